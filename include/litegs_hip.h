@@ -412,6 +412,24 @@ long long lg_morton_order_temp_bytes(long long n);
 int lg_morton_order(const float* xyz, long long n, int64_t* codes, int32_t* order, void* temp, long long temp_bytes, void* stream);
 int lg_permute_columns(const float* src, const int32_t* order, long long rows, long long n_src, long long n_dst, float* dst, void* stream);
 
+/* ---- draws.hip, sample.hip : random draws of training (litegs_amd/stochastic.py) -----------------------------------------------------
+ * dtype: 0 = float32, 1 = float16, 2 = bfloat16.  Word i of a draw is a function of (seed, offset, i) only (csrc/lg_philox.h);
+ * offset_dev (nullable, int64[1] on the device) is added to offset inside the kernel, so that a captured graph draws anew on every replay.
+ * lg_dropout: y[r,i] = word(index(i)) >= p * 2^32 ? x[r,i] / (1 - p) : 0 for x, y [lead, M]: one mask for all `lead` rows, never stored;
+ *   the backward pass is the same call on the gradient.  index(i) = i, or chunk_ids[i / S] * S + i % S (chunk_ids int64[M / S], nullable).
+ * lg_random_draw: std NULL: n uniforms (word + 1/2) / 2^32, kept below one; else n normals std[i] * N(0,1) (Box-Muller, two words a pair).
+ * lg_sample: R rows of V scores (row stride in elements, innermost contiguous), V < 2^31, n int64 indices per row to out [R, n]:
+ *   distinct = 0: n draws with replacement, u [R, n];  distinct = 1: the n largest keys of the exponential race, u [R, V], ascending, n <= V.
+ *   logits = 0: the scores are weights.  temperature > 0; top_k 0 = off; top_p in (0, 1]; min_p in [0, 1].  -1 = nothing (left) to draw.
+ *   temp: lg_sample_temp_bytes bytes, 16-byte aligned, contents irrelevant. */
+int lg_dropout(const void* x, void* y, int dtype, long long lead, long long M, double p, long long seed, long long offset,
+               const int64_t* offset_dev, const int64_t* chunk_ids, int S, void* stream);
+int lg_random_draw(const void* std_, void* out, int dtype, long long n, long long seed, long long offset, const int64_t* offset_dev, void* stream);
+long long lg_sample_temp_bytes(long long R, long long V, long long n, int distinct, int filtered);
+int lg_sample(const void* scores, int dtype, long long score_stride, const float* u, long long u_stride, long long R, long long V,
+              long long n, int distinct, int logits, double temperature, long long top_k, double top_p, double min_p,
+              int64_t* out, void* temp, long long temp_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

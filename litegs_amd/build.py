@@ -17,6 +17,7 @@ OBJ = os.path.join(HERE, "csrc", "_obj")
 ARCH = "gfx950"
 COMMON = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
           "-Wno-deprecated-declarations", "-I", CSRC, "-I", os.path.join(os.path.dirname(HERE), "include")]
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-file extra flags: exact (contraction-free) arithmetic where integer/index decisions must match the oracle
 SOURCES = {
     "transform.hip": ["-ffp-contract=off"],
@@ -29,6 +30,8 @@ SOURCES = {
     "dp.hip": ["-ffp-contract=off"],
     "knn.hip": [],
     "refine.hip": ["-ffp-contract=off"],
+    "draws.hip": NO_PACKED_FP32 + ["-ffp-contract=off"],
+    "sample.hip": NO_PACKED_FP32 + ["-ffp-contract=off"],
 }
 
 

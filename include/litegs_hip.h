@@ -420,12 +420,12 @@ int lg_permute_columns(const float* src, const int32_t* order, long long rows, l
  * lg_random_draw: std NULL: n uniforms (word + 1/2) / 2^32, kept below one; else n normals std[i] * N(0,1) (Box-Muller, two words a pair).
  * lg_sample: R rows of V scores (row stride in elements, innermost contiguous), V < 2^31, n int64 indices per row to out [R, n]:
  *   distinct = 0: n draws with replacement, u [R, n];  distinct = 1: the n largest keys of the exponential race, u [R, V], ascending, n <= V.
- *   logits = 0: the scores are weights.  temperature > 0; top_k 0 = off; top_p in (0, 1]; min_p in [0, 1].  -1 = nothing (left) to draw.
+ *   logits = 0: the scores are weights.  1e-30 <= temperature <= 1e30; top_k 0 = off; top_p in (0, 1]; min_p in [0, 1].  -1 = nothing (left) to draw.
  *   temp: lg_sample_temp_bytes bytes, 16-byte aligned, contents irrelevant. */
 int lg_dropout(const void* x, void* y, int dtype, long long lead, long long M, double p, long long seed, long long offset,
                const int64_t* offset_dev, const int64_t* chunk_ids, int S, void* stream);
 int lg_random_draw(const void* std_, void* out, int dtype, long long n, long long seed, long long offset, const int64_t* offset_dev, void* stream);
-long long lg_sample_temp_bytes(long long R, long long V, long long n, int distinct, int filtered);
+long long lg_sample_temp_bytes(long long R, long long V, long long n, int distinct);
 int lg_sample(const void* scores, int dtype, long long score_stride, const float* u, long long u_stride, long long R, long long V,
               long long n, int distinct, int logits, double temperature, long long top_k, double top_p, double min_p,
               int64_t* out, void* temp, long long temp_bytes, void* stream);

@@ -15,10 +15,9 @@
 #include "lg_types.h"
 #include "litegs_hip.h"
 
-#define SM_TPB 1024
-#define SM_BINS 2048
-#define SM_EPT 4                       // consecutive elements per thread of a prefix-sum step
-#define SM_STEP (SM_TPB * SM_EPT)
+
+#define SM_BINS 2048                   // bins of one level of a radix selection
+#define SM_MAX_WAVES 16
 
 enum { SM_LOGITS = 0, SM_LINEAR = 1, SM_POWER = 2 };
 
@@ -91,35 +90,46 @@ __device__ __forceinline__ double sm_sum_value(SmSum s)
 }
 
 // ---- workgroup-wide scans (fixed order) ----------------------------------------------------------------------------------------------
-template <typename V> __device__ __forceinline__ V sm_shfl_up(V v, int d) { return __shfl_up(v, d); }
+struct SmScratch { unsigned long long a[SM_MAX_WAVES + 1], b[SM_MAX_WAVES + 1], c[SM_MAX_WAVES + 1], word[4]; };
 
-// exclusive prefix of v over the workgroup and the total; `part` is LDS for one value per wave (+ 1)
-template <typename V> __device__ __forceinline__ V sm_block_scan(V v, V* part, V& total)
+// exclusive prefix of v over the workgroup, and the total; `part`: LDS for one 8-byte value per wave and one more
+template <typename V> __device__ __forceinline__ V sm_block_scan(V v, void* lds, V& total)
 {
+    V* part = (V*)lds;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     V inc = v;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const V o = sm_shfl_up(inc, d);
+        const V o = __shfl_up(inc, d);
         if (lane >= d) inc += o;
     }
     __syncthreads();
     if (lane == 63) part[wave] = inc;
     __syncthreads();
-    if (wave == 0) {
-        V w = lane < waves ? part[lane] : (V)0;
-        V winc = w;
+    V base = (V)0, sum = (V)0;                                         // every thread adds the waves up: no third barrier
+    for (int w = 0; w < waves; w++) {
+        if (w == wave) base = sum;
+        sum += part[w];
+    }
+    total = sum;
+    return base + (inc - v);
+}
+
+// inclusive maximum over the threads up to this one: sums that rounding made fall, or rise without a mass, are flat again
+__device__ __forceinline__ double sm_block_rise(double v, void* lds)
+{
+    double* part = (double*)lds;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            const V o = sm_shfl_up(winc, d);
-            if (lane >= d) winc += o;
-        }
-        if (lane < waves) part[lane] = winc - w;
-        if (lane == waves - 1) part[waves] = winc;
+    for (int d = 1; d < 64; d <<= 1) {
+        const double o = __shfl_up(v, d);
+        if (lane >= d) v = fmax(v, o);
     }
     __syncthreads();
-    total = part[waves];
-    return part[wave] + (inc - v);
+    if (lane == 63) part[wave] = v;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) v = fmax(v, part[w]);
+    return v;
 }
 
 __device__ __forceinline__ unsigned long long sm_block_max(unsigned long long v, unsigned long long* part)
@@ -135,50 +145,43 @@ __device__ __forceinline__ unsigned long long sm_block_max(unsigned long long v,
     return v;
 }
 
-// ---- histogram of one level of a radix selection, and the bin in which the selection ends ---------------------------------------------
+// ---- radix selection: histograms of one level, and the bin in which the selection ends -------------------------------------------------
 struct SmHist { uint32_t n[SM_BINS]; unsigned long long hi[SM_BINS], lo[SM_BINS]; };
 
-// An element is taken while what lies before it (best first) is less than the target.  `by_mass` false: counted in elements; true: in mass.
-struct SmTake { bool by_mass; double target; unsigned long long before_n; SmSum before_m; };
-
-struct SmScratch { unsigned long long u64[20], u64b[20], u64c[20]; double f64[20]; uint32_t u32[20]; unsigned long long word[4]; };
+// An element is taken while what lies before it (best first) is less than the target, counted in elements or in mass.
+struct SmTake { double target; unsigned long long before_n; SmSum before_m; };
 
 // The lowest non-empty bin whose predecessors (the bins above it) leave room.  Updates take.before_* to the amount above that bin and
-// returns the bin and its count; bin = -1: nothing there.
+// returns the bin and its count; -1: there is none.
+template <bool MASS>
 __device__ int sm_boundary(const SmHist& h, int nbins, SmTake& take, SmScratch& sc, unsigned long long& count)
 {
-    const int per = (nbins + SM_TPB - 1) / SM_TPB;                     // 1 or 2; thread t owns the bins nbins-1 - per*t - k
-    unsigned long long n[2] = { 0, 0 }, hi[2] = { 0, 0 }, lo[2] = { 0, 0 };
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
+    const int per = (nbins + (int)blockDim.x - 1) / (int)blockDim.x;   // thread t owns the bins nbins - 1 - (per * t + k), k < per
+    unsigned long long n = 0, hi = 0, lo = 0;
+    for (int k = 0; k < per; k++) {
         const int b = nbins - 1 - ((int)threadIdx.x * per + k);
-        if (k < per && b >= 0) {
-            n[k] = h.n[b];
-            if (take.by_mass) { hi[k] = h.hi[b]; lo[k] = h.lo[b]; }
-        }
+        if (b < 0) break;
+        n += h.n[b];
+        if (MASS) { hi += h.hi[b]; lo += h.lo[b]; }
     }
     unsigned long long tn, thi = 0, tlo = 0, bhi = 0, blo = 0;
-    unsigned long long bn = sm_block_scan<unsigned long long>(n[0] + n[1], sc.u64, tn);
-    if (take.by_mass) {
-        bhi = sm_block_scan<unsigned long long>(hi[0] + hi[1], sc.u64b, thi);
-        blo = sm_block_scan<unsigned long long>(lo[0] + lo[1], sc.u64c, tlo);
+    unsigned long long bn = take.before_n + sm_block_scan<unsigned long long>(n, sc.a, tn);
+    if (MASS) {
+        bhi = take.before_m.hi + sm_block_scan<unsigned long long>(hi, sc.b, thi);
+        blo = take.before_m.lo + sm_block_scan<unsigned long long>(lo, sc.c, tlo);
     }
-    unsigned long long mine = 0;                                       // 1 + position in descending order of the last bin that is entered
-    unsigned long long an = 0, ahi = 0, alo = 0, ac = 0;
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const unsigned long long before_n = take.before_n + bn;
-        const SmSum before_m = { take.before_m.hi + bhi, take.before_m.lo + blo };
-        const bool room = take.by_mass ? sm_sum_value(before_m) < take.target : (double)before_n < take.target;
-        if (k < per && n[k] != 0 && room) {
-            mine = (unsigned long long)threadIdx.x * per + k + 1;
-            an = before_n; ahi = before_m.hi; alo = before_m.lo; ac = n[k];
-        }
-        bn += n[k]; bhi += hi[k]; blo += lo[k];
+    unsigned long long mine = 0, an = 0, ahi = 0, alo = 0, ac = 0;     // mine: 1 + position, best first, of the last bin that is entered
+    for (int k = 0; k < per; k++) {
+        const int b = nbins - 1 - ((int)threadIdx.x * per + k);
+        if (b < 0) break;
+        const unsigned long long c = h.n[b];
+        const bool room = MASS ? sm_sum_value(SmSum{ bhi, blo }) < take.target : (double)bn < take.target;
+        if (c != 0 && room) { mine = (unsigned long long)(nbins - b); an = bn; ahi = bhi; alo = blo; ac = c; }
+        bn += c;
+        if (MASS) { bhi += h.hi[b]; blo += h.lo[b]; }
     }
-    const unsigned long long best = sm_block_max(mine, sc.u64);
+    const unsigned long long best = sm_block_max(mine, sc.a);
     if (best == 0) { count = 0; return -1; }
-    __syncthreads();
     if (mine == best) { sc.word[0] = an; sc.word[1] = ahi; sc.word[2] = alo; sc.word[3] = ac; }
     __syncthreads();
     take.before_n = sc.word[0];
@@ -189,256 +192,966 @@ __device__ int sm_boundary(const SmHist& h, int nbins, SmTake& take, SmScratch& 
 }
 
 // of `count` elements of equal key behind what is before them: how many are taken (at least one, by the choice of the bin)
-__device__ __forceinline__ unsigned long long sm_ties(const SmTake& take, unsigned long long count, double mass)
+template <bool MASS> __device__ __forceinline__ unsigned long long sm_ties(const SmTake& take, unsigned long long count, double mass)
 {
-    if (!take.by_mass) {
+    if (!MASS) {
         const double left = take.target - (double)take.before_n;
         return left >= (double)count ? count : (unsigned long long)ceil(left);
     }
     const SmSum one = sm_limbs(mass);
-    auto room = [&](unsigned long long j) {                            // is the j-th equal (from 0) taken?
-        return sm_sum_value(SmSum{ take.before_m.hi + j * one.hi, take.before_m.lo + j * one.lo }) < take.target;
-    };
-    unsigned long long lo = 1, hi = count;                             // room(0) holds; the answer is the first j without room
+    unsigned long long lo = 1, hi = count;                             // the first j (from 0) that finds no room
     while (lo < hi) {
         const unsigned long long mid = lo + (hi - lo) / 2;
-        if (room(mid)) lo = mid + 1; else hi = mid;
+        if (sm_sum_value(SmSum{ take.before_m.hi + mid * one.hi, take.before_m.lo + mid * one.lo }) < take.target) lo = mid + 1; else hi = mid;
     }
     return lo;
 }
-
-// ---- one workgroup per row -----------------------------------------------------------------------------------------------------------
-// what passes the filters: key > thr, or key == thr and index <= last; and mass >= least
-struct SmKept { uint32_t thr; long long last; double least; };
-
-template <typename T> struct SmRow {
-    const T* x; long long V; bool logits; SmScale scale;
-    __device__ __forceinline__ uint32_t key(long long i) const { return sm_key(x[i], logits); }
-    __device__ __forceinline__ bool in(const SmKept& k, uint32_t key, long long i) const
-    {
-        return key != 0u && (key > k.thr || (key == k.thr && i <= k.last)) && (k.least <= 0.0 || sm_mass(scale, key) >= k.least);
-    }
-};
-
-// shrinks `kept` to the elements that `take` leaves; keys(i) is an unsigned key of `bits` bits (0: not a candidate)
-template <int BITS, typename Key, typename Mass>
-__device__ void sm_select(long long V, const Key& keys, const Mass& mass_of, SmTake take, SmHist& h, SmScratch& sc,
-                          unsigned long long& thr, unsigned long long& ties, unsigned long long& equal)
+// every element of the boundary bin is taken: the selection needs no further level
+template <bool MASS> __device__ __forceinline__ bool sm_whole_bin(const SmTake& take, unsigned long long count)
 {
-    unsigned long long prefix = 0, count = 0;
+    return count == 1 || (!MASS && take.target - (double)take.before_n >= (double)count);
+}
+
+// What passes the filters: key > thr, or key == thr and index <= last (key 0 never does).
+struct SmKept { uint32_t thr, last; };
+#define SM_ALL 0xffffffffu
+__device__ __forceinline__ bool sm_in(const SmKept& k, uint32_t key, uint32_t i) { return key != 0u && (key > k.thr || (key == k.thr && i <= k.last)); }
+
+// min-p as a cut of the keys: the smallest key whose mass is at least min_p of the best one's (the mass grows with the key)
+__device__ __forceinline__ void sm_min_p(const SmScale& s, uint32_t best, double min_p, SmKept& kept)
+{
+    const double least = min_p * sm_mass(s, best);
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = 1, hi = best;                                        // 64 probes a round; the mass at hi is enough
+    while (lo < hi) {
+        const uint32_t gap = (hi - lo) / 64 + 1;
+        const unsigned long long p = (unsigned long long)lo + (unsigned long long)lane * gap;
+        const unsigned long long ok = __ballot(p >= hi || sm_mass(s, (uint32_t)p) >= least);
+        const uint32_t f = ok ? (uint32_t)__ffsll((long long)ok) - 1 : 64;
+        const unsigned long long nhi = (unsigned long long)lo + (unsigned long long)f * gap;
+        if (f) lo += (f - 1) * gap + 1;
+        hi = nhi < hi ? (uint32_t)nhi : hi;
+    }
+    if (lo > kept.thr) kept = SmKept{ lo, SM_ALL };
+}
+
+// Unrolled 64-bit exponentials and logarithms are kept apart: interleaved by the scheduler, sixteen of them spill two thousand registers.
+#define SM_ONE_AT_A_TIME() __builtin_amdgcn_sched_barrier(0)
+
+// ---- short rows: one workgroup per row, EPT consecutive elements of a thread in registers ----------------------------------------------
+// Narrows `kept` (or, for 64-bit race keys, finds thr / ties): each[k] is the key of element threadIdx.x * EPT + k, 0: not a candidate.
+template <bool MASS, int BITS, int EPT, typename Word, typename Mass>
+__device__ void sm_select_short(const Word (&key)[EPT], const Mass& mass_of, SmTake take, SmHist& h, SmScratch& sc,
+                                Word& thr, unsigned long long& ties, unsigned long long& equal)
+{
+    Word prefix = 0;
+    unsigned long long count = 0;
     int shift = BITS;
+    thr = 0; ties = equal = 0;
     while (shift > 0) {
-        const int width = shift >= 11 ? 11 : shift;
-        const int at = shift - width, nbins = 1 << width;
+        const int width = shift >= 11 ? 11 : shift, at = shift - width, nbins = 1 << width;
         __syncthreads();
-        for (int b = threadIdx.x; b < nbins; b += SM_TPB) { h.n[b] = 0; if (take.by_mass) { h.hi[b] = 0; h.lo[b] = 0; } }
+        for (int b = threadIdx.x; b < nbins; b += blockDim.x) { h.n[b] = 0; if (MASS) { h.hi[b] = 0; h.lo[b] = 0; } }
         __syncthreads();
-        for (long long i = threadIdx.x; i < V; i += SM_TPB) {
-            const unsigned long long k = keys(i);
-            if (k == 0ull || (shift < 64 && (k >> shift) != prefix)) continue;
-            const int b = (int)((k >> at) & (unsigned long long)(nbins - 1));
+#pragma unroll
+        for (int k = 0; k < EPT; k++) {
+            if (key[k] == 0 || (shift < BITS && (key[k] >> shift) != prefix)) continue;
+            const int b = (int)(key[k] >> at) & (nbins - 1);
             atomicAdd(&h.n[b], 1u);
-            if (take.by_mass) {
-                const SmSum m = sm_limbs(mass_of(k));
+            if (MASS) {
+                SM_ONE_AT_A_TIME();
+                const SmSum m = sm_limbs(mass_of(key[k]));
                 if (m.hi) atomicAdd(&h.hi[b], m.hi);
                 if (m.lo) atomicAdd(&h.lo[b], m.lo);
             }
         }
         __syncthreads();
-        const int b = sm_boundary(h, nbins, take, sc, count);
-        if (b < 0) { thr = ~0ull; ties = 0; equal = 0; return; }       // no candidate at all
-        prefix = (prefix << width) | (unsigned)b;
+        const int b = sm_boundary<MASS>(h, nbins, take, sc, count);
+        if (b < 0) { thr = ~(Word)0; return; }                         // no candidate at all
+        prefix = (Word)(prefix << width) | (Word)b;
         shift = at;
+        if (sm_whole_bin<MASS>(take, count)) { thr = prefix << at; ties = equal = 1; return; }
     }
     thr = prefix;
     equal = count;
-    ties = sm_ties(take, count, take.by_mass ? mass_of(thr) : 0.0);
+    ties = sm_ties<MASS>(take, count, MASS ? mass_of(thr) : 0.0);
 }
 
-// index of the n-th (from 1) element with is(i), in index order
-template <typename Is> __device__ long long sm_nth(long long V, unsigned long long n, const Is& is, SmScratch& sc)
+// index of the n-th (from 1) flagged element
+template <int EPT> __device__ uint32_t sm_nth_short(const bool (&flag)[EPT], unsigned long long n, SmScratch& sc)
 {
-    unsigned long long done = 0;
+    uint32_t c = 0, total;
+#pragma unroll
+    for (int k = 0; k < EPT; k++) c += flag[k];
+    uint32_t at = sm_block_scan<uint32_t>(c, sc.a, total);
+#pragma unroll
+    for (int k = 0; k < EPT; k++) if (flag[k] && ++at == n) sc.word[0] = threadIdx.x * EPT + k;
     __syncthreads();
-    if (threadIdx.x == 0) sc.word[0] = ~0ull;
+    const uint32_t i = (uint32_t)sc.word[0];
     __syncthreads();
-    for (long long base = 0; base < V; base += SM_TPB) {
-        const long long i = base + threadIdx.x;
-        const bool f = i < V && is(i);
-        uint32_t total;
-        const uint32_t before = sm_block_scan<uint32_t>(f ? 1u : 0u, sc.u32, total);
-        if (f && done + before + 1 == n) sc.word[0] = (unsigned long long)i;
-        done += total;
-        if (done >= n) break;
+    return i;
+}
+
+// four consecutive scores from i on as keys; beyond V: 0
+template <typename T> __device__ __forceinline__ void sm_load4(const T* x, long long i, long long V, bool vec, bool logits, uint32_t* key)
+{
+    if (vec && i + 4 <= V) {
+        const LgVec4<T> v = *(const LgVec4<T>*)(x + i);
+#pragma unroll
+        for (int k = 0; k < 4; k++) key[k] = sm_key(v.v[k], logits);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) key[k] = i + k < V ? sm_key(x[i + k], logits) : 0u;
     }
+}
+template <typename T> __device__ __forceinline__ bool sm_aligned(const T* x) { return (uintptr_t)x % (4 * sizeof(T)) == 0; }
+
+template <typename T, int TPB, int EPT, bool DISTINCT>
+__global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
+                                                            int V, long long n, SmRule rule, long long* __restrict__ out)
+{
+    __shared__ union { SmHist hist; double cdf[DISTINCT ? 1 : TPB * EPT]; } h;
+    __shared__ uint16_t pos[DISTINCT ? 1 : TPB];
+    __shared__ SmScratch sc;
+    const long long r = blockIdx.x;
+    const T* x = scores + r * sstride;
+    const bool logits = rule.mode == SM_LOGITS;
+    u += r * ustride;
+    out += r * n;
+    const int i0 = threadIdx.x * EPT;
+    uint32_t key[EPT], best = 0;
+#pragma unroll
+    for (int k = 0; k < EPT; k += 4) sm_load4(x, i0 + k, V, sm_aligned(x), logits, key + k);
+    float uk[EPT];
+    if (DISTINCT) {
+#pragma unroll
+        for (int k = 0; k < EPT; k++) uk[k] = i0 + k < V ? u[i0 + k] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < EPT; k++) best = key[k] > best ? key[k] : best;
+    best = (uint32_t)sm_block_max(best, sc.a);
+    if (best == 0) {                                                   // nothing to draw from
+        for (long long j = threadIdx.x; j < n; j += blockDim.x) out[j] = -1;
+        return;
+    }
+    const SmScale scale = sm_scale(rule, best);
+    const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
+    auto mass_of = [&](uint32_t k) { return sm_mass(scale, k) * unit; };
+    // filters: an element that one of them drops becomes key 0
+    for (int pass = 0; pass < 2; pass++) {
+        SmTake take = { 0.0, 0, { 0, 0 } };
+        uint32_t thr;
+        unsigned long long ties, equal;
+        if (pass == 0) {
+            if (rule.top_k <= 0 || rule.top_k >= V) continue;
+            take.target = (double)rule.top_k;
+            sm_select_short<false, 32, EPT, uint32_t>(key, mass_of, take, h.hist, sc, thr, ties, equal);
+        } else {
+            if (rule.top_p >= 1.0) continue;
+            SmSum mine = { 0, 0 }, total;
+#pragma unroll
+            for (int k = 0; k < EPT; k++)
+                if (key[k]) { SM_ONE_AT_A_TIME(); const SmSum m = sm_limbs(mass_of(key[k])); mine.hi += m.hi; mine.lo += m.lo; }
+            sm_block_scan<unsigned long long>(mine.hi, sc.a, total.hi);
+            sm_block_scan<unsigned long long>(mine.lo, sc.b, total.lo);
+            take.target = rule.top_p * sm_sum_value(total);
+            sm_select_short<true, 32, EPT, uint32_t>(key, mass_of, take, h.hist, sc, thr, ties, equal);
+        }
+        SmKept kept = { thr, SM_ALL };
+        if (ties < equal) {
+            bool tie[EPT];
+#pragma unroll
+            for (int k = 0; k < EPT; k++) tie[k] = key[k] == thr;
+            kept.last = sm_nth_short<EPT>(tie, ties, sc);
+        }
+#pragma unroll
+        for (int k = 0; k < EPT; k++) if (!sm_in(kept, key[k], (uint32_t)(i0 + k))) key[k] = 0;
+    }
+    if (rule.min_p > 0.0) {
+        SmKept kept = { 0u, SM_ALL };
+        sm_min_p(scale, best, rule.min_p, kept);
+#pragma unroll
+        for (int k = 0; k < EPT; k++) if (!sm_in(kept, key[k], (uint32_t)(i0 + k))) key[k] = 0;
+    }
+    if (DISTINCT) {
+        unsigned long long race[EPT], thr, ties, equal;
+#pragma unroll
+        for (int k = 0; k < EPT; k++) { race[k] = sm_race(scale, key[k], uk[k]); SM_ONE_AT_A_TIME(); }
+        const SmTake take = { (double)n, 0, { 0, 0 } };
+        sm_select_short<false, 64, EPT, unsigned long long>(race, [](unsigned long long) { return 0.0; }, take, h.hist, sc, thr, ties, equal);
+        uint32_t last = SM_ALL, c = 0, total;
+        if (ties < equal) {
+            bool tie[EPT];
+#pragma unroll
+            for (int k = 0; k < EPT; k++) tie[k] = race[k] == thr;
+            last = sm_nth_short<EPT>(tie, ties, sc);
+        }
+        bool win[EPT];
+#pragma unroll
+        for (int k = 0; k < EPT; k++) {
+            win[k] = race[k] != 0 && (race[k] > thr || (race[k] == thr && (uint32_t)(i0 + k) <= last));
+            c += win[k];
+        }
+        long long at = sm_block_scan<uint32_t>(c, sc.a, total);
+#pragma unroll
+        for (int k = 0; k < EPT; k++) if (win[k]) out[at++] = i0 + k;
+        for (long long j = (long long)total + threadIdx.x; j < n; j += blockDim.x) out[j] = -1;
+    } else {
+        double* cdf = h.cdf;                                           // the histograms are done
+        double w[EPT], sum = 0.0, total;
+        uint32_t positive = 0, last = 0;
+#pragma unroll
+        for (int k = 0; k < EPT; k++) {
+            w[k] = sm_mass(scale, key[k]);
+            sum += w[k];
+            if (w[k] > 0.0) { positive |= 1u << k; last = (uint32_t)(i0 + k) + 1; }
+            SM_ONE_AT_A_TIME();
+        }
+        double at = sm_block_scan<double>(sum, sc.a, total);
+        last = (uint32_t)sm_block_max(last, sc.b);
+#pragma unroll
+        for (int k = 0; k < EPT; k++) { at += w[k]; cdf[i0 + k] = at; }
+        pos[threadIdx.x] = (uint16_t)positive;
+        __syncthreads();
+        for (long long j = threadIdx.x; j < n; j += TPB) {
+            const float uj = u[j];
+            const double t = (uj > 0.0f ? (double)uj : 0.0) * total;
+            uint32_t lo = 0, hi = last - 1;                            // first element whose sum passes t; at the end the last one with a mass
+            while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (cdf[mid] > t) hi = mid; else lo = mid + 1; }
+            while (lo < last - 1 && !((pos[lo / EPT] >> (lo % EPT)) & 1)) lo++;      // rounding at a border never lands on a masked element
+            out[j] = lo;
+        }
+    }
+}
+
+// ---- long rows: B workgroups per row ---------------------------------------------------------------------------------------------------
+// Every step is one launch over (row, workgroup); the last workgroup of a row to finish a step (SmRowState::ticket) draws its conclusion and
+// leaves it in the row's state for the next launch.
+#define SM_LTPB 512
+#define SM_RBINS 4096                  // bins of a level of the race's approximate keys
+#define SM_TILE 8192                   // elements per workgroup step of the race's last pass: 128 words of winners
+#define SM_STILE 4096                  // elements per tile of prefix sums
+#define SM_GROUP 16                    // elements per stored prefix
+#define SM_STEPS 12
+
+struct SmRowState {
+    SmKept kept, before;               // what passes the filters; ... before the selection under way
+    SmTake take;
+    unsigned long long prefix, count, ties;
+    double total, top;                 // sample: total mass of the kept; the largest l
+    unsigned long long sure;           // race: winners outside the zone
+    uint32_t best, ended, cut, zone_lo, zone_hi, candidates;
+    uint32_t ticket[SM_STEPS];
+};
+
+struct SmWork {                        // workspace of a call: everything per row
+    SmRowState* state; SmHist* hist; uint32_t* rbins;
+    uint32_t* tile_n; uint32_t* keys; unsigned long long* words; uint32_t* list;
+    double *group, *tile_sum, *tile_top;
+    long long B, tiles, stiles, capacity, vpad;
+};
+
+__device__ __forceinline__ bool sm_last_block(uint32_t* ticket, uint32_t blocks, uint32_t* lds)
+{
+    __threadfence();
     __syncthreads();
-    const long long at = (long long)sc.word[0];
+    if (threadIdx.x == 0) *lds = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    return at;
+    const bool last = *lds == blocks - 1;
+    if (last) __threadfence();
+    return last;
+}
+template <typename V> __device__ __forceinline__ V sm_peek(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+__global__ void __launch_bounds__(256) sm_clear_kernel(uint4* p, long long n)
+{
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) p[i] = uint4{ 0, 0, 0, 0 };
 }
 
 template <typename T>
-__device__ SmKept sm_filter_row(SmRow<T>& row, const SmRule& rule, SmHist& h, SmScratch& sc)
+__global__ void __launch_bounds__(SM_LTPB) sm_best_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step)
 {
-    unsigned long long best = 0;
-    for (long long i = threadIdx.x; i < row.V; i += SM_TPB) { const unsigned long long k = row.key(i); best = k > best ? k : best; }
-    best = sm_block_max(best, sc.u64);
-    row.scale = sm_scale(rule, (uint32_t)best);
-    SmKept kept = { 0u, 0x7fffffffffffffffll, 0.0 };
-    if (best == 0) return kept;
-    const double unit = row.scale.mode == SM_LINEAR ? row.scale.shift : 1.0;
-    auto mass_of = [&](unsigned long long k) { return sm_mass(row.scale, (uint32_t)k) * unit; };
-    for (int pass = 0; pass < 2; pass++) {
-        SmTake take = { pass == 1, 0.0, 0, { 0, 0 } };
-        if (pass == 0) {
-            if (rule.top_k <= 0 || rule.top_k >= row.V) continue;
-            take.target = (double)rule.top_k;
-        } else {
-            if (rule.top_p >= 1.0) continue;
-            unsigned long long hi = 0, lo = 0;
-            for (long long i = threadIdx.x; i < row.V; i += SM_TPB) {
-                const uint32_t k = row.key(i);
-                if (!row.in(kept, k, i)) continue;
-                const SmSum m = sm_limbs(mass_of(k));
-                hi += m.hi; lo += m.lo;
+    __shared__ unsigned long long part[SM_MAX_WAVES + 1];
+    const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
+    const T* x = scores + r * sstride;
+    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    uint32_t best = 0;
+    for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += wk.B * SM_LTPB * 4) {
+        uint32_t k[4];
+        sm_load4(x, i, V, vec, logits, k);
+#pragma unroll
+        for (int j = 0; j < 4; j++) best = k[j] > best ? k[j] : best;
+    }
+    best = (uint32_t)sm_block_max(best, part);
+    if (threadIdx.x == 0 && best) atomicMax(&wk.state[r].best, best);
+    (void)step;
+}
+
+// one level of top-k (MASS false) or top-p: bits [at, at + width) of the keys that pass the filters and match the prefix found so far
+template <typename T, bool MASS>
+__global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step,
+                                                           int shift, int width)
+{
+    __shared__ SmHist h;
+    __shared__ SmScratch sc;
+    __shared__ uint32_t ticket;
+    const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
+    SmRowState& st = wk.state[r];
+    const bool first = shift == 32;
+    if (!first && st.ended) return;
+    const T* x = scores + r * sstride;
+    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const SmKept kept = first ? st.kept : st.before;
+    const uint32_t prefix = (uint32_t)st.prefix;
+    const int at = shift - width, nbins = 1 << width;
+    const SmScale scale = sm_scale(rule, MASS ? st.best : 0u);
+    const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
+    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) { h.n[i] = 0; if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } }
+    __syncthreads();
+    for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += wk.B * SM_LTPB * 4) {
+        uint32_t key[4];
+        sm_load4(x, i, V, vec, logits, key);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (!sm_in(kept, key[j], (uint32_t)(i + j)) || (!first && (key[j] >> shift) != prefix)) continue;
+            const int bin = (int)(key[j] >> at) & (nbins - 1);
+            atomicAdd(&h.n[bin], 1u);
+            if (MASS) {
+                const SmSum m = sm_limbs(sm_mass(scale, key[j]) * unit);
+                if (m.hi) atomicAdd(&h.hi[bin], m.hi);
+                if (m.lo) atomicAdd(&h.lo[bin], m.lo);
             }
-            SmSum total;
-            sm_block_scan<unsigned long long>(hi, sc.u64, total.hi);
-            sm_block_scan<unsigned long long>(lo, sc.u64b, total.lo);
+        }
+    }
+    __syncthreads();
+    SmHist& g = wk.hist[r];
+    for (int i = threadIdx.x; i < nbins; i += SM_LTPB)
+        if (h.n[i]) {
+            atomicAdd(&g.n[i], h.n[i]);
+            if (MASS) { if (h.hi[i]) atomicAdd(&g.hi[i], h.hi[i]); if (h.lo[i]) atomicAdd(&g.lo[i], h.lo[i]); }
+        }
+    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) {               // taken over, and left clear for the next level
+        h.n[i] = sm_peek(&g.n[i]); g.n[i] = 0;
+        if (MASS) { h.hi[i] = sm_peek(&g.hi[i]); h.lo[i] = sm_peek(&g.lo[i]); g.hi[i] = 0; g.lo[i] = 0; }
+    }
+    __syncthreads();
+    SmTake take = st.take;
+    if (first) {
+        take = SmTake{ (double)rule.top_k, 0, { 0, 0 } };
+        if (MASS) {
+            SmSum mine = { 0, 0 }, total;
+            for (int i = threadIdx.x; i < nbins; i += SM_LTPB) { mine.hi += h.hi[i]; mine.lo += h.lo[i]; }
+            sm_block_scan<unsigned long long>(mine.hi, sc.a, total.hi);
+            sm_block_scan<unsigned long long>(mine.lo, sc.b, total.lo);
             take.target = rule.top_p * sm_sum_value(total);
         }
-        unsigned long long thr, ties, equal;
-        const SmKept before = kept;
-        auto keys = [&](long long i) { const uint32_t k = row.key(i); return row.in(before, k, i) ? (unsigned long long)k : 0ull; };
-        sm_select<32>(row.V, keys, mass_of, take, h, sc, thr, ties, equal);
-        kept.thr = (uint32_t)thr;
-        if (kept.thr != before.thr) kept.last = 0x7fffffffffffffffll;      // an earlier filter's cut was among other equals
-        if (ties < equal) kept.last = sm_nth(row.V, ties, [&](long long i) { return keys(i) == thr; }, sc);
     }
-    if (rule.min_p > 0.0) kept.least = rule.min_p * sm_mass(row.scale, (uint32_t)best);
+    unsigned long long count;
+    const int bin = sm_boundary<MASS>(h, nbins, take, sc, count);
+    if (threadIdx.x != 0) return;
+    st.before = kept;
+    st.take = take;
+    st.ended = 0;
+    st.cut = 0;
+    if (bin < 0) { st.ended = 1; return; }                             // no candidate: the filter in force (or an empty row) stands
+    const uint32_t p = (first ? 0u : prefix << width) | (uint32_t)bin;
+    st.prefix = p;
+    const bool whole = sm_whole_bin<MASS>(take, count);
+    if (!whole && at > (sizeof(T) == 2 ? 10 : 0)) return;
+    // the key is found (or the lowest key of a bin that is taken whole); a cut among the equal ones is left to sm_tie_kernel.  Scores of 16
+    // bits differ in the 22 leading bits of their keys: what follows is all zeros, or all ones for a negative score.
+    const uint32_t thr = !whole && at && !(p >> (31 - at)) ? (p << at) | ((1u << at) - 1) : p << at;
+    unsigned long long ties = count;
+    if (!whole) ties = sm_ties<MASS>(take, count, MASS ? sm_mass(scale, thr) * unit : 0.0);
+    st.ended = 1;
+    if (thr < kept.thr) return;                                        // a whole bin around the earlier filter's cut: that one stands
+    st.kept = SmKept{ thr, thr == kept.thr ? kept.last : SM_ALL };
+    if (ties < count) { st.cut = 1; st.ties = ties; }
+}
+
+// index of the last equal element that is kept, where a selection ends inside equal keys; and min-p, once, behind the last filter
+template <typename T>
+__global__ void __launch_bounds__(SM_LTPB) sm_tie_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step)
+{
+    __shared__ SmScratch sc;
+    __shared__ uint32_t ticket;
+    const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
+    SmRowState& st = wk.state[r];
+    if (!st.cut) return;
+    const T* x = scores + r * sstride;
+    const bool logits = rule.mode == SM_LOGITS;
+    const SmKept kept = st.kept;
+    uint32_t* tile_n = wk.tile_n + r * wk.tiles;
+    auto tie = [&](long long i) { const uint32_t k = i < V ? sm_key(x[i], logits) : 0u; return k != 0u && k == kept.thr && (uint32_t)i <= kept.last; };
+    for (long long t = b; t < wk.tiles; t += wk.B) {
+        uint32_t c = 0, total;
+        for (int k = 0; k < SM_TILE / SM_LTPB; k++) c += tie(t * SM_TILE + k * SM_LTPB + threadIdx.x);
+        sm_block_scan<uint32_t>(c, sc.a, total);
+        if (threadIdx.x == 0) __hip_atomic_store(&tile_n[t], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    const unsigned long long want = st.ties;
+    unsigned long long done = 0;
+    long long tile = -1;
+    for (long long base = 0; base < wk.tiles && tile < 0; base += SM_LTPB) {
+        const long long t = base + threadIdx.x;
+        const uint32_t c = t < wk.tiles ? sm_peek(&tile_n[t]) : 0u;
+        uint32_t total;
+        const uint32_t before = sm_block_scan<uint32_t>(c, sc.a, total);
+        const bool here = done + before < want && want <= done + before + c;
+        if (here) { sc.word[0] = (unsigned long long)t; sc.word[1] = done + before; }
+        if (want <= done + total) {                                    // uniform
+            __syncthreads();
+            tile = (long long)sc.word[0];
+            done = sc.word[1];
+        } else done += total;
+    }
+    if (tile < 0) return;                                              // cannot be: `want` counts these very elements
+    for (int k = 0; k < SM_TILE / SM_LTPB; k++) {
+        const long long i = tile * SM_TILE + k * SM_LTPB + threadIdx.x;
+        const bool f = tie(i);
+        uint32_t total;
+        const uint32_t before = sm_block_scan<uint32_t>(f ? 1u : 0u, sc.a, total);
+        if (f && done + before + 1 == want) { st.kept.last = (uint32_t)i; st.cut = 0; }
+        done += total;
+        if (done >= want) break;                                       // uniform
+    }
+}
+
+// filter in force with min-p (every wave works the cut out for itself)
+__device__ __forceinline__ SmKept sm_final(const SmRowState& st, const SmRule& rule)
+{
+    SmKept kept = st.kept;
+    if (rule.min_p > 0.0 && st.best) sm_min_p(sm_scale(rule, st.best), st.best, rule.min_p, kept);
     return kept;
 }
 
+// ---- long rows, with replacement -------------------------------------------------------------------------------------------------------
+// Prefix sums of the kept masses inside tiles, one stored per SM_GROUP elements, relative to the tile's best element (so that no pass for the
+// row's best is needed); the last workgroup puts the tiles on a common scale.  Fixed order everywhere.
 template <typename T>
-__global__ void __launch_bounds__(SM_TPB) sample_row_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
-                                                            long long V, long long n, SmRule rule, long long* __restrict__ out)
+__global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step)
 {
-    __shared__ SmHist h;
     __shared__ SmScratch sc;
-    double* cdf = (double*)&h;                                         // the histograms are done when the prefix sums begin
-    static_assert(sizeof(SmHist) >= SM_STEP * sizeof(double), "");
-    const long long r = blockIdx.x;
-    SmRow<T> row = { scores + r * sstride, V, rule.mode == SM_LOGITS, {} };
-    const SmKept kept = sm_filter_row(row, rule, h, sc);
-    out += r * n;
-    u += r * ustride;
-    // two passes over the prefix sums of the kept masses, in the same order: the first for the total, the second finds the draws of each step
-    auto weight = [&](long long i) {
-        if (i >= V) return 0.0;
-        const uint32_t k = row.key(i);
-        return row.in(kept, k, i) ? sm_mass(row.scale, k) : 0.0;
-    };
-    double total = 0.0;
-    unsigned long long last = 0;
-    for (int pass = 0; pass < 2; pass++) {
-        double run = 0.0;
-        for (long long base = 0; base < V; base += SM_STEP) {
-            double w[SM_EPT], sum = 0.0, step;
+    __shared__ uint32_t ticket;
+    const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
+    SmRowState& st = wk.state[r];
+    const T* x = scores + r * sstride;
+    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const SmKept kept = sm_final(st, rule);
+    double *sums = wk.tile_sum + r * (wk.stiles + 1), *tops = wk.tile_top + r * wk.stiles, *groups = wk.group + r * wk.stiles * (SM_STILE / SM_GROUP);
+    for (long long t = b; t < wk.stiles; t += wk.B) {
+        const long long i0 = t * SM_STILE + threadIdx.x * SM_GROUP;
+        uint32_t key[SM_GROUP], best = 0;
 #pragma unroll
-            for (int k = 0; k < SM_EPT; k++) {
-                const long long i = base + (long long)threadIdx.x * SM_EPT + k;
-                w[k] = weight(i);
-                sum += w[k];
-                if (pass == 0 && w[k] > 0.0) last = (unsigned long long)i + 1;
-            }
-            double at = run + sm_block_scan<double>(sum, sc.f64, step);
-            if (pass == 1) {
+        for (int k = 0; k < SM_GROUP; k += 4) sm_load4(x, i0 + k, V, vec, logits, key + k);
 #pragma unroll
-                for (int k = 0; k < SM_EPT; k++) { at += w[k]; cdf[threadIdx.x * SM_EPT + k] = at; }
-                __syncthreads();
-                const double end = run + step;
-                for (long long j = threadIdx.x; j < n; j += SM_TPB) {
-                    const float uj = u[j];
-                    const double t = (uj > 0.0f ? (double)uj : 0.0) * total;
-                    if (!(t >= run && (t < end || base + SM_STEP >= V))) continue;
-                    int lo = 0, hi = SM_STEP;                          // first position with cdf > t
-                    while (lo < hi) { const int mid = (lo + hi) >> 1; if (cdf[mid] > t) hi = mid; else lo = mid + 1; }
-                    long long i = base + lo;
-                    while (i < (long long)last && !(weight(i) > 0.0)) i++;      // rounding at a border never lands on an excluded element
-                    out[j] = i < (long long)last ? i : (long long)last - 1;
-                }
-            }
-            run += step;
+        for (int k = 0; k < SM_GROUP; k++) {
+            if (!sm_in(kept, key[k], (uint32_t)(i0 + k))) key[k] = 0;
+            best = key[k] > best ? key[k] : best;
         }
-        if (pass == 0) {
-            total = run;
-            last = sm_block_max(last, sc.u64);
-            if (last == 0) {                                           // nothing to draw from
-                for (long long j = threadIdx.x; j < n; j += SM_TPB) out[j] = -1;
-                return;
+        best = (uint32_t)sm_block_max(best, sc.b);
+        const SmScale scale = sm_scale(rule, best);
+        double sum = 0.0, total;
+#pragma unroll
+        for (int k = 0; k < SM_GROUP; k++) sum += sm_mass(scale, key[k]);
+        const double before = sm_block_scan<double>(sum, sc.a, total);
+        groups[t * (SM_STILE / SM_GROUP) + threadIdx.x] = sm_block_rise(sum > 0.0 ? before + sum : 0.0, sc.b);
+        if (threadIdx.x == 0) {
+            __hip_atomic_store(&sums[t], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(&tops[t], best ? scale.top : -INFINITY, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    double top = -INFINITY;
+    for (long long t = threadIdx.x; t < wk.stiles; t += 256) top = fmax(top, sm_peek(&tops[t]));
+    const unsigned long long ordered = (unsigned long long)__double_as_longlong(top + 0.0);
+    const unsigned long long m = sm_block_max((ordered >> 63) ? ~ordered : (ordered | 0x8000000000000000ull), sc.b);
+    top = __longlong_as_double((long long)((m >> 63) ? (m & 0x7fffffffffffffffull) : ~m));
+    double run = 0.0, risen = 0.0;
+    for (long long base = 0; base < wk.stiles; base += 256) {
+        const long long t = base + threadIdx.x;
+        double mass = 0.0, total;
+        if (t < wk.stiles) {
+            const double tt = sm_peek(&tops[t]);
+            mass = sm_peek(&sums[t]) * (rule.mode == SM_LINEAR || tt == -INFINITY ? 1.0 : exp(tt - top));
+        }
+        const double before = sm_block_scan<double>(mass, sc.a, total);
+        const double upto = fmax(sm_block_rise(mass > 0.0 ? run + before + mass : 0.0, sc.b), risen);
+        if (t < wk.stiles) sums[t] = upto;
+        __syncthreads();
+        if (threadIdx.x == 255) sc.word[0] = (unsigned long long)__double_as_longlong(upto);
+        __syncthreads();
+        risen = __longlong_as_double((long long)sc.word[0]);
+        run += total;
+    }
+    if (threadIdx.x == 0) { st.total = run; st.top = top; st.kept = kept; }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
+                                                      long long R, long long V, long long n, SmRule rule, SmWork wk, long long* __restrict__ out)
+{
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= R * n) return;
+    const long long r = at / n, j = at - r * n;
+    const SmRowState& st = wk.state[r];
+    const double* sums = wk.tile_sum + r * (wk.stiles + 1);
+    const double* tops = wk.tile_top + r * wk.stiles;
+    const double total = sums[wk.stiles - 1];
+    if (!(total > 0.0)) { out[at] = -1; return; }
+    const float uj = u[r * ustride + j];
+    const double target = (uj > 0.0f ? (double)uj : 0.0) * st.total;
+    auto first = [](const double* a, long long n, auto&& past) {       // first position with past(a[.]), or n - 1
+        long long lo = 0, hi = n - 1;
+        while (lo < hi) { const long long mid = (lo + hi) >> 1; if (past(a[mid])) hi = mid; else lo = mid + 1; }
+        return lo;
+    };
+    long long t = first(sums, wk.stiles, [&](double s) { return s > target; });
+    if (!(sums[t] > target)) t = first(sums, wk.stiles, [&](double s) { return s >= total; });
+    const double* g = wk.group + (r * wk.stiles + t) * (SM_STILE / SM_GROUP);
+    const int ng = SM_STILE / SM_GROUP;
+    const double scale_up = rule.mode == SM_LINEAR ? 1.0 : exp(tops[t] - st.top);
+    const double local = fmax((target - (t ? sums[t - 1] : 0.0)) / scale_up, 0.0);
+    long long k = first(g, ng, [&](double s) { return s > local; });
+    if (!(g[k] > local)) k = first(g, ng, [&](double s) { return s >= g[ng - 1]; });
+    // inside the group: the masses once more, in the same order
+    const T* x = scores + r * sstride;
+    SmScale scale = { rule.mode, rule.temperature, tops[t], 1.0 };
+    const SmKept kept = st.kept;
+    const long long i0 = t * SM_STILE + k * SM_GROUP;
+    double acc = k ? g[k - 1] : 0.0;
+    long long found = -1, any = -1;
+    for (int e = 0; e < SM_GROUP; e++) {
+        const long long i = i0 + e;
+        const uint32_t key = i < V ? sm_key(x[i], rule.mode == SM_LOGITS) : 0u;
+        const double w = sm_in(kept, key, (uint32_t)i) ? sm_mass(scale, key) : 0.0;
+        acc += w;
+        if (w > 0.0) { any = i; if (found < 0 && acc > local) found = i; }
+    }
+    out[at] = found >= 0 ? found : any;
+}
+
+// ---- long rows, without replacement ----------------------------------------------------------------------------------------------------
+// The n-th largest race key is found from approximate keys in 32 bits: k ~ log2(mass) - log2(-ln(1 - u)).  Two levels of histograms (12 bits
+// each of the ordered float) bound it to a bin; what lies above the bin by more than twice the approximation's error wins, what lies below
+// by as much loses, and the few in the zone between are ranked by their exact 64-bit keys.
+//
+// Error of k: the logarithm instruction is good to a step of its result or 2^-22 (arguments next to one), log2(e) / T and the products round
+// three times, -ln(1 - u) is good to 2^-19 relative (below 2^-6 a series, above it 1 - u is off by 2^-25 of at least 2^-6): together less
+// than 2^-17 + |log2(mass)| 2^-21 + |log2(-ln(1-u))| 2^-21, the last at most 33, and for weights 2^-22 of the slope 1 / T (the logarithm of a
+// weight next to one).  sm_margin allows twice that and more.
+__device__ __forceinline__ float sm_log2(float x)                      // x > 0, subnormals too
+{
+    const bool small = x < 0x1p-100f;
+    return __builtin_amdgcn_logf(small ? x * 0x1p64f : x) - (small ? 64.0f : 0.0f);
+}
+__device__ __forceinline__ float sm_margin(float k, float slope) { return 0x1p-13f + fabsf(k) * 0x1p-18f + slope * 0x1p-21f; }
+__device__ __forceinline__ float sm_slope(const SmRule& r) { return (float)((r.mode == SM_LOGITS ? 1.4426950408889634 : 1.0) / r.temperature); }
+
+__device__ __forceinline__ uint32_t sm_order(float k)
+{
+    const uint32_t b = __float_as_uint(k);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float sm_unorder(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
+
+// ordered approximate key; 0 = excluded.  `slope`: log2(e) / T or 1 / T in 32 bits
+__device__ __forceinline__ uint32_t sm_race32(bool logits, float slope, uint32_t key, float u)
+{
+    if (key == 0u) return 0u;
+    u = u == u ? fminf(fmaxf(u, 0x1p-33f), 1.0f - 0x1p-24f) : 1.0f - 0x1p-24f;
+    const float x = __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+    const float a = (logits ? x : sm_log2(x)) * slope;
+    const float e = u < 0x1p-6f ? u * (1.0f + u * (0.5f + u * (0.33333333f + u * 0.25f))) : -0.69314718f * __builtin_amdgcn_logf(1.0f - u);
+    const float k = fminf(fmaxf(a, -3e38f), 3e38f) - __builtin_amdgcn_logf(e);
+    return sm_order(k + 0.0f);
+}
+
+// bin of the boundary in a histogram of counts (the lowest non-empty one with fewer than `target` before it), what lies before it, and the
+// histogram's total
+__device__ int sm_boundary_counts(const uint32_t* h, int nbins, double target, unsigned long long& before, unsigned long long& total, SmScratch& sc)
+{
+    const int per = (nbins + (int)blockDim.x - 1) / (int)blockDim.x;
+    unsigned long long n = 0;
+    for (int k = 0; k < per; k++) { const int b = nbins - 1 - ((int)threadIdx.x * per + k); if (b >= 0) n += h[b]; }
+    unsigned long long bn = before + sm_block_scan<unsigned long long>(n, sc.a, total);
+    unsigned long long mine = 0, an = 0;
+    for (int k = 0; k < per; k++) {
+        const int b = nbins - 1 - ((int)threadIdx.x * per + k);
+        if (b < 0) break;
+        if (h[b] != 0 && (double)bn < target) { mine = (unsigned long long)(nbins - b); an = bn; }
+        bn += h[b];
+    }
+    const unsigned long long best = sm_block_max(mine, sc.a);
+    if (best == 0) return -1;
+    if (mine == best) sc.word[0] = an;
+    __syncthreads();
+    before = sc.word[0];
+    __syncthreads();
+    return nbins - (int)best;
+}
+
+// approximate keys and their first level
+template <typename T>
+__global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
+                                                          long long V, long long n, SmRule rule, SmWork wk, int step)
+{
+    __shared__ uint32_t h[SM_RBINS];
+    __shared__ SmScratch sc;
+    __shared__ uint32_t ticket;
+    const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
+    SmRowState& st = wk.state[r];
+    const T* x = scores + r * sstride;
+    u += r * ustride;
+    uint32_t* keys = wk.keys + r * wk.vpad;
+    const bool logits = rule.mode == SM_LOGITS, vec = sm_aligned(x), uvec = sm_aligned(u);
+    const float slope = sm_slope(rule);
+    const SmKept kept = sm_final(st, rule);
+    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) h[i] = 0;
+    __syncthreads();
+    for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += wk.B * SM_LTPB * 4) {
+        uint32_t key[4];
+        float uk[4];
+        sm_load4(x, i, V, vec, logits, key);
+        if (uvec && i + 4 <= V) {
+            const LgVec4<float> q = *(const LgVec4<float>*)(u + i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) uk[j] = q.v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) uk[j] = i + j < V ? u[i + j] : 0.5f;
+        }
+        LgVec4<uint32_t> o;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            o.v[j] = sm_race32(logits, slope, sm_in(kept, key[j], (uint32_t)(i + j)) ? key[j] : 0u, uk[j]);
+            if (o.v[j]) atomicAdd(&h[o.v[j] >> 20], 1u);
+        }
+        *(LgVec4<uint32_t>*)(keys + i) = o;                            // (padded to a multiple of four: what lies behind V is key 0)
+    }
+    __syncthreads();
+    uint32_t* g = wk.rbins + r * SM_RBINS;
+    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) if (h[i]) atomicAdd(&g[i], h[i]);
+    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) { h[i] = sm_peek(&g[i]); g[i] = 0; }
+    __syncthreads();
+    unsigned long long before = 0, all;
+    const int bin = sm_boundary_counts(h, SM_RBINS, (double)n, before, all, sc);
+    if (threadIdx.x != 0) return;
+    st.kept = kept;
+    st.candidates = 0;
+    st.take.before_n = before;
+    st.prefix = (unsigned long long)(bin < 0 ? 0 : bin);
+    st.ended = 0;
+    if (all <= (unsigned long long)n) { st.ended = 1; st.zone_lo = st.zone_hi = 0u; }        // whatever is left wins: nothing to rank
+}
+
+// second level, and the zone
+__global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, long long n, SmRule rule, SmWork wk, int step)
+{
+    __shared__ uint32_t h[SM_RBINS];
+    __shared__ SmScratch sc;
+    __shared__ uint32_t ticket;
+    const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
+    SmRowState& st = wk.state[r];
+    if (st.ended) return;
+    const uint32_t* keys = wk.keys + r * wk.vpad;
+    const uint32_t prefix = (uint32_t)st.prefix;
+    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) h[i] = 0;
+    __syncthreads();
+    for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += wk.B * SM_LTPB * 4) {
+        const LgVec4<uint32_t> o = *(const LgVec4<uint32_t>*)(keys + i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) if (o.v[j] && (o.v[j] >> 20) == prefix) atomicAdd(&h[(o.v[j] >> 8) & (SM_RBINS - 1)], 1u);
+    }
+    __syncthreads();
+    uint32_t* g = wk.rbins + r * SM_RBINS;
+    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) if (h[i]) atomicAdd(&g[i], h[i]);
+    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) h[i] = sm_peek(&g[i]);
+    __syncthreads();
+    unsigned long long before = st.take.before_n, all;
+    const int bin = sm_boundary_counts(h, SM_RBINS, (double)n, before, all, sc);
+    if (threadIdx.x != 0) return;
+    const uint32_t lo = (prefix << 20) | ((uint32_t)(bin < 0 ? 0 : bin) << 8), hi = lo | 0xffu;
+    const float klo = sm_unorder(lo), khi = sm_unorder(hi), slope = sm_slope(rule);
+    st.zone_lo = sm_order(klo - 2.0f * sm_margin(klo, slope));                // losers: ordered key < zone_lo
+    st.zone_hi = sm_order(khi + 2.0f * sm_margin(khi, slope));                // winners: > zone_hi
+    if (st.zone_lo == 0u) st.zone_lo = 1u;
+}
+
+// winners as a bit per element, the zone's elements as a list, winners counted per tile; the last workgroup ranks the list
+template <typename T>
+__global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
+                                                          long long V, long long n, SmRule rule, SmWork wk, int step)
+{
+    __shared__ union { SmHist hist; unsigned long long rank[SM_BINS]; } h;
+    __shared__ SmScratch sc;
+    __shared__ uint32_t ticket;
+    const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
+    SmRowState& st = wk.state[r];
+    const uint32_t zlo = st.zone_lo, zhi = st.zone_hi;
+    const uint32_t* keys = wk.keys + r * wk.vpad;
+    unsigned long long* words = wk.words + r * wk.tiles * (SM_TILE / 64);
+    uint32_t* tile_n = wk.tile_n + r * wk.tiles;
+    uint32_t* list = wk.list + r * wk.capacity;
+    const int lane = threadIdx.x & 63;
+    for (long long t = b; t < wk.tiles; t += wk.B) {
+        uint32_t c = 0, total;
+        uint32_t key[SM_TILE / SM_LTPB];
+#pragma unroll
+        for (int k = 0; k < SM_TILE / SM_LTPB; k++) {
+            const long long i = t * SM_TILE + k * SM_LTPB + threadIdx.x;
+            key[k] = i < V ? keys[i] : 0u;
+        }
+#pragma unroll
+        for (int k = 0; k < SM_TILE / SM_LTPB; k++) {
+            const long long i = t * SM_TILE + k * SM_LTPB + threadIdx.x;
+            const unsigned long long w = __ballot(key[k] > zhi);
+            if (lane == 0) { words[i >> 6] = w; c += (uint32_t)__popcll(w); }
+            if (key[k] >= zlo && key[k] <= zhi && key[k] != 0u) {
+                const uint32_t at = atomicAdd(&st.candidates, 1u);
+                if (at < (uint32_t)wk.capacity) __hip_atomic_store(&list[at], (uint32_t)i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
+        }
+        sm_block_scan<uint32_t>(c, sc.a, total);
+        if (threadIdx.x == 0) { __hip_atomic_store(&tile_n[t], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+    }
+    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    unsigned long long mine = 0, sure;
+    for (long long t = threadIdx.x; t < wk.tiles; t += SM_LTPB) mine += sm_peek(&tile_n[t]);
+    sm_block_scan<unsigned long long>(mine, sc.a, sure);
+    const uint32_t found = sm_peek(&st.candidates);
+    const T* x = scores + r * sstride;
+    u += r * ustride;
+    const bool logits = rule.mode == SM_LOGITS;
+    const SmKept kept = st.kept;
+    const SmScale scale = sm_scale(rule, 0u);                          // (race keys need no common scale)
+    auto race = [&](long long i) {
+        const uint32_t k = sm_key(x[i], logits);
+        return sm_race(scale, sm_in(kept, k, (uint32_t)i) ? k : 0u, u[i]);
+    };
+    auto win = [&](uint32_t i) {
+        atomicOr(&words[i >> 6], 1ull << (i & 63));
+        atomicAdd(&tile_n[i / SM_TILE], 1u);
+    };
+    const unsigned long long room = (unsigned long long)n - sure;      // winners still to be named
+    if (found <= (uint32_t)wk.capacity && found <= SM_BINS) {
+        for (uint32_t a = threadIdx.x; a < found; a += SM_LTPB) h.rank[a] = race((long long)sm_peek(&list[a]));
+        __syncthreads();
+        for (uint32_t a = threadIdx.x; a < found; a += SM_LTPB) {
+            const uint32_t i = sm_peek(&list[a]);
+            const unsigned long long k = h.rank[a];
+            unsigned long long ahead = 0;
+            for (uint32_t c = 0; c < found && ahead < room; c++) {
+                const unsigned long long o = h.rank[c];
+                ahead += o > k || (o == k && c != a && sm_peek(&list[c]) < i);
+            }
+            if (ahead < room) win(i);
+        }
+    } else {
+        // many elements next to the border: all but equal keys in numbers.  Radix selection of the exact keys by this workgroup, over the list
+        // or, where that was too short, over the row.
+        const bool all = found > (uint32_t)wk.capacity;
+        const long long m = all ? V : (long long)found;
+        auto index = [&](long long a) { return all ? a : (long long)sm_peek(&list[a]); };
+        auto key_of = [&](long long a) {
+            const long long i = index(a);
+            const uint32_t o = keys[i];
+            return o >= zlo && o <= zhi && o != 0u ? race(i) : 0ull;
+        };
+        SmTake take = { (double)room, 0, { 0, 0 } };
+        unsigned long long prefix = 0, count = 0, thr = 0, ties = 0;
+        bool whole = room == 0;
+        int shift = 64;
+        if (room == 0) thr = ~0ull;
+        while (shift > 0 && !whole) {
+            const int width = shift >= 11 ? 11 : shift, at = shift - width, nbins = 1 << width;
+            __syncthreads();
+            for (int k = threadIdx.x; k < nbins; k += SM_LTPB) h.hist.n[k] = 0;
+            __syncthreads();
+            for (long long a = threadIdx.x; a < m; a += SM_LTPB) {
+                const unsigned long long k = key_of(a);
+                if (k != 0ull && (shift == 64 || (k >> shift) == prefix)) atomicAdd(&h.hist.n[(k >> at) & (unsigned long long)(nbins - 1)], 1u);
+            }
+            __syncthreads();
+            const int bin = sm_boundary<false>(h.hist, nbins, take, sc, count);
+            if (bin < 0) { thr = ~0ull; whole = true; break; }
+            prefix = (prefix << width) | (unsigned)bin;
+            shift = at;
+            thr = prefix << at;
+            whole = sm_whole_bin<false>(take, count);
+        }
+        uint32_t last = SM_ALL;
+        if (!whole) {
+            // the ties-th lowest index among equal keys: the same selection on the (unique) indices, from the top of their complement
+            ties = sm_ties<false>(take, count, 0.0);
+            SmTake by = { (double)ties, 0, { 0, 0 } };
+            unsigned long long p = 0;
+            int s = 32;
+            while (s > 0) {
+                const int width = s >= 11 ? 11 : s, at = s - width, nbins = 1 << width;
+                __syncthreads();
+                for (int k = threadIdx.x; k < nbins; k += SM_LTPB) h.hist.n[k] = 0;
+                __syncthreads();
+                for (long long a = threadIdx.x; a < m; a += SM_LTPB) {
+                    const uint32_t o = ~(uint32_t)index(a);
+                    if ((s == 32 || (o >> s) == (uint32_t)p) && key_of(a) == thr) atomicAdd(&h.hist.n[(o >> at) & (uint32_t)(nbins - 1)], 1u);
+                }
+                __syncthreads();
+                const int bin = sm_boundary<false>(h.hist, nbins, by, sc, count);
+                if (bin < 0) break;                                    // cannot be: ties >= 1 of them exist
+                p = (p << width) | (unsigned)bin;
+                s = at;
+            }
+            last = ~(uint32_t)p;
         }
         __syncthreads();
+        for (long long a = threadIdx.x; a < m; a += SM_LTPB) {
+            const unsigned long long k = key_of(a);
+            const uint32_t i = (uint32_t)index(a);
+            if (k != 0ull && (k > thr || (k == thr && i <= last))) win(i);
+        }
     }
+    __threadfence();
+    __syncthreads();
+    // tiles' first positions in the output
+    unsigned long long run = 0;
+    for (long long base = 0; base < wk.tiles; base += SM_LTPB) {
+        const long long t = base + threadIdx.x;
+        const uint32_t c = t < wk.tiles ? sm_peek(&tile_n[t]) : 0u;
+        unsigned long long total;
+        const unsigned long long before = sm_block_scan<unsigned long long>(c, sc.a, total);
+        if (t < wk.tiles) tile_n[t] = (uint32_t)(run + before);
+        run += total;
+    }
+    if (threadIdx.x == 0) st.sure = run;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SM_TPB) sample_distinct_row_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u,
-                                                                     long long ustride, long long V, long long n, SmRule rule, long long* __restrict__ out)
+// winners' indices, ascending; one workgroup of two waves per tile, one word of winners per thread
+__global__ void __launch_bounds__(SM_TILE / 64) sm_emit_kernel(long long n, SmWork wk, long long* __restrict__ out)
 {
-    __shared__ SmHist h;
     __shared__ SmScratch sc;
-    const long long r = blockIdx.x;
-    SmRow<T> row = { scores + r * sstride, V, rule.mode == SM_LOGITS, {} };
-    const SmKept kept = sm_filter_row(row, rule, h, sc);
+    const long long r = blockIdx.x / wk.tiles, t = blockIdx.x % wk.tiles;
     out += r * n;
-    u += r * ustride;
-    auto race = [&](long long i) {
-        const uint32_t k = row.key(i);
-        return row.in(kept, k, i) ? sm_race(row.scale, k, u[i]) : 0ull;
-    };
-    unsigned long long thr, ties, equal;
-    const SmTake take = { false, (double)n, 0, { 0, 0 } };
-    sm_select<64>(V, race, [](unsigned long long) { return 0.0; }, take, h, sc, thr, ties, equal);
-    // winners in index order; of the last key's ties the first ones
-    unsigned long long done = 0, tied = 0;
-    for (long long base = 0; base < V && done < (unsigned long long)n; base += SM_TPB) {
-        const long long i = base + threadIdx.x;
-        const unsigned long long k = i < V ? race(i) : 0ull;
-        bool win = k > thr;
-        uint32_t total;
-        if (ties < equal) {
-            const uint32_t before = sm_block_scan<uint32_t>(k != 0 && k == thr ? 1u : 0u, sc.u32, total);
-            win = win || (k != 0 && k == thr && tied + before < ties);
-            tied += total;
-        } else win = win || (k != 0 && k == thr);
-        const uint32_t before = sm_block_scan<uint32_t>(win ? 1u : 0u, sc.u32, total);
-        if (win) out[done + before] = i;
-        done += total;
+    unsigned long long w = wk.words[(r * wk.tiles + t) * (SM_TILE / 64) + threadIdx.x];
+    uint32_t total;
+    long long at = (long long)wk.tile_n[r * wk.tiles + t] + sm_block_scan<uint32_t>((uint32_t)__popcll(w), sc.a, total);
+    const long long i0 = t * SM_TILE + (long long)threadIdx.x * 64;
+    while (w) {
+        const int k = __ffsll((long long)w) - 1;
+        w &= w - 1;
+        if (at < n) out[at] = i0 + k;
+        at++;
     }
-    for (long long j = (long long)done + threadIdx.x; j < n; j += SM_TPB) out[j] = -1;
+    // the row's end where fewer than n were left
+    const long long m = (long long)wk.state[r].sure;
+    for (long long j = m + t * (SM_TILE / 64) + threadIdx.x; j < n; j += wk.tiles * (SM_TILE / 64)) out[j] = -1;
 }
 
-// ---- entry points --------------------------------------------------------------------------------------------------------------------
+// ---- entry points ----------------------------------------------------------------------------------------------------------------------
 static bool sm_rule(int logits, double temperature, long long top_k, double top_p, double min_p, SmRule& r)
 {
-    if (!(temperature > 0.0) || !(temperature <= 1e30) || top_k < 0 || !(top_p > 0.0 && top_p <= 1.0) || !(min_p >= 0.0 && min_p <= 1.0)) return false;
+    if (!(temperature >= 1e-30 && temperature <= 1e30) || top_k < 0 || !(top_p > 0.0 && top_p <= 1.0) || !(min_p >= 0.0 && min_p <= 1.0)) return false;
     r = SmRule{ logits ? SM_LOGITS : temperature == 1.0 ? SM_LINEAR : SM_POWER, temperature, top_p, min_p, top_k };
     return true;
 }
 
-template <typename T>
-static int sample_launch(const T* scores, long long sstride, const float* u, long long ustride, long long R, long long V, long long n,
-                         const SmRule& rule, long long* out, bool distinct, hipStream_t s)
+#define SM_SHORT 16384                 // longest row of the one-workgroup kernels
+
+// lays the workspace out; returns its size in bytes.  The cleared part (states, histograms) comes first.
+static long long sm_layout(long long R, long long V, bool distinct, char* base, SmWork& w, long long& clear_bytes)
 {
-    if (distinct)
-        hipLaunchKernelGGL((sample_distinct_row_kernel<T>), dim3((unsigned)R), dim3(SM_TPB), 0, s, scores, sstride, u, ustride, V, n, rule, out);
-    else
-        hipLaunchKernelGGL((sample_row_kernel<T>), dim3((unsigned)R), dim3(SM_TPB), 0, s, scores, sstride, u, ustride, V, n, rule, out);
+    char* p = base;
+    auto take = [&](long long bytes) { char* at = p; p += (bytes + 255) & ~255ll; return at; };
+    w.state = (SmRowState*)take(R * (long long)sizeof(SmRowState));
+    w.hist = (SmHist*)take(R * (long long)sizeof(SmHist));
+    w.rbins = distinct ? (uint32_t*)take(R * SM_RBINS * 4) : nullptr;
+    clear_bytes = p - base;
+    w.tiles = (V + SM_TILE - 1) / SM_TILE;
+    w.stiles = (V + SM_STILE - 1) / SM_STILE;
+    w.vpad = (V + 3) & ~3ll;
+    w.capacity = V / 256 > 4096 ? V / 256 : 4096;
+    const long long want = (V + SM_LTPB * 8 - 1) / (SM_LTPB * 8), most = R >= 1024 ? 1 : 1024 / R;
+    w.B = want < most ? want : most;
+    w.tile_n = (uint32_t*)take(R * w.tiles * 4);
+    w.keys = nullptr; w.words = nullptr; w.list = nullptr; w.group = w.tile_sum = w.tile_top = nullptr;
+    if (distinct) {
+        w.keys = (uint32_t*)take(R * w.vpad * 4);
+        w.words = (unsigned long long*)take(R * w.tiles * (SM_TILE / 64) * 8);
+        w.list = (uint32_t*)take(R * w.capacity * 4);
+    } else {
+        w.group = (double*)take(R * w.stiles * (SM_STILE / SM_GROUP) * 8);
+        w.tile_sum = (double*)take(R * (w.stiles + 1) * 8);
+        w.tile_top = (double*)take(R * w.stiles * 8);
+    }
+    return p - base;
+}
+
+template <typename T>
+static int sample_launch(const T* scores, long long ss, const float* u, long long us, long long R, long long V, long long n,
+                         const SmRule& rule, long long* out, bool distinct, void* temp, long long temp_bytes, hipStream_t s)
+{
+    if (V <= SM_SHORT) {
+        const dim3 grid((unsigned)R);
+#define SM_LAUNCH_SHORT(TPB_, EPT_)                                                                                                                    \
+        do {                                                                                                                                           \
+            if (distinct) hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, true>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, out);  \
+            else hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, false>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, out);     \
+        } while (0)
+        if (V <= 1024) SM_LAUNCH_SHORT(256, 4);
+        else if (V <= 4096) SM_LAUNCH_SHORT(1024, 4);
+        else SM_LAUNCH_SHORT(1024, 16);
+#undef SM_LAUNCH_SHORT
+        LG_RETURN_LAST();
+    }
+    SmWork wk;
+    long long clear_bytes;
+    const long long need = sm_layout(R, V, distinct, (char*)temp, wk, clear_bytes);
+    if (temp == nullptr || temp_bytes < need || (uintptr_t)temp % 16 != 0 || R * wk.B > 0x7fffffffll || R * wk.tiles > 0x7fffffffll) return (int)hipErrorInvalidValue;
+    const dim3 grid((unsigned)(R * wk.B)), block(SM_LTPB);
+    const long long words = clear_bytes / 16, cblocks = (words + 255) / 256;
+    hipLaunchKernelGGL(sm_clear_kernel, dim3((unsigned)(cblocks < 2048 ? cblocks : 2048)), dim3(256), 0, s, (uint4*)temp, words);
+    int step = 0;
+    const bool top_k = rule.top_k > 0 && rule.top_k < V, top_p = rule.top_p < 1.0;
+    if (top_p || rule.min_p > 0.0) hipLaunchKernelGGL((sm_best_kernel<T>), grid, block, 0, s, scores, ss, V, rule, wk, step++);
+    for (int pass = 0; pass < 2; pass++) {
+        if (!(pass == 0 ? top_k : top_p)) continue;
+        for (int shift = 32; shift > (sizeof(T) == 2 ? 10 : 0); ) {
+            const int width = shift >= 11 ? 11 : shift;
+            if (pass == 0) hipLaunchKernelGGL((sm_level_kernel<T, false>), grid, block, 0, s, scores, ss, V, rule, wk, step++, shift, width);
+            else hipLaunchKernelGGL((sm_level_kernel<T, true>), grid, block, 0, s, scores, ss, V, rule, wk, step++, shift, width);
+            shift -= width;
+        }
+        hipLaunchKernelGGL((sm_tie_kernel<T>), grid, block, 0, s, scores, ss, V, rule, wk, step++);
+    }
+    if (!distinct) {
+        SmWork sw = wk;
+        sw.B = wk.stiles < 2 * wk.B ? wk.stiles : 2 * wk.B;
+        hipLaunchKernelGGL((sm_sums_kernel<T>), dim3((unsigned)(R * sw.B)), dim3(256), 0, s, scores, ss, V, rule, sw, step++);
+        const long long blocks = (R * n + 255) / 256;
+        if (blocks > 0x7fffffffll) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL((sm_draw_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, scores, ss, u, us, R, V, n, rule, sw, out);
+        LG_RETURN_LAST();
+    }
+    hipLaunchKernelGGL((sm_race_kernel<T>), grid, block, 0, s, scores, ss, u, us, V, n, rule, wk, step++);
+    hipLaunchKernelGGL(sm_race_level_kernel, grid, block, 0, s, V, n, rule, wk, step++);
+    SmWork zw = wk;
+    zw.B = wk.tiles < wk.B ? wk.tiles : wk.B;
+    hipLaunchKernelGGL((sm_zone_kernel<T>), dim3((unsigned)(R * zw.B)), block, 0, s, scores, ss, u, us, V, n, rule, zw, step++);
+    hipLaunchKernelGGL(sm_emit_kernel, dim3((unsigned)(R * wk.tiles)), dim3(SM_TILE / 64), 0, s, n, wk, out);
     LG_RETURN_LAST();
 }
 
-LG_API long long lg_sample_temp_bytes(long long R, long long V, long long n, int distinct, int filtered) { return 0; }
+LG_API long long lg_sample_temp_bytes(long long R, long long V, long long n, int distinct)
+{
+    if (R <= 0 || n <= 0 || V <= SM_SHORT || V >= (1ll << 31)) return 0;
+    SmWork w;
+    long long clear_bytes;
+    return sm_layout(R, V, distinct != 0, nullptr, w, clear_bytes);
+}
 
 LG_API int lg_sample(const void* scores, int dtype, long long score_stride, const float* u, long long u_stride, long long R, long long V,
                      long long n, int distinct, int logits, double temperature, long long top_k, double top_p, double min_p,
@@ -452,9 +1165,9 @@ LG_API int lg_sample(const void* scores, int dtype, long long score_stride, cons
     if (distinct && n > V) return (int)hipErrorInvalidValue;
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
-    case LG_F32: return sample_launch((const float*)scores, score_stride, u, u_stride, R, V, n, rule, (long long*)out, distinct != 0, s);
-    case LG_F16: return sample_launch((const LgHalf*)scores, score_stride, u, u_stride, R, V, n, rule, (long long*)out, distinct != 0, s);
-    case LG_BF16: return sample_launch((const LgBf16*)scores, score_stride, u, u_stride, R, V, n, rule, (long long*)out, distinct != 0, s);
+    case LG_F32: return sample_launch((const float*)scores, score_stride, u, u_stride, R, V, n, rule, (long long*)out, distinct != 0, temp, temp_bytes, s);
+    case LG_F16: return sample_launch((const LgHalf*)scores, score_stride, u, u_stride, R, V, n, rule, (long long*)out, distinct != 0, temp, temp_bytes, s);
+    case LG_BF16: return sample_launch((const LgBf16*)scores, score_stride, u, u_stride, R, V, n, rule, (long long*)out, distinct != 0, temp, temp_bytes, s);
     }
     return (int)hipErrorInvalidValue;
 }

@@ -143,7 +143,7 @@ def _sample(what: str, scores, u, n: int, distinct: bool, temperature, top_k, to
     V = scores.shape[-1]
     if V >= 1 << 31:
         raise ValueError(f"{what}: at most 2^31 - 1 categories")
-    temperature = _real(temperature, f"{what}: temperature", lambda v: 0.0 < v <= 1e30)
+    temperature = _real(temperature, f"{what}: temperature", lambda v: 1e-30 <= v <= 1e30)
     top_k = _integer(top_k, f"{what}: top_k", 0, 1 << 62)
     top_p = _real(top_p, f"{what}: top_p", lambda v: 0.0 < v <= 1.0)
     min_p = _real(min_p, f"{what}: min_p", lambda v: 0.0 <= v <= 1.0)
@@ -151,7 +151,7 @@ def _sample(what: str, scores, u, n: int, distinct: bool, temperature, top_k, to
     R = x.shape[0]
     out = torch.empty((*scores.shape[:-1], n), dtype=torch.int64, device=x.device)
     L = lib()
-    tb = L.lg_sample_temp_bytes(R, V, n, int(distinct), int(top_k > 0 or top_p < 1.0))
+    tb = L.lg_sample_temp_bytes(R, V, n, int(distinct))
     temp = torch.empty((max(tb, 1),), dtype=torch.uint8, device=x.device)
     with _on(x.device):
         check(L.lg_sample(x.data_ptr(), _DTYPES[x.dtype], x.stride(0), uu.data_ptr(), uu.stride(0), R, V, n, int(distinct), int(bool(logits)),

@@ -235,8 +235,9 @@ __device__ __forceinline__ void sm_min_p(const SmScale& s, uint32_t best, double
     if (lo > kept.thr) kept = SmKept{ lo, SM_ALL };
 }
 
-// Unrolled 64-bit exponentials and logarithms are kept apart: interleaved by the scheduler, sixteen of them spill two thousand registers.
-#define SM_ONE_AT_A_TIME() __builtin_amdgcn_sched_barrier(0)
+// Unrolled 64-bit exponentials and logarithms stay out of line: sixteen of them inlined, with their constants, spill two thousand registers.
+__device__ __attribute__((noinline)) double sm_mass_call(SmScale s, uint32_t key) { return sm_mass(s, key); }
+__device__ __attribute__((noinline)) unsigned long long sm_race_call(SmScale s, uint32_t key, float u) { return sm_race(s, key, u); }
 
 // ---- short rows: one workgroup per row, EPT consecutive elements of a thread in registers ----------------------------------------------
 // Narrows `kept` (or, for 64-bit race keys, finds thr / ties): each[k] is the key of element threadIdx.x * EPT + k, 0: not a candidate.
@@ -259,7 +260,6 @@ __device__ void sm_select_short(const Word (&key)[EPT], const Mass& mass_of, SmT
             const int b = (int)(key[k] >> at) & (nbins - 1);
             atomicAdd(&h.n[b], 1u);
             if (MASS) {
-                SM_ONE_AT_A_TIME();
                 const SmSum m = sm_limbs(mass_of(key[k]));
                 if (m.hi) atomicAdd(&h.hi[b], m.hi);
                 if (m.lo) atomicAdd(&h.lo[b], m.lo);
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     }
     const SmScale scale = sm_scale(rule, best);
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
-    auto mass_of = [&](uint32_t k) { return sm_mass(scale, k) * unit; };
+    auto mass_of = [&](uint32_t k) { return sm_mass_call(scale, k) * unit; };
     // filters: an element that one of them drops becomes key 0
     for (int pass = 0; pass < 2; pass++) {
         SmTake take = { 0.0, 0, { 0, 0 } };
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             SmSum mine = { 0, 0 }, total;
 #pragma unroll
             for (int k = 0; k < EPT; k++)
-                if (key[k]) { SM_ONE_AT_A_TIME(); const SmSum m = sm_limbs(mass_of(key[k])); mine.hi += m.hi; mine.lo += m.lo; }
+                if (key[k]) { const SmSum m = sm_limbs(mass_of(key[k])); mine.hi += m.hi; mine.lo += m.lo; }
             sm_block_scan<unsigned long long>(mine.hi, sc.a, total.hi);
             sm_block_scan<unsigned long long>(mine.lo, sc.b, total.lo);
             take.target = rule.top_p * sm_sum_value(total);
@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     if (DISTINCT) {
         unsigned long long race[EPT], thr, ties, equal;
 #pragma unroll
-        for (int k = 0; k < EPT; k++) { race[k] = sm_race(scale, key[k], uk[k]); SM_ONE_AT_A_TIME(); }
+        for (int k = 0; k < EPT; k++) { race[k] = sm_race_call(scale, key[k], uk[k]); }
         const SmTake take = { (double)n, 0, { 0, 0 } };
         sm_select_short<false, 64, EPT, unsigned long long>(race, [](unsigned long long) { return 0.0; }, take, h.hist, sc, thr, ties, equal);
         uint32_t last = SM_ALL, c = 0, total;
@@ -402,10 +402,9 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         uint32_t positive = 0, last = 0;
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
-            w[k] = sm_mass(scale, key[k]);
+            w[k] = sm_mass_call(scale, key[k]);
             sum += w[k];
             if (w[k] > 0.0) { positive |= 1u << k; last = (uint32_t)(i0 + k) + 1; }
-            SM_ONE_AT_A_TIME();
         }
         double at = sm_block_scan<double>(sum, sc.a, total);
         last = (uint32_t)sm_block_max(last, sc.b);
@@ -427,7 +426,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
 // ---- long rows: B workgroups per row ---------------------------------------------------------------------------------------------------
 // Every step is one launch over (row, workgroup); the last workgroup of a row to finish a step (SmRowState::ticket) draws its conclusion and
 // leaves it in the row's state for the next launch.
-#define SM_LTPB 512
+#define SM_LTPB 1024
 #define SM_RBINS 4096                  // bins of a level of the race's approximate keys
 #define SM_TILE 8192                   // elements per workgroup step of the race's last pass: 128 words of winners
 #define SM_STILE 4096                  // elements per tile of prefix sums
@@ -451,17 +450,20 @@ struct SmWork {                        // workspace of a call: everything per ro
     long long B, tiles, stiles, capacity, vpad;
 };
 
+// The last workgroup of a row to get here.  What it reads of the others' work was written by device-wide atomics (adds, or sm_poke's stores, which
+// go through the XCD's own L2) and is read by sm_peek: each wave waits for its own to be done before the ticket is drawn, and no L2 has to be
+// written back (a release fence in every wave of every workgroup took longer than the pass over the data).
 __device__ __forceinline__ bool sm_last_block(uint32_t* ticket, uint32_t blocks, uint32_t* lds)
 {
-    __threadfence();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) *lds = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) *lds = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    const bool last = *lds == blocks - 1;
-    if (last) __threadfence();
-    return last;
+    return *lds == blocks - 1;
 }
 template <typename V> __device__ __forceinline__ V sm_peek(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+template <typename V> __device__ __forceinline__ void sm_poke(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 __global__ void __launch_bounds__(256) sm_clear_kernel(uint4* p, long long n)
 {
@@ -588,7 +590,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_tie_kernel(const T* __restrict__ s
         uint32_t c = 0, total;
         for (int k = 0; k < SM_TILE / SM_LTPB; k++) c += tie(t * SM_TILE + k * SM_LTPB + threadIdx.x);
         sm_block_scan<uint32_t>(c, sc.a, total);
-        if (threadIdx.x == 0) __hip_atomic_store(&tile_n[t], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (threadIdx.x == 0) sm_poke(&tile_n[t], total);
     }
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
     const unsigned long long want = st.ties;
@@ -659,8 +661,8 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
         const double before = sm_block_scan<double>(sum, sc.a, total);
         groups[t * (SM_STILE / SM_GROUP) + threadIdx.x] = sm_block_rise(sum > 0.0 ? before + sum : 0.0, sc.b);
         if (threadIdx.x == 0) {
-            __hip_atomic_store(&sums[t], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(&tops[t], best ? scale.top : -INFINITY, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            sm_poke(&sums[t], total);
+            sm_poke(&tops[t], best ? scale.top : -INFINITY);
         }
     }
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
@@ -910,14 +912,14 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
         for (int k = 0; k < SM_TILE / SM_LTPB; k++) {
             const long long i = t * SM_TILE + k * SM_LTPB + threadIdx.x;
             const unsigned long long w = __ballot(key[k] > zhi);
-            if (lane == 0) { words[i >> 6] = w; c += (uint32_t)__popcll(w); }
+            if (lane == 0) { sm_poke(&words[i >> 6], w); c += (uint32_t)__popcll(w); }
             if (key[k] >= zlo && key[k] <= zhi && key[k] != 0u) {
                 const uint32_t at = atomicAdd(&st.candidates, 1u);
-                if (at < (uint32_t)wk.capacity) __hip_atomic_store(&list[at], (uint32_t)i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (at < (uint32_t)wk.capacity) sm_poke(&list[at], (uint32_t)i);
             }
         }
         sm_block_scan<uint32_t>(c, sc.a, total);
-        if (threadIdx.x == 0) { __hip_atomic_store(&tile_n[t], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+        if (threadIdx.x == 0) { sm_poke(&tile_n[t], total); }
     }
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
     unsigned long long mine = 0, sure;
@@ -1074,7 +1076,7 @@ static long long sm_layout(long long R, long long V, bool distinct, char* base, 
     w.stiles = (V + SM_STILE - 1) / SM_STILE;
     w.vpad = (V + 3) & ~3ll;
     w.capacity = V / 256 > 4096 ? V / 256 : 4096;
-    const long long want = (V + SM_LTPB * 8 - 1) / (SM_LTPB * 8), most = R >= 1024 ? 1 : 1024 / R;
+    const long long want = (V + SM_LTPB * 8 - 1) / (SM_LTPB * 8), most = R >= 256 ? 1 : 256 / R;
     w.B = want < most ? want : most;
     w.tile_n = (uint32_t*)take(R * w.tiles * 4);
     w.keys = nullptr; w.words = nullptr; w.list = nullptr; w.group = w.tile_sum = w.tile_top = nullptr;

@@ -15,19 +15,20 @@ import types
 from . import fused as _py
 
 
-def _load_compiled():
+def load_compiled(name: str = "_litegs_fused_C"):
+    """the compiled module of that name next to this file, or None (not built, or ``LITEGS_FUSED_BINDING=ctypes``)"""
     if os.environ.get("LITEGS_FUSED_BINDING", "ext") == "ctypes":
         return None
-    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_litegs_fused_C.so")
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), name + ".so")
     if not os.path.exists(path):
         return None
     import torch  # noqa: F401  (the extension links against libtorch)
     from ._lib import lib
     lib()                                  # liblitegs_hip.so first: the extension resolves its lg_* symbols from it
-    return importlib.import_module("litegs_amd._litegs_fused_C")
+    return importlib.import_module("litegs_amd." + name)
 
 
-compiled = _load_compiled()
+compiled = load_compiled()
 
 
 def _make_ops():

@@ -45,6 +45,8 @@ def _hipcc() -> str:
 ABI_HEADER = os.path.join(os.path.dirname(HERE), "include", "litegs_hip.h")
 EXT_SRC = os.path.join(CSRC, "ext", "litegs_fused_ext.cpp")
 EXT_LIB = os.path.join(HERE, "_litegs_fused_C.so")
+STOCHASTIC_SRC = os.path.join(CSRC, "ext", "stochastic_ext.cpp")
+STOCHASTIC_LIB = os.path.join(HERE, "_stochastic_C.so")
 
 
 def _newer(src: str, dst: str) -> bool:
@@ -57,20 +59,20 @@ def _newer(src: str, dst: str) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build_extension(force: bool = False, verbose: bool = False) -> str:
+def build_extension(force: bool = False, verbose: bool = False, src: str = EXT_SRC, out: str = EXT_LIB) -> str:
     """``litegs_fused`` as a compiled torch extension (csrc/ext/litegs_fused_ext.cpp): host-only C++ over the C ABI, built with g++
     against the torch headers and linked to liblitegs_hip.so next to it (rpath $ORIGIN).  The reference builds the module of the same
-    name with GR/setup.py."""
-    if not (force or _newer(EXT_SRC, EXT_LIB) or os.path.getmtime(LIB) > os.path.getmtime(EXT_LIB)):
-        return EXT_LIB
+    name with GR/setup.py.  csrc/ext/stochastic_ext.cpp is built the same way."""
+    if not (force or _newer(src, out) or os.path.getmtime(LIB) > os.path.getmtime(out)):
+        return out
     import sysconfig
     import torch
     from torch.utils import cpp_extension as ce
     inc = ce.include_paths("cuda") + [sysconfig.get_paths()["include"], "/opt/rocm/include", os.path.join(os.path.dirname(HERE), "include")]
     libdirs = ce.library_paths("cuda")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_litegs_fused_C",
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=" + os.path.splitext(os.path.basename(out))[0],
            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-Wno-deprecated-declarations",
-           EXT_SRC, "-o", EXT_LIB]
+           src, "-o", out]
     for p in inc:
         cmd += ["-I", p]
     for p in libdirs:
@@ -81,8 +83,8 @@ def build_extension(force: bool = False, verbose: bool = False) -> str:
     p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
     if p.returncode != 0:
         sys.stderr.write(p.stdout.decode())
-        raise RuntimeError("g++ failed on the litegs_fused extension")
-    return EXT_LIB
+        raise RuntimeError(f"g++ failed on the {os.path.basename(out)} extension")
+    return out
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -116,12 +118,16 @@ def build(force: bool = False, verbose: bool = False) -> str:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
     try:
-        build_extension(force=force, verbose=verbose)
+        from concurrent.futures import ThreadPoolExecutor
+        with ThreadPoolExecutor(2) as pool:
+            jobs = [pool.submit(build_extension, force, verbose, src, out) for src, out in ((EXT_SRC, EXT_LIB), (STOCHASTIC_SRC, STOCHASTIC_LIB))]
+            for job in jobs:
+                job.result()
     except (RuntimeError, OSError, ImportError) as e:
         # no g++ / no torch headers: the C-ABI library above is complete, and litegs_amd/fused.py binds the same 26 names through
-        # ctypes (litegs_amd/binding.py picks whichever is there)
+        # ctypes (litegs_amd/binding.py picks whichever is there); litegs_amd/stochastic.py likewise
         import warnings
-        warnings.warn(f"litegs_amd.build: the compiled litegs_fused extension was not built ({e}); using the ctypes binding")
+        warnings.warn(f"litegs_amd.build: the compiled torch extensions were not built ({e}); using the ctypes binding")
     return LIB
 
 

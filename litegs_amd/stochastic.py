@@ -19,7 +19,9 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._lib import check, lib
+from .binding import load_compiled
 
+_C = load_compiled("_stochastic_C")          # None: the same calls through ctypes (litegs_amd/binding.py)
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 Offset = Union[int, torch.Tensor]
 
@@ -39,13 +41,13 @@ def _float_tensor(t, what: str) -> None:
 
 
 def _integer(v, what: str, lo: int, hi: int) -> int:
-    if isinstance(v, bool) or not isinstance(v, numbers.Integral) or not lo <= int(v) < hi:
+    if (type(v) is not int and (isinstance(v, bool) or not isinstance(v, numbers.Integral))) or not lo <= int(v) < hi:
         raise ValueError(f"{what} must be an integer in [{lo}, {hi}), got {v!r}")
     return int(v)
 
 
 def _real(v, what: str, ok) -> float:
-    if isinstance(v, bool) or not isinstance(v, numbers.Real) or not ok(float(v)):
+    if (type(v) is not float and (isinstance(v, bool) or not isinstance(v, numbers.Real))) or not ok(float(v)):
         raise ValueError(f"{what}: {v!r} is out of range")
     return float(v)
 
@@ -101,12 +103,20 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Offset = 0, shared: in
         if shared not in (0, x.dim() - 2):
             raise ValueError("dropout: chunk_ids share the mask over all leading dimensions")
         shared, S, chunk_ids = x.dim() - 2, x.shape[-1], chunk_ids.contiguous()
-    lead = math.prod(x.shape[:shared])
     M = math.prod(x.shape[shared:])
-    return _Dropout.apply(x, lead, M, p, *key, chunk_ids, S)
+    lead = math.prod(x.shape[:shared])
+    return (_Dropout.apply if _C is None else _C.dropout)(x, lead, M, p, *key, chunk_ids, S)
 
 
-@torch.no_grad()
+def _draw(std, out, seed, offset, offset_dev, what: str) -> None:
+    if _C is not None:
+        _C.random_draw(std, out, seed, offset, offset_dev)
+        return
+    with _on(out.device):
+        check(lib().lg_random_draw(None if std is None else std.data_ptr(), out.data_ptr(), _DTYPES[out.dtype], out.numel(), seed, offset,
+                                   None if offset_dev is None else offset_dev.data_ptr(), _s()), what)
+
+
 def uniform(shape, seed: int, offset: Offset = 0, dtype: torch.dtype = torch.float32, device: Optional[torch.device] = None) -> torch.Tensor:
     """``(word(i) + 1/2) / 2^32`` rounded to ``dtype`` and kept below one: in (0, 1) in float32 (in half width the smallest round to 0)"""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
@@ -114,22 +124,17 @@ def uniform(shape, seed: int, offset: Offset = 0, dtype: torch.dtype = torch.flo
         raise RuntimeError("uniform: float32, float16 or bfloat16 on a GPU (no CPU path)")
     out = torch.empty(shape, dtype=dtype, device=device)
     seed, offset, offset_dev = _key(seed, offset, out.device, "uniform")
-    with _on(out.device):
-        check(lib().lg_random_draw(None, out.data_ptr(), _DTYPES[dtype], out.numel(), seed, offset,
-                                   None if offset_dev is None else offset_dev.data_ptr(), _s()), "uniform")
+    _draw(None, out, seed, offset, offset_dev, "uniform")
     return out
 
 
-@torch.no_grad()
 def normal(std: torch.Tensor, seed: int, offset: Offset = 0) -> torch.Tensor:
     """``std * N(0,1)``, element for element (Box-Muller: the words 2j and 2j + 1 give the elements 2j and 2j + 1); not differentiable"""
     _float_tensor(std, "normal")
     seed, offset, offset_dev = _key(seed, offset, std.device, "normal")
-    std = std.contiguous()
+    std = std.detach().contiguous()
     out = torch.empty_like(std)
-    with _on(std.device):
-        check(lib().lg_random_draw(std.data_ptr(), out.data_ptr(), _DTYPES[std.dtype], out.numel(), seed, offset,
-                                   None if offset_dev is None else offset_dev.data_ptr(), _s()), "normal")
+    _draw(std, out, seed, offset, offset_dev, "normal")
     return out
 
 
@@ -147,9 +152,12 @@ def _sample(what: str, scores, u, n: int, distinct: bool, temperature, top_k, to
     top_k = _integer(top_k, f"{what}: top_k", 0, 1 << 62)
     top_p = _real(top_p, f"{what}: top_p", lambda v: 0.0 < v <= 1.0)
     min_p = _real(min_p, f"{what}: min_p", lambda v: 0.0 <= v <= 1.0)
-    x, uu = _rows(scores.detach()), _rows(u)
+    x, uu = _rows(scores.detach()), _rows(u.detach())
     R = x.shape[0]
     out = torch.empty((*scores.shape[:-1], n), dtype=torch.int64, device=x.device)
+    if _C is not None:
+        _C.sample(x, uu, out, n, distinct, bool(logits), temperature, top_k, top_p, min_p)
+        return out
     L = lib()
     tb = L.lg_sample_temp_bytes(R, V, n, int(distinct))
     temp = torch.empty((max(tb, 1),), dtype=torch.uint8, device=x.device)
@@ -167,7 +175,6 @@ def _check_scores(scores, u, what: str) -> None:
         raise ValueError(f"{what}: scores [..., V] and u [..., K] must have the same leading dimensions")
 
 
-@torch.no_grad()
 def sample(scores: torch.Tensor, u: torch.Tensor, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
            logits: bool = True) -> torch.Tensor:
     """Categories drawn with replacement: ``scores`` [..., V], ``u`` [..., n] float32 in [0, 1) -> int64 [..., n].
@@ -181,7 +188,6 @@ def sample(scores: torch.Tensor, u: torch.Tensor, *, temperature: float = 1.0, t
     return _sample("sample", scores, u, u.shape[-1], False, temperature, top_k, top_p, min_p, logits)
 
 
-@torch.no_grad()
 def sample_distinct(scores: torch.Tensor, u: torch.Tensor, n: int, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
                     min_p: float = 0.0, logits: bool = True) -> torch.Tensor:
     """``n`` different categories drawn one after the other without replacement, in ascending order: ``scores`` and ``u`` [..., V] -> int64 [..., n].

@@ -358,3 +358,25 @@ def test_sampling_refusals():
     for a, b in ((x.double(), u), (x, u.double()), (x.cpu(), u.cpu()), (x, u.cpu()), (x.long(), u)):
         with pytest.raises(RuntimeError):
             stochastic.sample(a, b)
+
+
+# ---- the two bindings ----------------------------------------------------------------------------------------------------------------
+def test_compiled_and_ctypes_bindings_agree(monkeypatch):
+    assert stochastic._C is not None, "the compiled binding is built by litegs_amd.build"
+    x = torch.randn((3, 5, 128), device=DEV, requires_grad=True)
+    dy, ids, step = torch.randn_like(x), torch.tensor([9, 4, 2, 8, 70], device=DEV), torch.tensor([6], device=DEV)
+    z, u = scores_of("normal", 2, 40000, torch.float16, True), draws_of((2, 40000))
+
+    def everything():
+        out = []
+        for kw in (dict(), dict(shared=1), dict(chunk_ids=ids), dict(offset=step)):
+            y = stochastic.dropout(x, 0.4, 2 ** 64 - 1, **kw)
+            out += [y, torch.autograd.grad(y, x, dy)[0]]
+        out += [stochastic.uniform((7, 3), 5, 6), stochastic.normal(x, 5, step), stochastic.normal(x.detach(), 5, 6)]
+        out += [stochastic.sample(z, u[:, :9], top_p=0.9), stochastic.sample_distinct(z, u, 77, top_k=500), stochastic.sample(z[:, :50], u[:, :3])]
+        return out
+
+    compiled = everything()
+    monkeypatch.setattr(stochastic, "_C", None)
+    for a, b in zip(compiled, everything()):
+        assert torch.equal(a, b) and a.requires_grad == b.requires_grad

@@ -43,22 +43,22 @@ __device__ __forceinline__ double sm_value(uint32_t key)
     return (double)__uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 
-struct SmScale { int mode; double temperature, top /*l of the best score, or its weight*/, shift /*power of two that brings a linear weight below one*/; };
+struct SmScale { int mode; double inv_t, top /*l of the best score, or its weight*/, shift /*power of two that brings a linear weight below one*/; };
 
 __device__ __forceinline__ SmScale sm_scale(const SmRule& r, uint32_t best)
 {
-    SmScale s = { r.mode, r.temperature, 0.0, 1.0 };
+    SmScale s = { r.mode, 1.0 / r.temperature, 0.0, 1.0 };
     if (best == 0u) return s;
     const double x = sm_value(best);
-    if (r.mode == SM_LOGITS) s.top = x / r.temperature;
-    else if (r.mode == SM_POWER) s.top = log(x) / r.temperature;
+    if (r.mode == SM_LOGITS) s.top = x * s.inv_t;
+    else if (r.mode == SM_POWER) s.top = log(x) * s.inv_t;
     else { s.top = x; s.shift = ldexp(1.0, -ilogb(x) - 1); }
     return s;
 }
 __device__ __forceinline__ double sm_log(const SmScale& s, uint32_t key)
 {
     const double x = sm_value(key);
-    return s.mode == SM_LOGITS ? x / s.temperature : s.mode == SM_POWER ? log(x) / s.temperature : log(x);
+    return s.mode == SM_LOGITS ? x * s.inv_t : s.mode == SM_POWER ? log(x) * s.inv_t : log(x);
 }
 __device__ __forceinline__ double sm_mass(const SmScale& s, uint32_t key)
 {
@@ -89,125 +89,162 @@ __device__ __forceinline__ double sm_sum_value(SmSum s)
     return (double)hi * 0x1p-32 + (double)lo * 0x1p-64;
 }
 
-// ---- workgroup-wide scans (fixed order) ----------------------------------------------------------------------------------------------
-struct SmScratch { unsigned long long a[SM_MAX_WAVES + 1], b[SM_MAX_WAVES + 1], c[SM_MAX_WAVES + 1], word[4]; };
+// ---- scans of a wave and of a workgroup, in one fixed order ----------------------------------------------------------------------------
+// Lane exchange by DPP (row shifts of 16 lanes, then two broadcasts): a shuffle through the LDS crossbar costs a hundred cycles a step, and a
+// selection is little else than scans.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t sm_dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS> __device__ __forceinline__ unsigned long long sm_dpp(unsigned long long v)
+{
+    return (unsigned long long)sm_dpp<CTRL, ROWS>((uint32_t)v) | (unsigned long long)sm_dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32;
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ double sm_dpp(double v)
+{
+    return __longlong_as_double((long long)sm_dpp<CTRL, ROWS>((unsigned long long)__double_as_longlong(v)));
+}
+__device__ __forceinline__ uint32_t sm_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ unsigned long long sm_lane(unsigned long long v, int lane)
+{
+    return (unsigned long long)sm_lane((uint32_t)v, lane) | (unsigned long long)sm_lane((uint32_t)(v >> 32), lane) << 32;
+}
+__device__ __forceinline__ double sm_lane(double v, int lane) { return __longlong_as_double((long long)sm_lane((unsigned long long)__double_as_longlong(v), lane)); }
 
-// exclusive prefix of v over the workgroup, and the total; `part`: LDS for one 8-byte value per wave and one more
-template <typename V> __device__ __forceinline__ V sm_block_scan(V v, void* lds, V& total)
+struct SmAdd { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; } };
+struct SmMaxOf { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; } };
+
+// inclusive scan over the wave (ROWS16: over each row of 16 lanes); lanes without a neighbour see 0, the identity of both operations here
+template <bool ROWS16, typename Op, typename V> __device__ __forceinline__ V sm_wave_scan(V v, Op op)
+{
+    v = op(v, sm_dpp<0x111, 0xf>(v));
+    v = op(v, sm_dpp<0x112, 0xf>(v));
+    v = op(v, sm_dpp<0x114, 0xf>(v));
+    v = op(v, sm_dpp<0x118, 0xf>(v));
+    if (!ROWS16) {
+        v = op(v, sm_dpp<0x142, 0xa>(v));
+        v = op(v, sm_dpp<0x143, 0xc>(v));
+    }
+    return v;
+}
+
+struct SmScratch { unsigned long long a[SM_MAX_WAVES], b[SM_MAX_WAVES], word[6]; };
+
+// inclusive scan over the workgroup; `before` and `total` are the operation over the waves before this one and over all.  lds: 8 bytes a wave
+template <typename Op, typename V> __device__ __forceinline__ V sm_block_op(V v, Op op, void* lds, V& before, V& total)
 {
     V* part = (V*)lds;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    V inc = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const V o = __shfl_up(inc, d);
-        if (lane >= d) inc += o;
-    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const V inc = sm_wave_scan<false>(v, op);
     __syncthreads();
     if (lane == 63) part[wave] = inc;
     __syncthreads();
-    V base = (V)0, sum = (V)0;                                         // every thread adds the waves up: no third barrier
-    for (int w = 0; w < waves; w++) {
-        if (w == wave) base = sum;
-        sum += part[w];
-    }
-    total = sum;
-    return base + (inc - v);
+    const V p = sm_wave_scan<true>((lane & 15) < waves ? part[lane & 15] : (V)0, op);
+    total = sm_lane(p, 15);
+    before = wave ? sm_lane(p, wave - 1) : (V)0;
+    return op(before, inc);
 }
-
+// exclusive prefix sum over the workgroup, and the total
+template <typename V> __device__ __forceinline__ V sm_block_scan(V v, void* lds, V& total)
+{
+    V before;
+    return sm_block_op(v, SmAdd(), lds, before, total) - v;
+}
 // inclusive maximum over the threads up to this one: sums that rounding made fall, or rise without a mass, are flat again
-__device__ __forceinline__ double sm_block_rise(double v, void* lds)
+__device__ __forceinline__ double sm_block_rise(double v, void* lds, double& total)
 {
-    double* part = (double*)lds;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(v, d);
-        if (lane >= d) v = fmax(v, o);
-    }
-    __syncthreads();
-    if (lane == 63) part[wave] = v;
-    __syncthreads();
-    for (int w = 0; w < wave; w++) v = fmax(v, part[w]);
-    return v;
+    double before;
+    return sm_block_op(v, SmMaxOf(), lds, before, total);
 }
-
-__device__ __forceinline__ unsigned long long sm_block_max(unsigned long long v, unsigned long long* part)
+template <typename V> __device__ __forceinline__ V sm_block_max(V v, void* lds)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) { const unsigned long long o = __shfl_xor(v, d); v = o > v ? o : v; }
-    __syncthreads();
-    if (lane == 0) part[wave] = v;
-    __syncthreads();
-    v = part[0];
-    for (int w = 1; w < waves; w++) v = part[w] > v ? part[w] : v;
-    return v;
+    V before, total;
+    sm_block_op(v, SmMaxOf(), lds, before, total);
+    return total;
 }
 
 // ---- radix selection: histograms of one level, and the bin in which the selection ends -------------------------------------------------
+// Bin b of 64 * 2^p lies at sm_slot(b, p): the 2^p bins of one lane of the wave that walks them lie 64 apart.
 struct SmHist { uint32_t n[SM_BINS]; unsigned long long hi[SM_BINS], lo[SM_BINS]; };
+__device__ __forceinline__ int sm_slot(int b, int p) { return ((b & ((1 << p) - 1)) << 6) | (b >> p); }
 
 // An element is taken while what lies before it (best first) is less than the target, counted in elements or in mass.
-struct SmTake { double target; unsigned long long before_n; SmSum before_m; };
+struct SmTake { double target; uint32_t before_n; SmSum before_m; };
+struct SmBin { int bin; uint32_t count, total; };
 
-// The lowest non-empty bin whose predecessors (the bins above it) leave room.  Updates take.before_* to the amount above that bin and
-// returns the bin and its count; -1: there is none.
-template <bool MASS>
-__device__ int sm_boundary(const SmHist& h, int nbins, SmTake& take, SmScratch& sc, unsigned long long& count)
+template <bool MASS> __device__ __forceinline__ bool sm_room(const SmTake& t, uint32_t n, unsigned long long hi, unsigned long long lo)
 {
-    const int per = (nbins + (int)blockDim.x - 1) / (int)blockDim.x;   // thread t owns the bins nbins - 1 - (per * t + k), k < per
-    unsigned long long n = 0, hi = 0, lo = 0;
-    for (int k = 0; k < per; k++) {
-        const int b = nbins - 1 - ((int)threadIdx.x * per + k);
-        if (b < 0) break;
-        n += h.n[b];
-        if (MASS) { hi += h.hi[b]; lo += h.lo[b]; }
+    return MASS ? sm_sum_value(SmSum{ t.before_m.hi + hi, t.before_m.lo + lo }) < t.target : (double)(t.before_n + n) < t.target;
+}
+
+// The lowest non-empty bin whose predecessors (the bins above it) leave room: a wave sums 2^p bins a lane, best first, scans, and does the
+// same once more inside the lane it ends in.  Updates take.before_* to the amount above that bin; bin -1: there is none.  All threads call it
+// behind a barrier; a barrier has to follow before the histogram or sc is written again.
+template <bool MASS> __device__ SmBin sm_boundary(const uint32_t* hn, const unsigned long long* hhi, const unsigned long long* hlo, int p, SmTake& take, SmScratch& sc)
+{
+    if (threadIdx.x < 64) {
+        const int lane = threadIdx.x, per = 1 << p;
+        uint32_t n = 0;
+        unsigned long long hi = 0, lo = 0;
+        for (int k = 0; k < per; k++) {
+            const int at = (k << 6) | (63 - lane);
+            n += hn[at];
+            if (MASS) { hi += hhi[at]; lo += hlo[at]; }
+        }
+        const uint32_t in = sm_wave_scan<false>(n, SmAdd());
+        unsigned long long ihi = 0, ilo = 0;
+        if (MASS) { ihi = sm_wave_scan<false>(hi, SmAdd()); ilo = sm_wave_scan<false>(lo, SmAdd()); }
+        const unsigned long long enter = __ballot(n != 0 && sm_room<MASS>(take, in - n, ihi - hi, ilo - lo));
+        const uint32_t total = sm_lane(in, 63);
+        int bin = -1;
+        uint32_t bn = take.before_n, count = 0;
+        SmSum bm = take.before_m;
+        if (enter) {
+            const int l = 63 - __clzll((long long)enter);
+            bn += sm_lane(in - n, l);
+            if (MASS) { bm.hi += sm_lane(ihi - hi, l); bm.lo += sm_lane(ilo - lo, l); }
+            const int at = ((per - 1 - lane) << 6) | (63 - l);
+            const uint32_t n2 = lane < per ? hn[at] : 0u;
+            unsigned long long hi2 = 0, lo2 = 0, ihi2 = 0, ilo2 = 0;
+            if (MASS && lane < per) { hi2 = hhi[at]; lo2 = hlo[at]; }
+            const uint32_t in2 = sm_wave_scan<false>(n2, SmAdd());
+            if (MASS) { ihi2 = sm_wave_scan<false>(hi2, SmAdd()); ilo2 = sm_wave_scan<false>(lo2, SmAdd()); }
+            const SmTake inner = { take.target, bn, bm };
+            const int l2 = 63 - __clzll((long long)__ballot(n2 != 0 && sm_room<MASS>(inner, in2 - n2, ihi2 - hi2, ilo2 - lo2)));
+            bin = ((63 - l) << p) | (per - 1 - l2);
+            bn += sm_lane(in2 - n2, l2);
+            count = sm_lane(n2, l2);
+            if (MASS) { bm.hi += sm_lane(ihi2 - hi2, l2); bm.lo += sm_lane(ilo2 - lo2, l2); }
+        }
+        if (lane == 0) {
+            sc.word[0] = (unsigned long long)(long long)bin;
+            sc.word[1] = bn;
+            sc.word[2] = (unsigned long long)count | (unsigned long long)total << 32;
+            sc.word[3] = bm.hi;
+            sc.word[4] = bm.lo;
+        }
     }
-    unsigned long long tn, thi = 0, tlo = 0, bhi = 0, blo = 0;
-    unsigned long long bn = take.before_n + sm_block_scan<unsigned long long>(n, sc.a, tn);
-    if (MASS) {
-        bhi = take.before_m.hi + sm_block_scan<unsigned long long>(hi, sc.b, thi);
-        blo = take.before_m.lo + sm_block_scan<unsigned long long>(lo, sc.c, tlo);
-    }
-    unsigned long long mine = 0, an = 0, ahi = 0, alo = 0, ac = 0;     // mine: 1 + position, best first, of the last bin that is entered
-    for (int k = 0; k < per; k++) {
-        const int b = nbins - 1 - ((int)threadIdx.x * per + k);
-        if (b < 0) break;
-        const unsigned long long c = h.n[b];
-        const bool room = MASS ? sm_sum_value(SmSum{ bhi, blo }) < take.target : (double)bn < take.target;
-        if (c != 0 && room) { mine = (unsigned long long)(nbins - b); an = bn; ahi = bhi; alo = blo; ac = c; }
-        bn += c;
-        if (MASS) { bhi += h.hi[b]; blo += h.lo[b]; }
-    }
-    const unsigned long long best = sm_block_max(mine, sc.a);
-    if (best == 0) { count = 0; return -1; }
-    if (mine == best) { sc.word[0] = an; sc.word[1] = ahi; sc.word[2] = alo; sc.word[3] = ac; }
     __syncthreads();
-    take.before_n = sc.word[0];
-    take.before_m = SmSum{ sc.word[1], sc.word[2] };
-    count = sc.word[3];
-    __syncthreads();
-    return nbins - (int)best;
+    const SmBin b = { (int)(long long)sc.word[0], (uint32_t)sc.word[2], (uint32_t)(sc.word[2] >> 32) };
+    take.before_n = (uint32_t)sc.word[1];
+    take.before_m = SmSum{ sc.word[3], sc.word[4] };
+    return b;
 }
 
 // of `count` elements of equal key behind what is before them: how many are taken (at least one, by the choice of the bin)
-template <bool MASS> __device__ __forceinline__ unsigned long long sm_ties(const SmTake& take, unsigned long long count, double mass)
+template <bool MASS> __device__ __forceinline__ uint32_t sm_ties(const SmTake& take, uint32_t count, double mass)
 {
     if (!MASS) {
         const double left = take.target - (double)take.before_n;
-        return left >= (double)count ? count : (unsigned long long)ceil(left);
+        return left >= (double)count ? count : (uint32_t)ceil(left);
     }
     const SmSum one = sm_limbs(mass);
-    unsigned long long lo = 1, hi = count;                             // the first j (from 0) that finds no room
+    uint32_t lo = 1, hi = count;                                       // the first j (from 0) that finds no room
     while (lo < hi) {
-        const unsigned long long mid = lo + (hi - lo) / 2;
-        if (sm_sum_value(SmSum{ take.before_m.hi + mid * one.hi, take.before_m.lo + mid * one.lo }) < take.target) lo = mid + 1; else hi = mid;
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (sm_room<true>(take, 0, mid * one.hi, mid * one.lo)) lo = mid + 1; else hi = mid;
     }
     return lo;
 }
 // every element of the boundary bin is taken: the selection needs no further level
-template <bool MASS> __device__ __forceinline__ bool sm_whole_bin(const SmTake& take, unsigned long long count)
+template <bool MASS> __device__ __forceinline__ bool sm_whole_bin(const SmTake& take, uint32_t count)
 {
     return count == 1 || (!MASS && take.target - (double)take.before_n >= (double)count);
 }
@@ -235,50 +272,97 @@ __device__ __forceinline__ void sm_min_p(const SmScale& s, uint32_t best, double
     if (lo > kept.thr) kept = SmKept{ lo, SM_ALL };
 }
 
+// ---- approximate race keys ---------------------------------------------------------------------------------------------------------------
+// The n-th largest race key is found from approximate keys in 32 bits: k ~ log2(mass) - log2(-ln(1 - u)).  Levels of histograms of the ordered
+// float bound it to a bin; what lies above the bin by more than twice the approximation's error wins, what lies below by as much loses, and
+// the few in the zone between are ranked by their exact 64-bit keys.
+//
+// Error of k: the logarithm instruction is good to a step of its result or 2^-22 (arguments next to one), log2(e) / T and the products round
+// three times, -ln(1 - u) is good to 2^-19 relative (below 2^-6 a series, above it 1 - u is off by 2^-25 of at least 2^-6): together less
+// than 2^-17 + |log2(mass)| 2^-21 + |log2(-ln(1-u))| 2^-21, the last at most 33, and for weights 2^-22 of the slope 1 / T (the logarithm of a
+// weight next to one).  sm_margin allows twice that and more.
+__device__ __forceinline__ float sm_log2(float x)                      // x > 0, subnormals too
+{
+    const bool small = x < 0x1p-100f;
+    return __builtin_amdgcn_logf(small ? x * 0x1p64f : x) - (small ? 64.0f : 0.0f);
+}
+__device__ __forceinline__ float sm_margin(float k, float slope) { return 0x1p-13f + fabsf(k) * 0x1p-18f + slope * 0x1p-21f; }
+__device__ __forceinline__ float sm_slope(const SmRule& r) { return (float)((r.mode == SM_LOGITS ? 1.4426950408889634 : 1.0) / r.temperature); }
+
+__device__ __forceinline__ uint32_t sm_order(float k)
+{
+    const uint32_t b = __float_as_uint(k);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float sm_unorder(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
+
+// ordered approximate key; 0 = excluded.  `slope`: log2(e) / T or 1 / T in 32 bits
+__device__ __forceinline__ uint32_t sm_race32(bool logits, float slope, uint32_t key, float u)
+{
+    if (key == 0u) return 0u;
+    u = u == u ? fminf(fmaxf(u, 0x1p-33f), 1.0f - 0x1p-24f) : 1.0f - 0x1p-24f;
+    const float x = __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+    const float a = (logits ? x : sm_log2(x)) * slope;
+    const float e = u < 0x1p-6f ? u * (1.0f + u * (0.5f + u * (0.33333333f + u * 0.25f))) : -0.69314718f * __builtin_amdgcn_logf(1.0f - u);
+    const float k = fminf(fmaxf(a, -3e38f), 3e38f) - __builtin_amdgcn_logf(e);
+    return sm_order(k + 0.0f);
+}
+
+// zone of the n-th key given that its approximation lies in [lo, hi]: ordered keys below zone.lo lose, above zone.hi win
+struct SmZone { uint32_t lo, hi; };
+__device__ __forceinline__ SmZone sm_zone(uint32_t lo, uint32_t hi, float slope)
+{
+    const float klo = sm_unorder(lo), khi = sm_unorder(hi);
+    const uint32_t a = sm_order(klo - 2.0f * sm_margin(klo, slope)), b = sm_order(khi + 2.0f * sm_margin(khi, slope));
+    return SmZone{ a ? a : 1u, b };
+}
+
 // Unrolled 64-bit exponentials and logarithms stay out of line: sixteen of them inlined, with their constants, spill two thousand registers.
 __device__ __attribute__((noinline)) double sm_mass_call(SmScale s, uint32_t key) { return sm_mass(s, key); }
 __device__ __attribute__((noinline)) unsigned long long sm_race_call(SmScale s, uint32_t key, float u) { return sm_race(s, key, u); }
 
 // ---- short rows: one workgroup per row, EPT consecutive elements of a thread in registers ----------------------------------------------
-// Narrows `kept` (or, for 64-bit race keys, finds thr / ties): each[k] is the key of element threadIdx.x * EPT + k, 0: not a candidate.
+// key[k] is the key of element threadIdx.x * EPT + k, 0: not a candidate.  Ends when the boundary bin holds at most `small` elements:
+// [lo, hi] is then the bin's range of keys, take.before_* what lies above it, and the result its count and the number of candidates.
 template <bool MASS, int BITS, int EPT, typename Word, typename Mass>
-__device__ void sm_select_short(const Word (&key)[EPT], const Mass& mass_of, SmTake take, SmHist& h, SmScratch& sc,
-                                Word& thr, unsigned long long& ties, unsigned long long& equal)
+__device__ SmBin sm_select_short(const Word (&key)[EPT], const Mass& mass_of, SmTake& take, uint32_t small, SmHist& h, SmScratch& sc, Word& lo, Word& hi)
 {
     Word prefix = 0;
-    unsigned long long count = 0;
     int shift = BITS;
-    thr = 0; ties = equal = 0;
+    SmBin b = { -1, 0, 0 };
+    uint32_t candidates = 0;
     while (shift > 0) {
-        const int width = shift >= 11 ? 11 : shift, at = shift - width, nbins = 1 << width;
+        const int width = shift >= 11 ? 11 : shift < 6 ? 6 : shift, at = shift > width ? shift - width : 0, p = width - 6;
         __syncthreads();
-        for (int b = threadIdx.x; b < nbins; b += blockDim.x) { h.n[b] = 0; if (MASS) { h.hi[b] = 0; h.lo[b] = 0; } }
+        for (int i = threadIdx.x; i < 1 << width; i += blockDim.x) { h.n[i] = 0; if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
             if (key[k] == 0 || (shift < BITS && (key[k] >> shift) != prefix)) continue;
-            const int b = (int)(key[k] >> at) & (nbins - 1);
-            atomicAdd(&h.n[b], 1u);
+            const int i = sm_slot((int)((key[k] >> at) & (((Word)1 << (shift - at)) - 1)), p);
+            atomicAdd(&h.n[i], 1u);
             if (MASS) {
                 const SmSum m = sm_limbs(mass_of(key[k]));
-                if (m.hi) atomicAdd(&h.hi[b], m.hi);
-                if (m.lo) atomicAdd(&h.lo[b], m.lo);
+                if (m.hi) atomicAdd(&h.hi[i], m.hi);
+                if (m.lo) atomicAdd(&h.lo[i], m.lo);
             }
         }
         __syncthreads();
-        const int b = sm_boundary<MASS>(h, nbins, take, sc, count);
-        if (b < 0) { thr = ~(Word)0; return; }                         // no candidate at all
-        prefix = (Word)(prefix << width) | (Word)b;
+        b = sm_boundary<MASS>(h.n, h.hi, h.lo, p, take, sc);
+        if (shift == BITS) candidates = b.total;
+        if (b.bin < 0) break;                                          // no candidate at all
+        prefix = (Word)(prefix << (shift - at)) | (Word)b.bin;
         shift = at;
-        if (sm_whole_bin<MASS>(take, count)) { thr = prefix << at; ties = equal = 1; return; }
+        if (b.count <= small) break;
     }
-    thr = prefix;
-    equal = count;
-    ties = sm_ties<MASS>(take, count, MASS ? mass_of(thr) : 0.0);
+    lo = prefix << shift;
+    hi = lo | (((Word)1 << shift) - 1);
+    b.total = candidates;
+    return b;
 }
 
 // index of the n-th (from 1) flagged element
-template <int EPT> __device__ uint32_t sm_nth_short(const bool (&flag)[EPT], unsigned long long n, SmScratch& sc)
+template <int EPT> __device__ uint32_t sm_nth_short(const bool (&flag)[EPT], uint32_t n, SmScratch& sc)
 {
     uint32_t c = 0, total;
 #pragma unroll
@@ -287,9 +371,7 @@ template <int EPT> __device__ uint32_t sm_nth_short(const bool (&flag)[EPT], uns
 #pragma unroll
     for (int k = 0; k < EPT; k++) if (flag[k] && ++at == n) sc.word[0] = threadIdx.x * EPT + k;
     __syncthreads();
-    const uint32_t i = (uint32_t)sc.word[0];
-    __syncthreads();
-    return i;
+    return (uint32_t)sc.word[0];
 }
 
 // four consecutive scores from i on as keys; beyond V: 0
@@ -310,7 +392,8 @@ template <typename T, int TPB, int EPT, bool DISTINCT>
 __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                             int V, long long n, SmRule rule, long long* __restrict__ out)
 {
-    __shared__ union { SmHist hist; double cdf[DISTINCT ? 1 : TPB * EPT]; } h;
+    __shared__ union { SmHist hist; double cdf[DISTINCT ? 1 : TPB * EPT]; struct { unsigned long long rank[SM_BINS]; uint32_t index[SM_BINS]; } zone; } h;
+    __shared__ uint32_t won[DISTINCT ? TPB * EPT / 32 : 1];
     __shared__ uint16_t pos[DISTINCT ? 1 : TPB];
     __shared__ SmScratch sc;
     const long long r = blockIdx.x;
@@ -329,7 +412,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     }
 #pragma unroll
     for (int k = 0; k < EPT; k++) best = key[k] > best ? key[k] : best;
-    best = (uint32_t)sm_block_max(best, sc.a);
+    best = sm_block_max(best, sc.a);
     if (best == 0) {                                                   // nothing to draw from
         for (long long j = threadIdx.x; j < n; j += blockDim.x) out[j] = -1;
         return;
@@ -340,12 +423,12 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     // filters: an element that one of them drops becomes key 0
     for (int pass = 0; pass < 2; pass++) {
         SmTake take = { 0.0, 0, { 0, 0 } };
-        uint32_t thr;
-        unsigned long long ties, equal;
+        uint32_t lo, hi;
+        SmBin bin;
         if (pass == 0) {
             if (rule.top_k <= 0 || rule.top_k >= V) continue;
             take.target = (double)rule.top_k;
-            sm_select_short<false, 32, EPT, uint32_t>(key, mass_of, take, h.hist, sc, thr, ties, equal);
+            bin = sm_select_short<false, 32, EPT, uint32_t>(key, mass_of, take, 1, h.hist, sc, lo, hi);
         } else {
             if (rule.top_p >= 1.0) continue;
             SmSum mine = { 0, 0 }, total;
@@ -355,13 +438,15 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             sm_block_scan<unsigned long long>(mine.hi, sc.a, total.hi);
             sm_block_scan<unsigned long long>(mine.lo, sc.b, total.lo);
             take.target = rule.top_p * sm_sum_value(total);
-            sm_select_short<true, 32, EPT, uint32_t>(key, mass_of, take, h.hist, sc, thr, ties, equal);
+            bin = sm_select_short<true, 32, EPT, uint32_t>(key, mass_of, take, 1, h.hist, sc, lo, hi);
         }
-        SmKept kept = { thr, SM_ALL };
-        if (ties < equal) {
+        // a bin of one element is taken whole; one of equal elements up to the cut
+        SmKept kept = { lo, SM_ALL };
+        const uint32_t ties = bin.count == 1 ? 1 : pass == 0 ? sm_ties<false>(take, bin.count, 0.0) : sm_ties<true>(take, bin.count, mass_of(lo));
+        if (ties < bin.count) {
             bool tie[EPT];
 #pragma unroll
-            for (int k = 0; k < EPT; k++) tie[k] = key[k] == thr;
+            for (int k = 0; k < EPT; k++) tie[k] = key[k] == lo;
             kept.last = sm_nth_short<EPT>(tie, ties, sc);
         }
 #pragma unroll
@@ -374,28 +459,69 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         for (int k = 0; k < EPT; k++) if (!sm_in(kept, key[k], (uint32_t)(i0 + k))) key[k] = 0;
     }
     if (DISTINCT) {
-        unsigned long long race[EPT], thr, ties, equal;
+        uint32_t race[EPT], lo, hi, wins = 0;
+        const float slope = sm_slope(rule);
 #pragma unroll
-        for (int k = 0; k < EPT; k++) { race[k] = sm_race_call(scale, key[k], uk[k]); }
-        const SmTake take = { (double)n, 0, { 0, 0 } };
-        sm_select_short<false, 64, EPT, unsigned long long>(race, [](unsigned long long) { return 0.0; }, take, h.hist, sc, thr, ties, equal);
-        uint32_t last = SM_ALL, c = 0, total;
-        if (ties < equal) {
-            bool tie[EPT];
-#pragma unroll
-            for (int k = 0; k < EPT; k++) tie[k] = race[k] == thr;
-            last = sm_nth_short<EPT>(tie, ties, sc);
-        }
-        bool win[EPT];
+        for (int k = 0; k < EPT; k++) race[k] = sm_race32(logits, slope, key[k], uk[k]);
+        SmTake take = { (double)n, 0, { 0, 0 } };
+        const SmBin bin = sm_select_short<false, 32, EPT, uint32_t>(race, [](uint32_t) { return 0.0; }, take, 16, h.hist, sc, lo, hi);
+        SmZone zone = { 1u, 0u };                                      // nothing to rank where everything wins
+        if (bin.total > n) zone = sm_zone(lo, hi, slope);
+        __syncthreads();
+        if (threadIdx.x == 0) sc.word[5] = 0;
+        for (int i = threadIdx.x; i < TPB * EPT / 32; i += TPB) won[i] = 0;
+        __syncthreads();
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
-            win[k] = race[k] != 0 && (race[k] > thr || (race[k] == thr && (uint32_t)(i0 + k) <= last));
-            c += win[k];
+            if (race[k] > zone.hi) wins |= 1u << k;
+            else if (race[k] >= zone.lo) {
+                const uint32_t at = (uint32_t)atomicAdd(&sc.word[5], 1ull);
+                if (at < SM_BINS) h.zone.index[at] = i0 + k;
+            }
         }
-        long long at = sm_block_scan<uint32_t>(c, sc.a, total);
+        uint32_t sure;
+        sm_block_scan<uint32_t>(__popc(wins), sc.a, sure);
+        const uint32_t found = (uint32_t)sc.word[5], room = (uint32_t)n > sure ? (uint32_t)n - sure : 0;
+        if (found <= SM_BINS) {
+            for (uint32_t a = threadIdx.x; a < found; a += TPB) {
+                const uint32_t i = h.zone.index[a];
+                h.zone.rank[a] = sm_race(scale, sm_key(x[i], logits), u[i]);
+            }
+            __syncthreads();
+            for (uint32_t a = threadIdx.x; a < found; a += TPB) {
+                const unsigned long long mine = h.zone.rank[a];
+                const uint32_t i = h.zone.index[a];
+                uint32_t ahead = 0;
+                for (uint32_t c = 0; c < found; c++) ahead += h.zone.rank[c] > mine || (h.zone.rank[c] == mine && h.zone.index[c] < i);
+                if (ahead < room) atomicOr(&won[i >> 5], 1u << (i & 31));
+            }
+            __syncthreads();
+            wins |= (won[i0 >> 5] >> (i0 & 31)) & ((1u << EPT) - 1);
+        } else {
+            // many elements next to the border (equal numbers, or a slope that spreads nothing): radix selection of their exact keys
+            unsigned long long exact[EPT], elo, ehi;
 #pragma unroll
-        for (int k = 0; k < EPT; k++) if (win[k]) out[at++] = i0 + k;
-        for (long long j = (long long)total + threadIdx.x; j < n; j += blockDim.x) out[j] = -1;
+            for (int k = 0; k < EPT; k++) exact[k] = race[k] >= zone.lo && race[k] <= zone.hi ? sm_race_call(scale, key[k], uk[k]) : 0ull;
+            SmTake left = { (double)room, 0, { 0, 0 } };
+            const SmBin e = sm_select_short<false, 64, EPT, unsigned long long>(exact, [](unsigned long long) { return 0.0; }, left, 1, h.hist, sc, elo, ehi);
+            const uint32_t ties = e.bin < 0 ? 0 : e.count == 1 ? 1 : sm_ties<false>(left, e.count, 0.0);
+            uint32_t last = SM_ALL;
+            if (ties < e.count) {
+                bool tie[EPT];
+#pragma unroll
+                for (int k = 0; k < EPT; k++) tie[k] = exact[k] == elo;
+                last = sm_nth_short<EPT>(tie, ties, sc);
+            }
+            if (e.bin >= 0)
+#pragma unroll
+                for (int k = 0; k < EPT; k++)
+                    if (exact[k] != 0 && (exact[k] > elo || (exact[k] == elo && (uint32_t)(i0 + k) <= last))) wins |= 1u << k;
+        }
+        uint32_t total;
+        long long at = sm_block_scan<uint32_t>(__popc(wins), sc.a, total);
+#pragma unroll
+        for (int k = 0; k < EPT; k++) if ((wins >> k) & 1) out[at++] = i0 + k;
+        for (long long j = (long long)total + threadIdx.x; j < n; j += TPB) out[j] = -1;
     } else {
         double* cdf = h.cdf;                                           // the histograms are done
         double w[EPT], sum = 0.0, total;
@@ -407,7 +533,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             if (w[k] > 0.0) { positive |= 1u << k; last = (uint32_t)(i0 + k) + 1; }
         }
         double at = sm_block_scan<double>(sum, sc.a, total);
-        last = (uint32_t)sm_block_max(last, sc.b);
+        last = sm_block_max(last, sc.b);
 #pragma unroll
         for (int k = 0; k < EPT; k++) { at += w[k]; cdf[i0 + k] = at; }
         pos[threadIdx.x] = (uint16_t)positive;
@@ -427,7 +553,9 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
 // Every step is one launch over (row, workgroup); the last workgroup of a row to finish a step (SmRowState::ticket) draws its conclusion and
 // leaves it in the row's state for the next launch.
 #define SM_LTPB 1024
-#define SM_RBINS 4096                  // bins of a level of the race's approximate keys
+#define SM_RBITS1 12                   // levels of the race's approximate keys: 12 bits, then 10 (a finer second level costs more to merge than it saves to rank)
+#define SM_RBITS2 10
+#define SM_RBINS (1 << SM_RBITS1)
 #define SM_TILE 8192                   // elements per workgroup step of the race's last pass: 128 words of winners
 #define SM_STILE 4096                  // elements per tile of prefix sums
 #define SM_GROUP 16                    // elements per stored prefix
@@ -473,7 +601,7 @@ __global__ void __launch_bounds__(256) sm_clear_kernel(uint4* p, long long n)
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_best_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step)
 {
-    __shared__ unsigned long long part[SM_MAX_WAVES + 1];
+    __shared__ unsigned long long part[SM_MAX_WAVES];
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
     const T* x = scores + r * sstride;
     const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
@@ -484,7 +612,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_best_kernel(const T* __restrict__ 
 #pragma unroll
         for (int j = 0; j < 4; j++) best = k[j] > best ? k[j] : best;
     }
-    best = (uint32_t)sm_block_max(best, part);
+    best = sm_block_max(best, part);
     if (threadIdx.x == 0 && best) atomicMax(&wk.state[r].best, best);
     (void)step;
 }
@@ -505,7 +633,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
     const SmKept kept = first ? st.kept : st.before;
     const uint32_t prefix = (uint32_t)st.prefix;
-    const int at = shift - width, nbins = 1 << width;
+    const int at = shift - width, nbins = 1 << width, p = width - 6;
     const SmScale scale = sm_scale(rule, MASS ? st.best : 0u);
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
     for (int i = threadIdx.x; i < nbins; i += SM_LTPB) { h.n[i] = 0; if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } }
@@ -516,7 +644,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (!sm_in(kept, key[j], (uint32_t)(i + j)) || (!first && (key[j] >> shift) != prefix)) continue;
-            const int bin = (int)(key[j] >> at) & (nbins - 1);
+            const int bin = sm_slot((int)(key[j] >> at) & (nbins - 1), p);
             atomicAdd(&h.n[bin], 1u);
             if (MASS) {
                 const SmSum m = sm_limbs(sm_mass(scale, key[j]) * unit);
@@ -549,27 +677,26 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
             take.target = rule.top_p * sm_sum_value(total);
         }
     }
-    unsigned long long count;
-    const int bin = sm_boundary<MASS>(h, nbins, take, sc, count);
+    const SmBin bin = sm_boundary<MASS>(h.n, h.hi, h.lo, p, take, sc);
     if (threadIdx.x != 0) return;
     st.before = kept;
     st.take = take;
     st.ended = 0;
     st.cut = 0;
-    if (bin < 0) { st.ended = 1; return; }                             // no candidate: the filter in force (or an empty row) stands
-    const uint32_t p = (first ? 0u : prefix << width) | (uint32_t)bin;
-    st.prefix = p;
-    const bool whole = sm_whole_bin<MASS>(take, count);
+    if (bin.bin < 0) { st.ended = 1; return; }                         // no candidate: the filter in force (or an empty row) stands
+    const uint32_t found = (first ? 0u : prefix << width) | (uint32_t)bin.bin;
+    st.prefix = found;
+    const bool whole = sm_whole_bin<MASS>(take, bin.count);
     if (!whole && at > (sizeof(T) == 2 ? 10 : 0)) return;
     // the key is found (or the lowest key of a bin that is taken whole); a cut among the equal ones is left to sm_tie_kernel.  Scores of 16
     // bits differ in the 22 leading bits of their keys: what follows is all zeros, or all ones for a negative score.
-    const uint32_t thr = !whole && at && !(p >> (31 - at)) ? (p << at) | ((1u << at) - 1) : p << at;
-    unsigned long long ties = count;
-    if (!whole) ties = sm_ties<MASS>(take, count, MASS ? sm_mass(scale, thr) * unit : 0.0);
+    const uint32_t thr = !whole && at && !(found >> (31 - at)) ? (found << at) | ((1u << at) - 1) : found << at;
+    uint32_t ties = bin.count;
+    if (!whole) ties = sm_ties<MASS>(take, bin.count, MASS ? sm_mass(scale, thr) * unit : 0.0);
     st.ended = 1;
     if (thr < kept.thr) return;                                        // a whole bin around the earlier filter's cut: that one stands
     st.kept = SmKept{ thr, thr == kept.thr ? kept.last : SM_ALL };
-    if (ties < count) { st.cut = 1; st.ties = ties; }
+    if (ties < bin.count) { st.cut = 1; st.ties = ties; }
 }
 
 // index of the last equal element that is kept, where a selection ends inside equal keys; and min-p, once, behind the last filter
@@ -653,15 +780,16 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
             if (!sm_in(kept, key[k], (uint32_t)(i0 + k))) key[k] = 0;
             best = key[k] > best ? key[k] : best;
         }
-        best = (uint32_t)sm_block_max(best, sc.b);
+        best = sm_block_max(best, sc.b);
         const SmScale scale = sm_scale(rule, best);
         double sum = 0.0, total;
 #pragma unroll
         for (int k = 0; k < SM_GROUP; k++) sum += sm_mass(scale, key[k]);
         const double before = sm_block_scan<double>(sum, sc.a, total);
-        groups[t * (SM_STILE / SM_GROUP) + threadIdx.x] = sm_block_rise(sum > 0.0 ? before + sum : 0.0, sc.b);
+        const double mass = total;
+        groups[t * (SM_STILE / SM_GROUP) + threadIdx.x] = sm_block_rise(sum > 0.0 ? before + sum : 0.0, sc.b, total);
         if (threadIdx.x == 0) {
-            sm_poke(&sums[t], total);
+            sm_poke(&sums[t], mass);
             sm_poke(&tops[t], best ? scale.top : -INFINITY);
         }
     }
@@ -669,7 +797,7 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
     double top = -INFINITY;
     for (long long t = threadIdx.x; t < wk.stiles; t += 256) top = fmax(top, sm_peek(&tops[t]));
     const unsigned long long ordered = (unsigned long long)__double_as_longlong(top + 0.0);
-    const unsigned long long m = sm_block_max((ordered >> 63) ? ~ordered : (ordered | 0x8000000000000000ull), sc.b);
+    const unsigned long long m = sm_block_max<unsigned long long>((ordered >> 63) ? ~ordered : (ordered | 0x8000000000000000ull), sc.b);
     top = __longlong_as_double((long long)((m >> 63) ? (m & 0x7fffffffffffffffull) : ~m));
     double run = 0.0, risen = 0.0;
     for (long long base = 0; base < wk.stiles; base += 256) {
@@ -680,12 +808,10 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
             mass = sm_peek(&sums[t]) * (rule.mode == SM_LINEAR || tt == -INFINITY ? 1.0 : exp(tt - top));
         }
         const double before = sm_block_scan<double>(mass, sc.a, total);
-        const double upto = fmax(sm_block_rise(mass > 0.0 ? run + before + mass : 0.0, sc.b), risen);
+        double most;
+        const double upto = fmax(sm_block_rise(mass > 0.0 ? run + before + mass : 0.0, sc.b, most), risen);
         if (t < wk.stiles) sums[t] = upto;
-        __syncthreads();
-        if (threadIdx.x == 255) sc.word[0] = (unsigned long long)__double_as_longlong(upto);
-        __syncthreads();
-        risen = __longlong_as_double((long long)sc.word[0]);
+        risen = fmax(risen, most);
         run += total;
     }
     if (threadIdx.x == 0) { st.total = run; st.top = top; st.kept = kept; }
@@ -720,7 +846,7 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
     if (!(g[k] > local)) k = first(g, ng, [&](double s) { return s >= g[ng - 1]; });
     // inside the group: the masses once more, in the same order
     const T* x = scores + r * sstride;
-    SmScale scale = { rule.mode, rule.temperature, tops[t], 1.0 };
+    const SmScale scale = { rule.mode, 1.0 / rule.temperature, tops[t], 1.0 };
     const SmKept kept = st.kept;
     const long long i0 = t * SM_STILE + k * SM_GROUP;
     double acc = k ? g[k - 1] : 0.0;
@@ -736,65 +862,6 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
 }
 
 // ---- long rows, without replacement ----------------------------------------------------------------------------------------------------
-// The n-th largest race key is found from approximate keys in 32 bits: k ~ log2(mass) - log2(-ln(1 - u)).  Two levels of histograms (12 bits
-// each of the ordered float) bound it to a bin; what lies above the bin by more than twice the approximation's error wins, what lies below
-// by as much loses, and the few in the zone between are ranked by their exact 64-bit keys.
-//
-// Error of k: the logarithm instruction is good to a step of its result or 2^-22 (arguments next to one), log2(e) / T and the products round
-// three times, -ln(1 - u) is good to 2^-19 relative (below 2^-6 a series, above it 1 - u is off by 2^-25 of at least 2^-6): together less
-// than 2^-17 + |log2(mass)| 2^-21 + |log2(-ln(1-u))| 2^-21, the last at most 33, and for weights 2^-22 of the slope 1 / T (the logarithm of a
-// weight next to one).  sm_margin allows twice that and more.
-__device__ __forceinline__ float sm_log2(float x)                      // x > 0, subnormals too
-{
-    const bool small = x < 0x1p-100f;
-    return __builtin_amdgcn_logf(small ? x * 0x1p64f : x) - (small ? 64.0f : 0.0f);
-}
-__device__ __forceinline__ float sm_margin(float k, float slope) { return 0x1p-13f + fabsf(k) * 0x1p-18f + slope * 0x1p-21f; }
-__device__ __forceinline__ float sm_slope(const SmRule& r) { return (float)((r.mode == SM_LOGITS ? 1.4426950408889634 : 1.0) / r.temperature); }
-
-__device__ __forceinline__ uint32_t sm_order(float k)
-{
-    const uint32_t b = __float_as_uint(k);
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float sm_unorder(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
-
-// ordered approximate key; 0 = excluded.  `slope`: log2(e) / T or 1 / T in 32 bits
-__device__ __forceinline__ uint32_t sm_race32(bool logits, float slope, uint32_t key, float u)
-{
-    if (key == 0u) return 0u;
-    u = u == u ? fminf(fmaxf(u, 0x1p-33f), 1.0f - 0x1p-24f) : 1.0f - 0x1p-24f;
-    const float x = __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
-    const float a = (logits ? x : sm_log2(x)) * slope;
-    const float e = u < 0x1p-6f ? u * (1.0f + u * (0.5f + u * (0.33333333f + u * 0.25f))) : -0.69314718f * __builtin_amdgcn_logf(1.0f - u);
-    const float k = fminf(fmaxf(a, -3e38f), 3e38f) - __builtin_amdgcn_logf(e);
-    return sm_order(k + 0.0f);
-}
-
-// bin of the boundary in a histogram of counts (the lowest non-empty one with fewer than `target` before it), what lies before it, and the
-// histogram's total
-__device__ int sm_boundary_counts(const uint32_t* h, int nbins, double target, unsigned long long& before, unsigned long long& total, SmScratch& sc)
-{
-    const int per = (nbins + (int)blockDim.x - 1) / (int)blockDim.x;
-    unsigned long long n = 0;
-    for (int k = 0; k < per; k++) { const int b = nbins - 1 - ((int)threadIdx.x * per + k); if (b >= 0) n += h[b]; }
-    unsigned long long bn = before + sm_block_scan<unsigned long long>(n, sc.a, total);
-    unsigned long long mine = 0, an = 0;
-    for (int k = 0; k < per; k++) {
-        const int b = nbins - 1 - ((int)threadIdx.x * per + k);
-        if (b < 0) break;
-        if (h[b] != 0 && (double)bn < target) { mine = (unsigned long long)(nbins - b); an = bn; }
-        bn += h[b];
-    }
-    const unsigned long long best = sm_block_max(mine, sc.a);
-    if (best == 0) return -1;
-    if (mine == best) sc.word[0] = an;
-    __syncthreads();
-    before = sc.word[0];
-    __syncthreads();
-    return nbins - (int)best;
-}
-
 // approximate keys and their first level
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
@@ -829,7 +896,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             o.v[j] = sm_race32(logits, slope, sm_in(kept, key[j], (uint32_t)(i + j)) ? key[j] : 0u, uk[j]);
-            if (o.v[j]) atomicAdd(&h[o.v[j] >> 20], 1u);
+            if (o.v[j]) atomicAdd(&h[sm_slot((int)(o.v[j] >> (32 - SM_RBITS1)), SM_RBITS1 - 6)], 1u);
         }
         *(LgVec4<uint32_t>*)(keys + i) = o;                            // (padded to a multiple of four: what lies behind V is key 0)
     }
@@ -839,15 +906,15 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
     for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) { h[i] = sm_peek(&g[i]); g[i] = 0; }
     __syncthreads();
-    unsigned long long before = 0, all;
-    const int bin = sm_boundary_counts(h, SM_RBINS, (double)n, before, all, sc);
+    SmTake take = { (double)n, 0, { 0, 0 } };
+    const SmBin bin = sm_boundary<false>(h, nullptr, nullptr, SM_RBITS1 - 6, take, sc);
     if (threadIdx.x != 0) return;
     st.kept = kept;
     st.candidates = 0;
-    st.take.before_n = before;
-    st.prefix = (unsigned long long)(bin < 0 ? 0 : bin);
+    st.take = take;
+    st.prefix = (unsigned long long)(bin.bin < 0 ? 0 : bin.bin);
     st.ended = 0;
-    if (all <= (unsigned long long)n) { st.ended = 1; st.zone_lo = st.zone_hi = 0u; }        // whatever is left wins: nothing to rank
+    if (bin.total <= (unsigned long long)n) { st.ended = 1; st.zone_lo = 1u; st.zone_hi = 0u; }        // whatever is left wins: nothing to rank
 }
 
 // second level, and the zone
@@ -861,27 +928,28 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, lon
     if (st.ended) return;
     const uint32_t* keys = wk.keys + r * wk.vpad;
     const uint32_t prefix = (uint32_t)st.prefix;
-    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) h[i] = 0;
+    const int nbins = 1 << SM_RBITS2, at = 32 - SM_RBITS1 - SM_RBITS2;
+    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) h[i] = 0;
     __syncthreads();
     for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += wk.B * SM_LTPB * 4) {
         const LgVec4<uint32_t> o = *(const LgVec4<uint32_t>*)(keys + i);
 #pragma unroll
-        for (int j = 0; j < 4; j++) if (o.v[j] && (o.v[j] >> 20) == prefix) atomicAdd(&h[(o.v[j] >> 8) & (SM_RBINS - 1)], 1u);
+        for (int j = 0; j < 4; j++)
+            if (o.v[j] && (o.v[j] >> (32 - SM_RBITS1)) == prefix) atomicAdd(&h[sm_slot((int)(o.v[j] >> at) & (nbins - 1), SM_RBITS2 - 6)], 1u);
     }
     __syncthreads();
     uint32_t* g = wk.rbins + r * SM_RBINS;
-    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) if (h[i]) atomicAdd(&g[i], h[i]);
+    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) if (h[i]) atomicAdd(&g[i], h[i]);
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
-    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) h[i] = sm_peek(&g[i]);
+    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) h[i] = sm_peek(&g[i]);
     __syncthreads();
-    unsigned long long before = st.take.before_n, all;
-    const int bin = sm_boundary_counts(h, SM_RBINS, (double)n, before, all, sc);
+    SmTake take = st.take;
+    const SmBin bin = sm_boundary<false>(h, nullptr, nullptr, SM_RBITS2 - 6, take, sc);
     if (threadIdx.x != 0) return;
-    const uint32_t lo = (prefix << 20) | ((uint32_t)(bin < 0 ? 0 : bin) << 8), hi = lo | 0xffu;
-    const float klo = sm_unorder(lo), khi = sm_unorder(hi), slope = sm_slope(rule);
-    st.zone_lo = sm_order(klo - 2.0f * sm_margin(klo, slope));                // losers: ordered key < zone_lo
-    st.zone_hi = sm_order(khi + 2.0f * sm_margin(khi, slope));                // winners: > zone_hi
-    if (st.zone_lo == 0u) st.zone_lo = 1u;
+    const uint32_t lo = (prefix << (32 - SM_RBITS1)) | ((uint32_t)(bin.bin < 0 ? 0 : bin.bin) << at);
+    const SmZone zone = sm_zone(lo, lo | ((1u << at) - 1), sm_slope(rule));
+    st.zone_lo = zone.lo;
+    st.zone_hi = zone.hi;
 }
 
 // winners as a bit per element, the zone's elements as a list, winners counted per tile; the last workgroup ranks the list
@@ -913,7 +981,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
             const long long i = t * SM_TILE + k * SM_LTPB + threadIdx.x;
             const unsigned long long w = __ballot(key[k] > zhi);
             if (lane == 0) { sm_poke(&words[i >> 6], w); c += (uint32_t)__popcll(w); }
-            if (key[k] >= zlo && key[k] <= zhi && key[k] != 0u) {
+            if (key[k] >= zlo && key[k] <= zhi) {
                 const uint32_t at = atomicAdd(&st.candidates, 1u);
                 if (at < (uint32_t)wk.capacity) sm_poke(&list[at], (uint32_t)i);
             }
@@ -962,53 +1030,46 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
         auto key_of = [&](long long a) {
             const long long i = index(a);
             const uint32_t o = keys[i];
-            return o >= zlo && o <= zhi && o != 0u ? race(i) : 0ull;
+            return o >= zlo && o <= zhi ? race(i) : 0ull;
         };
-        SmTake take = { (double)room, 0, { 0, 0 } };
-        unsigned long long prefix = 0, count = 0, thr = 0, ties = 0;
-        bool whole = room == 0;
-        int shift = 64;
-        if (room == 0) thr = ~0ull;
-        while (shift > 0 && !whole) {
-            const int width = shift >= 11 ? 11 : shift, at = shift - width, nbins = 1 << width;
-            __syncthreads();
-            for (int k = threadIdx.x; k < nbins; k += SM_LTPB) h.hist.n[k] = 0;
-            __syncthreads();
-            for (long long a = threadIdx.x; a < m; a += SM_LTPB) {
-                const unsigned long long k = key_of(a);
-                if (k != 0ull && (shift == 64 || (k >> shift) == prefix)) atomicAdd(&h.hist.n[(k >> at) & (unsigned long long)(nbins - 1)], 1u);
-            }
-            __syncthreads();
-            const int bin = sm_boundary<false>(h.hist, nbins, take, sc, count);
-            if (bin < 0) { thr = ~0ull; whole = true; break; }
-            prefix = (prefix << width) | (unsigned)bin;
-            shift = at;
-            thr = prefix << at;
-            whole = sm_whole_bin<false>(take, count);
-        }
-        uint32_t last = SM_ALL;
-        if (!whole) {
-            // the ties-th lowest index among equal keys: the same selection on the (unique) indices, from the top of their complement
-            ties = sm_ties<false>(take, count, 0.0);
-            SmTake by = { (double)ties, 0, { 0, 0 } };
-            unsigned long long p = 0;
-            int s = 32;
-            while (s > 0) {
-                const int width = s >= 11 ? 11 : s, at = s - width, nbins = 1 << width;
+        // one selection of `bits` bits among of(a) != 0: lowest key of the bin it ends in, and that bin
+        auto select = [&](int bits, double target, auto&& of, unsigned long long& thr, SmTake& take) {
+            take = SmTake{ target, 0, { 0, 0 } };
+            SmBin bin = { -1, 0, 0 };
+            unsigned long long prefix = 0;
+            int shift = bits;
+            while (shift > 0) {
+                const int width = shift >= 11 ? 11 : shift < 6 ? 6 : shift, low = shift > width ? shift - width : 0;
                 __syncthreads();
-                for (int k = threadIdx.x; k < nbins; k += SM_LTPB) h.hist.n[k] = 0;
+                for (int k = threadIdx.x; k < 1 << width; k += SM_LTPB) h.hist.n[k] = 0;
                 __syncthreads();
                 for (long long a = threadIdx.x; a < m; a += SM_LTPB) {
-                    const uint32_t o = ~(uint32_t)index(a);
-                    if ((s == 32 || (o >> s) == (uint32_t)p) && key_of(a) == thr) atomicAdd(&h.hist.n[(o >> at) & (uint32_t)(nbins - 1)], 1u);
+                    const unsigned long long k = of(a);
+                    if (k != 0ull && (shift == 64 || (k >> shift) == prefix)) atomicAdd(&h.hist.n[sm_slot((int)((k >> low) & ((1ull << (shift - low)) - 1)), width - 6)], 1u);
                 }
                 __syncthreads();
-                const int bin = sm_boundary<false>(h.hist, nbins, by, sc, count);
-                if (bin < 0) break;                                    // cannot be: ties >= 1 of them exist
-                p = (p << width) | (unsigned)bin;
-                s = at;
+                bin = sm_boundary<false>(h.hist.n, nullptr, nullptr, width - 6, take, sc);
+                if (bin.bin < 0) break;
+                prefix = (prefix << (shift - low)) | (unsigned)bin.bin;
+                shift = low;
+                if (bin.count == 1) break;
             }
-            last = ~(uint32_t)p;
+            thr = prefix << shift;
+            return bin;
+        };
+        unsigned long long thr = ~0ull;
+        uint32_t last = SM_ALL;
+        SmTake take;
+        const SmBin e = room ? select(64, (double)room, key_of, thr, take) : SmBin{ -1, 0, 0 };
+        if (e.bin < 0) thr = ~0ull;
+        else if (e.count > 1) {
+            const uint32_t ties = sm_ties<false>(take, e.count, 0.0);
+            if (ties < e.count) {                                      // the lowest indices among equal keys: selected by the indices' complement
+                unsigned long long cut;
+                const unsigned long long equal = thr;
+                select(32, (double)ties, [&](long long a) { return key_of(a) == equal ? (unsigned long long)~(uint32_t)index(a) : 0ull; }, cut, take);
+                last = ~(uint32_t)cut;
+            }
         }
         __syncthreads();
         for (long long a = threadIdx.x; a < m; a += SM_LTPB) {

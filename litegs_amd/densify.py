@@ -7,6 +7,8 @@ job, every rank must take IDENTICAL clone / split / prune decisions or the repli
 * ``Statistics.all_reduce`` is called first, so the moments equal those of one process that rendered every rank's frames;
 * the two random draws (the multinomial pick of densification candidates and the normal offsets of split children) come from a
   ``Sampler`` seeded by (seed, epoch) only -- parameters are bit-identical across ranks (synchronous updates), so are the draws.
+  ``CounterSampler`` (``DensifyParams.sampler = "counter"``) takes them from the counter-based generator of ``stochastic.py``: any number of
+  Gaussians (``torch.multinomial`` ends at 2^24), candidates in index order, and a pick that can be sharpened or cut off.
 
 Layout: every parameter is [..., chunks, S]; all decisions are taken on the flat [.., N] view and whole chunks are appended /
 removed (the reference's truncation rules: the appended set and the pruned set are cut to a multiple of S, densify.py:153-160,
@@ -39,6 +41,11 @@ class DensifyParams:
     opacity_threshold: float = 0.005
     screen_size_threshold: int = 128
     percent_dense: float = 0.01
+    sampler: str = "torch"                     # 'torch' | 'counter'; the rest applies to 'counter' (stochastic.sample_distinct)
+    sample_temperature: float = 1.0            # candidates are drawn by score ** (1 / temperature)
+    sample_top_k: int = 0                      # among the k best scores
+    sample_top_p: float = 1.0                  # ... that carry this part of the total
+    sample_min_p: float = 0.0                  # ... with at least this part of the best score
 
     def resolve_until(self, total_epochs: int) -> None:
         """trainer.py:103-104: a negative densify_until means 80 % of the run, rounded down to a reset boundary, plus one."""
@@ -63,6 +70,47 @@ class Sampler:
 
     def normal(self, std: torch.Tensor) -> torch.Tensor:
         return torch.normal(mean=torch.zeros_like(std), std=std, generator=self._gen["g"])
+
+
+class CounterSampler(Sampler):
+    """The same draws from ``litegs_amd.stochastic``: functions of (seed, epoch, number of the draw, Gaussian) alone.  Gaussians without a
+    score are never picked; where fewer have one than the budget asks for, all of them are."""
+
+    def __init__(self, seed: int = 0, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
+        super().__init__(seed)
+        self.rule = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        self._draw = 0
+
+    def begin(self, epoch: int, device: torch.device) -> None:
+        self._draw = epoch << 8                                      # one counter per draw of an epoch
+
+    def _next(self) -> int:
+        self._draw += 1
+        return self._draw - 1
+
+    def multinomial(self, score: torch.Tensor, budget: int) -> torch.Tensor:
+        from . import stochastic
+        u = stochastic.uniform(score.shape, self.seed, self._next(), device=score.device)
+        picked = stochastic.sample_distinct(score, u, budget, logits=False, **self.rule)
+        return picked[picked >= 0]
+
+    def normal(self, std: torch.Tensor) -> torch.Tensor:
+        from . import stochastic
+        return stochastic.normal(std, self.seed, self._next())
+
+
+def make_sampler(params, seed: int = 0) -> Sampler:
+    """the sampler that ``params`` names; parameter objects without these fields (the reference's own) get the default one"""
+    plain = DensifyParams()
+    rule = {k: getattr(params, "sample_" + k, getattr(plain, "sample_" + k)) for k in ("temperature", "top_k", "top_p", "min_p")}
+    name = getattr(params, "sampler", plain.sampler)
+    if name == "counter":
+        return CounterSampler(seed, **rule)
+    if name != "torch":
+        raise ValueError(f"DensifyParams.sampler: {name!r} is neither 'torch' nor 'counter'")
+    if any(v != getattr(plain, "sample_" + k) for k, v in rule.items()):
+        raise ValueError("DensifyParams.sample_*: only the 'counter' sampler shapes its draws")
+    return Sampler(seed)
 
 
 def rotation_rows(rot: torch.Tensor) -> torch.Tensor:

@@ -30,6 +30,7 @@ class OptimizationParams:
     lambda_dssim: float = 0.2            # unused by the reference as well (the fused loss fixes 0.8 L1 + 0.2 D-SSIM)
     reg_weight: float = 0.0
     learnable_viewproj: bool = False
+    opacity_dropout: float = 0.0         # part of the Gaussians dropped by each training step (not in the reference; operator path, one GPU)
 
 
 class SparseGaussianAdam(torch.optim.Adam):

@@ -13,6 +13,7 @@ from typing import Optional, Tuple
 
 import torch
 
+from . import stochastic
 from . import wrapper
 from .binding import ops as fused
 from .statistics import STATS
@@ -51,8 +52,11 @@ def get_cluster_AABB(clustered_xyz, clustered_scale, clustered_rot):
 def render_preprocess(cluster_origin: Optional[torch.Tensor], cluster_extend: Optional[torch.Tensor], frustumplane: torch.Tensor,
                       view_matrix: torch.Tensor, xyz: torch.Tensor, scale: torch.Tensor, rot: torch.Tensor, sh_0: torch.Tensor,
                       sh_rest: torch.Tensor, opacity: torch.Tensor, feedback_buffer: Optional[torch.Tensor],
-                      idx_tensor: Optional[torch.Tensor], pp, actived_sh_degree: int):
-    """-> (visible_chunkid, visible_chunks_num, culled_xyz, culled_scale, culled_rot, color, culled_opacity)."""
+                      idx_tensor: Optional[torch.Tensor], pp, actived_sh_degree: int, opacity_dropout: Optional[Tuple[float, int, int]] = None):
+    """-> (visible_chunkid, visible_chunks_num, culled_xyz, culled_scale, culled_rot, color, culled_opacity).
+
+    ``opacity_dropout`` (not in the reference): (p, seed, offset) of ``stochastic.dropout`` on the activated opacities; a Gaussian's decision
+    depends on its place in the whole cloud, not on the chunks that this view keeps.  A dropped Gaussian (opacity 0) emits no tile instances."""
     visible_chunkid = None
     visible_chunks_num = None
     if pp.cluster_size:
@@ -63,6 +67,8 @@ def render_preprocess(cluster_origin: Optional[torch.Tensor], cluster_extend: Op
             STATS.set_compaction(visible_chunkid, visible_chunks_num)
         culled = wrapper.CullCompactActivateWithSparseGrad.apply(pp.sparse_grad, actived_sh_degree, visible_chunkid, visible_chunks_num,
                                                                  view_matrix, xyz, scale, rot, sh_0, sh_rest, opacity)
+        if opacity_dropout is not None:
+            culled = (*culled[:-1], stochastic.dropout(culled[-1], *opacity_dropout, chunk_ids=visible_chunkid))
         culled_xyz, culled_scale, culled_rot, color, culled_opacity = uncluster(*culled)
     else:
         pad_one = torch.ones((1, xyz.shape[-1]), dtype=xyz.dtype, device=xyz.device)
@@ -70,6 +76,8 @@ def render_preprocess(cluster_origin: Optional[torch.Tensor], cluster_extend: Op
         culled_scale = scale.exp()
         culled_rot = torch.nn.functional.normalize(rot, dim=0)
         culled_opacity = opacity.sigmoid()
+        if opacity_dropout is not None:
+            culled_opacity = stochastic.dropout(culled_opacity, *opacity_dropout)
         with torch.no_grad():
             camera_center = (-view_matrix[..., 3:4, :3] @ (view_matrix[..., :3, :3].transpose(-1, -2))).squeeze(1)
             dirs = torch.nn.functional.normalize(culled_xyz[:3] - camera_center.unsqueeze(-1), dim=-2)

@@ -68,6 +68,12 @@ class FrameTrainer:
         # (litegs/training/trainer.py:108: total_epoch = iterations / frames), so training.start sets this to the world size and the
         # position learning rate reaches its final value after the same number of FRAMES as on one GPU
         self.sched_ticks = 1
+        # opacity dropout (stochastic.dropout) of training steps: each step drops this part of the Gaussians and scales the others by
+        # 1 / (1 - p).  Operator path only (fused=False): the native executor activates opacities inside its own kernels.  A step's mask is a
+        # function of (opacity_dropout_seed, training_steps, Gaussian), whichever chunks the frame sees.
+        self.opacity_dropout = 0.0
+        self.opacity_dropout_seed = 0
+        self.training_steps = 0
         self.last = {}
         # speculative culling (csrc/fused.hip): culled steps enqueue no gated repeat; a failed step poisons the Adam launches from there on
         # and is replayed here, unculled, together with the steps enqueued behind it.  Parameters are final only after flush().
@@ -90,7 +96,7 @@ class FrameTrainer:
         self.sanitised = {}               # site -> garbage table words neutralised by a kernel so far (csrc/lg_sanity.h); empty = none
 
     # -------------------------------------------------------------------------------------------
-    def forward(self, frame: Frame, raw: bool = False):
+    def forward(self, frame: Frame, raw: bool = False, training: bool = False):
         xyz, scale, rot, sh_0, sh_rest, opacity = self.params
         STATS.current_frame = int(frame.idx_tensor[0])
         if self.fused:
@@ -99,7 +105,8 @@ class FrameTrainer:
             return img, vis_id, vis_num, None
         vis_id, vis_num, cx, cs, cr, cc, co = R.render_preprocess(
             self.cluster_origin, self.cluster_extend, frame.planes, frame.view, xyz, scale, rot, sh_0, sh_rest, opacity,
-            self.feedback_visible_chunks_num, frame.idx_tensor, self.pp, self.degree)
+            self.feedback_visible_chunks_num, frame.idx_tensor, self.pp, self.degree,
+            (self.opacity_dropout, self.opacity_dropout_seed, self.training_steps) if training and self.opacity_dropout > 0.0 else None)
         valid_length = vis_num * self.pp.cluster_size
         img, trans, depth, normal, prim_vis = R.render(frame.view, frame.proj, cx, cs, cr, cc, co, valid_length,
                                                        self.feedback_binning_allocate_size, frame.idx_tensor, self.degree,
@@ -286,6 +293,8 @@ class FrameTrainer:
     def _step_body(self, frame_index: int, grad_hook=None, hook_slot: int = 0, peer_frames=None):
         frame = self.frames[frame_index % len(self.frames)]
         moments = grad_hook is not None and hasattr(grad_hook, "step") and not callable(grad_hook)
+        if self.opacity_dropout > 0.0 and self.fused:
+            raise RuntimeError("opacity dropout needs the operator path (fused=False)")
         if moments and not (self.fused and self.fuse_adam):
             raise RuntimeError("MomentExchange needs the native executor (fused=True)")
         # gradients are only materialised when something consumes them between backward and the optimizer (gradient-hook DP exchange)
@@ -294,7 +303,8 @@ class FrameTrainer:
         # gradient replicas whenever every consumer of the records folds them: the fused backward + Adam and the moment exchange's
         # compaction (csrc/dp.hip) do
         self.renderer.fold_only_consumer = grad_hook is None or moments
-        img, vis_id, vis_num, prim_vis = self.forward(frame, raw=self.raw_loss)
+        img, vis_id, vis_num, prim_vis = self.forward(frame, raw=self.raw_loss, training=True)
+        self.training_steps += 1
         if self.raw_loss:
             from . import loss_hip
             loss = loss_hip.raster_l1_ssim_loss(img, frame.gt, value_in_backward=True)      # backward() follows at once
@@ -372,7 +382,7 @@ class FrameTrainer:
         from . import densify as D
         dp = params or D.DensifyParams()
         dp.resolve_until(total_epochs)
-        self.controller = D.DensityController(screen_extent, dp, self.S, init_points_num or self.n_chunks * self.S, STATS, D.Sampler(seed), group)
+        self.controller = D.DensityController(screen_extent, dp, self.S, init_points_num or self.n_chunks * self.S, STATS, D.make_sampler(dp, seed), group)
         self.controller.on_change = self._rebind
         STATS.reset(self.n_chunks, self.S, self.controller.is_densify_actived, device=self.device)
         return self.controller

@@ -18,6 +18,8 @@ Differences from the reference, all deliberate:
   ever broadcast.  Frames are grouped into fixed sets of ``world`` (seeded once); the ORDER of the sets is re-drawn every epoch,
   so the exchange's per-set size predictions stay valid.  Only rank 0 writes files and prints;
 * frames are drawn by a seeded permutation per epoch instead of a ``DataLoader(shuffle=True)`` (same distribution, reproducible);
+* ``op.opacity_dropout`` (not in the reference): every training step drops that part of the Gaussians (litegs_amd/stochastic.py), on the
+  operator path; evaluation renders all of them;
 * ``op.learnable_viewproj`` (trainer.py:84-91, 117-123, 158-162, 183-191, 221-222): the cameras are built from their parameters -- the
   frames' COLMAP poses as a sparse ``nn.Embedding`` [frames, 7] (quaternion + translation) and the first camera's 1 / tan(fov_x / 2) --
   by the ``create_viewproj`` operator, ``SparseAdam(lr 1e-4)`` steps the embedding after every iteration, evaluation frames take the
@@ -145,6 +147,12 @@ def start(lp, op, pp, dp, test_epochs: Sequence[int] = (), save_ply: Sequence[in
     if getattr(pp, "enable_transmitance", False):
         raise ValueError("pp.enable_transmitance (transmittance loss term) is not implemented in litegs_amd.training.start")
 
+    drop = float(getattr(op, "opacity_dropout", 0.0) or 0.0)
+    if not 0.0 <= drop < 1.0:
+        raise ValueError("op.opacity_dropout must lie in [0, 1)")
+    if drop > 0.0 and world > 1:
+        raise ValueError("op.opacity_dropout runs on the operator path, which has no moment exchange: one GPU only")
+
     cameras_info, camera_frames, init_xyz, init_color = io_manager.load_colmap_result(lp.source_path, lp.images)
     training_frames, test_frames = split_frames(lp, camera_frames)
     trainingset = data_mod.CameraFrameDataset(cameras_info, training_frames, lp.resolution, device if pp.device_preload else None)
@@ -178,7 +186,10 @@ def start(lp, op, pp, dp, test_epochs: Sequence[int] = (), save_ply: Sequence[in
     cam_state = None
     if getattr(op, "learnable_viewproj", False):
         cam_state = _learnable_cameras(cameras_info, training_frames, test_frames, frames, test_frames_dev, H, W, device)
+    fused = bool(fused) and drop == 0.0               # opacity dropout is a step of the operator path
     trainer = FrameTrainer(params, frames, H, W, opt, sched, pp, sh_degree=0, device=device, fused=fused, extra_slots=len(test_frames_dev))
+    trainer.opacity_dropout, trainer.opacity_dropout_seed = drop, seed
+    trainer.training_steps = start_epoch * len(frames)
 
     total_epoch = int(op.iterations / len(trainingset))
     dp.resolve_until(total_epoch)

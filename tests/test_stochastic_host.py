@@ -95,3 +95,37 @@ def test_c_entry_refuses_bad_dropout_arguments(kw):
 def test_c_entry_refuses_a_bad_draw():
     assert lib().lg_random_draw(None, None, 0, 8, 0, 0, None, None) == INVALID
     assert lib().lg_random_draw(None, 16, 5, 8, 0, 0, None, None) == INVALID
+
+
+# ---- where the framework takes them from ----------------------------------------------------------------------------------------------
+def test_sampler_of_the_density_controller_is_chosen_by_its_parameters():
+    from types import SimpleNamespace
+    from litegs_amd import densify as D
+    assert type(D.make_sampler(D.DensifyParams(), 3)) is D.Sampler and type(D.make_sampler(SimpleNamespace(), 3)) is D.Sampler
+    s = D.make_sampler(D.DensifyParams(sampler="counter", sample_top_p=0.9, sample_temperature=0.5), 3)
+    assert type(s) is D.CounterSampler and s.seed == 3 and s.rule == dict(temperature=0.5, top_k=0, top_p=0.9, min_p=0.0)
+    for bad in (dict(sampler="other"), dict(sample_top_k=5), dict(sample_min_p=0.1), dict(sample_temperature=2.0)):
+        with pytest.raises(ValueError):
+            D.make_sampler(D.DensifyParams(**bad))
+
+
+def test_every_draw_of_a_run_has_a_counter_of_its_own():
+    from litegs_amd import densify as D
+    s, seen = D.CounterSampler(1), []
+    for epoch in range(3):
+        s.begin(epoch, torch.device("cpu"))
+        seen += [s._next() for _ in range(4)]
+    assert len(set(seen)) == len(seen)
+    s.begin(1, torch.device("cpu"))
+    assert s._next() == seen[4]                                      # ... and a repeated epoch the same ones
+
+
+def test_command_line_carries_the_options():
+    from argparse import ArgumentParser
+    from litegs_amd import arguments as A
+    parser = ArgumentParser()
+    A.add_cmdline_args(parser)
+    _, op, _, dp = A.extract(parser.parse_args(["--opacity_dropout", "0.1", "--sampler", "counter", "--sample_top_p", "0.95", "--sample_top_k", "7"]))
+    assert op.opacity_dropout == 0.1 and (dp.sampler, dp.sample_top_p, dp.sample_top_k) == ("counter", 0.95, 7)
+    _, op, _, dp = A.extract(parser.parse_args([]))
+    assert op.opacity_dropout == 0.0 and dp.sampler == "torch"

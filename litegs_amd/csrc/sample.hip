@@ -9,7 +9,7 @@
 //   without:             the n largest l_i - log(-log(1 - u_i)), in index order
 //
 // All masses, sums and keys are in 64 bits: an index has to be the same as the definition's however many categories there are.  Masses that
-// are added by atomics (top-p's histograms) are added as integers (two 64-bit limbs of 32 fraction bits each, relative to the largest mass),
+// are added by atomics (top-p's histograms) are added as integers (two 64-bit limbs of 31 and 32 fraction bits, relative to the largest mass),
 // so that neither their order nor the launch changes a result; floating sums have one fixed order.
 #include "lg_common.h"
 #include "lg_types.h"
@@ -18,6 +18,7 @@
 
 #define SM_BINS 2048                   // bins of one level of a radix selection
 #define SM_MAX_WAVES 16
+#define SM_SHORT 15360                 // longest row of one workgroup: 960 threads of 16 elements, whose masses and a histogram fill the LDS
 
 enum { SM_LOGITS = 0, SM_LINEAR = 1, SM_POWER = 2 };
 
@@ -43,6 +44,48 @@ __device__ __forceinline__ double sm_value(uint32_t key)
     return (double)__uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 
+// exp(x) for x <= 0 and log(x) for x > 0 in 64 bits, without the general functions' special cases (which cost as much again, and registers):
+// x = n ln 2 + r with |r| <= ln 2 / 2 and the Taylor polynomial of degree 13 (first term left out < 5e-18);  x = 2^e m with m in
+// [sqrt(1/2), sqrt(2)), log m = 2 atanh(s), s = (m - 1) / (m + 1), |s| < 0.172, eleven terms behind the first (next: 4e-19).  ln 2 in two
+// parts, the first of 32 bits so that its products with n are exact.  Good to about one step.
+__device__ __forceinline__ double sm_exp(double x)
+{
+    x = fmax(x, -800.0);                                               // (below 2^-1074 all is 0)
+    const double n = rint(x * 1.4426950408889634);
+    const double r = fma(n, -1.90821492927058770e-10, fma(n, -6.93147180369123816e-01, x));
+    double p = fma(r, 1.6059043836821613e-10, 2.08767569878681e-09);
+    p = fma(r, p, 2.505210838544172e-08);
+    p = fma(r, p, 2.755731922398589e-07);
+    p = fma(r, p, 2.7557319223985893e-06);
+    p = fma(r, p, 2.48015873015873e-05);
+    p = fma(r, p, 0.0001984126984126984);
+    p = fma(r, p, 0.001388888888888889);
+    p = fma(r, p, 0.008333333333333333);
+    p = fma(r, p, 0.041666666666666664);
+    p = fma(r, p, 0.16666666666666666);
+    p = fma(r, p, 0.5);
+    return ldexp(fma(r * r, p, r) + 1.0, (int)n);
+}
+__device__ __forceinline__ double sm_ln(double x)
+{
+    int e = __builtin_amdgcn_frexp_exp(x);
+    double m = __builtin_amdgcn_frexp_mant(x);                          // [1/2, 1)
+    if (m < 0.70710678118654752) { m *= 2.0; e -= 1; }
+    const double f = m - 1.0, s = f / (m + 1.0), z = s * s;
+    double p = fma(z, 1.0 / 23, 1.0 / 21);
+    p = fma(z, p, 1.0 / 19);
+    p = fma(z, p, 1.0 / 17);
+    p = fma(z, p, 1.0 / 15);
+    p = fma(z, p, 1.0 / 13);
+    p = fma(z, p, 1.0 / 11);
+    p = fma(z, p, 1.0 / 9);
+    p = fma(z, p, 1.0 / 7);
+    p = fma(z, p, 1.0 / 5);
+    p = fma(z, p, 1.0 / 3);
+    const double n = (double)e;
+    return fma(n, 6.93147180369123816e-01, fma(n, 1.90821492927058770e-10, 2.0 * fma(s * z, p, s)));
+}
+
 struct SmScale { int mode; double inv_t, top /*l of the best score, or its weight*/, shift /*power of two that brings a linear weight below one*/; };
 
 __device__ __forceinline__ SmScale sm_scale(const SmRule& r, uint32_t best)
@@ -51,19 +94,19 @@ __device__ __forceinline__ SmScale sm_scale(const SmRule& r, uint32_t best)
     if (best == 0u) return s;
     const double x = sm_value(best);
     if (r.mode == SM_LOGITS) s.top = x * s.inv_t;
-    else if (r.mode == SM_POWER) s.top = log(x) * s.inv_t;
+    else if (r.mode == SM_POWER) s.top = sm_ln(x) * s.inv_t;
     else { s.top = x; s.shift = ldexp(1.0, -ilogb(x) - 1); }
     return s;
 }
 __device__ __forceinline__ double sm_log(const SmScale& s, uint32_t key)
 {
     const double x = sm_value(key);
-    return s.mode == SM_LOGITS ? x * s.inv_t : s.mode == SM_POWER ? log(x) * s.inv_t : log(x);
+    return s.mode == SM_LOGITS ? x * s.inv_t : s.mode == SM_POWER ? sm_ln(x) * s.inv_t : sm_ln(x);
 }
 __device__ __forceinline__ double sm_mass(const SmScale& s, uint32_t key)
 {
     if (key == 0u) return 0.0;
-    return s.mode == SM_LINEAR ? sm_value(key) : exp(sm_log(s, key) - s.top);
+    return s.mode == SM_LINEAR ? sm_value(key) : sm_exp(sm_log(s, key) - s.top);
 }
 // key of the exponential race, ordered as an unsigned integer; 0 = excluded
 __device__ __forceinline__ unsigned long long sm_race(const SmScale& s, uint32_t key, float u)
@@ -76,17 +119,18 @@ __device__ __forceinline__ unsigned long long sm_race(const SmScale& s, uint32_t
 }
 
 // ---- sums of masses that do not depend on their order --------------------------------------------------------------------------------
-struct SmSum { unsigned long long hi, lo; };                           // (hi + lo / 2^32) / 2^32, both limbs carry-free up to 2^31 terms
-__device__ __forceinline__ SmSum sm_limbs(double m)                    // 0 <= m <= 1
+struct SmSum { unsigned long long hi, lo; };                           // (hi + lo / 2^32) / 2^31, both limbs carry-free up to 2^31 terms
+struct SmLimbs { uint32_t hi, lo; };
+__device__ __forceinline__ SmLimbs sm_limbs(double m)                  // 0 <= m <= 1
 {
-    const double a = m * 4294967296.0;
-    const unsigned long long hi = (unsigned long long)a;
-    return SmSum{ hi, (unsigned long long)((a - (double)hi) * 4294967296.0) };
+    const double a = m * 0x1p31;
+    const uint32_t hi = (uint32_t)a;
+    return SmLimbs{ hi, (uint32_t)((a - (double)hi) * 0x1p32) };
 }
 __device__ __forceinline__ double sm_sum_value(SmSum s)
 {
     const unsigned long long hi = s.hi + (s.lo >> 32), lo = s.lo & 0xffffffffull;
-    return (double)hi * 0x1p-32 + (double)lo * 0x1p-64;
+    return (double)hi * 0x1p-31 + (double)lo * 0x1p-63;
 }
 
 // ---- scans of a wave and of a workgroup, in one fixed order ----------------------------------------------------------------------------
@@ -162,7 +206,10 @@ template <typename V> __device__ __forceinline__ V sm_block_max(V v, void* lds)
 
 // ---- radix selection: histograms of one level, and the bin in which the selection ends -------------------------------------------------
 // Bin b of 64 * 2^p lies at sm_slot(b, p): the 2^p bins of one lane of the wave that walks them lie 64 apart.
+// A row of one workgroup keeps the counts above bit 48 of the low limb's sums (at most SM_SHORT terms: 46 bits), one atomic less an element.
 struct SmHist { uint32_t n[SM_BINS]; unsigned long long hi[SM_BINS], lo[SM_BINS]; };
+union SmShortHist { uint32_t n[SM_BINS]; struct { unsigned long long hi[SM_BINS], lo[SM_BINS]; }; };
+#define SM_PACK 48
 __device__ __forceinline__ int sm_slot(int b, int p) { return ((b & ((1 << p) - 1)) << 6) | (b >> p); }
 
 // An element is taken while what lies before it (best first) is less than the target, counted in elements or in mass.
@@ -177,16 +224,19 @@ template <bool MASS> __device__ __forceinline__ bool sm_room(const SmTake& t, ui
 // The lowest non-empty bin whose predecessors (the bins above it) leave room: a wave sums 2^p bins a lane, best first, scans, and does the
 // same once more inside the lane it ends in.  Updates take.before_* to the amount above that bin; bin -1: there is none.  All threads call it
 // behind a barrier; a barrier has to follow before the histogram or sc is written again.
-template <bool MASS> __device__ SmBin sm_boundary(const uint32_t* hn, const unsigned long long* hhi, const unsigned long long* hlo, int p, SmTake& take, SmScratch& sc)
+template <bool MASS, bool PACKED = false>
+__device__ SmBin sm_boundary(const uint32_t* hn, const unsigned long long* hhi, const unsigned long long* hlo, int p, SmTake& take, SmScratch& sc)
 {
+    const unsigned long long low = PACKED ? (1ull << SM_PACK) - 1 : ~0ull;
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x, per = 1 << p;
         uint32_t n = 0;
         unsigned long long hi = 0, lo = 0;
+#pragma unroll 8
         for (int k = 0; k < per; k++) {
             const int at = (k << 6) | (63 - lane);
-            n += hn[at];
-            if (MASS) { hi += hhi[at]; lo += hlo[at]; }
+            if (!PACKED) n += hn[at];
+            if (MASS) { const unsigned long long v = hlo[at]; hi += hhi[at]; lo += v & low; if (PACKED) n += (uint32_t)(v >> SM_PACK); }
         }
         const uint32_t in = sm_wave_scan<false>(n, SmAdd());
         unsigned long long ihi = 0, ilo = 0;
@@ -201,9 +251,12 @@ template <bool MASS> __device__ SmBin sm_boundary(const uint32_t* hn, const unsi
             bn += sm_lane(in - n, l);
             if (MASS) { bm.hi += sm_lane(ihi - hi, l); bm.lo += sm_lane(ilo - lo, l); }
             const int at = ((per - 1 - lane) << 6) | (63 - l);
-            const uint32_t n2 = lane < per ? hn[at] : 0u;
+            uint32_t n2 = 0;
             unsigned long long hi2 = 0, lo2 = 0, ihi2 = 0, ilo2 = 0;
-            if (MASS && lane < per) { hi2 = hhi[at]; lo2 = hlo[at]; }
+            if (lane < per) {
+                if (!PACKED) n2 = hn[at];
+                if (MASS) { hi2 = hhi[at]; lo2 = hlo[at] & low; if (PACKED) n2 = (uint32_t)(hlo[at] >> SM_PACK); }
+            }
             const uint32_t in2 = sm_wave_scan<false>(n2, SmAdd());
             if (MASS) { ihi2 = sm_wave_scan<false>(hi2, SmAdd()); ilo2 = sm_wave_scan<false>(lo2, SmAdd()); }
             const SmTake inner = { take.target, bn, bm };
@@ -235,7 +288,8 @@ template <bool MASS> __device__ __forceinline__ uint32_t sm_ties(const SmTake& t
         const double left = take.target - (double)take.before_n;
         return left >= (double)count ? count : (uint32_t)ceil(left);
     }
-    const SmSum one = sm_limbs(mass);
+    const SmLimbs l = sm_limbs(mass);
+    const SmSum one = { l.hi, l.lo };
     uint32_t lo = 1, hi = count;                                       // the first j (from 0) that finds no room
     while (lo < hi) {
         const uint32_t mid = lo + (hi - lo) / 2;
@@ -322,10 +376,11 @@ __device__ __attribute__((noinline)) double sm_mass_call(SmScale s, uint32_t key
 __device__ __attribute__((noinline)) unsigned long long sm_race_call(SmScale s, uint32_t key, float u) { return sm_race(s, key, u); }
 
 // ---- short rows: one workgroup per row, EPT consecutive elements of a thread in registers ----------------------------------------------
-// key[k] is the key of element threadIdx.x * EPT + k, 0: not a candidate.  Ends when the boundary bin holds at most `small` elements:
+// key(k) is the key of element threadIdx.x * EPT + k, 0: not a candidate.  Ends when the boundary bin holds at most `small` elements:
 // [lo, hi] is then the bin's range of keys, take.before_* what lies above it, and the result its count and the number of candidates.
-template <bool MASS, int BITS, int EPT, typename Word, typename Mass>
-__device__ SmBin sm_select_short(const Word (&key)[EPT], const Mass& mass_of, SmTake& take, uint32_t small, SmHist& h, SmScratch& sc, Word& lo, Word& hi)
+template <bool MASS, int BITS, int TPB, int EPT, typename Word, typename Key>
+__device__ SmBin sm_select_short(const Key& key, const double* mass /*LDS, [EPT][TPB], at most one each*/, SmTake& take, uint32_t small, SmShortHist& h, SmScratch& sc,
+                                 Word& lo, Word& hi)
 {
     Word prefix = 0;
     int shift = BITS;
@@ -334,21 +389,21 @@ __device__ SmBin sm_select_short(const Word (&key)[EPT], const Mass& mass_of, Sm
     while (shift > 0) {
         const int width = shift >= 11 ? 11 : shift < 6 ? 6 : shift, at = shift > width ? shift - width : 0, p = width - 6;
         __syncthreads();
-        for (int i = threadIdx.x; i < 1 << width; i += blockDim.x) { h.n[i] = 0; if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } }
+        for (int i = threadIdx.x; i < 1 << width; i += TPB) { if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } else h.n[i] = 0; }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
-            if (key[k] == 0 || (shift < BITS && (key[k] >> shift) != prefix)) continue;
-            const int i = sm_slot((int)((key[k] >> at) & (((Word)1 << (shift - at)) - 1)), p);
-            atomicAdd(&h.n[i], 1u);
+            const Word w = key(k);
+            if (w == 0 || (shift < BITS && (w >> shift) != prefix)) continue;
+            const int i = sm_slot((int)((w >> at) & (((Word)1 << (shift - at)) - 1)), p);
             if (MASS) {
-                const SmSum m = sm_limbs(mass_of(key[k]));
-                if (m.hi) atomicAdd(&h.hi[i], m.hi);
-                if (m.lo) atomicAdd(&h.lo[i], m.lo);
-            }
+                const SmLimbs m = sm_limbs(mass[k * TPB + threadIdx.x]);
+                if (m.hi) atomicAdd(&h.hi[i], (unsigned long long)m.hi);
+                atomicAdd(&h.lo[i], (unsigned long long)m.lo | 1ull << SM_PACK);
+            } else atomicAdd(&h.n[i], 1u);
         }
         __syncthreads();
-        b = sm_boundary<MASS>(h.n, h.hi, h.lo, p, take, sc);
+        b = sm_boundary<MASS, MASS>(h.n, h.hi, h.lo, p, take, sc);
         if (shift == BITS) candidates = b.total;
         if (b.bin < 0) break;                                          // no candidate at all
         prefix = (Word)(prefix << (shift - at)) | (Word)b.bin;
@@ -392,7 +447,8 @@ template <typename T, int TPB, int EPT, bool DISTINCT>
 __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                             int V, long long n, SmRule rule, long long* __restrict__ out)
 {
-    __shared__ union { SmHist hist; double cdf[DISTINCT ? 1 : TPB * EPT]; struct { unsigned long long rank[SM_BINS]; uint32_t index[SM_BINS]; } zone; } h;
+    __shared__ double mass[TPB * EPT];                                 // element k of thread t at k * TPB + t; at the end the cumulative ones
+    __shared__ union { SmShortHist hist; struct { unsigned long long rank[SM_BINS]; uint32_t index[SM_BINS]; } zone; } h;
     __shared__ uint32_t won[DISTINCT ? TPB * EPT / 32 : 1];
     __shared__ uint16_t pos[DISTINCT ? 1 : TPB];
     __shared__ SmScratch sc;
@@ -405,11 +461,6 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     uint32_t key[EPT], best = 0;
 #pragma unroll
     for (int k = 0; k < EPT; k += 4) sm_load4(x, i0 + k, V, sm_aligned(x), logits, key + k);
-    float uk[EPT];
-    if (DISTINCT) {
-#pragma unroll
-        for (int k = 0; k < EPT; k++) uk[k] = i0 + k < V ? u[i0 + k] : 0.0f;
-    }
 #pragma unroll
     for (int k = 0; k < EPT; k++) best = key[k] > best ? key[k] : best;
     best = sm_block_max(best, sc.a);
@@ -418,8 +469,12 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         return;
     }
     const SmScale scale = sm_scale(rule, best);
+    // masses, once: linear ones by a power of two below one
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
-    auto mass_of = [&](uint32_t k) { return sm_mass_call(scale, k) * unit; };
+    auto masses = [&]() {
+#pragma unroll
+        for (int k = 0; k < EPT; k++) mass[k * TPB + threadIdx.x] = sm_mass_call(scale, key[k]) * unit;
+    };
     // filters: an element that one of them drops becomes key 0
     for (int pass = 0; pass < 2; pass++) {
         SmTake take = { 0.0, 0, { 0, 0 } };
@@ -428,21 +483,21 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         if (pass == 0) {
             if (rule.top_k <= 0 || rule.top_k >= V) continue;
             take.target = (double)rule.top_k;
-            bin = sm_select_short<false, 32, EPT, uint32_t>(key, mass_of, take, 1, h.hist, sc, lo, hi);
+            bin = sm_select_short<false, 32, TPB, EPT, uint32_t>([&](int k) { return key[k]; }, nullptr, take, 1, h.hist, sc, lo, hi);
         } else {
             if (rule.top_p >= 1.0) continue;
             SmSum mine = { 0, 0 }, total;
+            masses();
 #pragma unroll
-            for (int k = 0; k < EPT; k++)
-                if (key[k]) { const SmSum m = sm_limbs(mass_of(key[k])); mine.hi += m.hi; mine.lo += m.lo; }
+            for (int k = 0; k < EPT; k++) { const SmLimbs m = sm_limbs(mass[k * TPB + threadIdx.x]); mine.hi += m.hi; mine.lo += m.lo; }
             sm_block_scan<unsigned long long>(mine.hi, sc.a, total.hi);
             sm_block_scan<unsigned long long>(mine.lo, sc.b, total.lo);
             take.target = rule.top_p * sm_sum_value(total);
-            bin = sm_select_short<true, 32, EPT, uint32_t>(key, mass_of, take, 1, h.hist, sc, lo, hi);
+            bin = sm_select_short<true, 32, TPB, EPT, uint32_t>([&](int k) { return key[k]; }, mass, take, 1, h.hist, sc, lo, hi);
         }
         // a bin of one element is taken whole; one of equal elements up to the cut
         SmKept kept = { lo, SM_ALL };
-        const uint32_t ties = bin.count == 1 ? 1 : pass == 0 ? sm_ties<false>(take, bin.count, 0.0) : sm_ties<true>(take, bin.count, mass_of(lo));
+        const uint32_t ties = bin.count == 1 ? 1 : pass == 0 ? sm_ties<false>(take, bin.count, 0.0) : sm_ties<true>(take, bin.count, sm_mass_call(scale, lo) * unit);
         if (ties < bin.count) {
             bool tie[EPT];
 #pragma unroll
@@ -462,9 +517,11 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         uint32_t race[EPT], lo, hi, wins = 0;
         const float slope = sm_slope(rule);
 #pragma unroll
-        for (int k = 0; k < EPT; k++) race[k] = sm_race32(logits, slope, key[k], uk[k]);
+        for (int k = 0; k < EPT; k++) race[k] = __float_as_uint(key[k] ? u[i0 + k] : 0.0f);        // (loads first; key 0 behind V)
+#pragma unroll
+        for (int k = 0; k < EPT; k++) race[k] = sm_race32(logits, slope, key[k], __uint_as_float(race[k]));
         SmTake take = { (double)n, 0, { 0, 0 } };
-        const SmBin bin = sm_select_short<false, 32, EPT, uint32_t>(race, [](uint32_t) { return 0.0; }, take, 16, h.hist, sc, lo, hi);
+        const SmBin bin = sm_select_short<false, 32, TPB, EPT, uint32_t>([&](int k) { return race[k]; }, nullptr, take, 16, h.hist, sc, lo, hi);
         SmZone zone = { 1u, 0u };                                      // nothing to rank where everything wins
         if (bin.total > n) zone = sm_zone(lo, hi, slope);
         __syncthreads();
@@ -499,23 +556,25 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             wins |= (won[i0 >> 5] >> (i0 & 31)) & ((1u << EPT) - 1);
         } else {
             // many elements next to the border (equal numbers, or a slope that spreads nothing): radix selection of their exact keys
-            unsigned long long exact[EPT], elo, ehi;
+            unsigned long long *mine = (unsigned long long*)mass + threadIdx.x, elo, ehi;        // (the masses are done)
 #pragma unroll
-            for (int k = 0; k < EPT; k++) exact[k] = race[k] >= zone.lo && race[k] <= zone.hi ? sm_race_call(scale, key[k], uk[k]) : 0ull;
+            for (int k = 0; k < EPT; k++) mine[k * TPB] = race[k] >= zone.lo && race[k] <= zone.hi ? sm_race_call(scale, key[k], u[i0 + k]) : 0ull;
             SmTake left = { (double)room, 0, { 0, 0 } };
-            const SmBin e = sm_select_short<false, 64, EPT, unsigned long long>(exact, [](unsigned long long) { return 0.0; }, left, 1, h.hist, sc, elo, ehi);
+            const SmBin e = sm_select_short<false, 64, TPB, EPT, unsigned long long>([&](int k) { return mine[k * TPB]; }, nullptr, left, 1, h.hist, sc, elo, ehi);
             const uint32_t ties = e.bin < 0 ? 0 : e.count == 1 ? 1 : sm_ties<false>(left, e.count, 0.0);
             uint32_t last = SM_ALL;
             if (ties < e.count) {
                 bool tie[EPT];
 #pragma unroll
-                for (int k = 0; k < EPT; k++) tie[k] = exact[k] == elo;
+                for (int k = 0; k < EPT; k++) tie[k] = mine[k * TPB] == elo;
                 last = sm_nth_short<EPT>(tie, ties, sc);
             }
             if (e.bin >= 0)
 #pragma unroll
-                for (int k = 0; k < EPT; k++)
-                    if (exact[k] != 0 && (exact[k] > elo || (exact[k] == elo && (uint32_t)(i0 + k) <= last))) wins |= 1u << k;
+                for (int k = 0; k < EPT; k++) {
+                    const unsigned long long w = mine[k * TPB];
+                    if (w != 0 && (w > elo || (w == elo && (uint32_t)(i0 + k) <= last))) wins |= 1u << k;
+                }
         }
         uint32_t total;
         long long at = sm_block_scan<uint32_t>(__popc(wins), sc.a, total);
@@ -523,26 +582,26 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         for (int k = 0; k < EPT; k++) if ((wins >> k) & 1) out[at++] = i0 + k;
         for (long long j = (long long)total + threadIdx.x; j < n; j += TPB) out[j] = -1;
     } else {
-        double* cdf = h.cdf;                                           // the histograms are done
-        double w[EPT], sum = 0.0, total;
+        double sum = 0.0, total;
         uint32_t positive = 0, last = 0;
+        if (rule.top_p >= 1.0) masses();
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
-            w[k] = sm_mass_call(scale, key[k]);
-            sum += w[k];
-            if (w[k] > 0.0) { positive |= 1u << k; last = (uint32_t)(i0 + k) + 1; }
+            const double m = key[k] ? mass[k * TPB + threadIdx.x] : 0.0;
+            sum += m;
+            if (m > 0.0) { positive |= 1u << k; last = (uint32_t)(i0 + k) + 1; }
         }
         double at = sm_block_scan<double>(sum, sc.a, total);
         last = sm_block_max(last, sc.b);
 #pragma unroll
-        for (int k = 0; k < EPT; k++) { at += w[k]; cdf[i0 + k] = at; }
+        for (int k = 0; k < EPT; k++) { if (key[k]) at += mass[k * TPB + threadIdx.x]; mass[k * TPB + threadIdx.x] = at; }
         pos[threadIdx.x] = (uint16_t)positive;
         __syncthreads();
         for (long long j = threadIdx.x; j < n; j += TPB) {
             const float uj = u[j];
             const double t = (uj > 0.0f ? (double)uj : 0.0) * total;
             uint32_t lo = 0, hi = last - 1;                            // first element whose sum passes t; at the end the last one with a mass
-            while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (cdf[mid] > t) hi = mid; else lo = mid + 1; }
+            while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (mass[mid % EPT * TPB + mid / EPT] > t) hi = mid; else lo = mid + 1; }
             while (lo < last - 1 && !((pos[lo / EPT] >> (lo % EPT)) & 1)) lo++;      // rounding at a border never lands on a masked element
             out[j] = lo;
         }
@@ -647,9 +706,9 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
             const int bin = sm_slot((int)(key[j] >> at) & (nbins - 1), p);
             atomicAdd(&h.n[bin], 1u);
             if (MASS) {
-                const SmSum m = sm_limbs(sm_mass(scale, key[j]) * unit);
-                if (m.hi) atomicAdd(&h.hi[bin], m.hi);
-                if (m.lo) atomicAdd(&h.lo[bin], m.lo);
+                const SmLimbs m = sm_limbs(sm_mass(scale, key[j]) * unit);
+                if (m.hi) atomicAdd(&h.hi[bin], (unsigned long long)m.hi);
+                if (m.lo) atomicAdd(&h.lo[bin], (unsigned long long)m.lo);
             }
         }
     }
@@ -1122,7 +1181,6 @@ static bool sm_rule(int logits, double temperature, long long top_k, double top_
     return true;
 }
 
-#define SM_SHORT 16384                 // longest row of the one-workgroup kernels
 
 // lays the workspace out; returns its size in bytes.  The cleared part (states, histograms) comes first.
 static long long sm_layout(long long R, long long V, bool distinct, char* base, SmWork& w, long long& clear_bytes)
@@ -1166,7 +1224,7 @@ static int sample_launch(const T* scores, long long ss, const float* u, long lon
         } while (0)
         if (V <= 1024) SM_LAUNCH_SHORT(256, 4);
         else if (V <= 4096) SM_LAUNCH_SHORT(1024, 4);
-        else SM_LAUNCH_SHORT(1024, 16);
+        else SM_LAUNCH_SHORT(960, 16);
 #undef SM_LAUNCH_SHORT
         LG_RETURN_LAST();
     }

@@ -425,7 +425,7 @@ int lg_permute_columns(const float* src, const int32_t* order, long long rows, l
 int lg_dropout(const void* x, void* y, int dtype, long long lead, long long M, double p, long long seed, long long offset,
                const int64_t* offset_dev, const int64_t* chunk_ids, int S, void* stream);
 int lg_random_draw(const void* std_, void* out, int dtype, long long n, long long seed, long long offset, const int64_t* offset_dev, void* stream);
-long long lg_sample_temp_bytes(long long R, long long V, long long n, int distinct);
+long long lg_sample_temp_bytes(long long R, long long V, long long n, int dtype, int distinct, long long top_k, double top_p);
 int lg_sample(const void* scores, int dtype, long long score_stride, const float* u, long long u_stride, long long R, long long V,
               long long n, int distinct, int logits, double temperature, long long top_k, double top_p, double min_p,
               int64_t* out, void* temp, long long temp_bytes, void* stream);

@@ -69,7 +69,7 @@ void sample(const Tensor& scores, const Tensor& u, Tensor out, int64_t n, bool d
 {
     const c10::OptionalDeviceGuard guard(at::device_of(scores));
     const int64_t R = scores.size(0), V = scores.size(1);
-    const long long bytes = lg_sample_temp_bytes(R, V, n, distinct);
+    const long long bytes = lg_sample_temp_bytes(R, V, n, dtype_code(scores, "sample"), distinct, top_k, top_p);
     Tensor temp;
     if (bytes) temp = at::empty({ bytes }, scores.options().dtype(at::kByte));
     check(lg_sample(scores.data_ptr(), dtype_code(scores, "sample"), scores.stride(0), (const float*)u.data_ptr(), u.stride(0), R, V, n, distinct, logits, temperature, top_k,

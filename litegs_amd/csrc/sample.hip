@@ -197,6 +197,13 @@ __device__ __forceinline__ double sm_block_rise(double v, void* lds, double& tot
     double before;
     return sm_block_op(v, SmMaxOf(), lds, before, total);
 }
+__device__ __forceinline__ double sm_block_rise_before(double v, void* lds, double& total)       // ... up to the thread before this one
+{
+    double before;
+    const double inc = sm_block_op(v, SmMaxOf(), lds, before, total);
+    const double prev = sm_dpp<0x138, 0xf>(inc);                       // one lane up; lane 0: 0
+    return fmax(before, prev);
+}
 template <typename V> __device__ __forceinline__ V sm_block_max(V v, void* lds)
 {
     V before, total;
@@ -429,23 +436,21 @@ template <int EPT> __device__ uint32_t sm_nth_short(const bool (&flag)[EPT], uin
     return (uint32_t)sc.word[0];
 }
 
-// four consecutive scores from i on as keys; beyond V: 0
-template <typename T> __device__ __forceinline__ void sm_load4(const T* x, long long i, long long V, bool vec, bool logits, uint32_t* key)
+// four consecutive scores from i on; what lies behind V is NaN, which is never drawn
+template <typename T> __device__ __forceinline__ LgVec4<T> sm_load4(const T* x, long long i, long long V, bool vec)
 {
-    if (vec && i + 4 <= V) {
-        const LgVec4<T> v = *(const LgVec4<T>*)(x + i);
+    if (vec && i + 4 <= V) return *(const LgVec4<T>*)(x + i);
+    LgVec4<T> v;
 #pragma unroll
-        for (int k = 0; k < 4; k++) key[k] = sm_key(v.v[k], logits);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++) key[k] = i + k < V ? sm_key(x[i + k], logits) : 0u;
-    }
+    for (int k = 0; k < 4; k++) v.v[k] = i + k < V ? x[i + k] : lg_from_float<T>(__uint_as_float(0x7fc00000u));
+    return v;
 }
 template <typename T> __device__ __forceinline__ bool sm_aligned(const T* x) { return (uintptr_t)x % (4 * sizeof(T)) == 0; }
 
 template <typename T, int TPB, int EPT, bool DISTINCT>
 __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
-                                                            int V, long long n, SmRule rule, long long* __restrict__ out)
+                                                            int V, long long n, SmRule rule, const uint32_t* __restrict__ names /*nullable [R, V]*/,
+                                                            long long* __restrict__ out)
 {
     __shared__ double mass[TPB * EPT];                                 // element k of thread t at k * TPB + t; at the end the cumulative ones
     __shared__ union { SmShortHist hist; struct { unsigned long long rank[SM_BINS]; uint32_t index[SM_BINS]; } zone; } h;
@@ -457,15 +462,21 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     const bool logits = rule.mode == SM_LOGITS;
     u += r * ustride;
     out += r * n;
+    if (names) names += r * V;
+    auto name = [&](uint32_t i) { return names ? (long long)names[i] : (long long)i; };          // of element i, where the row is what a filter left
     const int i0 = threadIdx.x * EPT;
     uint32_t key[EPT], best = 0;
 #pragma unroll
-    for (int k = 0; k < EPT; k += 4) sm_load4(x, i0 + k, V, sm_aligned(x), logits, key + k);
+    for (int k = 0; k < EPT; k += 4) {
+        const LgVec4<T> v = sm_load4(x, i0 + k, V, sm_aligned(x));
+#pragma unroll
+        for (int j = 0; j < 4; j++) key[k + j] = sm_key(v.v[j], logits);
+    }
 #pragma unroll
     for (int k = 0; k < EPT; k++) best = key[k] > best ? key[k] : best;
     best = sm_block_max(best, sc.a);
     if (best == 0) {                                                   // nothing to draw from
-        for (long long j = threadIdx.x; j < n; j += blockDim.x) out[j] = -1;
+        for (long long j = (long long)blockIdx.y * TPB + threadIdx.x; j < n; j += (long long)gridDim.y * TPB) out[j] = -1;
         return;
     }
     const SmScale scale = sm_scale(rule, best);
@@ -579,7 +590,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         uint32_t total;
         long long at = sm_block_scan<uint32_t>(__popc(wins), sc.a, total);
 #pragma unroll
-        for (int k = 0; k < EPT; k++) if ((wins >> k) & 1) out[at++] = i0 + k;
+        for (int k = 0; k < EPT; k++) if ((wins >> k) & 1) out[at++] = name(i0 + k);
         for (long long j = (long long)total + threadIdx.x; j < n; j += TPB) out[j] = -1;
     } else {
         double sum = 0.0, total;
@@ -597,13 +608,13 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         for (int k = 0; k < EPT; k++) { if (key[k]) at += mass[k * TPB + threadIdx.x]; mass[k * TPB + threadIdx.x] = at; }
         pos[threadIdx.x] = (uint16_t)positive;
         __syncthreads();
-        for (long long j = threadIdx.x; j < n; j += TPB) {
+        for (long long j = (long long)blockIdx.y * TPB + threadIdx.x; j < n; j += (long long)gridDim.y * TPB) {         // (blockIdx.y: its share of the draws)
             const float uj = u[j];
             const double t = (uj > 0.0f ? (double)uj : 0.0) * total;
             uint32_t lo = 0, hi = last - 1;                            // first element whose sum passes t; at the end the last one with a mass
             while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (mass[mid % EPT * TPB + mid / EPT] > t) hi = mid; else lo = mid + 1; }
             while (lo < last - 1 && !((pos[lo / EPT] >> (lo % EPT)) & 1)) lo++;      // rounding at a border never lands on a masked element
-            out[j] = lo;
+            out[j] = name(lo);
         }
     }
 }
@@ -623,60 +634,84 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
 struct SmRowState {
     SmKept kept, before;               // what passes the filters; ... before the selection under way
     SmTake take;
-    unsigned long long prefix, count, ties;
-    double total, top;                 // sample: total mass of the kept; the largest l
-    unsigned long long sure;           // race: winners outside the zone
-    uint32_t best, ended, cut, zone_lo, zone_hi, candidates;
+    double total, top;                 // with replacement: total mass of the kept; the largest l
+    unsigned long long sure;           // race: winners
+    uint32_t prefix, ties, best, ended, cut, zone_lo, zone_hi, candidates;
     uint32_t ticket[SM_STEPS];
 };
 
-struct SmWork {                        // workspace of a call: everything per row
-    SmRowState* state; SmHist* hist; uint32_t* rbins;
-    uint32_t* tile_n; uint32_t* keys; unsigned long long* words; uint32_t* list;
+struct SmWork {                        // workspace of a call
+    char* clear;                       // per row, `clear_bytes` each: state, then what is there of: race bins, histogram or 16-bit counts
+    long long clear_bytes, rbins_at, hist_at;
+    uint32_t *best, *tile_n, *tile_eq, *keys, *list, *names;
+    unsigned long long* words;
     double *group, *tile_sum, *tile_top;
+    char *few, *few_u;                 // what top-k left: scores and numbers, rule.top_k a row
     long long B, tiles, stiles, capacity, vpad;
+    __device__ __forceinline__ SmRowState& state(long long r) const { return *(SmRowState*)(clear + r * clear_bytes); }
+    __device__ __forceinline__ uint32_t* rbins(long long r) const { return (uint32_t*)(clear + r * clear_bytes + rbins_at); }
+    __device__ __forceinline__ SmHist& hist(long long r) const { return *(SmHist*)(clear + r * clear_bytes + hist_at); }
+    __device__ __forceinline__ uint32_t* counts(long long r) const { return (uint32_t*)(clear + r * clear_bytes + hist_at); }
 };
+
+template <typename V> __device__ __forceinline__ V sm_peek(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename V> __device__ __forceinline__ void sm_poke(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // The last workgroup of a row to get here.  What it reads of the others' work was written by device-wide atomics (adds, or sm_poke's stores, which
 // go through the XCD's own L2) and is read by sm_peek: each wave waits for its own to be done before the ticket is drawn, and no L2 has to be
 // written back (a release fence in every wave of every workgroup took longer than the pass over the data).
 __device__ __forceinline__ bool sm_last_block(uint32_t* ticket, uint32_t blocks, uint32_t* lds)
 {
+    if (blocks == 1) { __syncthreads(); return true; }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) *lds = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     return *lds == blocks - 1;
 }
-template <typename V> __device__ __forceinline__ V sm_peek(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-template <typename V> __device__ __forceinline__ void sm_poke(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
-__global__ void __launch_bounds__(256) sm_clear_kernel(uint4* p, long long n)
-{
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) p[i] = uint4{ 0, 0, 0, 0 };
-}
-
+// Clears the row's part of the workspace and, where a mass needs the row's best score, leaves the best of each workgroup's share.
 template <typename T>
-__global__ void __launch_bounds__(SM_LTPB) sm_best_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step)
+__global__ void __launch_bounds__(SM_LTPB) sm_begin_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int want_best)
 {
-    __shared__ unsigned long long part[SM_MAX_WAVES];
+    __shared__ SmScratch sc;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
+    uint4* clear = (uint4*)(wk.clear + r * wk.clear_bytes);
+    for (long long i = b * SM_LTPB + threadIdx.x; i < wk.clear_bytes / 16; i += wk.B * SM_LTPB) clear[i] = uint4{ 0, 0, 0, 0 };
+    if (!want_best) return;
     const T* x = scores + r * sstride;
     const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const long long stride = wk.B * SM_LTPB * 4;
     uint32_t best = 0;
-    for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += wk.B * SM_LTPB * 4) {
-        uint32_t k[4];
-        sm_load4(x, i, V, vec, logits, k);
+    for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += 4 * stride) {
+        LgVec4<T> v[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) best = k[j] > best ? k[j] : best;
+        for (int g = 0; g < 4; g++) v[g] = sm_load4(x, i + g * stride, V, vec);
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) { const uint32_t k = sm_key(v[g].v[j], logits); best = k > best ? k : best; }
     }
-    best = sm_block_max(best, part);
-    if (threadIdx.x == 0 && best) atomicMax(&wk.state[r].best, best);
-    (void)step;
+    best = sm_block_max(best, sc.a);
+    if (threadIdx.x == 0) wk.best[r * wk.B + b] = best;
+}
+// the row's best (every wave on its own)
+__device__ __forceinline__ uint32_t sm_best(const SmWork& wk, long long r)
+{
+    uint32_t best = 0;
+    for (long long i = threadIdx.x & 63; i < wk.B; i += 64) { const uint32_t k = wk.best[r * wk.B + i]; best = k > best ? k : best; }
+    return sm_lane(sm_wave_scan<false>(best, SmMaxOf()), 63);
 }
 
-// one level of top-k (MASS false) or top-p: bits [at, at + width) of the keys that pass the filters and match the prefix found so far
+// what a selection leaves in the row's state (one thread): `ties` of `count` elements of key thr are taken, and all above it
+__device__ __forceinline__ void sm_conclude(SmRowState& st, const SmKept& kept, uint32_t thr, uint32_t ties, uint32_t count)
+{
+    if (thr < kept.thr) return;                                        // a whole bin around the earlier filter's cut: that one stands
+    st.kept = SmKept{ thr, thr == kept.thr ? kept.last : SM_ALL };
+    if (ties < count) { st.cut = 1; st.ties = ties; }
+}
+
+// one level of top-k (MASS false) or top-p: bits [shift - width, shift) of the keys that pass the filters and match the prefix found so far
 template <typename T, bool MASS>
 __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step,
                                                            int shift, int width)
@@ -684,53 +719,67 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     __shared__ SmHist h;
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
+    constexpr int G = MASS ? 2 : 4;                                    // groups of four loaded ahead
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
-    SmRowState& st = wk.state[r];
+    SmRowState& st = wk.state(r);
     const bool first = shift == 32;
-    if (!first && st.ended) return;
     const T* x = scores + r * sstride;
     const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
-    const SmKept kept = first ? st.kept : st.before;
-    const uint32_t prefix = (uint32_t)st.prefix;
     const int at = shift - width, nbins = 1 << width, p = width - 6;
-    const SmScale scale = sm_scale(rule, MASS ? st.best : 0u);
-    const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
-    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) { h.n[i] = 0; if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } }
-    __syncthreads();
-    for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += wk.B * SM_LTPB * 4) {
-        uint32_t key[4];
-        sm_load4(x, i, V, vec, logits, key);
+    const long long stride = wk.B * SM_LTPB * 4;
+    long long i = (b * SM_LTPB + threadIdx.x) * 4;
+    LgVec4<T> v[G];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (!sm_in(kept, key[j], (uint32_t)(i + j)) || (!first && (key[j] >> shift) != prefix)) continue;
-            const int bin = sm_slot((int)(key[j] >> at) & (nbins - 1), p);
-            atomicAdd(&h.n[bin], 1u);
-            if (MASS) {
-                const SmLimbs m = sm_limbs(sm_mass(scale, key[j]) * unit);
-                if (m.hi) atomicAdd(&h.hi[bin], (unsigned long long)m.hi);
-                if (m.lo) atomicAdd(&h.lo[bin], (unsigned long long)m.lo);
+    for (int g = 0; g < G; g++) v[g] = sm_load4(x, i + g * stride, V, vec);
+    if (!first && st.ended) return;
+    const SmKept kept = first ? st.kept : st.before;
+    const uint32_t prefix = st.prefix;
+    const uint32_t best = MASS ? (first ? sm_best(wk, r) : st.best) : 0u;
+    const SmScale scale = sm_scale(rule, best);
+    const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
+    for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { h.n[k] = 0; if (MASS) { h.hi[k] = 0; h.lo[k] = 0; } }
+    __syncthreads();
+    while (i < V) {
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t key = sm_key(v[g].v[j], logits);
+                if (!sm_in(kept, key, (uint32_t)(i + g * stride + j)) || (!first && (key >> shift) != prefix)) continue;
+                const int bin = sm_slot((int)(key >> at) & (nbins - 1), p);
+                atomicAdd(&h.n[bin], 1u);
+                if (MASS) {
+                    const SmLimbs m = sm_limbs(sm_mass(scale, key) * unit);
+                    if (m.hi) atomicAdd(&h.hi[bin], (unsigned long long)m.hi);
+                    if (m.lo) atomicAdd(&h.lo[bin], (unsigned long long)m.lo);
+                }
             }
-        }
+        i += G * stride;
+        if (i >= V) break;
+#pragma unroll
+        for (int g = 0; g < G; g++) v[g] = sm_load4(x, i + g * stride, V, vec);
     }
     __syncthreads();
-    SmHist& g = wk.hist[r];
-    for (int i = threadIdx.x; i < nbins; i += SM_LTPB)
-        if (h.n[i]) {
-            atomicAdd(&g.n[i], h.n[i]);
-            if (MASS) { if (h.hi[i]) atomicAdd(&g.hi[i], h.hi[i]); if (h.lo[i]) atomicAdd(&g.lo[i], h.lo[i]); }
+    if (wk.B > 1) {
+        SmHist& g = wk.hist(r);
+        for (int k = threadIdx.x; k < nbins; k += SM_LTPB)
+            if (h.n[k]) {
+                atomicAdd(&g.n[k], h.n[k]);
+                if (MASS) { if (h.hi[k]) atomicAdd(&g.hi[k], h.hi[k]); if (h.lo[k]) atomicAdd(&g.lo[k], h.lo[k]); }
+            }
+        if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+        for (int k = threadIdx.x; k < nbins; k += SM_LTPB) {           // taken over, and left clear for the next level
+            h.n[k] = sm_peek(&g.n[k]); g.n[k] = 0;
+            if (MASS) { h.hi[k] = sm_peek(&g.hi[k]); h.lo[k] = sm_peek(&g.lo[k]); g.hi[k] = 0; g.lo[k] = 0; }
         }
-    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
-    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) {               // taken over, and left clear for the next level
-        h.n[i] = sm_peek(&g.n[i]); g.n[i] = 0;
-        if (MASS) { h.hi[i] = sm_peek(&g.hi[i]); h.lo[i] = sm_peek(&g.lo[i]); g.hi[i] = 0; g.lo[i] = 0; }
+        __syncthreads();
     }
-    __syncthreads();
     SmTake take = st.take;
     if (first) {
         take = SmTake{ (double)rule.top_k, 0, { 0, 0 } };
         if (MASS) {
             SmSum mine = { 0, 0 }, total;
-            for (int i = threadIdx.x; i < nbins; i += SM_LTPB) { mine.hi += h.hi[i]; mine.lo += h.lo[i]; }
+            for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { mine.hi += h.hi[k]; mine.lo += h.lo[k]; }
             sm_block_scan<unsigned long long>(mine.hi, sc.a, total.hi);
             sm_block_scan<unsigned long long>(mine.lo, sc.b, total.lo);
             take.target = rule.top_p * sm_sum_value(total);
@@ -740,78 +789,305 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     if (threadIdx.x != 0) return;
     st.before = kept;
     st.take = take;
+    st.best = best;
     st.ended = 0;
     st.cut = 0;
     if (bin.bin < 0) { st.ended = 1; return; }                         // no candidate: the filter in force (or an empty row) stands
     const uint32_t found = (first ? 0u : prefix << width) | (uint32_t)bin.bin;
     st.prefix = found;
     const bool whole = sm_whole_bin<MASS>(take, bin.count);
-    if (!whole && at > (sizeof(T) == 2 ? 10 : 0)) return;
-    // the key is found (or the lowest key of a bin that is taken whole); a cut among the equal ones is left to sm_tie_kernel.  Scores of 16
-    // bits differ in the 22 leading bits of their keys: what follows is all zeros, or all ones for a negative score.
-    const uint32_t thr = !whole && at && !(found >> (31 - at)) ? (found << at) | ((1u << at) - 1) : found << at;
-    uint32_t ties = bin.count;
-    if (!whole) ties = sm_ties<MASS>(take, bin.count, MASS ? sm_mass(scale, thr) * unit : 0.0);
+    if (!whole && at > 0) return;
+    // the key is found, or the lowest key of a bin that is taken whole; a cut among the equal ones is left to sm_cut_kernel
+    const uint32_t thr = found << at;
     st.ended = 1;
-    if (thr < kept.thr) return;                                        // a whole bin around the earlier filter's cut: that one stands
-    st.kept = SmKept{ thr, thr == kept.thr ? kept.last : SM_ALL };
-    if (ties < bin.count) { st.cut = 1; st.ties = ties; }
+    sm_conclude(st, kept, thr, whole ? bin.count : sm_ties<MASS>(take, bin.count, MASS ? sm_mass(scale, thr) * unit : 0.0), bin.count);
 }
 
-// index of the last equal element that is kept, where a selection ends inside equal keys; and min-p, once, behind the last filter
+// ---- scores of 16 bits: both filters from one histogram of all keys ----------------------------------------------------------------------
+// The 65536 ordered keys of a 16-bit type are counted in LDS (two counters a word: a workgroup takes at most SM_SHARE16 elements), added up in
+// memory, and the last workgroup works top-k and top-p out of the counts: one pass over the row and one exponential per distinct score, in
+// the place of one pass for the best and two for each filter.
+#define SM_SHARE16 32768
+__device__ __forceinline__ uint32_t sm_bits(LgHalf v) { return (uint32_t)__builtin_bit_cast(uint16_t, v); }
+__device__ __forceinline__ uint32_t sm_bits(LgBf16 v) { return v.bits; }
+__device__ __forceinline__ uint32_t sm_bits(float) { return 0u; }                            // (no such path)
+template <typename T> __device__ __forceinline__ T sm_from_bits(uint32_t b);
+template <> __device__ __forceinline__ LgHalf sm_from_bits<LgHalf>(uint32_t b) { return __builtin_bit_cast(LgHalf, (uint16_t)b); }
+template <> __device__ __forceinline__ LgBf16 sm_from_bits<LgBf16>(uint32_t b) { return LgBf16{ (uint16_t)b }; }
+
+// ordered key of 16 bits; 0 = excluded.  sm_key(sm_unkey16(k)) orders like k
+template <typename T> __device__ __forceinline__ uint32_t sm_key16(T raw, bool logits)
+{
+    const uint32_t key = sm_key(raw, logits);
+    if (key == 0u) return 0u;
+    const float x = __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);        // canonical: no -0, no infinity
+    const uint32_t b = sm_bits(lg_from_float<T>(x));
+    return (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
+}
+template <typename T> __device__ __forceinline__ uint32_t sm_key_of16(uint32_t k, bool logits)
+{
+    return k == 0u ? 0u : sm_key(sm_from_bits<T>((k & 0x8000u) ? (k & 0x7fffu) : (~k & 0xffffu)), logits);
+}
+
+// per chunk of 64 keys: count, and mass in limbs, of what a filter left
+struct SmChunks { uint32_t n[1024]; unsigned long long hi[1024], lo[1024]; };
+
 template <typename T>
-__global__ void __launch_bounds__(SM_LTPB) sm_tie_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step)
+__global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step, int top_k, int top_p)
+{
+    __shared__ union { uint32_t pair[32768]; SmChunks chunk; } h;
+    __shared__ SmScratch sc;
+    __shared__ uint32_t ticket;
+    const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
+    SmRowState& st = wk.state(r);
+    const T* x = scores + r * sstride;
+    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const long long stride = wk.B * 4096;
+    long long i = (b * 1024 + threadIdx.x) * 4;
+    LgVec4<T> v[4];
+#pragma unroll
+    for (int g = 0; g < 4; g++) v[g] = sm_load4(x, i + g * stride, V, vec);
+    for (int k = threadIdx.x; k < 8192; k += 1024) ((uint4*)h.pair)[k] = uint4{ 0, 0, 0, 0 };
+    __syncthreads();
+    while (i < V) {
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t k = sm_key16(v[g].v[j], logits);
+                if (k) atomicAdd(&h.pair[k >> 1], 1u << (16 * (k & 1)));
+            }
+        i += 4 * stride;
+        if (i >= V) break;
+#pragma unroll
+        for (int g = 0; g < 4; g++) v[g] = sm_load4(x, i + g * stride, V, vec);
+    }
+    __syncthreads();
+    uint32_t* counts = wk.counts(r);
+    for (int k = threadIdx.x; k < 32768; k += 1024) {
+        const uint32_t w = h.pair[k];
+        if (w & 0xffffu) atomicAdd(&counts[2 * k], w & 0xffffu);
+        if (w >> 16) atomicAdd(&counts[2 * k + 1], w >> 16);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // chunk c: keys 64 c ... 64 c + 63, one a lane; wave w takes the chunks w, w + 16, ... (the scores that occur lie close together)
+    uint32_t best = 0;
+    for (int c0 = 0; c0 < 64; c0 += 16) {
+        uint32_t n[16];
+#pragma unroll
+        for (int c = 0; c < 16; c++) n[c] = sm_peek(&counts[((c0 + c) * 16 + wave) * 64 + lane]);
+#pragma unroll
+        for (int c = 0; c < 16; c++) {
+            const int chunk = (c0 + c) * 16 + wave;
+            const unsigned long long any = __ballot(n[c] != 0);
+            if (any) best = (uint32_t)(chunk * 64 + 63 - __clzll((long long)any));
+            const uint32_t sum = any ? sm_lane(sm_wave_scan<false>(n[c], SmAdd()), 63) : 0u;
+            if (lane == 0) h.chunk.n[chunk] = sum;
+        }
+    }
+    best = sm_block_max(best, sc.a);
+    const uint32_t best_key = sm_key_of16<T>(best, logits);
+    const SmScale scale = sm_scale(rule, best_key);
+    const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
+    SmKept kept = { 0u, SM_ALL };
+    uint32_t cut_key = 0, cut_n = 0;                                   // top-k: keys above cut_key whole, cut_n of it
+    uint32_t thr = 0, ties = 0, equal = 0;
+    for (int pass = 0; pass < 2 && best != 0; pass++) {
+        if (!(pass == 0 ? top_k : top_p)) continue;
+        const bool mass = pass == 1;
+        SmTake take = { (double)rule.top_k, 0, { 0, 0 } };
+        // what is left of key k's count
+        auto left = [&](uint32_t k) {
+            const uint32_t n = sm_peek(&counts[k]);
+            return k > cut_key ? n : k == cut_key ? cut_n : 0u;
+        };
+        auto limbs = [&](uint32_t k, uint32_t n) {
+            SmSum m = { 0, 0 };
+            if (n) { const SmLimbs one = sm_limbs(sm_mass(scale, sm_key_of16<T>(k, logits)) * unit); m = SmSum{ (unsigned long long)one.hi * n, (unsigned long long)one.lo * n }; }
+            return m;
+        };
+        if (mass) {
+            for (int c = 0; c < 64; c++) {
+                const int chunk = c * 16 + wave;
+                SmSum m = { 0, 0 };
+                if (h.chunk.n[chunk] != 0 && (uint32_t)chunk * 64 + 63 >= cut_key) {          // (uniform over the wave)
+                    const uint32_t k = (uint32_t)chunk * 64 + lane;
+                    m = limbs(k, left(k));
+                    m.hi = sm_lane(sm_wave_scan<false>(m.hi, SmAdd()), 63);
+                    m.lo = sm_lane(sm_wave_scan<false>(m.lo, SmAdd()), 63);
+                }
+                if (lane == 0) { h.chunk.hi[chunk] = m.hi; h.chunk.lo[chunk] = m.lo; }
+            }
+            __syncthreads();
+        }
+        // the chunk in which the selection ends: thread t stands for chunk 1023 - t
+        const int chunk = 1023 - (int)threadIdx.x;
+        const uint32_t n = h.chunk.n[chunk];
+        SmSum m = { 0, 0 }, total = { 0, 0 }, upto = { 0, 0 };
+        uint32_t all, before = sm_block_scan<uint32_t>(n, sc.a, all);
+        if (mass) {
+            m = SmSum{ h.chunk.hi[chunk], h.chunk.lo[chunk] };
+            upto.hi = sm_block_scan<unsigned long long>(m.hi, sc.a, total.hi);
+            upto.lo = sm_block_scan<unsigned long long>(m.lo, sc.b, total.lo);
+            take.target = rule.top_p * sm_sum_value(total);
+        }
+        const bool room = mass ? (m.hi | m.lo) != 0 && sm_room<true>(take, 0, upto.hi, upto.lo) : n != 0 && sm_room<false>(take, before, 0, 0);
+        const uint32_t end = sm_block_max<uint32_t>(room ? threadIdx.x + 1 : 0u, sc.a);
+        if (room && threadIdx.x + 1 == end) { sc.word[0] = before; sc.word[1] = upto.hi; sc.word[2] = upto.lo; }
+        __syncthreads();
+        take.before_n = (uint32_t)sc.word[0];
+        take.before_m = SmSum{ sc.word[1], sc.word[2] };
+        // inside it: lane l stands for its key 63 - l (every wave the same)
+        const uint32_t k = (1024 - end) * 64 + 63 - (uint32_t)lane;
+        const uint32_t n2 = left(k);
+        SmSum m2 = { 0, 0 }, in2 = { 0, 0 };
+        const uint32_t in = sm_wave_scan<false>(n2, SmAdd());
+        if (mass) {
+            m2 = limbs(k, n2);
+            in2.hi = sm_wave_scan<false>(m2.hi, SmAdd());
+            in2.lo = sm_wave_scan<false>(m2.lo, SmAdd());
+        }
+        const unsigned long long enter = __ballot(mass ? (m2.hi | m2.lo) != 0 && sm_room<true>(take, 0, in2.hi - m2.hi, in2.lo - m2.lo) : n2 != 0 && sm_room<false>(take, in - n2, 0, 0));
+        const int l = enter ? 63 - __clzll((long long)enter) : 0;
+        equal = sm_lane(n2, l);
+        thr = sm_lane(k, l);
+        take.before_n += sm_lane(in - n2, l);
+        if (mass) { take.before_m.hi += sm_lane(in2.hi - m2.hi, l); take.before_m.lo += sm_lane(in2.lo - m2.lo, l); }
+        const double unit_mass = mass ? sm_mass(scale, sm_key_of16<T>(thr, logits)) * unit : 0.0;
+        ties = mass ? sm_ties<true>(take, equal, unit_mass) : sm_ties<false>(take, equal, 0.0);
+        // equal ones that top-k had left out count as cut too
+        equal = sm_peek(&counts[thr]);
+        cut_key = thr;
+        cut_n = ties;
+        __syncthreads();
+    }
+    if (threadIdx.x != 0) return;
+    st.before = kept;
+    st.best = best_key;
+    st.ended = 1;
+    st.cut = 0;
+    if (best != 0) sm_conclude(st, kept, sm_key_of16<T>(thr, logits), ties, equal);
+}
+
+// ---- cuts among equal keys, and what top-k left ------------------------------------------------------------------------------------------
+// Index of the last equal element that is kept, where a selection ends inside equal keys.  GATHER: also every tile's first place among the
+// elements that are left.
+template <typename T, bool GATHER>
+__global__ void __launch_bounds__(SM_LTPB) sm_cut_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step)
 {
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
-    SmRowState& st = wk.state[r];
-    if (!st.cut) return;
+    SmRowState& st = wk.state(r);
+    const bool cut = st.cut;
+    if (!GATHER && !cut) return;
     const T* x = scores + r * sstride;
-    const bool logits = rule.mode == SM_LOGITS;
+    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
     const SmKept kept = st.kept;
-    uint32_t* tile_n = wk.tile_n + r * wk.tiles;
-    auto tie = [&](long long i) { const uint32_t k = i < V ? sm_key(x[i], logits) : 0u; return k != 0u && k == kept.thr && (uint32_t)i <= kept.last; };
+    uint32_t *tile_n = wk.tile_n + r * wk.tiles, *tile_eq = wk.tile_eq + r * wk.tiles;
     for (long long t = b; t < wk.tiles; t += wk.B) {
-        uint32_t c = 0, total;
-        for (int k = 0; k < SM_TILE / SM_LTPB; k++) c += tie(t * SM_TILE + k * SM_LTPB + threadIdx.x);
-        sm_block_scan<uint32_t>(c, sc.a, total);
-        if (threadIdx.x == 0) sm_poke(&tile_n[t], total);
+        // (counts do not care for the order: groups of four as they load best)
+        LgVec4<T> v[SM_TILE / SM_LTPB / 4];
+#pragma unroll
+        for (int g = 0; g < SM_TILE / SM_LTPB / 4; g++) v[g] = sm_load4(x, t * SM_TILE + (g * SM_LTPB + threadIdx.x) * 4, V, vec);
+        uint32_t eq = 0, more = 0, total;
+#pragma unroll
+        for (int g = 0; g < SM_TILE / SM_LTPB / 4; g++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t k = sm_key(v[g].v[j], logits), i = (uint32_t)(t * SM_TILE + (g * SM_LTPB + threadIdx.x) * 4 + j);
+                eq += k != 0u && k == kept.thr && i <= kept.last;
+                more += k > kept.thr;
+            }
+        sm_block_scan<uint32_t>(eq, sc.a, total);
+        if (threadIdx.x == 0) sm_poke(&tile_eq[t], total);
+        if (GATHER) {
+            sm_block_scan<uint32_t>(more, sc.b, total);
+            if (threadIdx.x == 0) sm_poke(&tile_n[t], total);
+        }
     }
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
-    const unsigned long long want = st.ties;
-    unsigned long long done = 0;
+    const uint32_t want = cut ? st.ties : SM_ALL;                      // equal elements that are kept
+    unsigned long long equal = 0, run = 0;
     long long tile = -1;
-    for (long long base = 0; base < wk.tiles && tile < 0; base += SM_LTPB) {
+    uint32_t rest = 0;
+    for (long long base = 0; base < wk.tiles; base += SM_LTPB) {
         const long long t = base + threadIdx.x;
-        const uint32_t c = t < wk.tiles ? sm_peek(&tile_n[t]) : 0u;
+        const uint32_t c = t < wk.tiles ? sm_peek(&tile_eq[t]) : 0u;
         uint32_t total;
         const uint32_t before = sm_block_scan<uint32_t>(c, sc.a, total);
-        const bool here = done + before < want && want <= done + before + c;
-        if (here) { sc.word[0] = (unsigned long long)t; sc.word[1] = done + before; }
-        if (want <= done + total) {                                    // uniform
-            __syncthreads();
-            tile = (long long)sc.word[0];
-            done = sc.word[1];
-        } else done += total;
+        const unsigned long long from = equal + before;                // equal ones before this tile
+        const uint32_t mine = from >= want ? 0u : want - from < c ? (uint32_t)(want - from) : c;
+        if (cut && mine != 0 && from + mine == want) { sc.word[0] = (unsigned long long)t; sc.word[1] = want - from; }
+        if (GATHER) {
+            uint32_t kept_here = mine + (t < wk.tiles ? sm_peek(&tile_n[t]) : 0u), all;
+            const uint32_t at = sm_block_scan<uint32_t>(kept_here, sc.b, all);
+            if (t < wk.tiles) tile_n[t] = (uint32_t)(run + at);
+            run += all;
+        }
+        __syncthreads();
+        if (cut && tile < 0 && equal + total >= want) { tile = (long long)sc.word[0]; rest = (uint32_t)sc.word[1]; }        // uniform
+        equal += total;
+        __syncthreads();
     }
-    if (tile < 0) return;                                              // cannot be: `want` counts these very elements
+    if (GATHER && threadIdx.x == 0) st.sure = run;
+    if (tile < 0) return;
     for (int k = 0; k < SM_TILE / SM_LTPB; k++) {
         const long long i = tile * SM_TILE + k * SM_LTPB + threadIdx.x;
-        const bool f = tie(i);
+        const uint32_t key = i < V ? sm_key(x[i], logits) : 0u;
+        const bool f = key != 0u && key == kept.thr && (uint32_t)i <= kept.last;
         uint32_t total;
         const uint32_t before = sm_block_scan<uint32_t>(f ? 1u : 0u, sc.a, total);
-        if (f && done + before + 1 == want) { st.kept.last = (uint32_t)i; st.cut = 0; }
-        done += total;
-        if (done >= want) break;                                       // uniform
+        if (f && before + 1 == rest) { st.kept.last = (uint32_t)i; st.cut = 0; }
+        if (total >= rest) break;                                      // uniform
+        rest -= total;
     }
 }
 
+// what top-k left, in index order: scores, their names and (without replacement) their numbers; rule.top_k places a row, the last ones empty
+template <typename T>
+__global__ void __launch_bounds__(SM_LTPB) sm_gather_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u /*nullable*/, long long ustride,
+                                                            long long V, SmRule rule, SmWork wk)
+{
+    __shared__ SmScratch sc;
+    const long long r = blockIdx.x / wk.tiles, t = blockIdx.x % wk.tiles, K = rule.top_k;
+    const SmRowState& st = wk.state(r);
+    const T* x = scores + r * sstride;
+    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const SmKept kept = st.kept;
+    constexpr int E = SM_TILE / SM_LTPB;                               // consecutive elements a thread
+    const long long i0 = t * SM_TILE + (long long)threadIdx.x * E;
+    LgVec4<T> v[E / 4];
+#pragma unroll
+    for (int g = 0; g < E / 4; g++) v[g] = sm_load4(x, i0 + 4 * g, V, vec);
+    uint32_t in = 0, total;
+#pragma unroll
+    for (int k = 0; k < E; k++) if (sm_in(kept, sm_key(v[k / 4].v[k % 4], logits), (uint32_t)(i0 + k))) in |= 1u << k;
+    long long at = (long long)wk.tile_n[r * wk.tiles + t] + sm_block_scan<uint32_t>(__popc(in), sc.a, total);
+    T* few = (T*)wk.few + r * K;
+    uint32_t* names = wk.names + r * K;
+    float* few_u = (float*)wk.few_u + r * K;
+#pragma unroll
+    for (int k = 0; k < E; k++)
+        if ((in >> k) & 1) {
+            if (at < K) {
+                few[at] = v[k / 4].v[k % 4];
+                names[at] = (uint32_t)(i0 + k);
+                if (u) few_u[at] = u[r * ustride + i0 + k];
+            }
+            at++;
+        }
+    for (long long j = (long long)st.sure + t * SM_LTPB + threadIdx.x; j < K; j += wk.tiles * SM_LTPB) few[j] = lg_from_float<T>(__uint_as_float(0x7fc00000u));
+}
+
 // filter in force with min-p (every wave works the cut out for itself)
-__device__ __forceinline__ SmKept sm_final(const SmRowState& st, const SmRule& rule)
+__device__ __forceinline__ SmKept sm_final(const SmWork& wk, long long r, const SmRowState& st, const SmRule& rule)
 {
     SmKept kept = st.kept;
-    if (rule.min_p > 0.0 && st.best) sm_min_p(sm_scale(rule, st.best), st.best, rule.min_p, kept);
+    const uint32_t best = rule.min_p > 0.0 ? sm_best(wk, r) : 0u;
+    if (best) sm_min_p(sm_scale(rule, best), best, rule.min_p, kept);
     return kept;
 }
 
@@ -819,36 +1095,37 @@ __device__ __forceinline__ SmKept sm_final(const SmRowState& st, const SmRule& r
 // Prefix sums of the kept masses inside tiles, one stored per SM_GROUP elements, relative to the tile's best element (so that no pass for the
 // row's best is needed); the last workgroup puts the tiles on a common scale.  Fixed order everywhere.
 template <typename T>
-__global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step)
+__global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, SmWork whole, int step)
 {
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
-    SmRowState& st = wk.state[r];
+    SmRowState& st = wk.state(r);
     const T* x = scores + r * sstride;
     const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
-    const SmKept kept = sm_final(st, rule);
-    double *sums = wk.tile_sum + r * (wk.stiles + 1), *tops = wk.tile_top + r * wk.stiles, *groups = wk.group + r * wk.stiles * (SM_STILE / SM_GROUP);
+    const SmKept kept = sm_final(whole, r, st, rule);
+    double *sums = wk.tile_sum + r * wk.stiles, *tops = wk.tile_top + r * wk.stiles, *groups = wk.group + r * wk.stiles * (SM_STILE / SM_GROUP);
     for (long long t = b; t < wk.stiles; t += wk.B) {
         const long long i0 = t * SM_STILE + threadIdx.x * SM_GROUP;
+        LgVec4<T> v[SM_GROUP / 4];
+#pragma unroll
+        for (int k = 0; k < SM_GROUP / 4; k++) v[k] = sm_load4(x, i0 + 4 * k, V, vec);
         uint32_t key[SM_GROUP], best = 0;
 #pragma unroll
-        for (int k = 0; k < SM_GROUP; k += 4) sm_load4(x, i0 + k, V, vec, logits, key + k);
-#pragma unroll
         for (int k = 0; k < SM_GROUP; k++) {
+            key[k] = sm_key(v[k / 4].v[k % 4], logits);
             if (!sm_in(kept, key[k], (uint32_t)(i0 + k))) key[k] = 0;
             best = key[k] > best ? key[k] : best;
         }
         best = sm_block_max(best, sc.b);
         const SmScale scale = sm_scale(rule, best);
-        double sum = 0.0, total;
+        double sum = 0.0, total, most;
 #pragma unroll
         for (int k = 0; k < SM_GROUP; k++) sum += sm_mass(scale, key[k]);
         const double before = sm_block_scan<double>(sum, sc.a, total);
-        const double mass = total;
-        groups[t * (SM_STILE / SM_GROUP) + threadIdx.x] = sm_block_rise(sum > 0.0 ? before + sum : 0.0, sc.b, total);
+        groups[t * (SM_STILE / SM_GROUP) + threadIdx.x] = sm_block_rise(sum > 0.0 ? before + sum : 0.0, sc.b, most);
         if (threadIdx.x == 0) {
-            sm_poke(&sums[t], mass);
+            sm_poke(&sums[t], total);
             sm_poke(&tops[t], best ? scale.top : -INFINITY);
         }
     }
@@ -859,60 +1136,107 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
     const unsigned long long m = sm_block_max<unsigned long long>((ordered >> 63) ? ~ordered : (ordered | 0x8000000000000000ull), sc.b);
     top = __longlong_as_double((long long)((m >> 63) ? (m & 0x7fffffffffffffffull) : ~m));
     double run = 0.0, risen = 0.0;
-    for (long long base = 0; base < wk.stiles; base += 256) {
-        const long long t = base + threadIdx.x;
-        double mass = 0.0, total;
-        if (t < wk.stiles) {
-            const double tt = sm_peek(&tops[t]);
-            mass = sm_peek(&sums[t]) * (rule.mode == SM_LINEAR || tt == -INFINITY ? 1.0 : exp(tt - top));
+    constexpr int K = 4;                                               // tiles a thread
+    for (long long base = 0; base < wk.stiles; base += 256 * K) {
+        const long long t0 = base + threadIdx.x * K;
+        double mass[K], tt[K], sum = 0.0, total, most;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            mass[k] = t0 + k < wk.stiles ? sm_peek(&sums[t0 + k]) : 0.0;
+            tt[k] = t0 + k < wk.stiles ? sm_peek(&tops[t0 + k]) : -INFINITY;
         }
-        const double before = sm_block_scan<double>(mass, sc.a, total);
-        double most;
-        const double upto = fmax(sm_block_rise(mass > 0.0 ? run + before + mass : 0.0, sc.b, most), risen);
-        if (t < wk.stiles) sums[t] = upto;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            if (rule.mode != SM_LINEAR) mass[k] = tt[k] == -INFINITY ? 0.0 : mass[k] * sm_exp(tt[k] - top);
+            sum += mass[k];
+        }
+        double at = run + sm_block_scan<double>(sum, sc.a, total);
+        double rise[K], high = 0.0;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            at += mass[k];
+            if (mass[k] > 0.0 && at > high) high = at;
+            rise[k] = high;
+        }
+        const double below = fmax(sm_block_rise_before(high, sc.b, most), risen);
+#pragma unroll
+        for (int k = 0; k < K; k++) if (t0 + k < wk.stiles) sums[t0 + k] = fmax(rise[k], below);
         risen = fmax(risen, most);
         run += total;
     }
     if (threadIdx.x == 0) { st.total = run; st.top = top; st.kept = kept; }
 }
 
+// how many of the n ascending values are not past (`past(a[i])` is false up to there and true behind)
+template <typename Past> __device__ __forceinline__ int sm_rank(const double* a, int n, const Past& past)
+{
+    int lo = 0;
+    while (n > 0) {
+        const int half = n >> 1;
+        if (past(a[lo + half])) n = half; else { lo += half + 1; n -= half + 1; }
+    }
+    return lo;
+}
+// the same, three values a round loaded together (half the round trips to memory for half as many loads again)
+template <typename Past> __device__ __forceinline__ int sm_rank4(const double* a, int n, const Past& past)
+{
+    int lo = 0;
+    while (n >= 4) {
+        const int part = n >> 2;
+        const bool x = past(a[lo + part - 1]), y = past(a[lo + 2 * part - 1]), z = past(a[lo + 3 * part - 1]);
+        const int c = x ? 0 : y ? 1 : z ? 2 : 3;
+        lo += c * part;
+        n = c < 3 ? part - 1 : n - 3 * part;
+    }
+    return lo + sm_rank(a + lo, n, past);
+}
+
+#define SM_DRAW_ENDS 2048              // tiles whose ends a workgroup of draws keeps in LDS (or ends of groups of tiles, where there are more)
+
 template <typename T>
 __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                       long long R, long long V, long long n, SmRule rule, SmWork wk, long long* __restrict__ out)
 {
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (at >= R * n) return;
-    const long long r = at / n, j = at - r * n;
-    const SmRowState& st = wk.state[r];
-    const double* sums = wk.tile_sum + r * (wk.stiles + 1);
+    __shared__ double ends[SM_DRAW_ENDS];
+    const long long blocks = (n + 255) / 256, r = blockIdx.x / blocks, j = blockIdx.x % blocks * 256 + threadIdx.x, at = r * n + j;
+    const SmRowState& st = wk.state(r);
+    const double* sums = wk.tile_sum + r * wk.stiles;
+    const int tiles = (int)wk.stiles, group = (tiles + SM_DRAW_ENDS - 1) / SM_DRAW_ENDS, ngroups = (tiles + group - 1) / group;
+    for (int k = threadIdx.x; k < ngroups; k += 256) ends[k] = sums[((k + 1) * group < tiles ? (k + 1) * group : tiles) - 1];
+    __syncthreads();
+    if (j >= n) return;
     const double* tops = wk.tile_top + r * wk.stiles;
-    const double total = sums[wk.stiles - 1];
+    const double total = ends[ngroups - 1];
     if (!(total > 0.0)) { out[at] = -1; return; }
     const float uj = u[r * ustride + j];
     const double target = (uj > 0.0f ? (double)uj : 0.0) * st.total;
-    auto first = [](const double* a, long long n, auto&& past) {       // first position with past(a[.]), or n - 1
-        long long lo = 0, hi = n - 1;
-        while (lo < hi) { const long long mid = (lo + hi) >> 1; if (past(a[mid])) hi = mid; else lo = mid + 1; }
-        return lo;
+    auto tile_of = [&](auto&& past) {
+        const int k = sm_rank(ends, ngroups, past), t = k * group;
+        return k < ngroups && group > 1 ? t + sm_rank(sums + t, t + group < tiles ? group : tiles - t, past) : t;
     };
-    long long t = first(sums, wk.stiles, [&](double s) { return s > target; });
-    if (!(sums[t] > target)) t = first(sums, wk.stiles, [&](double s) { return s >= total; });
-    const double* g = wk.group + (r * wk.stiles + t) * (SM_STILE / SM_GROUP);
+    int t = tile_of([&](double s) { return s > target; });
+    if (t >= tiles) t = tile_of([&](double s) { return s >= total; });                                  // rounding, or u >= 1: where the masses end
+    const double* g = wk.group + (r * wk.stiles + t) * (long long)(SM_STILE / SM_GROUP);
     const int ng = SM_STILE / SM_GROUP;
-    const double scale_up = rule.mode == SM_LINEAR ? 1.0 : exp(tops[t] - st.top);
-    const double local = fmax((target - (t ? sums[t - 1] : 0.0)) / scale_up, 0.0);
-    long long k = first(g, ng, [&](double s) { return s > local; });
-    if (!(g[k] > local)) k = first(g, ng, [&](double s) { return s >= g[ng - 1]; });
+    const double scale_up = rule.mode == SM_LINEAR ? 1.0 : sm_exp(tops[t] - st.top);
+    const double local = fmax((target - (t ? sums[t - 1] : 0.0)) / scale_up, 0.0), here = g[ng - 1];
+    int k = sm_rank4(g, ng, [&](double s) { return s > local; });
+    if (k >= ng) k = sm_rank4(g, ng, [&](double s) { return s >= here; });
     // inside the group: the masses once more, in the same order
     const T* x = scores + r * sstride;
     const SmScale scale = { rule.mode, 1.0 / rule.temperature, tops[t], 1.0 };
     const SmKept kept = st.kept;
-    const long long i0 = t * SM_STILE + k * SM_GROUP;
+    const long long i0 = (long long)t * SM_STILE + k * SM_GROUP;
     double acc = k ? g[k - 1] : 0.0;
     long long found = -1, any = -1;
+    LgVec4<T> v[SM_GROUP / 4];
+    const bool vec = sm_aligned(x);
+#pragma unroll
+    for (int e = 0; e < SM_GROUP / 4; e++) v[e] = sm_load4(x, i0 + 4 * e, V, vec);
+#pragma unroll
     for (int e = 0; e < SM_GROUP; e++) {
         const long long i = i0 + e;
-        const uint32_t key = i < V ? sm_key(x[i], rule.mode == SM_LOGITS) : 0u;
+        const uint32_t key = sm_key(v[e / 4].v[e % 4], rule.mode == SM_LOGITS);
         const double w = sm_in(kept, key, (uint32_t)i) ? sm_mass(scale, key) : 0.0;
         acc += w;
         if (w > 0.0) { any = i; if (found < 0 && acc > local) found = i; }
@@ -930,37 +1254,42 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
-    SmRowState& st = wk.state[r];
+    SmRowState& st = wk.state(r);
     const T* x = scores + r * sstride;
     u += r * ustride;
     uint32_t* keys = wk.keys + r * wk.vpad;
     const bool logits = rule.mode == SM_LOGITS, vec = sm_aligned(x), uvec = sm_aligned(u);
     const float slope = sm_slope(rule);
-    const SmKept kept = sm_final(st, rule);
-    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) h[i] = 0;
+    const SmKept kept = sm_final(wk, r, st, rule);
+    const long long stride = wk.B * SM_LTPB * 4;
+    constexpr int G = 2;
+    long long i = (b * SM_LTPB + threadIdx.x) * 4;
+    LgVec4<T> v[G];
+    LgVec4<float> uk[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) { v[g] = sm_load4(x, i + g * stride, V, vec); uk[g] = sm_load4(u, i + g * stride, V, uvec); }
+    for (int k = threadIdx.x; k < SM_RBINS; k += SM_LTPB) h[k] = 0;
     __syncthreads();
-    for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += wk.B * SM_LTPB * 4) {
-        uint32_t key[4];
-        float uk[4];
-        sm_load4(x, i, V, vec, logits, key);
-        if (uvec && i + 4 <= V) {
-            const LgVec4<float> q = *(const LgVec4<float>*)(u + i);
+    while (i < V) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) uk[j] = q.v[j];
-        } else {
+        for (int g = 0; g < G; g++) {
+            const long long at = i + g * stride;
+            LgVec4<uint32_t> o;
 #pragma unroll
-            for (int j = 0; j < 4; j++) uk[j] = i + j < V ? u[i + j] : 0.5f;
+            for (int j = 0; j < 4; j++) {
+                const uint32_t key = sm_key(v[g].v[j], logits);
+                o.v[j] = sm_race32(logits, slope, sm_in(kept, key, (uint32_t)(at + j)) ? key : 0u, uk[g].v[j]);
+                if (o.v[j]) atomicAdd(&h[sm_slot((int)(o.v[j] >> (32 - SM_RBITS1)), SM_RBITS1 - 6)], 1u);
+            }
+            if (at < V) *(LgVec4<uint32_t>*)(keys + at) = o;           // (padded to a multiple of four: what lies behind V is key 0)
         }
-        LgVec4<uint32_t> o;
+        i += G * stride;
+        if (i >= V) break;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            o.v[j] = sm_race32(logits, slope, sm_in(kept, key[j], (uint32_t)(i + j)) ? key[j] : 0u, uk[j]);
-            if (o.v[j]) atomicAdd(&h[sm_slot((int)(o.v[j] >> (32 - SM_RBITS1)), SM_RBITS1 - 6)], 1u);
-        }
-        *(LgVec4<uint32_t>*)(keys + i) = o;                            // (padded to a multiple of four: what lies behind V is key 0)
+        for (int g = 0; g < G; g++) { v[g] = sm_load4(x, i + g * stride, V, vec); uk[g] = sm_load4(u, i + g * stride, V, uvec); }
     }
     __syncthreads();
-    uint32_t* g = wk.rbins + r * SM_RBINS;
+    uint32_t* g = wk.rbins(r);
     for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) if (h[i]) atomicAdd(&g[i], h[i]);
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
     for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) { h[i] = sm_peek(&g[i]); g[i] = 0; }
@@ -971,7 +1300,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
     st.kept = kept;
     st.candidates = 0;
     st.take = take;
-    st.prefix = (unsigned long long)(bin.bin < 0 ? 0 : bin.bin);
+    st.prefix = (uint32_t)(bin.bin < 0 ? 0 : bin.bin);
     st.ended = 0;
     if (bin.total <= (unsigned long long)n) { st.ended = 1; st.zone_lo = 1u; st.zone_hi = 0u; }        // whatever is left wins: nothing to rank
 }
@@ -983,21 +1312,26 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, lon
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
-    SmRowState& st = wk.state[r];
+    SmRowState& st = wk.state(r);
     if (st.ended) return;
     const uint32_t* keys = wk.keys + r * wk.vpad;
-    const uint32_t prefix = (uint32_t)st.prefix;
+    const uint32_t prefix = st.prefix;
     const int nbins = 1 << SM_RBITS2, at = 32 - SM_RBITS1 - SM_RBITS2;
     for (int i = threadIdx.x; i < nbins; i += SM_LTPB) h[i] = 0;
     __syncthreads();
-    for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += wk.B * SM_LTPB * 4) {
-        const LgVec4<uint32_t> o = *(const LgVec4<uint32_t>*)(keys + i);
+    const long long stride = wk.B * SM_LTPB * 4;
+    for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += 4 * stride) {
+        LgVec4<uint32_t> o[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (o.v[j] && (o.v[j] >> (32 - SM_RBITS1)) == prefix) atomicAdd(&h[sm_slot((int)(o.v[j] >> at) & (nbins - 1), SM_RBITS2 - 6)], 1u);
+        for (int g = 0; g < 4; g++) o[g] = i + g * stride < V ? *(const LgVec4<uint32_t>*)(keys + i + g * stride) : LgVec4<uint32_t>{ { 0, 0, 0, 0 } };
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (o[g].v[j] && (o[g].v[j] >> (32 - SM_RBITS1)) == prefix) atomicAdd(&h[sm_slot((int)(o[g].v[j] >> at) & (nbins - 1), SM_RBITS2 - 6)], 1u);
     }
     __syncthreads();
-    uint32_t* g = wk.rbins + r * SM_RBINS;
+    uint32_t* g = wk.rbins(r);
     for (int i = threadIdx.x; i < nbins; i += SM_LTPB) if (h[i]) atomicAdd(&g[i], h[i]);
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
     for (int i = threadIdx.x; i < nbins; i += SM_LTPB) h[i] = sm_peek(&g[i]);
@@ -1011,16 +1345,18 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, lon
     st.zone_hi = zone.hi;
 }
 
+#define SM_ZTILES 4096                 // tiles whose winners are counted in LDS
 // winners as a bit per element, the zone's elements as a list, winners counted per tile; the last workgroup ranks the list
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                           long long V, long long n, SmRule rule, SmWork wk, int step)
 {
-    __shared__ union { SmHist hist; unsigned long long rank[SM_BINS]; } h;
+    __shared__ union { SmHist hist; struct { unsigned long long rank[SM_BINS]; uint32_t index[SM_BINS]; }; } h;
+    __shared__ uint32_t wins[SM_ZTILES];
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
-    SmRowState& st = wk.state[r];
+    SmRowState& st = wk.state(r);
     const uint32_t zlo = st.zone_lo, zhi = st.zone_hi;
     const uint32_t* keys = wk.keys + r * wk.vpad;
     unsigned long long* words = wk.words + r * wk.tiles * (SM_TILE / 64);
@@ -1050,9 +1386,15 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
     }
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
     unsigned long long mine = 0, sure;
-    for (long long t = threadIdx.x; t < wk.tiles; t += SM_LTPB) mine += sm_peek(&tile_n[t]);
-    sm_block_scan<unsigned long long>(mine, sc.a, sure);
+    const bool in_lds = wk.tiles <= SM_ZTILES;
     const uint32_t found = sm_peek(&st.candidates);
+    for (uint32_t a = threadIdx.x; a < found && a < SM_BINS; a += SM_LTPB) h.index[a] = sm_peek(&list[a]);
+    for (long long t = threadIdx.x; t < wk.tiles; t += SM_LTPB) {
+        const uint32_t c = sm_peek(&tile_n[t]);
+        mine += c;
+        if (in_lds) wins[t] = c;
+    }
+    sm_block_scan<unsigned long long>(mine, sc.a, sure);
     const T* x = scores + r * sstride;
     u += r * ustride;
     const bool logits = rule.mode == SM_LOGITS;
@@ -1064,20 +1406,17 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
     };
     auto win = [&](uint32_t i) {
         atomicOr(&words[i >> 6], 1ull << (i & 63));
-        atomicAdd(&tile_n[i / SM_TILE], 1u);
+        if (in_lds) atomicAdd(&wins[i / SM_TILE], 1u); else atomicAdd(&tile_n[i / SM_TILE], 1u);
     };
     const unsigned long long room = (unsigned long long)n - sure;      // winners still to be named
     if (found <= (uint32_t)wk.capacity && found <= SM_BINS) {
-        for (uint32_t a = threadIdx.x; a < found; a += SM_LTPB) h.rank[a] = race((long long)sm_peek(&list[a]));
+        for (uint32_t a = threadIdx.x; a < found; a += SM_LTPB) h.rank[a] = race((long long)h.index[a]);
         __syncthreads();
         for (uint32_t a = threadIdx.x; a < found; a += SM_LTPB) {
-            const uint32_t i = sm_peek(&list[a]);
+            const uint32_t i = h.index[a];
             const unsigned long long k = h.rank[a];
-            unsigned long long ahead = 0;
-            for (uint32_t c = 0; c < found && ahead < room; c++) {
-                const unsigned long long o = h.rank[c];
-                ahead += o > k || (o == k && c != a && sm_peek(&list[c]) < i);
-            }
+            uint32_t ahead = 0;
+            for (uint32_t c = 0; c < found; c++) ahead += h.rank[c] > k || (h.rank[c] == k && h.index[c] < i);
             if (ahead < room) win(i);
         }
     } else {
@@ -1137,13 +1476,13 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
             if (k != 0ull && (k > thr || (k == thr && i <= last))) win(i);
         }
     }
-    __threadfence();
+    if (!in_lds) __threadfence();
     __syncthreads();
     // tiles' first positions in the output
     unsigned long long run = 0;
     for (long long base = 0; base < wk.tiles; base += SM_LTPB) {
         const long long t = base + threadIdx.x;
-        const uint32_t c = t < wk.tiles ? sm_peek(&tile_n[t]) : 0u;
+        const uint32_t c = t < wk.tiles ? (in_lds ? wins[t] : sm_peek(&tile_n[t])) : 0u;
         unsigned long long total;
         const unsigned long long before = sm_block_scan<unsigned long long>(c, sc.a, total);
         if (t < wk.tiles) tile_n[t] = (uint32_t)(run + before);
@@ -1169,7 +1508,7 @@ __global__ void __launch_bounds__(SM_TILE / 64) sm_emit_kernel(long long n, SmWo
         at++;
     }
     // the row's end where fewer than n were left
-    const long long m = (long long)wk.state[r].sure;
+    const long long m = (long long)wk.state(r).sure;
     for (long long j = m + t * (SM_TILE / 64) + threadIdx.x; j < n; j += wk.tiles * (SM_TILE / 64)) out[j] = -1;
 }
 
@@ -1182,79 +1521,130 @@ static bool sm_rule(int logits, double temperature, long long top_k, double top_
 }
 
 
-// lays the workspace out; returns its size in bytes.  The cleared part (states, histograms) comes first.
-static long long sm_layout(long long R, long long V, bool distinct, char* base, SmWork& w, long long& clear_bytes)
+// How a call runs.  Short rows: one workgroup each.  Long ones: the filters by levels of a histogram, or, for 16-bit scores, from one histogram
+// of all keys where its 256 KB a row are little next to the work (R rows at most); what a small top-k leaves goes on as a short row.
+struct SmPlan { bool is_short, top_k, top_p, counts, few; };
+#define SM_COUNTS_ROWS 256
+
+static SmPlan sm_plan(long long R, long long V, int bytes, long long top_k, double top_p)
+{
+    SmPlan p;
+    p.is_short = V <= SM_SHORT;
+    p.top_k = top_k > 0 && top_k < V;
+    p.top_p = top_p < 1.0;
+    p.counts = bytes == 2 && (p.top_k || p.top_p) && R <= SM_COUNTS_ROWS;
+    p.few = p.top_k && top_k <= SM_SHORT;
+    return p;
+}
+
+// lays the workspace out; returns its size in bytes
+static long long sm_layout(const SmPlan& plan, long long R, long long V, int bytes, bool distinct, long long top_k, char* base, SmWork& w)
 {
     char* p = base;
-    auto take = [&](long long bytes) { char* at = p; p += (bytes + 255) & ~255ll; return at; };
-    w.state = (SmRowState*)take(R * (long long)sizeof(SmRowState));
-    w.hist = (SmHist*)take(R * (long long)sizeof(SmHist));
-    w.rbins = distinct ? (uint32_t*)take(R * SM_RBINS * 4) : nullptr;
-    clear_bytes = p - base;
+    auto align = [](long long b) { return (b + 255) & ~255ll; };
+    auto take = [&](bool want, long long b) { char* at = p; if (want) p += align(b); return at; };
+    const bool race = distinct && !plan.few;
+    w.rbins_at = align(sizeof(SmRowState));
+    w.hist_at = w.rbins_at + (race ? align(SM_RBINS * 4) : 0);
+    w.clear_bytes = w.hist_at + (plan.counts ? 65536 * 4 : plan.top_k || plan.top_p ? align(sizeof(SmHist)) : 0);
     w.tiles = (V + SM_TILE - 1) / SM_TILE;
     w.stiles = (V + SM_STILE - 1) / SM_STILE;
     w.vpad = (V + 3) & ~3ll;
     w.capacity = V / 256 > 4096 ? V / 256 : 4096;
+    // 256 workgroups fill the chip, and every further one adds its histogram to the same words of memory
     const long long want = (V + SM_LTPB * 8 - 1) / (SM_LTPB * 8), most = R >= 256 ? 1 : 256 / R;
     w.B = want < most ? want : most;
-    w.tile_n = (uint32_t*)take(R * w.tiles * 4);
-    w.keys = nullptr; w.words = nullptr; w.list = nullptr; w.group = w.tile_sum = w.tile_top = nullptr;
-    if (distinct) {
-        w.keys = (uint32_t*)take(R * w.vpad * 4);
-        w.words = (unsigned long long*)take(R * w.tiles * (SM_TILE / 64) * 8);
-        w.list = (uint32_t*)take(R * w.capacity * 4);
-    } else {
-        w.group = (double*)take(R * w.stiles * (SM_STILE / SM_GROUP) * 8);
-        w.tile_sum = (double*)take(R * (w.stiles + 1) * 8);
-        w.tile_top = (double*)take(R * w.stiles * 8);
-    }
+    w.clear = take(true, R * w.clear_bytes);
+    w.best = (uint32_t*)take(true, R * w.B * 4);
+    w.tile_n = (uint32_t*)take(true, R * w.tiles * 4);
+    w.tile_eq = (uint32_t*)take(true, R * w.tiles * 4);
+    w.names = (uint32_t*)take(plan.few, R * top_k * 4);
+    w.few = take(plan.few, R * top_k * bytes);
+    w.few_u = take(plan.few && distinct, R * top_k * 4);
+    w.keys = (uint32_t*)take(race, R * w.vpad * 4);
+    w.words = (unsigned long long*)take(race, R * w.tiles * (SM_TILE / 64) * 8);
+    w.list = (uint32_t*)take(race, R * w.capacity * 4);
+    const bool sums = !distinct && !plan.few;
+    w.group = (double*)take(sums, R * w.stiles * (SM_STILE / SM_GROUP) * 8);
+    w.tile_sum = (double*)take(sums, R * w.stiles * 8);
+    w.tile_top = (double*)take(sums, R * w.stiles * 8);
     return p - base;
+}
+
+template <typename T>
+static void sample_short(const T* scores, long long ss, const float* u, long long us, long long R, long long V, long long n, const SmRule& rule,
+                         const uint32_t* names, long long* out, bool distinct, hipStream_t s)
+{
+    // many draws of few rows: several workgroups filter the row again and share its draws (binary searches, 4096 of them cost a filtering)
+    const long long share = (n + 4095) / 4096, most = R < 256 ? 256 / R : 1;
+    const dim3 grid((unsigned)R, distinct ? 1u : (unsigned)(share < most ? share : most));
+#define SM_LAUNCH_SHORT(TPB_, EPT_)                                                                                                                            \
+    do {                                                                                                                                                       \
+        if (distinct) hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, true>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, names, out);  \
+        else hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, false>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, names, out);          \
+    } while (0)
+    if (V <= 1024) SM_LAUNCH_SHORT(256, 4);
+    else if (V <= 4096) SM_LAUNCH_SHORT(1024, 4);
+    else SM_LAUNCH_SHORT(960, 16);
+#undef SM_LAUNCH_SHORT
 }
 
 template <typename T>
 static int sample_launch(const T* scores, long long ss, const float* u, long long us, long long R, long long V, long long n,
                          const SmRule& rule, long long* out, bool distinct, void* temp, long long temp_bytes, hipStream_t s)
 {
-    if (V <= SM_SHORT) {
-        const dim3 grid((unsigned)R);
-#define SM_LAUNCH_SHORT(TPB_, EPT_)                                                                                                                    \
-        do {                                                                                                                                           \
-            if (distinct) hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, true>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, out);  \
-            else hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, false>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, out);     \
-        } while (0)
-        if (V <= 1024) SM_LAUNCH_SHORT(256, 4);
-        else if (V <= 4096) SM_LAUNCH_SHORT(1024, 4);
-        else SM_LAUNCH_SHORT(960, 16);
-#undef SM_LAUNCH_SHORT
+    const SmPlan plan = sm_plan(R, V, (int)sizeof(T), rule.top_k, rule.top_p);
+    if (plan.is_short) {
+        sample_short(scores, ss, u, us, R, V, n, rule, nullptr, out, distinct, s);
         LG_RETURN_LAST();
     }
     SmWork wk;
-    long long clear_bytes;
-    const long long need = sm_layout(R, V, distinct, (char*)temp, wk, clear_bytes);
-    if (temp == nullptr || temp_bytes < need || (uintptr_t)temp % 16 != 0 || R * wk.B > 0x7fffffffll || R * wk.tiles > 0x7fffffffll) return (int)hipErrorInvalidValue;
+    const long long need = sm_layout(plan, R, V, (int)sizeof(T), distinct, rule.top_k, (char*)temp, wk);
+    const long long draws = R * ((n + 255) / 256);
+    if (temp == nullptr || temp_bytes < need || (uintptr_t)temp % 16 != 0 || R * wk.tiles > 0x7fffffffll || draws > 0x7fffffffll) return (int)hipErrorInvalidValue;
     const dim3 grid((unsigned)(R * wk.B)), block(SM_LTPB);
-    const long long words = clear_bytes / 16, cblocks = (words + 255) / 256;
-    hipLaunchKernelGGL(sm_clear_kernel, dim3((unsigned)(cblocks < 2048 ? cblocks : 2048)), dim3(256), 0, s, (uint4*)temp, words);
     int step = 0;
-    const bool top_k = rule.top_k > 0 && rule.top_k < V, top_p = rule.top_p < 1.0;
-    if (top_p || rule.min_p > 0.0) hipLaunchKernelGGL((sm_best_kernel<T>), grid, block, 0, s, scores, ss, V, rule, wk, step++);
-    for (int pass = 0; pass < 2; pass++) {
-        if (!(pass == 0 ? top_k : top_p)) continue;
-        for (int shift = 32; shift > (sizeof(T) == 2 ? 10 : 0); ) {
-            const int width = shift >= 11 ? 11 : shift;
-            if (pass == 0) hipLaunchKernelGGL((sm_level_kernel<T, false>), grid, block, 0, s, scores, ss, V, rule, wk, step++, shift, width);
-            else hipLaunchKernelGGL((sm_level_kernel<T, true>), grid, block, 0, s, scores, ss, V, rule, wk, step++, shift, width);
-            shift -= width;
+    const int want_best = (plan.top_p && !plan.counts) || rule.min_p > 0.0;
+    hipLaunchKernelGGL((sm_begin_kernel<T>), grid, block, 0, s, scores, ss, V, rule, wk, want_best);
+    if (plan.counts) {
+        if constexpr (sizeof(T) == 2) {
+            SmWork cw = wk;                                            // counters of 16 bits: a bounded share of the row each
+            const long long shares = (V + SM_SHARE16 - 1) / SM_SHARE16;
+            cw.B = shares > wk.B ? shares : wk.B;
+            if (R * cw.B > 0x7fffffffll) return (int)hipErrorInvalidValue;
+            hipLaunchKernelGGL((sm_count16_kernel<T>), dim3((unsigned)(R * cw.B)), dim3(1024), 0, s, scores, ss, V, rule, cw, step++, (int)plan.top_k, (int)plan.top_p);
         }
-        hipLaunchKernelGGL((sm_tie_kernel<T>), grid, block, 0, s, scores, ss, V, rule, wk, step++);
+    }
+    for (int pass = 0; pass < 2; pass++) {
+        if (plan.counts ? pass == 0 : !(pass == 0 ? plan.top_k : plan.top_p && !plan.few)) continue;
+        if (!plan.counts)
+            for (int shift = 32; shift > 0; ) {
+                const int width = shift >= 11 ? 11 : shift;
+                if (pass == 0) hipLaunchKernelGGL((sm_level_kernel<T, false>), grid, block, 0, s, scores, ss, V, rule, wk, step++, shift, width);
+                else hipLaunchKernelGGL((sm_level_kernel<T, true>), grid, block, 0, s, scores, ss, V, rule, wk, step++, shift, width);
+                shift -= width;
+            }
+        SmWork tw = wk;
+        tw.B = wk.tiles < 256 ? wk.tiles : 256;
+        const dim3 tgrid((unsigned)(R * tw.B));
+        if (plan.few) hipLaunchKernelGGL((sm_cut_kernel<T, true>), tgrid, block, 0, s, scores, ss, V, rule, tw, step++);
+        else hipLaunchKernelGGL((sm_cut_kernel<T, false>), tgrid, block, 0, s, scores, ss, V, rule, tw, step++);
+    }
+    if (plan.few) {
+        const long long K = rule.top_k;
+        hipLaunchKernelGGL((sm_gather_kernel<T>), dim3((unsigned)(R * wk.tiles)), block, 0, s, scores, ss, distinct ? u : nullptr, us, V, rule, wk);
+        SmRule rest = rule;
+        rest.top_k = 0;
+        if (plan.counts) rest.top_p = 1.0;
+        if (distinct) sample_short((const T*)wk.few, K, (const float*)wk.few_u, K, R, K, n, rest, wk.names, out, true, s);
+        else sample_short((const T*)wk.few, K, u, us, R, K, n, rest, wk.names, out, false, s);
+        LG_RETURN_LAST();
     }
     if (!distinct) {
         SmWork sw = wk;
         sw.B = wk.stiles < 2 * wk.B ? wk.stiles : 2 * wk.B;
-        hipLaunchKernelGGL((sm_sums_kernel<T>), dim3((unsigned)(R * sw.B)), dim3(256), 0, s, scores, ss, V, rule, sw, step++);
-        const long long blocks = (R * n + 255) / 256;
-        if (blocks > 0x7fffffffll) return (int)hipErrorInvalidValue;
-        hipLaunchKernelGGL((sm_draw_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, scores, ss, u, us, R, V, n, rule, sw, out);
+        hipLaunchKernelGGL((sm_sums_kernel<T>), dim3((unsigned)(R * sw.B)), dim3(256), 0, s, scores, ss, V, rule, sw, wk, step++);
+        hipLaunchKernelGGL((sm_draw_kernel<T>), dim3((unsigned)draws), dim3(256), 0, s, scores, ss, u, us, R, V, n, rule, wk, out);
         LG_RETURN_LAST();
     }
     hipLaunchKernelGGL((sm_race_kernel<T>), grid, block, 0, s, scores, ss, u, us, V, n, rule, wk, step++);
@@ -1266,12 +1656,12 @@ static int sample_launch(const T* scores, long long ss, const float* u, long lon
     LG_RETURN_LAST();
 }
 
-LG_API long long lg_sample_temp_bytes(long long R, long long V, long long n, int distinct)
+LG_API long long lg_sample_temp_bytes(long long R, long long V, long long n, int dtype, int distinct, long long top_k, double top_p)
 {
     if (R <= 0 || n <= 0 || V <= SM_SHORT || V >= (1ll << 31)) return 0;
+    const int bytes = dtype == LG_F32 ? 4 : 2;
     SmWork w;
-    long long clear_bytes;
-    return sm_layout(R, V, distinct != 0, nullptr, w, clear_bytes);
+    return sm_layout(sm_plan(R, V, bytes, top_k, top_p), R, V, bytes, distinct != 0, top_k, nullptr, w);
 }
 
 LG_API int lg_sample(const void* scores, int dtype, long long score_stride, const float* u, long long u_stride, long long R, long long V,

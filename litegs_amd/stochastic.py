@@ -159,7 +159,7 @@ def _sample(what: str, scores, u, n: int, distinct: bool, temperature, top_k, to
         _C.sample(x, uu, out, n, distinct, bool(logits), temperature, top_k, top_p, min_p)
         return out
     L = lib()
-    tb = L.lg_sample_temp_bytes(R, V, n, int(distinct))
+    tb = L.lg_sample_temp_bytes(R, V, n, _DTYPES[x.dtype], int(distinct), top_k, top_p)
     temp = torch.empty((max(tb, 1),), dtype=torch.uint8, device=x.device)
     with _on(x.device):
         check(L.lg_sample(x.data_ptr(), _DTYPES[x.dtype], x.stride(0), uu.data_ptr(), uu.stride(0), R, V, n, int(distinct), int(bool(logits)),

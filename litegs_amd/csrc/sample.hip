@@ -108,6 +108,52 @@ __device__ __forceinline__ double sm_mass(const SmScale& s, uint32_t key)
     if (key == 0u) return 0.0;
     return s.mode == SM_LINEAR ? sm_value(key) : sm_exp(sm_log(s, key) - s.top);
 }
+// The same masses in about a third of the instructions, for passes over whole rows, with two tables in LDS that each workgroup works out for
+// itself: 1 / c and log c for the middles c of 128 parts of [1, 2) -- a score has 24 bits, m / c - 1 is one product, below 1 / 256, and six
+// terms of its logarithm remain -- and 2^(j / 64): five terms of the exponential.  Good to two steps of the logarithm, as the above.
+struct SmTables { double inv[128], log[128], exp[64]; };
+
+__device__ __forceinline__ void sm_tables(SmTables& t, int mode)      // a barrier has to follow
+{
+    const int k = threadIdx.x;
+    if (mode == SM_POWER && k < 128) {
+        const double inv = 1.0 / (1.0 + (k + 0.5) * 0x1p-7);
+        t.inv[k] = inv;
+        t.log[k] = -sm_ln(inv);
+    }
+    if (mode != SM_LINEAR && k >= 128 && k < 192) t.exp[k - 128] = 2.0 * sm_exp((k - 192) * (0.69314718055994531 / 64));
+}
+__device__ __forceinline__ double sm_exp(const SmTables& t, double x)
+{
+    x = fmax(x, -800.0);
+    const double k = rint(x * 92.332482616893657);                     // 64 / ln 2
+    const double r = fma(k, -1.90821492927058770e-10 / 64, fma(k, -6.93147180369123816e-01 / 64, x));
+    double p = fma(r, 1.0 / 120, 1.0 / 24);
+    p = fma(r, p, 1.0 / 6);
+    p = fma(r, p, 0.5);
+    const int i = (int)k;
+    const double e = t.exp[i & 63];
+    return ldexp(fma(e, fma(r * r, p, r), e), i >> 6);
+}
+__device__ __forceinline__ double sm_ln(const SmTables& t, float x)
+{
+    const bool small = x < 0x1p-126f;
+    const uint32_t b = __float_as_uint(small ? x * 0x1p32f : x);
+    const int i = (int)(b >> 16) & 127;
+    const double r = fma((double)__uint_as_float((b & 0x7fffffu) | 0x3f800000u), t.inv[i], -1.0), n = (double)((int)(b >> 23) - (small ? 159 : 127));
+    double p = fma(r, -1.0 / 6, 1.0 / 5);
+    p = fma(r, p, -1.0 / 4);
+    p = fma(r, p, 1.0 / 3);
+    p = fma(r, p, -0.5);
+    return fma(n, 6.93147180369123816e-01, fma(n, 1.90821492927058770e-10, t.log[i] + fma(r * r, p, r)));
+}
+__device__ __forceinline__ double sm_mass(const SmTables& t, const SmScale& s, uint32_t key)
+{
+    if (key == 0u) return 0.0;
+    const float x = __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+    return s.mode == SM_LINEAR ? (double)x : sm_exp(t, (s.mode == SM_LOGITS ? (double)x : sm_ln(t, x)) * s.inv_t - s.top);
+}
+
 // key of the exponential race, ordered as an unsigned integer; 0 = excluded
 __device__ __forceinline__ unsigned long long sm_race(const SmScale& s, uint32_t key, float u)
 {
@@ -228,7 +274,7 @@ template <bool MASS> __device__ __forceinline__ bool sm_room(const SmTake& t, ui
     return MASS ? sm_sum_value(SmSum{ t.before_m.hi + hi, t.before_m.lo + lo }) < t.target : (double)(t.before_n + n) < t.target;
 }
 
-// The lowest non-empty bin whose predecessors (the bins above it) leave room: a wave sums 2^p bins a lane, best first, scans, and does the
+// The lowest bin with anything in it (a mass, where mass is what counts) whose predecessors (the bins above it) leave room: a wave sums 2^p bins a lane, best first, scans, and does the
 // same once more inside the lane it ends in.  Updates take.before_* to the amount above that bin; bin -1: there is none.  All threads call it
 // behind a barrier; a barrier has to follow before the histogram or sc is written again.
 template <bool MASS, bool PACKED = false>
@@ -248,7 +294,7 @@ __device__ SmBin sm_boundary(const uint32_t* hn, const unsigned long long* hhi, 
         const uint32_t in = sm_wave_scan<false>(n, SmAdd());
         unsigned long long ihi = 0, ilo = 0;
         if (MASS) { ihi = sm_wave_scan<false>(hi, SmAdd()); ilo = sm_wave_scan<false>(lo, SmAdd()); }
-        const unsigned long long enter = __ballot(n != 0 && sm_room<MASS>(take, in - n, ihi - hi, ilo - lo));
+        const unsigned long long enter = __ballot((MASS ? (hi | lo) != 0 : n != 0) && sm_room<MASS>(take, in - n, ihi - hi, ilo - lo));
         const uint32_t total = sm_lane(in, 63);
         int bin = -1;
         uint32_t bn = take.before_n, count = 0;
@@ -267,7 +313,7 @@ __device__ SmBin sm_boundary(const uint32_t* hn, const unsigned long long* hhi, 
             const uint32_t in2 = sm_wave_scan<false>(n2, SmAdd());
             if (MASS) { ihi2 = sm_wave_scan<false>(hi2, SmAdd()); ilo2 = sm_wave_scan<false>(lo2, SmAdd()); }
             const SmTake inner = { take.target, bn, bm };
-            const int l2 = 63 - __clzll((long long)__ballot(n2 != 0 && sm_room<MASS>(inner, in2 - n2, ihi2 - hi2, ilo2 - lo2)));
+            const int l2 = 63 - __clzll((long long)__ballot((MASS ? (hi2 | lo2) != 0 : n2 != 0) && sm_room<MASS>(inner, in2 - n2, ihi2 - hi2, ilo2 - lo2)));
             bin = ((63 - l) << p) | (per - 1 - l2);
             bn += sm_lane(in2 - n2, l2);
             count = sm_lane(n2, l2);
@@ -717,6 +763,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
                                                            int shift, int width)
 {
     __shared__ SmHist h;
+    __shared__ SmTables tables;
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
     constexpr int G = MASS ? 2 : 4;                                    // groups of four loaded ahead
@@ -737,6 +784,8 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     const uint32_t best = MASS ? (first ? sm_best(wk, r) : st.best) : 0u;
     const SmScale scale = sm_scale(rule, best);
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
+    const bool counted = !MASS || at == 0;                             // masses need no counts before the last level
+    if (MASS) sm_tables(tables, rule.mode);
     for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { h.n[k] = 0; if (MASS) { h.hi[k] = 0; h.lo[k] = 0; } }
     __syncthreads();
     while (i < V) {
@@ -747,9 +796,9 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
                 const uint32_t key = sm_key(v[g].v[j], logits);
                 if (!sm_in(kept, key, (uint32_t)(i + g * stride + j)) || (!first && (key >> shift) != prefix)) continue;
                 const int bin = sm_slot((int)(key >> at) & (nbins - 1), p);
-                atomicAdd(&h.n[bin], 1u);
+                if (counted) atomicAdd(&h.n[bin], 1u);
                 if (MASS) {
-                    const SmLimbs m = sm_limbs(sm_mass(scale, key) * unit);
+                    const SmLimbs m = sm_limbs(sm_mass(tables, scale, key) * unit);
                     if (m.hi) atomicAdd(&h.hi[bin], (unsigned long long)m.hi);
                     if (m.lo) atomicAdd(&h.lo[bin], (unsigned long long)m.lo);
                 }
@@ -762,15 +811,26 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     __syncthreads();
     if (wk.B > 1) {
         SmHist& g = wk.hist(r);
-        for (int k = threadIdx.x; k < nbins; k += SM_LTPB)
-            if (h.n[k]) {
-                atomicAdd(&g.n[k], h.n[k]);
-                if (MASS) { if (h.hi[k]) atomicAdd(&g.hi[k], h.hi[k]); if (h.lo[k]) atomicAdd(&g.lo[k], h.lo[k]); }
-            }
+        for (int k = threadIdx.x; k < nbins; k += SM_LTPB) {
+            if (counted && h.n[k]) atomicAdd(&g.n[k], h.n[k]);
+            if (MASS) { if (h.hi[k]) atomicAdd(&g.hi[k], h.hi[k]); if (h.lo[k]) atomicAdd(&g.lo[k], h.lo[k]); }
+        }
         if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
-        for (int k = threadIdx.x; k < nbins; k += SM_LTPB) {           // taken over, and left clear for the next level
-            h.n[k] = sm_peek(&g.n[k]); g.n[k] = 0;
-            if (MASS) { h.hi[k] = sm_peek(&g.hi[k]); h.lo[k] = sm_peek(&g.lo[k]); g.hi[k] = 0; g.lo[k] = 0; }
+        // taken over (all loads before the first store: each is a round trip to memory), and left clear for the next level
+        constexpr int K = SM_BINS / SM_LTPB;
+        uint32_t n[K];
+        unsigned long long hi[K], lo[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int at = k * SM_LTPB + threadIdx.x;
+            n[k] = counted ? sm_peek(&g.n[at]) : 0u;
+            if (MASS) { hi[k] = sm_peek(&g.hi[at]); lo[k] = sm_peek(&g.lo[at]); }
+        }
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int at = k * SM_LTPB + threadIdx.x;
+            h.n[at] = n[k]; g.n[at] = 0;
+            if (MASS) { h.hi[at] = hi[k]; h.lo[at] = lo[k]; g.hi[at] = 0; g.lo[at] = 0; }
         }
         __syncthreads();
     }
@@ -795,7 +855,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     if (bin.bin < 0) { st.ended = 1; return; }                         // no candidate: the filter in force (or an empty row) stands
     const uint32_t found = (first ? 0u : prefix << width) | (uint32_t)bin.bin;
     st.prefix = found;
-    const bool whole = sm_whole_bin<MASS>(take, bin.count);
+    const bool whole = counted && sm_whole_bin<MASS>(take, bin.count);
     if (!whole && at > 0) return;
     // the key is found, or the lowest key of a bin that is taken whole; a cut among the equal ones is left to sm_cut_kernel
     const uint32_t thr = found << at;
@@ -1097,12 +1157,14 @@ __device__ __forceinline__ SmKept sm_final(const SmWork& wk, long long r, const 
 template <typename T>
 __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, SmWork whole, int step)
 {
+    __shared__ SmTables tables;
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
     SmRowState& st = wk.state(r);
     const T* x = scores + r * sstride;
     const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    sm_tables(tables, rule.mode);                                      // (the scans below are the barrier)
     const SmKept kept = sm_final(whole, r, st, rule);
     double *sums = wk.tile_sum + r * wk.stiles, *tops = wk.tile_top + r * wk.stiles, *groups = wk.group + r * wk.stiles * (SM_STILE / SM_GROUP);
     for (long long t = b; t < wk.stiles; t += wk.B) {
@@ -1121,7 +1183,7 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
         const SmScale scale = sm_scale(rule, best);
         double sum = 0.0, total, most;
 #pragma unroll
-        for (int k = 0; k < SM_GROUP; k++) sum += sm_mass(scale, key[k]);
+        for (int k = 0; k < SM_GROUP; k++) sum += sm_mass(tables, scale, key[k]);
         const double before = sm_block_scan<double>(sum, sc.a, total);
         groups[t * (SM_STILE / SM_GROUP) + threadIdx.x] = sm_block_rise(sum > 0.0 ? before + sum : 0.0, sc.b, most);
         if (threadIdx.x == 0) {
@@ -1147,7 +1209,7 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
         }
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            if (rule.mode != SM_LINEAR) mass[k] = tt[k] == -INFINITY ? 0.0 : mass[k] * sm_exp(tt[k] - top);
+            if (rule.mode != SM_LINEAR) mass[k] = tt[k] == -INFINITY ? 0.0 : mass[k] * sm_exp(tables, tt[k] - top);
             sum += mass[k];
         }
         double at = run + sm_block_scan<double>(sum, sc.a, total);
@@ -1198,10 +1260,12 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
                                                       long long R, long long V, long long n, SmRule rule, SmWork wk, long long* __restrict__ out)
 {
     __shared__ double ends[SM_DRAW_ENDS];
+    __shared__ SmTables tables;
     const long long blocks = (n + 255) / 256, r = blockIdx.x / blocks, j = blockIdx.x % blocks * 256 + threadIdx.x, at = r * n + j;
     const SmRowState& st = wk.state(r);
     const double* sums = wk.tile_sum + r * wk.stiles;
     const int tiles = (int)wk.stiles, group = (tiles + SM_DRAW_ENDS - 1) / SM_DRAW_ENDS, ngroups = (tiles + group - 1) / group;
+    sm_tables(tables, rule.mode);
     for (int k = threadIdx.x; k < ngroups; k += 256) ends[k] = sums[((k + 1) * group < tiles ? (k + 1) * group : tiles) - 1];
     __syncthreads();
     if (j >= n) return;
@@ -1218,7 +1282,7 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
     if (t >= tiles) t = tile_of([&](double s) { return s >= total; });                                  // rounding, or u >= 1: where the masses end
     const double* g = wk.group + (r * wk.stiles + t) * (long long)(SM_STILE / SM_GROUP);
     const int ng = SM_STILE / SM_GROUP;
-    const double scale_up = rule.mode == SM_LINEAR ? 1.0 : sm_exp(tops[t] - st.top);
+    const double scale_up = rule.mode == SM_LINEAR ? 1.0 : sm_exp(tables, tops[t] - st.top);
     const double local = fmax((target - (t ? sums[t - 1] : 0.0)) / scale_up, 0.0), here = g[ng - 1];
     int k = sm_rank4(g, ng, [&](double s) { return s > local; });
     if (k >= ng) k = sm_rank4(g, ng, [&](double s) { return s >= here; });
@@ -1237,7 +1301,7 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
     for (int e = 0; e < SM_GROUP; e++) {
         const long long i = i0 + e;
         const uint32_t key = sm_key(v[e / 4].v[e % 4], rule.mode == SM_LOGITS);
-        const double w = sm_in(kept, key, (uint32_t)i) ? sm_mass(scale, key) : 0.0;
+        const double w = sm_in(kept, key, (uint32_t)i) ? sm_mass(tables, scale, key) : 0.0;
         acc += w;
         if (w > 0.0) { any = i; if (found < 0 && acc > local) found = i; }
     }
@@ -1292,7 +1356,11 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
     uint32_t* g = wk.rbins(r);
     for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) if (h[i]) atomicAdd(&g[i], h[i]);
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
-    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) { h[i] = sm_peek(&g[i]); g[i] = 0; }
+    uint32_t n4[SM_RBINS / SM_LTPB];
+#pragma unroll
+    for (int k = 0; k < SM_RBINS / SM_LTPB; k++) n4[k] = sm_peek(&g[k * SM_LTPB + threadIdx.x]);
+#pragma unroll
+    for (int k = 0; k < SM_RBINS / SM_LTPB; k++) { h[k * SM_LTPB + threadIdx.x] = n4[k]; g[k * SM_LTPB + threadIdx.x] = 0; }
     __syncthreads();
     SmTake take = { (double)n, 0, { 0, 0 } };
     const SmBin bin = sm_boundary<false>(h, nullptr, nullptr, SM_RBITS1 - 6, take, sc);
@@ -1352,7 +1420,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
                                                           long long V, long long n, SmRule rule, SmWork wk, int step)
 {
     __shared__ union { SmHist hist; struct { unsigned long long rank[SM_BINS]; uint32_t index[SM_BINS]; }; } h;
-    __shared__ uint32_t wins[SM_ZTILES];
+    __shared__ uint32_t wins[SM_ZTILES], ahead[SM_BINS];
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
@@ -1412,13 +1480,19 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
     if (found <= (uint32_t)wk.capacity && found <= SM_BINS) {
         for (uint32_t a = threadIdx.x; a < found; a += SM_LTPB) h.rank[a] = race((long long)h.index[a]);
         __syncthreads();
-        for (uint32_t a = threadIdx.x; a < found; a += SM_LTPB) {
-            const uint32_t i = h.index[a];
+        // `parts` threads share a candidate's comparisons
+        const uint32_t parts = found <= SM_LTPB / 8 ? 8 : found <= SM_LTPB / 2 ? 2 : 1, each = (found + parts - 1) / parts;
+        for (uint32_t a = threadIdx.x; a < found; a += SM_LTPB) ahead[a] = 0;
+        __syncthreads();
+        for (uint32_t q = threadIdx.x; q < found * parts; q += SM_LTPB) {
+            const uint32_t a = q / parts, part = q % parts, i = h.index[a];
             const unsigned long long k = h.rank[a];
-            uint32_t ahead = 0;
-            for (uint32_t c = 0; c < found; c++) ahead += h.rank[c] > k || (h.rank[c] == k && h.index[c] < i);
-            if (ahead < room) win(i);
+            uint32_t n = 0;
+            for (uint32_t c = part * each; c < found && c < (part + 1) * each; c++) n += h.rank[c] > k || (h.rank[c] == k && h.index[c] < i);
+            if (n) atomicAdd(&ahead[a], n);
         }
+        __syncthreads();
+        for (uint32_t a = threadIdx.x; a < found; a += SM_LTPB) if (ahead[a] < room) win(h.index[a]);
     } else {
         // many elements next to the border: all but equal keys in numbers.  Radix selection of the exact keys by this workgroup, over the list
         // or, where that was too short, over the row.

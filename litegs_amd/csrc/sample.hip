@@ -934,16 +934,22 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // chunk c: keys 64 c ... 64 c + 63, one a lane; wave w takes the chunks w, w + 16, ... (the scores that occur lie close together)
     uint32_t best = 0;
-    for (int c0 = 0; c0 < 64; c0 += 16) {
-        uint32_t n[16];
+    unsigned long long live = 0;                                       // chunks of this wave with a score in them
 #pragma unroll
-        for (int c = 0; c < 16; c++) n[c] = sm_peek(&counts[((c0 + c) * 16 + wave) * 64 + lane]);
+    for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t n[32];
 #pragma unroll
-        for (int c = 0; c < 16; c++) {
+        for (int c = 0; c < 32; c++) n[c] = sm_peek(&counts[((c0 + c) * 16 + wave) * 64 + lane]);
+#pragma unroll
+        for (int c = 0; c < 32; c++) {
             const int chunk = (c0 + c) * 16 + wave;
             const unsigned long long any = __ballot(n[c] != 0);
-            if (any) best = (uint32_t)(chunk * 64 + 63 - __clzll((long long)any));
-            const uint32_t sum = any ? sm_lane(sm_wave_scan<false>(n[c], SmAdd()), 63) : 0u;
+            uint32_t sum = 0;
+            if (any) {
+                best = (uint32_t)(chunk * 64 + 63 - __clzll((long long)any));
+                live |= 1ull << (c0 + c);
+                sum = sm_lane(sm_wave_scan<false>(n[c], SmAdd()), 63);
+            }
             if (lane == 0) h.chunk.n[chunk] = sum;
         }
     }
@@ -969,16 +975,27 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
             return m;
         };
         if (mass) {
-            for (int c = 0; c < 64; c++) {
-                const int chunk = c * 16 + wave;
-                SmSum m = { 0, 0 };
-                if (h.chunk.n[chunk] != 0 && (uint32_t)chunk * 64 + 63 >= cut_key) {          // (uniform over the wave)
-                    const uint32_t k = (uint32_t)chunk * 64 + lane;
-                    m = limbs(k, left(k));
+            h.chunk.hi[threadIdx.x] = 0;
+            h.chunk.lo[threadIdx.x] = 0;
+            __syncthreads();
+            // four chunks a round: their counts are four round trips to memory otherwise
+            for (unsigned long long todo = live; todo; ) {
+                uint32_t key[4], n[4];
+                int chunk[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    chunk[q] = todo ? (__ffsll((long long)todo) - 1) * 16 + wave : -1;
+                    todo &= todo - 1;
+                    key[q] = (uint32_t)(chunk[q] < 0 ? 0 : chunk[q]) * 64 + lane;
+                    n[q] = chunk[q] < 0 ? 0u : left(key[q]);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    SmSum m = limbs(key[q], n[q]);
                     m.hi = sm_lane(sm_wave_scan<false>(m.hi, SmAdd()), 63);
                     m.lo = sm_lane(sm_wave_scan<false>(m.lo, SmAdd()), 63);
+                    if (lane == 0 && chunk[q] >= 0) { h.chunk.hi[chunk[q]] = m.hi; h.chunk.lo[chunk[q]] = m.lo; }
                 }
-                if (lane == 0) { h.chunk.hi[chunk] = m.hi; h.chunk.lo[chunk] = m.lo; }
             }
             __syncthreads();
         }
@@ -1094,16 +1111,21 @@ __global__ void __launch_bounds__(SM_LTPB) sm_cut_kernel(const T* __restrict__ s
     }
     if (GATHER && threadIdx.x == 0) st.sure = run;
     if (tile < 0) return;
-    for (int k = 0; k < SM_TILE / SM_LTPB; k++) {
-        const long long i = tile * SM_TILE + k * SM_LTPB + threadIdx.x;
-        const uint32_t key = i < V ? sm_key(x[i], logits) : 0u;
-        const bool f = key != 0u && key == kept.thr && (uint32_t)i <= kept.last;
-        uint32_t total;
-        const uint32_t before = sm_block_scan<uint32_t>(f ? 1u : 0u, sc.a, total);
-        if (f && before + 1 == rest) { st.kept.last = (uint32_t)i; st.cut = 0; }
-        if (total >= rest) break;                                      // uniform
-        rest -= total;
+    // inside the tile: eight consecutive elements a thread
+    constexpr int E = SM_TILE / SM_LTPB;
+    const long long i0 = tile * SM_TILE + (long long)threadIdx.x * E;
+    LgVec4<T> v[E / 4];
+#pragma unroll
+    for (int g = 0; g < E / 4; g++) v[g] = sm_load4(x, i0 + 4 * g, V, vec);
+    uint32_t is = 0, total;
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+        const uint32_t key = sm_key(v[k / 4].v[k % 4], logits);
+        if (key != 0u && key == kept.thr && (uint32_t)(i0 + k) <= kept.last) is |= 1u << k;
     }
+    uint32_t before = sm_block_scan<uint32_t>(__popc(is), sc.a, total);
+#pragma unroll
+    for (int k = 0; k < E; k++) if (((is >> k) & 1) && ++before == rest) { st.kept.last = (uint32_t)(i0 + k); st.cut = 0; }
 }
 
 // what top-k left, in index order: scores, their names and (without replacement) their numbers; rule.top_k places a row, the last ones empty
@@ -1146,7 +1168,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_gather_kernel(const T* __restrict_
 __device__ __forceinline__ SmKept sm_final(const SmWork& wk, long long r, const SmRowState& st, const SmRule& rule)
 {
     SmKept kept = st.kept;
-    const uint32_t best = rule.min_p > 0.0 ? sm_best(wk, r) : 0u;
+    const uint32_t best = rule.min_p <= 0.0 ? 0u : wk.best ? sm_best(wk, r) : st.best;
     if (best) sm_min_p(sm_scale(rule, best), best, rule.min_p, kept);
     return kept;
 }
@@ -1629,7 +1651,7 @@ static long long sm_layout(const SmPlan& plan, long long R, long long V, int byt
     const long long want = (V + SM_LTPB * 8 - 1) / (SM_LTPB * 8), most = R >= 256 ? 1 : 256 / R;
     w.B = want < most ? want : most;
     w.clear = take(true, R * w.clear_bytes);
-    w.best = (uint32_t*)take(true, R * w.B * 4);
+    w.best = plan.counts ? nullptr : (uint32_t*)take(true, R * w.B * 4);        // (else the histogram of all keys tells)
     w.tile_n = (uint32_t*)take(true, R * w.tiles * 4);
     w.tile_eq = (uint32_t*)take(true, R * w.tiles * 4);
     w.names = (uint32_t*)take(plan.few, R * top_k * 4);
@@ -1678,7 +1700,7 @@ static int sample_launch(const T* scores, long long ss, const float* u, long lon
     if (temp == nullptr || temp_bytes < need || (uintptr_t)temp % 16 != 0 || R * wk.tiles > 0x7fffffffll || draws > 0x7fffffffll) return (int)hipErrorInvalidValue;
     const dim3 grid((unsigned)(R * wk.B)), block(SM_LTPB);
     int step = 0;
-    const int want_best = (plan.top_p && !plan.counts) || rule.min_p > 0.0;
+    const int want_best = !plan.counts && (plan.top_p || rule.min_p > 0.0);
     hipLaunchKernelGGL((sm_begin_kernel<T>), grid, block, 0, s, scores, ss, V, rule, wk, want_best);
     if (plan.counts) {
         if constexpr (sizeof(T) == 2) {
@@ -1716,7 +1738,7 @@ static int sample_launch(const T* scores, long long ss, const float* u, long lon
     }
     if (!distinct) {
         SmWork sw = wk;
-        sw.B = wk.stiles < 2 * wk.B ? wk.stiles : 2 * wk.B;
+        sw.B = wk.stiles < 5 * wk.B ? wk.stiles : 5 * wk.B;            // (five workgroups of four waves fit a CU)
         hipLaunchKernelGGL((sm_sums_kernel<T>), dim3((unsigned)(R * sw.B)), dim3(256), 0, s, scores, ss, V, rule, sw, wk, step++);
         hipLaunchKernelGGL((sm_draw_kernel<T>), dim3((unsigned)draws), dim3(256), 0, s, scores, ss, u, us, R, V, n, rule, wk, out);
         LG_RETURN_LAST();

@@ -147,11 +147,30 @@ __device__ __forceinline__ double sm_ln(const SmTables& t, float x)
     p = fma(r, p, -0.5);
     return fma(n, 6.93147180369123816e-01, fma(n, 1.90821492927058770e-10, t.log[i] + fma(r * r, p, r)));
 }
-__device__ __forceinline__ double sm_mass(const SmTables& t, const SmScale& s, uint32_t key)
+// N masses at once, without a branch between them: one after the other each waits for its own chain of some twenty dependent instructions
+template <int N> __device__ __forceinline__ void sm_masses(const SmTables& t, const SmScale& s, const uint32_t (&key)[N], double (&m)[N])
 {
-    if (key == 0u) return 0.0;
-    const float x = __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
-    return s.mode == SM_LINEAR ? (double)x : sm_exp(t, (s.mode == SM_LOGITS ? (double)x : sm_ln(t, x)) * s.inv_t - s.top);
+    bool any = false;
+#pragma unroll
+    for (int k = 0; k < N; k++) any = any || key[k] != 0u;
+    if (__ballot(any) == 0) {                                          // (the same for the wave)
+#pragma unroll
+        for (int k = 0; k < N; k++) m[k] = 0.0;
+        return;
+    }
+    double x[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) x[k] = (double)__uint_as_float((key[k] & 0x80000000u) ? (key[k] & 0x7fffffffu) : key[k] ? ~key[k] : 0x3f800000u);
+    if (s.mode == SM_POWER) {
+#pragma unroll
+        for (int k = 0; k < N; k++) x[k] = sm_ln(t, (float)x[k]);
+    }
+    if (s.mode != SM_LINEAR) {
+#pragma unroll
+        for (int k = 0; k < N; k++) x[k] = sm_exp(t, x[k] * s.inv_t - s.top);
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) m[k] = key[k] ? x[k] : 0.0;
 }
 
 // key of the exponential race, ordered as an unsigned integer; 0 = excluded
@@ -682,8 +701,8 @@ struct SmRowState {
     SmTake take;
     double total, top;                 // with replacement: total mass of the kept; the largest l
     unsigned long long sure;           // race: winners
-    uint32_t prefix, ties, best, ended, cut, zone_lo, zone_hi, candidates;
-    uint32_t ticket[SM_STEPS];
+    uint32_t prefix, ties, best, least, ended, cut, zone_lo, zone_hi, candidates;
+    uint32_t ticket[SM_STEPS], sub[16];
 };
 
 struct SmWork {                        // workspace of a call
@@ -706,14 +725,28 @@ template <typename V> __device__ __forceinline__ void sm_poke(V* p, V v) { __hip
 // The last workgroup of a row to get here.  What it reads of the others' work was written by device-wide atomics (adds, or sm_poke's stores, which
 // go through the XCD's own L2) and is read by sm_peek: each wave waits for its own to be done before the ticket is drawn, and no L2 has to be
 // written back (a release fence in every wave of every workgroup took longer than the pass over the data).
+__device__ __forceinline__ uint32_t sm_draw_ticket(uint32_t* t) { return __hip_atomic_fetch_add(t, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ bool sm_last_block(uint32_t* ticket, uint32_t blocks, uint32_t* lds)
 {
     if (blocks == 1) { __syncthreads(); return true; }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) *lds = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) *lds = sm_draw_ticket(ticket) == blocks - 1;
     __syncthreads();
-    return *lds == blocks - 1;
+    return *lds != 0;
+}
+// ... of many workgroups: adds to one word take 10 ns each, so sixteen groups draw among themselves first.  `sub`: sixteen cleared words
+__device__ __forceinline__ bool sm_last_block_of_many(uint32_t* ticket, uint32_t* sub, uint32_t block, uint32_t blocks, uint32_t* lds)
+{
+    if (blocks <= 128) return sm_last_block(ticket, blocks, lds);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t g = block & 15;
+        *lds = sm_draw_ticket(&sub[g]) == (blocks - g + 15) / 16 - 1 && sm_draw_ticket(ticket) == 15;
+    }
+    __syncthreads();
+    return *lds != 0;
 }
 
 // Clears the row's part of the workspace and, where a mass needs the row's best score, leaves the best of each workgroup's share.
@@ -789,20 +822,28 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { h.n[k] = 0; if (MASS) { h.hi[k] = 0; h.lo[k] = 0; } }
     __syncthreads();
     while (i < V) {
+        uint32_t key[4 * G];
 #pragma unroll
         for (int g = 0; g < G; g++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint32_t key = sm_key(v[g].v[j], logits);
-                if (!sm_in(kept, key, (uint32_t)(i + g * stride + j)) || (!first && (key >> shift) != prefix)) continue;
-                const int bin = sm_slot((int)(key >> at) & (nbins - 1), p);
-                if (counted) atomicAdd(&h.n[bin], 1u);
-                if (MASS) {
-                    const SmLimbs m = sm_limbs(sm_mass(tables, scale, key) * unit);
-                    if (m.hi) atomicAdd(&h.hi[bin], (unsigned long long)m.hi);
-                    if (m.lo) atomicAdd(&h.lo[bin], (unsigned long long)m.lo);
-                }
+                const uint32_t k = sm_key(v[g].v[j], logits);
+                key[4 * g + j] = sm_in(kept, k, (uint32_t)(i + g * stride + j)) && (first || (k >> shift) == prefix) ? k : 0u;
             }
+        double mass[4 * G];
+        if (MASS && first) sm_masses(tables, scale, key, mass);        // (later levels: few are left, one at a time)
+#pragma unroll
+        for (int j = 0; j < 4 * G; j++) {
+            if (key[j] == 0u) continue;
+            const int bin = sm_slot((int)(key[j] >> at) & (nbins - 1), p);
+            if (counted) atomicAdd(&h.n[bin], 1u);
+            if (MASS) {
+                if (!first) { const uint32_t one[1] = { key[j] }; double m[1]; sm_masses(tables, scale, one, m); mass[j] = m[0]; }
+                const SmLimbs m = sm_limbs(mass[j] * unit);
+                if (m.hi) atomicAdd(&h.hi[bin], (unsigned long long)m.hi);
+                if (m.lo) atomicAdd(&h.lo[bin], (unsigned long long)m.lo);
+            }
+        }
         i += G * stride;
         if (i >= V) break;
 #pragma unroll
@@ -1040,9 +1081,12 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
         cut_n = ties;
         __syncthreads();
     }
+    SmKept least = { 0u, SM_ALL };
+    if (best != 0 && rule.min_p > 0.0) sm_min_p(scale, best_key, rule.min_p, least);
     if (threadIdx.x != 0) return;
     st.before = kept;
     st.best = best_key;
+    st.least = least.thr;
     st.ended = 1;
     st.cut = 0;
     if (best != 0) sm_conclude(st, kept, sm_key_of16<T>(thr, logits), ties, equal);
@@ -1164,11 +1208,13 @@ __global__ void __launch_bounds__(SM_LTPB) sm_gather_kernel(const T* __restrict_
     for (long long j = (long long)st.sure + t * SM_LTPB + threadIdx.x; j < K; j += wk.tiles * SM_LTPB) few[j] = lg_from_float<T>(__uint_as_float(0x7fc00000u));
 }
 
-// filter in force with min-p (every wave works the cut out for itself)
+// filter in force with min-p (every wave works the cut out for itself where the histogram of all keys has not)
 __device__ __forceinline__ SmKept sm_final(const SmWork& wk, long long r, const SmRowState& st, const SmRule& rule)
 {
     SmKept kept = st.kept;
-    const uint32_t best = rule.min_p <= 0.0 ? 0u : wk.best ? sm_best(wk, r) : st.best;
+    if (rule.min_p <= 0.0) return kept;
+    if (!wk.best) return st.least > kept.thr ? SmKept{ st.least, SM_ALL } : kept;
+    const uint32_t best = sm_best(wk, r);
     if (best) sm_min_p(sm_scale(rule, best), best, rule.min_p, kept);
     return kept;
 }
@@ -1203,9 +1249,10 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
         }
         best = sm_block_max(best, sc.b);
         const SmScale scale = sm_scale(rule, best);
-        double sum = 0.0, total, most;
+        double mass[SM_GROUP], sum = 0.0, total, most;
+        sm_masses(tables, scale, key, mass);
 #pragma unroll
-        for (int k = 0; k < SM_GROUP; k++) sum += sm_mass(tables, scale, key[k]);
+        for (int k = 0; k < SM_GROUP; k++) sum += mass[k];
         const double before = sm_block_scan<double>(sum, sc.a, total);
         groups[t * (SM_STILE / SM_GROUP) + threadIdx.x] = sm_block_rise(sum > 0.0 ? before + sum : 0.0, sc.b, most);
         if (threadIdx.x == 0) {
@@ -1213,7 +1260,7 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
             sm_poke(&tops[t], best ? scale.top : -INFINITY);
         }
     }
-    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    if (!sm_last_block_of_many(&st.ticket[step], st.sub, (uint32_t)b, (uint32_t)wk.B, &ticket)) return;
     double top = -INFINITY;
     for (long long t = threadIdx.x; t < wk.stiles; t += 256) top = fmax(top, sm_peek(&tops[t]));
     const unsigned long long ordered = (unsigned long long)__double_as_longlong(top + 0.0);
@@ -1314,20 +1361,25 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
     const SmKept kept = st.kept;
     const long long i0 = (long long)t * SM_STILE + k * SM_GROUP;
     double acc = k ? g[k - 1] : 0.0;
-    long long found = -1, any = -1;
+    int found = -1, any = -1;
     LgVec4<T> v[SM_GROUP / 4];
     const bool vec = sm_aligned(x);
 #pragma unroll
     for (int e = 0; e < SM_GROUP / 4; e++) v[e] = sm_load4(x, i0 + 4 * e, V, vec);
+    uint32_t key[SM_GROUP];
+    double mass[SM_GROUP];
 #pragma unroll
     for (int e = 0; e < SM_GROUP; e++) {
-        const long long i = i0 + e;
-        const uint32_t key = sm_key(v[e / 4].v[e % 4], rule.mode == SM_LOGITS);
-        const double w = sm_in(kept, key, (uint32_t)i) ? sm_mass(tables, scale, key) : 0.0;
-        acc += w;
-        if (w > 0.0) { any = i; if (found < 0 && acc > local) found = i; }
+        key[e] = sm_key(v[e / 4].v[e % 4], rule.mode == SM_LOGITS);
+        if (!sm_in(kept, key[e], (uint32_t)(i0 + e))) key[e] = 0u;
     }
-    out[at] = found >= 0 ? found : any;
+    sm_masses(tables, scale, key, mass);
+#pragma unroll
+    for (int e = 0; e < SM_GROUP; e++) {
+        acc += mass[e];
+        if (mass[e] > 0.0) { any = e; if (found < 0 && acc > local) found = e; }
+    }
+    out[at] = i0 + (found >= 0 ? found : any);
 }
 
 // ---- long rows, without replacement ----------------------------------------------------------------------------------------------------

@@ -40,27 +40,29 @@ def _float_tensor(t, what: str) -> None:
         raise RuntimeError(f"{what}: float32, float16 or bfloat16 GPU tensor required (no CPU path)")
 
 
-def _integer(v, what: str, lo: int, hi: int) -> int:
+def _integer(v, what: str, name: str, lo: int, hi: int) -> int:
+    """v as an int in [lo, hi)"""
     if (type(v) is not int and (isinstance(v, bool) or not isinstance(v, numbers.Integral))) or not lo <= int(v) < hi:
-        raise ValueError(f"{what} must be an integer in [{lo}, {hi}), got {v!r}")
+        raise ValueError(f"{what}: {name} must be an integer in [{lo}, {hi}), got {v!r}")
     return int(v)
 
 
-def _real(v, what: str, ok) -> float:
-    if (type(v) is not float and (isinstance(v, bool) or not isinstance(v, numbers.Real))) or not ok(float(v)):
-        raise ValueError(f"{what}: {v!r} is out of range")
+def _real(v, what: str, name: str, lo: float, hi: float) -> float:
+    """v as a float in [lo, hi]"""
+    if (type(v) is not float and (isinstance(v, bool) or not isinstance(v, numbers.Real))) or not lo <= float(v) <= hi:
+        raise ValueError(f"{what}: {name} must be a number in [{lo}, {hi}], got {v!r}")
     return float(v)
 
 
 def _key(seed, offset: Offset, device: torch.device, what: str) -> Tuple[int, int, Optional[torch.Tensor]]:
     """-> (seed as the int64 of the same bits, host offset, device offset or None)"""
-    seed = _integer(seed, f"{what}: seed", 0, 1 << 64)
+    seed = _integer(seed, what, "seed", 0, 1 << 64)
     seed -= (seed >> 63) << 64
     if isinstance(offset, torch.Tensor):
         if offset.dtype != torch.int64 or offset.numel() != 1 or offset.device != device:
             raise ValueError(f"{what}: an offset tensor must be one int64 on {device}")
         return seed, 0, offset
-    return seed, _integer(offset, f"{what}: offset", 0, 1 << 63), None
+    return seed, _integer(offset, what, "offset", 0, 1 << 63), None
 
 
 class _Dropout(torch.autograd.Function):
@@ -93,9 +95,9 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Offset = 0, shared: in
     ``chunk_ids[a] * S + s``, and that is its index, shared by all leading dimensions -- a Gaussian's decision is the same in every view,
     whatever slot its chunk was compacted to.  ``p = 1`` drops everything."""
     _float_tensor(x, "dropout")
-    p = _real(p, "dropout: p", lambda v: 0.0 <= v <= 1.0)
+    p = _real(p, "dropout", "p", 0.0, 1.0)
     key = _key(seed, offset, x.device, "dropout")
-    shared = _integer(shared, "dropout: shared", 0, x.dim() + 1)
+    shared = _integer(shared, "dropout", "shared", 0, x.dim() + 1)
     S = 1
     if chunk_ids is not None:
         if not isinstance(chunk_ids, torch.Tensor) or x.dim() < 2 or chunk_ids.dtype != torch.int64 or chunk_ids.device != x.device or tuple(chunk_ids.shape) != (x.shape[-2],):
@@ -140,7 +142,9 @@ def normal(std: torch.Tensor, seed: int, offset: Offset = 0) -> torch.Tensor:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., K] -> [R, K] with a contiguous innermost dimension (a view where the strides allow one)"""
-    t = t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.new_empty((math.prod(t.shape[:-1]), 0))
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t
+    t = t.detach().reshape(-1, t.shape[-1]) if t.shape[-1] else t.new_empty((math.prod(t.shape[:-1]), 0))
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
@@ -148,11 +152,13 @@ def _sample(what: str, scores, u, n: int, distinct: bool, temperature, top_k, to
     V = scores.shape[-1]
     if V >= 1 << 31:
         raise ValueError(f"{what}: at most 2^31 - 1 categories")
-    temperature = _real(temperature, f"{what}: temperature", lambda v: 1e-30 <= v <= 1e30)
-    top_k = _integer(top_k, f"{what}: top_k", 0, 1 << 62)
-    top_p = _real(top_p, f"{what}: top_p", lambda v: 0.0 < v <= 1.0)
-    min_p = _real(min_p, f"{what}: min_p", lambda v: 0.0 <= v <= 1.0)
-    x, uu = _rows(scores.detach()), _rows(u.detach())
+    temperature = _real(temperature, what, "temperature", 1e-30, 1e30)
+    top_k = _integer(top_k, what, "top_k", 0, 1 << 62)
+    top_p = _real(top_p, what, "top_p", 0.0, 1.0)
+    min_p = _real(min_p, what, "min_p", 0.0, 1.0)
+    if top_p == 0.0:
+        raise ValueError(f"{what}: top_p must be more than 0")
+    x, uu = _rows(scores), _rows(u)
     R = x.shape[0]
     out = torch.empty((*scores.shape[:-1], n), dtype=torch.int64, device=x.device)
     if _C is not None:
@@ -198,5 +204,5 @@ def sample_distinct(scores: torch.Tensor, u: torch.Tensor, n: int, *, temperatur
     _check_scores(scores, u, "sample_distinct")
     if u.shape != scores.shape:
         raise ValueError("sample_distinct: one u for every score")
-    n = _integer(n, "sample_distinct: n", 0, scores.shape[-1] + 1)
+    n = _integer(n, "sample_distinct", "n", 0, scores.shape[-1] + 1)
     return _sample("sample_distinct", scores, u, n, True, temperature, top_k, top_p, min_p, logits)

@@ -18,7 +18,7 @@
 
 #define SM_BINS 2048                   // bins of one level of a radix selection
 #define SM_MAX_WAVES 16
-#define SM_SHORT 15360                 // longest row of one workgroup: 960 threads of 16 elements, whose masses and a histogram fill the LDS
+#define SM_SHORT 12288                 // longest row of one workgroup: 768 threads of 16 elements (a CU has 168 registers for each of 12 waves; with 16 waves 128 are too few)
 
 enum { SM_LOGITS = 0, SM_LINEAR = 1, SM_POWER = 2 };
 
@@ -38,6 +38,12 @@ template <typename T> __device__ __forceinline__ uint32_t sm_key(T raw, bool log
     x = fminf(x, SmMax<T>::v) + 0.0f;                                  // (-0 + 0 = +0: equal scores have equal keys)
     const uint32_t b = __float_as_uint(x);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+// the score itself; -inf = excluded
+template <typename T> __device__ __forceinline__ float sm_score(T raw, bool logits)
+{
+    const float x = lg_to_float(raw);
+    return (logits ? x == x : x > 0.0f) ? fminf(x, SmMax<T>::v) + 0.0f : -INFINITY;
 }
 __device__ __forceinline__ double sm_value(uint32_t key)
 {
@@ -147,30 +153,42 @@ __device__ __forceinline__ double sm_ln(const SmTables& t, float x)
     p = fma(r, p, -0.5);
     return fma(n, 6.93147180369123816e-01, fma(n, 1.90821492927058770e-10, t.log[i] + fma(r * r, p, r)));
 }
-// N masses at once, without a branch between them: one after the other each waits for its own chain of some twenty dependent instructions
-template <int N> __device__ __forceinline__ void sm_masses(const SmTables& t, const SmScale& s, const uint32_t (&key)[N], double (&m)[N])
+// N masses at once (x: scores, -inf where excluded), without a branch between them: one after the other each waits for its own chain of some
+// twenty dependent instructions
+template <int N> __device__ __forceinline__ void sm_masses(const SmTables& t, const SmScale& s, const float (&x)[N], double (&m)[N])
 {
     bool any = false;
 #pragma unroll
-    for (int k = 0; k < N; k++) any = any || key[k] != 0u;
+    for (int k = 0; k < N; k++) any = any || x[k] > -INFINITY;
     if (__ballot(any) == 0) {                                          // (the same for the wave)
 #pragma unroll
         for (int k = 0; k < N; k++) m[k] = 0.0;
         return;
     }
-    double x[N];
+    if (s.mode == SM_LINEAR) {
 #pragma unroll
-    for (int k = 0; k < N; k++) x[k] = (double)__uint_as_float((key[k] & 0x80000000u) ? (key[k] & 0x7fffffffu) : key[k] ? ~key[k] : 0x3f800000u);
+        for (int k = 0; k < N; k++) m[k] = (double)fmaxf(x[k], 0.0f);
+        return;
+    }
     if (s.mode == SM_POWER) {
 #pragma unroll
-        for (int k = 0; k < N; k++) x[k] = sm_ln(t, (float)x[k]);
-    }
-    if (s.mode != SM_LINEAR) {
+        for (int k = 0; k < N; k++) m[k] = sm_ln(t, x[k] > -INFINITY ? x[k] : 1.0f);
+    } else {
 #pragma unroll
-        for (int k = 0; k < N; k++) x[k] = sm_exp(t, x[k] * s.inv_t - s.top);
+        for (int k = 0; k < N; k++) m[k] = (double)(x[k] > -INFINITY ? x[k] : 0.0f);
     }
 #pragma unroll
-    for (int k = 0; k < N; k++) m[k] = key[k] ? x[k] : 0.0;
+    for (int k = 0; k < N; k++) m[k] = sm_exp(t, m[k] * s.inv_t - s.top);
+#pragma unroll
+    for (int k = 0; k < N; k++) m[k] = x[k] > -INFINITY ? m[k] : 0.0;
+}
+__device__ __forceinline__ float sm_float(uint32_t key) { return key ? __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key) : -INFINITY; }
+template <int N> __device__ __forceinline__ void sm_masses(const SmTables& t, const SmScale& s, const uint32_t (&key)[N], double (&m)[N])
+{
+    float x[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) x[k] = sm_float(key[k]);
+    sm_masses(t, s, x, m);
 }
 
 // key of the exponential race, ordered as an unsigned integer; 0 = excluded
@@ -422,16 +440,14 @@ __device__ __forceinline__ uint32_t sm_order(float k)
 }
 __device__ __forceinline__ float sm_unorder(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
 
-// ordered approximate key; 0 = excluded.  `slope`: log2(e) / T or 1 / T in 32 bits
-__device__ __forceinline__ uint32_t sm_race32(bool logits, float slope, uint32_t key, float u)
+// approximate key of a candidate.  `slope`: log2(e) / T or 1 / T in 32 bits
+__device__ __forceinline__ float sm_race32(bool logits, float slope, float x, float u)
 {
-    if (key == 0u) return 0u;
     u = u == u ? fminf(fmaxf(u, 0x1p-33f), 1.0f - 0x1p-24f) : 1.0f - 0x1p-24f;
-    const float x = __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
     const float a = (logits ? x : sm_log2(x)) * slope;
     const float e = u < 0x1p-6f ? u * (1.0f + u * (0.5f + u * (0.33333333f + u * 0.25f))) : -0.69314718f * __builtin_amdgcn_logf(1.0f - u);
     const float k = fminf(fmaxf(a, -3e38f), 3e38f) - __builtin_amdgcn_logf(e);
-    return sm_order(k + 0.0f);
+    return k + 0.0f;
 }
 
 // zone of the n-th key given that its approximation lies in [lo, hi]: ordered keys below zone.lo lose, above zone.hi win
@@ -443,15 +459,18 @@ __device__ __forceinline__ SmZone sm_zone(uint32_t lo, uint32_t hi, float slope)
     return SmZone{ a ? a : 1u, b };
 }
 
-// Unrolled 64-bit exponentials and logarithms stay out of line: sixteen of them inlined, with their constants, spill two thousand registers.
-__device__ __attribute__((noinline)) double sm_mass_call(SmScale s, uint32_t key) { return sm_mass(s, key); }
+// (out of line: sixteen of them inlined, with their constants, spill two thousand registers)
 __device__ __attribute__((noinline)) unsigned long long sm_race_call(SmScale s, uint32_t key, float u) { return sm_race(s, key, u); }
 
 // ---- short rows: one workgroup per row, EPT consecutive elements of a thread in registers ----------------------------------------------
-// key(k) is the key of element threadIdx.x * EPT + k, 0: not a candidate.  Ends when the boundary bin holds at most `small` elements:
-// [lo, hi] is then the bin's range of keys, take.before_* what lies above it, and the result its count and the number of candidates.
-template <bool MASS, int BITS, int TPB, int EPT, typename Word, typename Key>
-__device__ SmBin sm_select_short(const Key& key, const double* mass /*LDS, [EPT][TPB], at most one each*/, SmTake& take, uint32_t small, SmShortHist& h, SmScratch& sc,
+// One CU works on a row, so that every instruction an element costs is 0.1 us for 15 k of them: scores are kept as floats (-inf: excluded)
+// and compared as they are, and a level of a selection spreads the range that is left evenly over its bins (floats of either sign linearly,
+// weights by their bits, i.e. by their logarithm).  A level leaves some tens of elements then, which a wave ranks.
+
+// at(k, w): whether element threadIdx.x * EPT + k is a candidate, and its word.  Ends when the boundary bin holds at most `small` elements:
+// [lo, hi] is then the bin's range of words, take.before_* what lies above it, and the result its count and the number of candidates.
+template <bool MASS, int BITS, int TPB, int EPT, typename Word, typename At>
+__device__ __forceinline__ SmBin sm_select_short(const At& at_, const double* mass /*LDS, [EPT][TPB], at most one each*/, SmTake& take, uint32_t small, SmShortHist& h, SmScratch& sc,
                                  Word& lo, Word& hi)
 {
     Word prefix = 0;
@@ -465,8 +484,8 @@ __device__ SmBin sm_select_short(const Key& key, const double* mass /*LDS, [EPT]
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
-            const Word w = key(k);
-            if (w == 0 || (shift < BITS && (w >> shift) != prefix)) continue;
+            Word w;
+            if (!at_(k, w) || (shift < BITS && (w >> shift) != prefix)) continue;
             const int i = sm_slot((int)((w >> at) & (((Word)1 << (shift - at)) - 1)), p);
             if (MASS) {
                 const SmLimbs m = sm_limbs(mass[k * TPB + threadIdx.x]);
@@ -477,7 +496,7 @@ __device__ SmBin sm_select_short(const Key& key, const double* mass /*LDS, [EPT]
         __syncthreads();
         b = sm_boundary<MASS, MASS>(h.n, h.hi, h.lo, p, take, sc);
         if (shift == BITS) candidates = b.total;
-        if (b.bin < 0) break;                                          // no candidate at all
+        if (b.bin < 0) { lo = hi = 0; b.total = candidates; return b; }                       // no candidate at all
         prefix = (Word)(prefix << (shift - at)) | (Word)b.bin;
         shift = at;
         if (b.count <= small) break;
@@ -489,7 +508,7 @@ __device__ SmBin sm_select_short(const Key& key, const double* mass /*LDS, [EPT]
 }
 
 // index of the n-th (from 1) flagged element
-template <int EPT> __device__ uint32_t sm_nth_short(const bool (&flag)[EPT], uint32_t n, SmScratch& sc)
+template <int EPT> __device__ __forceinline__ uint32_t sm_nth_short(const bool (&flag)[EPT], uint32_t n, SmScratch& sc)
 {
     uint32_t c = 0, total;
 #pragma unroll
@@ -512,54 +531,191 @@ template <typename T> __device__ __forceinline__ LgVec4<T> sm_load4(const T* x, 
 }
 template <typename T> __device__ __forceinline__ bool sm_aligned(const T* x) { return (uintptr_t)x % (4 * sizeof(T)) == 0; }
 
+// a boundary bin of at most 64 elements, ranked by a wave
+struct SmFew { unsigned long long hi[64], lo[64]; float x[64]; uint32_t index[64], order[64]; };
+union SmShortLds { SmShortHist hist; SmFew few; struct { unsigned long long rank[SM_BINS]; uint32_t index[SM_BINS]; } zone; };
+
+// Bins of the numbers from lo to hi, and the one that is wanted (-1: all of them).  Grows with x; lo and hi are never in one bin.
+struct SmBins {
+    float lo, hi, f, s;
+    uint32_t low;
+    int down, want;
+    bool linear;
+    __device__ __forceinline__ int of(float x) const
+    {
+        if (!linear) return (int)((__float_as_uint(x) - low) >> down);
+        return (int)fminf(fmaxf((x * f - lo * f) * s, 0.0f), (float)(SM_BINS - 1));
+    }
+    __device__ __forceinline__ bool in(float x) const { return x >= lo && x <= hi && (want < 0 || of(x) == want); }
+};
+__device__ __forceinline__ SmBins sm_bins(bool linear, float lo, float hi)
+{
+    SmBins b = { lo, hi, 1.0f, 0.0f, __float_as_uint(lo), 0, -1, linear };
+    if (linear) {
+        if (hi - lo == INFINITY) b.f = 0.25f;
+        b.s = (float)SM_BINS / (hi * b.f - lo * b.f);                  // (infinite for a range below 1e-35: lo is then in bin 0, the others in the last)
+    } else {
+        const uint32_t range = __float_as_uint(hi) - b.low;
+        b.down = range >> 11 ? 21 - __clz(range) : 0;
+    }
+    return b;
+}
+
+// the smallest and the largest of the numbers that are in
+template <int EPT, typename In> __device__ __forceinline__ void sm_range_short(const float (&x)[EPT], const In& in, SmScratch& sc, float& lo, float& hi)
+{
+    float a = INFINITY, b = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < EPT; k++) if (in(k)) { a = fminf(a, x[k]); b = fmaxf(b, x[k]); }
+    hi = sm_unorder(sm_block_max(sm_order(b), sc.a));
+    lo = sm_unorder(~sm_block_max(~sm_order(a), sc.b));
+}
+
+// Where a selection of the candidates x (> -inf) ends: the bins that are left hold at most `small` elements, or only equal ones (lo == hi).
+// take.before_* is what lies above them, the result their count and the number of candidates (0: there are none).
+template <bool MASS, int TPB, int EPT>
+__device__ __forceinline__ SmBin sm_find_short(const float (&x)[EPT], const double* mass /*LDS, [EPT][TPB], at most one each*/, bool linear, SmTake& take, uint32_t small, SmShortHist& h, SmScratch& sc,
+                               SmBins& bins)
+{
+    uint32_t candidates = 0;
+    bins.want = -1;
+    for (int level = 0; ; level++) {
+        float lo, hi;
+        sm_range_short<EPT>(x, [&](int k) { return x[k] > -INFINITY && (level == 0 || bins.in(x[k])); }, sc, lo, hi);
+        if (!(lo <= hi)) return SmBin{ -1, 0, 0 };
+        bins = sm_bins(linear, lo, hi);
+        for (int i = threadIdx.x; i < SM_BINS; i += TPB) { if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } else h.n[i] = 0; }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < EPT; k++) {
+            if (!(x[k] >= lo && x[k] <= hi)) continue;
+            const int i = sm_slot(bins.of(x[k]), 5);
+            if (MASS) {
+                const SmLimbs m = sm_limbs(mass[k * TPB + threadIdx.x]);
+                if (m.hi) atomicAdd(&h.hi[i], (unsigned long long)m.hi);
+                atomicAdd(&h.lo[i], (unsigned long long)m.lo | 1ull << SM_PACK);
+            } else atomicAdd(&h.n[i], 1u);
+        }
+        __syncthreads();
+        SmBin b = sm_boundary<MASS, MASS>(h.n, h.hi, h.lo, 5, take, sc);
+        if (level == 0) candidates = b.total;
+        b.total = candidates;
+        if (b.bin < 0) return b;
+        bins.want = b.bin;
+        if (b.count <= small || lo == hi) return b;
+        __syncthreads();                                               // (lo and hi are never in one bin: every round has fewer)
+    }
+}
+
+// what is left of a row: numbers above thr, and those equal to it up to index last
+struct SmLeft { float thr; uint32_t last; };
+
+// what a top-k (MASS false) or top-p with that target leaves of the candidates
+template <bool MASS, int TPB, int EPT>
+__device__ __forceinline__ SmLeft sm_filter_short(const float (&x)[EPT], const double* mass, bool linear, SmTake take, SmShortLds& h, SmScratch& sc)
+{
+    SmBins bins;
+    const SmBin bin = sm_find_short<MASS, TPB, EPT>(x, mass, linear, take, 64, h.hist, sc, bins);
+    if (bin.count > 64) {                                              // equal ones: the first of them
+        bool tie[EPT];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < EPT; k++) {
+            tie[k] = x[k] == bins.lo;
+            if (MASS && tie[k]) sc.word[5] = (unsigned long long)__double_as_longlong(mass[k * TPB + threadIdx.x]);        // (all the same)
+        }
+        __syncthreads();
+        const uint32_t ties = sm_ties<MASS>(take, bin.count, MASS ? __longlong_as_double((long long)sc.word[5]) : 0.0);
+        return SmLeft{ bins.lo, ties < bin.count ? sm_nth_short<EPT>(tie, ties, sc) : SM_ALL };
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) sc.word[5] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < EPT; k++)
+        if (bins.in(x[k])) {
+            const uint32_t a = (uint32_t)atomicAdd(&sc.word[5], 1ull);
+            h.few.x[a] = x[k];
+            h.few.index[a] = threadIdx.x * EPT + k;
+            if (MASS) { const SmLimbs m = sm_limbs(mass[k * TPB + threadIdx.x]); h.few.hi[a] = m.hi; h.few.lo[a] = m.lo; }
+        }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        const uint32_t n = bin.count, l = threadIdx.x, i = l < n ? h.few.index[l] : 0u;
+        const float mine = l < n ? h.few.x[l] : 0.0f;
+        uint32_t ahead = 0;
+        for (uint32_t c = 0; c < n; c++) ahead += h.few.x[c] > mine || (h.few.x[c] == mine && h.few.index[c] < i);
+        if (l < n) h.few.order[ahead] = l;
+        __threadfence_block();                                         // (one wave: in order, and the compiler is told)
+        const uint32_t a = l < n ? h.few.order[l] : 0u;                // the l-th best
+        bool room;
+        if (MASS) {
+            const SmSum m = { l < n ? h.few.hi[a] : 0ull, l < n ? h.few.lo[a] : 0ull };
+            room = sm_room<true>(take, 0, sm_wave_scan<false>(m.hi, SmAdd()) - m.hi, sm_wave_scan<false>(m.lo, SmAdd()) - m.lo);
+        } else room = sm_room<false>(take, l, 0, 0);
+        const unsigned long long taken = __ballot(l < n && room);
+        const int e = taken ? 63 - __clzll((long long)taken) : 0;      // (the first one always is)
+        if ((int)l == e) { sc.word[0] = __float_as_uint(h.few.x[a]); sc.word[1] = h.few.index[a]; }
+    }
+    __syncthreads();
+    return SmLeft{ __uint_as_float((uint32_t)sc.word[0]), (uint32_t)sc.word[1] };
+}
+
 template <typename T, int TPB, int EPT, bool DISTINCT>
 __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                             int V, long long n, SmRule rule, const uint32_t* __restrict__ names /*nullable [R, V]*/,
                                                             long long* __restrict__ out)
 {
     __shared__ double mass[TPB * EPT];                                 // element k of thread t at k * TPB + t; at the end the cumulative ones
-    __shared__ union { SmShortHist hist; struct { unsigned long long rank[SM_BINS]; uint32_t index[SM_BINS]; } zone; } h;
+    __shared__ SmShortLds h;
+    __shared__ SmTables tables;
     __shared__ uint32_t won[DISTINCT ? TPB * EPT / 32 : 1];
     __shared__ uint16_t pos[DISTINCT ? 1 : TPB];
     __shared__ SmScratch sc;
     const long long r = blockIdx.x;
-    const T* x = scores + r * sstride;
+    const T* row = scores + r * sstride;
     const bool logits = rule.mode == SM_LOGITS;
     u += r * ustride;
     out += r * n;
     if (names) names += r * V;
     auto name = [&](uint32_t i) { return names ? (long long)names[i] : (long long)i; };          // of element i, where the row is what a filter left
     const int i0 = threadIdx.x * EPT;
-    uint32_t key[EPT], best = 0;
+    float x[EPT], most = -INFINITY;
+    {
+        LgVec4<T> v[EPT / 4];
 #pragma unroll
-    for (int k = 0; k < EPT; k += 4) {
-        const LgVec4<T> v = sm_load4(x, i0 + k, V, sm_aligned(x));
+        for (int k = 0; k < EPT / 4; k++) v[k] = sm_load4(row, i0 + 4 * k, V, sm_aligned(row));
+        sm_tables(tables, rule.mode);                                  // (the first scan is the barrier)
 #pragma unroll
-        for (int j = 0; j < 4; j++) key[k + j] = sm_key(v.v[j], logits);
+        for (int k = 0; k < EPT; k++) { x[k] = sm_score(v[k / 4].v[k % 4], logits); most = fmaxf(most, x[k]); }
     }
-#pragma unroll
-    for (int k = 0; k < EPT; k++) best = key[k] > best ? key[k] : best;
-    best = sm_block_max(best, sc.a);
-    if (best == 0) {                                                   // nothing to draw from
+    most = sm_unorder(sm_block_max(sm_order(most), sc.a));
+    if (most == -INFINITY) {                                           // nothing to draw from
         for (long long j = (long long)blockIdx.y * TPB + threadIdx.x; j < n; j += (long long)gridDim.y * TPB) out[j] = -1;
         return;
     }
+    const uint32_t best = sm_order(most);
     const SmScale scale = sm_scale(rule, best);
     // masses, once: linear ones by a power of two below one
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
     auto masses = [&]() {
 #pragma unroll
-        for (int k = 0; k < EPT; k++) mass[k * TPB + threadIdx.x] = sm_mass_call(scale, key[k]) * unit;
+        for (int k = 0; k < EPT; k += 4) {
+            const float four[4] = { x[k], x[k + 1], x[k + 2], x[k + 3] };
+            double m[4];
+            sm_masses(tables, scale, four, m);
+#pragma unroll
+            for (int j = 0; j < 4; j++) mass[(k + j) * TPB + threadIdx.x] = m[j] * unit;
+        }
     };
-    // filters: an element that one of them drops becomes key 0
+    // filters: an element that one of them drops becomes -inf
     for (int pass = 0; pass < 2; pass++) {
         SmTake take = { 0.0, 0, { 0, 0 } };
-        uint32_t lo, hi;
-        SmBin bin;
+        SmLeft left;
         if (pass == 0) {
             if (rule.top_k <= 0 || rule.top_k >= V) continue;
             take.target = (double)rule.top_k;
-            bin = sm_select_short<false, 32, TPB, EPT, uint32_t>([&](int k) { return key[k]; }, nullptr, take, 1, h.hist, sc, lo, hi);
+            left = sm_filter_short<false, TPB, EPT>(x, mass, logits, take, h, sc);
         } else {
             if (rule.top_p >= 1.0) continue;
             SmSum mine = { 0, 0 }, total;
@@ -569,45 +725,44 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             sm_block_scan<unsigned long long>(mine.hi, sc.a, total.hi);
             sm_block_scan<unsigned long long>(mine.lo, sc.b, total.lo);
             take.target = rule.top_p * sm_sum_value(total);
-            bin = sm_select_short<true, 32, TPB, EPT, uint32_t>([&](int k) { return key[k]; }, mass, take, 1, h.hist, sc, lo, hi);
-        }
-        // a bin of one element is taken whole; one of equal elements up to the cut
-        SmKept kept = { lo, SM_ALL };
-        const uint32_t ties = bin.count == 1 ? 1 : pass == 0 ? sm_ties<false>(take, bin.count, 0.0) : sm_ties<true>(take, bin.count, sm_mass_call(scale, lo) * unit);
-        if (ties < bin.count) {
-            bool tie[EPT];
-#pragma unroll
-            for (int k = 0; k < EPT; k++) tie[k] = key[k] == lo;
-            kept.last = sm_nth_short<EPT>(tie, ties, sc);
+            left = sm_filter_short<true, TPB, EPT>(x, mass, logits, take, h, sc);
         }
 #pragma unroll
-        for (int k = 0; k < EPT; k++) if (!sm_in(kept, key[k], (uint32_t)(i0 + k))) key[k] = 0;
+        for (int k = 0; k < EPT; k++) if (!(x[k] > left.thr || (x[k] == left.thr && (uint32_t)(i0 + k) <= left.last))) x[k] = -INFINITY;
     }
     if (rule.min_p > 0.0) {
         SmKept kept = { 0u, SM_ALL };
         sm_min_p(scale, best, rule.min_p, kept);
+        const float least = sm_float(kept.thr);
 #pragma unroll
-        for (int k = 0; k < EPT; k++) if (!sm_in(kept, key[k], (uint32_t)(i0 + k))) key[k] = 0;
+        for (int k = 0; k < EPT; k++) if (!(x[k] >= least)) x[k] = -INFINITY;
     }
     if (DISTINCT) {
-        uint32_t race[EPT], lo, hi, wins = 0;
+        float race[EPT];                                               // approximate keys; -inf: not a candidate
+        uint32_t wins = 0;
         const float slope = sm_slope(rule);
 #pragma unroll
-        for (int k = 0; k < EPT; k++) race[k] = __float_as_uint(key[k] ? u[i0 + k] : 0.0f);        // (loads first; key 0 behind V)
+        for (int k = 0; k < EPT; k++) race[k] = x[k] > -INFINITY ? u[i0 + k] : 0.0f;              // (loads first; -inf behind V)
 #pragma unroll
-        for (int k = 0; k < EPT; k++) race[k] = sm_race32(logits, slope, key[k], __uint_as_float(race[k]));
+        for (int k = 0; k < EPT; k++) race[k] = x[k] > -INFINITY ? sm_race32(logits, slope, x[k], race[k]) : -INFINITY;
         SmTake take = { (double)n, 0, { 0, 0 } };
-        const SmBin bin = sm_select_short<false, 32, TPB, EPT, uint32_t>([&](int k) { return race[k]; }, nullptr, take, 16, h.hist, sc, lo, hi);
-        SmZone zone = { 1u, 0u };                                      // nothing to rank where everything wins
-        if (bin.total > n) zone = sm_zone(lo, hi, slope);
+        SmBins bins;
+        const SmBin bin = sm_find_short<false, TPB, EPT>(race, nullptr, true, take, 64, h.hist, sc, bins);
+        float zlo = -INFINITY, zhi = -INFINITY;                        // nothing to rank where everything wins
+        const bool ranked = bin.total > (uint32_t)n;
+        if (ranked) {
+            sm_range_short<EPT>(race, [&](int k) { return bins.in(race[k]); }, sc, zlo, zhi);
+            zlo -= 2.0f * sm_margin(zlo, slope);
+            zhi += 2.0f * sm_margin(zhi, slope);
+        }
         __syncthreads();
         if (threadIdx.x == 0) sc.word[5] = 0;
         for (int i = threadIdx.x; i < TPB * EPT / 32; i += TPB) won[i] = 0;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
-            if (race[k] > zone.hi) wins |= 1u << k;
-            else if (race[k] >= zone.lo) {
+            if (race[k] > zhi) wins |= 1u << k;
+            else if (ranked && race[k] >= zlo) {
                 const uint32_t at = (uint32_t)atomicAdd(&sc.word[5], 1ull);
                 if (at < SM_BINS) h.zone.index[at] = i0 + k;
             }
@@ -618,7 +773,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         if (found <= SM_BINS) {
             for (uint32_t a = threadIdx.x; a < found; a += TPB) {
                 const uint32_t i = h.zone.index[a];
-                h.zone.rank[a] = sm_race(scale, sm_key(x[i], logits), u[i]);
+                h.zone.rank[a] = sm_race_call(scale, sm_key(row[i], logits), u[i]);
             }
             __syncthreads();
             for (uint32_t a = threadIdx.x; a < found; a += TPB) {
@@ -634,13 +789,14 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             // many elements next to the border (equal numbers, or a slope that spreads nothing): radix selection of their exact keys
             unsigned long long *mine = (unsigned long long*)mass + threadIdx.x, elo, ehi;        // (the masses are done)
 #pragma unroll
-            for (int k = 0; k < EPT; k++) mine[k * TPB] = race[k] >= zone.lo && race[k] <= zone.hi ? sm_race_call(scale, key[k], u[i0 + k]) : 0ull;
+            for (int k = 0; k < EPT; k++) mine[k * TPB] = race[k] > -INFINITY && race[k] >= zlo && race[k] <= zhi ? sm_race_call(scale, sm_order(x[k]), u[i0 + k]) : 0ull;
             SmTake left = { (double)room, 0, { 0, 0 } };
-            const SmBin e = sm_select_short<false, 64, TPB, EPT, unsigned long long>([&](int k) { return mine[k * TPB]; }, nullptr, left, 1, h.hist, sc, elo, ehi);
+            const SmBin e = sm_select_short<false, 64, TPB, EPT, unsigned long long>([&](int k, unsigned long long& w) { w = mine[k * TPB]; return w != 0ull; }, nullptr, left, 1, h.hist, sc, elo, ehi);
             const uint32_t ties = e.bin < 0 ? 0 : e.count == 1 ? 1 : sm_ties<false>(left, e.count, 0.0);
             uint32_t last = SM_ALL;
             if (ties < e.count) {
                 bool tie[EPT];
+                __syncthreads();
 #pragma unroll
                 for (int k = 0; k < EPT; k++) tie[k] = mine[k * TPB] == elo;
                 last = sm_nth_short<EPT>(tie, ties, sc);
@@ -658,19 +814,20 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         for (int k = 0; k < EPT; k++) if ((wins >> k) & 1) out[at++] = name(i0 + k);
         for (long long j = (long long)total + threadIdx.x; j < n; j += TPB) out[j] = -1;
     } else {
-        double sum = 0.0, total;
+        double m[EPT], sum = 0.0, total;
         uint32_t positive = 0, last = 0;
         if (rule.top_p >= 1.0) masses();
 #pragma unroll
+        for (int k = 0; k < EPT; k++) m[k] = x[k] > -INFINITY ? mass[k * TPB + threadIdx.x] : 0.0;
+#pragma unroll
         for (int k = 0; k < EPT; k++) {
-            const double m = key[k] ? mass[k * TPB + threadIdx.x] : 0.0;
-            sum += m;
-            if (m > 0.0) { positive |= 1u << k; last = (uint32_t)(i0 + k) + 1; }
+            sum += m[k];
+            if (m[k] > 0.0) { positive |= 1u << k; last = (uint32_t)(i0 + k) + 1; }
         }
         double at = sm_block_scan<double>(sum, sc.a, total);
         last = sm_block_max(last, sc.b);
 #pragma unroll
-        for (int k = 0; k < EPT; k++) { if (key[k]) at += mass[k * TPB + threadIdx.x]; mass[k * TPB + threadIdx.x] = at; }
+        for (int k = 0; k < EPT; k++) { at += m[k]; mass[k * TPB + threadIdx.x] = at; }
         pos[threadIdx.x] = (uint16_t)positive;
         __syncthreads();
         for (long long j = (long long)blockIdx.y * TPB + threadIdx.x; j < n; j += (long long)gridDim.y * TPB) {         // (blockIdx.y: its share of the draws)
@@ -1416,7 +1573,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const uint32_t key = sm_key(v[g].v[j], logits);
-                o.v[j] = sm_race32(logits, slope, sm_in(kept, key, (uint32_t)(at + j)) ? key : 0u, uk[g].v[j]);
+                o.v[j] = sm_in(kept, key, (uint32_t)(at + j)) ? sm_order(sm_race32(logits, slope, sm_float(key), uk[g].v[j])) : 0u;
                 if (o.v[j]) atomicAdd(&h[sm_slot((int)(o.v[j] >> (32 - SM_RBITS1)), SM_RBITS1 - 6)], 1u);
             }
             if (at < V) *(LgVec4<uint32_t>*)(keys + at) = o;           // (padded to a multiple of four: what lies behind V is key 0)
@@ -1733,7 +1890,7 @@ static void sample_short(const T* scores, long long ss, const float* u, long lon
     } while (0)
     if (V <= 1024) SM_LAUNCH_SHORT(256, 4);
     else if (V <= 4096) SM_LAUNCH_SHORT(1024, 4);
-    else SM_LAUNCH_SHORT(960, 16);
+    else SM_LAUNCH_SHORT(768, 16);
 #undef SM_LAUNCH_SHORT
 }
 

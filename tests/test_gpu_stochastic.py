@@ -213,8 +213,12 @@ def scores_of(kind, R, V, dtype, logits, seed=0):
         z = torch.full((R, V), 0.75, device=DEV)
     elif kind == "wide":
         z = z * 20
+    elif kind == "steps":                                           # powers of two over the whole range of float32, either sign
+        z = torch.where(hole < 0.5, -1.0, 1.0) * torch.exp2(torch.randint(-140, 120, (R, V), generator=g, device=DEV).float())
+    elif kind == "near":                                            # floats next to each other, around one and around zero
+        z = torch.where(hole < 0.5, 1.0 + (z * 3).round() * 2.0 ** -23, (z * 3).round() * 2.0 ** -149)
     if not logits:
-        z = z.clamp(-40, 40).exp()
+        z = z.abs() if kind in ("steps", "near") else z.clamp(-40, 40).exp()
     z = z.to(dtype)
     if kind == "masked":
         z = torch.where(hole < 0.5, torch.tensor(-math.inf if logits else 0.0, dtype=dtype, device=DEV), z)
@@ -255,7 +259,7 @@ def check_distinct(x, u, n, **kw):
     assert got.dtype == torch.int64 and np.array_equal(got.cpu().numpy(), want), (x.shape, x.dtype, n, kw)
 
 
-LENGTHS = [1, 2, 63, 64, 65, 1000, 1025, 4095, 4097, 9000, 20001]
+LENGTHS = [1, 2, 63, 64, 65, 1000, 1024, 1025, 4095, 4096, 4097, 9000, 12288, 12289, 20001]
 
 
 @pytest.mark.parametrize("V", LENGTHS)
@@ -275,7 +279,7 @@ def test_distinct_lengths(V, logits):
             check_distinct(x, draws_of((2, V), V), n, logits=logits, **kw)
 
 
-KINDS = ["ties", "equal", "wide", "masked", "lowest", "nan", "inf", "zeros", "empty", "tiny"]
+KINDS = ["ties", "equal", "wide", "steps", "near", "masked", "lowest", "nan", "inf", "zeros", "empty", "tiny"]
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -328,6 +332,87 @@ def test_rows_with_strides(R):
     assert torch.equal(one, stochastic.sample(base[:1], u[:1, :3])[0])
     three = stochastic.sample_distinct(base.reshape(R, 3, 700), u.reshape(R, 3, 700), 5)
     assert torch.equal(three.reshape(-1, 5), stochastic.sample_distinct(base.reshape(-1, 700), u.reshape(-1, 700), 5))
+
+
+@pytest.mark.parametrize("R,V", [(2, 700), (2, 11000), (1, 50000), (3, 50000), (260, 13000), (300, 20000)])
+def test_many_rows_and_many_draws(R, V):
+    """several workgroups a row and one, shares of the draws, 16-bit scores in more rows than their histogram of all keys is made for"""
+    for dtype in (torch.float32, torch.bfloat16):
+        x = scores_of("normal", R, V, dtype, True, seed=R)
+        n = 9000 if R < 10 else 5
+        check_sample(x, draws_of((R, n)), logits=True, top_k=V // 3, top_p=0.9)
+        check_sample(x, draws_of((R, n)), logits=True, top_k=300, min_p=1e-4)
+        check_distinct(x, draws_of((R, V)), 50, logits=True, top_k=V // 3, top_p=0.9, min_p=1e-3)
+
+
+@pytest.mark.parametrize("equal", [2500, 5000])
+def test_distinct_with_many_candidates_next_to_the_border(equal):
+    """more elements of one race key than a workgroup ranks pairwise, then more than the list holds; the rest on either side of it"""
+    V = 60000
+    x = torch.zeros((2, V), device=DEV)
+    u = draws_of((2, V)) * 0.2 + 0.4
+    u[:, 7::23] = 0.1                                               # (a small u wins)
+    some = torch.randperm(V, generator=torch.Generator().manual_seed(1))[:equal].to(DEV)
+    u[:, some] = 0.25
+    ahead = int((u[0] < 0.25).sum())
+    for n in (ahead, ahead + 1, ahead + equal // 2, ahead + equal, ahead + equal + 1):
+        check_distinct(x, u, n, logits=True)
+
+
+def test_sample_of_more_tiles_than_a_workgroup_keeps():
+    V = 9000001
+    x = scores_of("masked", 1, V, torch.float32, False, seed=4)
+    u = draws_of((1, 3000))
+    u[0, 0], u[0, 1] = 0.0, 1.0
+    check_sample(x, u, logits=False)
+    check_sample(x, u, logits=False, temperature=0.7, top_p=0.8)
+
+
+def test_distinct_of_more_tiles_than_are_counted_in_lds():
+    V, n = 34000000, 100000
+    g = torch.Generator(device=DEV).manual_seed(8)
+    x, u = torch.rand((1, V), generator=g, device=DEV), torch.rand((1, V), generator=g, device=DEV)
+    got = stochastic.sample_distinct(x, u, n, logits=False)[0].cpu().numpy()
+    key = torch.log(x.double()) - torch.log(-torch.log1p(-u.double().clamp(2.0 ** -33, 1 - 2.0 ** -24)))
+    want = key[0].topk(n).indices.sort().values.cpu().numpy()       # (keys differ: 2^-24 steps of either number meet in few places, far from the border)
+    assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("distinct", [False, True])
+@pytest.mark.parametrize("R,V,n", [(1, 5, 3), (3, 4096, 17), (2, 12289, 333), (1, 100003, 1000), (300, 13001, 4)])
+def test_nothing_is_written_outside(distinct, R, V, n):
+    """the C entry with its output and its workspace inside larger buffers: what lies around them stays as it was"""
+    from litegs_amd._lib import lib
+    L = lib()
+    for code, dtype in enumerate(TYPES):
+        for top_k, top_p in ((0, 1.0), (9, 0.9), (V // 2, 0.9)):
+            x, u = scores_of("normal", R, V, dtype, True), draws_of((R, V if distinct else n))
+            need = L.lg_sample_temp_bytes(R, V, n, code, int(distinct), top_k, top_p)
+            out = torch.full((R * n + 512,), -77, dtype=torch.int64, device=DEV)
+            temp = torch.full((need + 8192,), 0xC1, dtype=torch.uint8, device=DEV)
+            rc = L.lg_sample(x.data_ptr(), code, V, u.data_ptr(), u.shape[1], R, V, n, int(distinct), 1, 1.0, top_k, top_p, 0.0, out.data_ptr() + 256 * 8,
+                             temp.data_ptr() + 4096, need, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            assert (out[:256] == -77).all() and (out[256 + R * n:] == -77).all() and (out[256:256 + R * n] >= -1).all()
+            assert (temp[:4096] == 0xC1).all() and (temp[4096 + need:] == 0xC1).all()
+            if need:                                                # a workspace that is too small or missing is refused
+                assert L.lg_sample(x.data_ptr(), code, V, u.data_ptr(), u.shape[1], R, V, n, int(distinct), 1, 1.0, top_k, top_p, 0.0, out.data_ptr(),
+                                   temp.data_ptr(), need - 1, None) != 0
+                assert L.lg_sample(x.data_ptr(), code, V, u.data_ptr(), u.shape[1], R, V, n, int(distinct), 1, 1.0, top_k, top_p, 0.0, out.data_ptr(),
+                                   None, 0, None) != 0
+
+
+def test_two_streams_at_once():
+    x, u = scores_of("normal", 4, 60000, torch.float32, True), draws_of((4, 60000))
+    want = [stochastic.sample_distinct(x, u, 100, top_p=0.9), stochastic.sample(x, u[:, :500], top_k=20000)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([stochastic.sample_distinct(x, u, 100, top_p=0.9), stochastic.sample(x, u[:, :500], top_k=20000)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for pair in got for a, b in zip(pair, want))
 
 
 def test_empty_calls():

@@ -94,15 +94,21 @@ __device__ __forceinline__ double sm_ln(double x)
 
 struct SmScale { int mode; double inv_t, top /*l of the best score, or its weight*/, shift /*power of two that brings a linear weight below one*/; };
 
-__device__ __forceinline__ SmScale sm_scale(const SmRule& r, uint32_t best)
+// The best one's l has to come from the function that gives the others' (`ln`): at a temperature of 1e-20 the last bit of a logarithm is
+// as much as e^1000.
+template <typename Ln> __device__ __forceinline__ SmScale sm_scale(const SmRule& r, uint32_t best, const Ln& ln)
 {
     SmScale s = { r.mode, 1.0 / r.temperature, 0.0, 1.0 };
     if (best == 0u) return s;
     const double x = sm_value(best);
     if (r.mode == SM_LOGITS) s.top = x * s.inv_t;
-    else if (r.mode == SM_POWER) s.top = sm_ln(x) * s.inv_t;
+    else if (r.mode == SM_POWER) s.top = ln(x) * s.inv_t;
     else { s.top = x; s.shift = ldexp(1.0, -ilogb(x) - 1); }
     return s;
+}
+__device__ __forceinline__ SmScale sm_scale(const SmRule& r, uint32_t best)                   // for sm_mass
+{
+    return sm_scale(r, best, [](double x) { return sm_ln(x); });
 }
 __device__ __forceinline__ double sm_log(const SmScale& s, uint32_t key)
 {
@@ -152,6 +158,10 @@ __device__ __forceinline__ double sm_ln(const SmTables& t, float x)
     p = fma(r, p, 1.0 / 3);
     p = fma(r, p, -0.5);
     return fma(n, 6.93147180369123816e-01, fma(n, 1.90821492927058770e-10, t.log[i] + fma(r * r, p, r)));
+}
+__device__ __forceinline__ SmScale sm_scale(const SmTables& t, const SmRule& r, uint32_t best)        // for sm_masses
+{
+    return sm_scale(r, best, [&](double x) { return sm_ln(t, (float)x); });
 }
 // N masses at once (x: scores, -inf where excluded), without a branch between them: one after the other each waits for its own chain of some
 // twenty dependent instructions
@@ -399,9 +409,10 @@ struct SmKept { uint32_t thr, last; };
 __device__ __forceinline__ bool sm_in(const SmKept& k, uint32_t key, uint32_t i) { return key != 0u && (key > k.thr || (key == k.thr && i <= k.last)); }
 
 // min-p as a cut of the keys: the smallest key whose mass is at least min_p of the best one's (the mass grows with the key)
-__device__ __forceinline__ void sm_min_p(const SmScale& s, uint32_t best, double min_p, SmKept& kept)
+__device__ __forceinline__ void sm_min_p(const SmRule& rule, uint32_t best, SmKept& kept)
 {
-    const double least = min_p * sm_mass(s, best);
+    const SmScale s = sm_scale(rule, best);
+    const double least = rule.min_p * sm_mass(s, best);
     const uint32_t lane = threadIdx.x & 63;
     uint32_t lo = 1, hi = best;                                        // 64 probes a round; the mass at hi is enough
     while (lo < hi) {
@@ -467,43 +478,33 @@ __device__ __attribute__((noinline)) unsigned long long sm_race_call(SmScale s, 
 // and compared as they are, and a level of a selection spreads the range that is left evenly over its bins (floats of either sign linearly,
 // weights by their bits, i.e. by their logarithm).  A level leaves some tens of elements then, which a wave ranks.
 
-// at(k, w): whether element threadIdx.x * EPT + k is a candidate, and its word.  Ends when the boundary bin holds at most `small` elements:
-// [lo, hi] is then the bin's range of words, take.before_* what lies above it, and the result its count and the number of candidates.
-template <bool MASS, int BITS, int TPB, int EPT, typename Word, typename At>
-__device__ __forceinline__ SmBin sm_select_short(const At& at_, const double* mass /*LDS, [EPT][TPB], at most one each*/, SmTake& take, uint32_t small, SmShortHist& h, SmScratch& sc,
-                                 Word& lo, Word& hi)
+// Radix selection.  at(k, w): whether element threadIdx.x * EPT + k is a candidate, and its word.  Ends with one element in the bin or one
+// word: lo is then the bin's lowest word, take.before_* what lies above it, and the result its count.
+template <int TPB, int EPT, typename At>
+__device__ __forceinline__ SmBin sm_select_short(const At& at_, SmTake& take, SmShortHist& h, SmScratch& sc, unsigned long long& lo)
 {
-    Word prefix = 0;
-    int shift = BITS;
+    unsigned long long prefix = 0;
+    int shift = 64;
     SmBin b = { -1, 0, 0 };
-    uint32_t candidates = 0;
     while (shift > 0) {
         const int width = shift >= 11 ? 11 : shift < 6 ? 6 : shift, at = shift > width ? shift - width : 0, p = width - 6;
         __syncthreads();
-        for (int i = threadIdx.x; i < 1 << width; i += TPB) { if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } else h.n[i] = 0; }
+        for (int i = threadIdx.x; i < 1 << width; i += TPB) h.n[i] = 0;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
-            Word w;
-            if (!at_(k, w) || (shift < BITS && (w >> shift) != prefix)) continue;
-            const int i = sm_slot((int)((w >> at) & (((Word)1 << (shift - at)) - 1)), p);
-            if (MASS) {
-                const SmLimbs m = sm_limbs(mass[k * TPB + threadIdx.x]);
-                if (m.hi) atomicAdd(&h.hi[i], (unsigned long long)m.hi);
-                atomicAdd(&h.lo[i], (unsigned long long)m.lo | 1ull << SM_PACK);
-            } else atomicAdd(&h.n[i], 1u);
+            unsigned long long w;
+            if (!at_(k, w) || (shift < 64 && (w >> shift) != prefix)) continue;
+            atomicAdd(&h.n[sm_slot((int)((w >> at) & ((1ull << (shift - at)) - 1)), p)], 1u);
         }
         __syncthreads();
-        b = sm_boundary<MASS, MASS>(h.n, h.hi, h.lo, p, take, sc);
-        if (shift == BITS) candidates = b.total;
-        if (b.bin < 0) { lo = hi = 0; b.total = candidates; return b; }                       // no candidate at all
-        prefix = (Word)(prefix << (shift - at)) | (Word)b.bin;
+        b = sm_boundary<false>(h.n, nullptr, nullptr, p, take, sc);
+        if (b.bin < 0) { lo = 0; return b; }                           // no candidate at all
+        prefix = (prefix << (shift - at)) | (unsigned)b.bin;
         shift = at;
-        if (b.count <= small) break;
+        if (b.count == 1) break;
     }
     lo = prefix << shift;
-    hi = lo | (((Word)1 << shift) - 1);
-    b.total = candidates;
     return b;
 }
 
@@ -695,7 +696,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         return;
     }
     const uint32_t best = sm_order(most);
-    const SmScale scale = sm_scale(rule, best);
+    const SmScale scale = sm_scale(tables, rule, best);
     // masses, once: linear ones by a power of two below one
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
     auto masses = [&]() {
@@ -732,7 +733,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     }
     if (rule.min_p > 0.0) {
         SmKept kept = { 0u, SM_ALL };
-        sm_min_p(scale, best, rule.min_p, kept);
+        sm_min_p(rule, best, kept);
         const float least = sm_float(kept.thr);
 #pragma unroll
         for (int k = 0; k < EPT; k++) if (!(x[k] >= least)) x[k] = -INFINITY;
@@ -787,11 +788,11 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             wins |= (won[i0 >> 5] >> (i0 & 31)) & ((1u << EPT) - 1);
         } else {
             // many elements next to the border (equal numbers, or a slope that spreads nothing): radix selection of their exact keys
-            unsigned long long *mine = (unsigned long long*)mass + threadIdx.x, elo, ehi;        // (the masses are done)
+            unsigned long long *mine = (unsigned long long*)mass + threadIdx.x, elo;        // (the masses are done)
 #pragma unroll
             for (int k = 0; k < EPT; k++) mine[k * TPB] = race[k] > -INFINITY && race[k] >= zlo && race[k] <= zhi ? sm_race_call(scale, sm_order(x[k]), u[i0 + k]) : 0ull;
             SmTake left = { (double)room, 0, { 0, 0 } };
-            const SmBin e = sm_select_short<false, 64, TPB, EPT, unsigned long long>([&](int k, unsigned long long& w) { w = mine[k * TPB]; return w != 0ull; }, nullptr, left, 1, h.hist, sc, elo, ehi);
+            const SmBin e = sm_select_short<TPB, EPT>([&](int k, unsigned long long& w) { w = mine[k * TPB]; return w != 0ull; }, left, h.hist, sc, elo);
             const uint32_t ties = e.bin < 0 ? 0 : e.count == 1 ? 1 : sm_ties<false>(left, e.count, 0.0);
             uint32_t last = SM_ALL;
             if (ties < e.count) {
@@ -972,12 +973,12 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     const SmKept kept = first ? st.kept : st.before;
     const uint32_t prefix = st.prefix;
     const uint32_t best = MASS ? (first ? sm_best(wk, r) : st.best) : 0u;
-    const SmScale scale = sm_scale(rule, best);
-    const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
     const bool counted = !MASS || at == 0;                             // masses need no counts before the last level
     if (MASS) sm_tables(tables, rule.mode);
     for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { h.n[k] = 0; if (MASS) { h.hi[k] = 0; h.lo[k] = 0; } }
     __syncthreads();
+    const SmScale scale = sm_scale(tables, rule, best);
+    const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
     while (i < V) {
         uint32_t key[4 * G];
 #pragma unroll
@@ -1056,9 +1057,11 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     const bool whole = counted && sm_whole_bin<MASS>(take, bin.count);
     if (!whole && at > 0) return;
     // the key is found, or the lowest key of a bin that is taken whole; a cut among the equal ones is left to sm_cut_kernel
-    const uint32_t thr = found << at;
+    const uint32_t thr = found << at, one[1] = { thr };
+    double mass[1] = { 0.0 };
+    if (MASS) sm_masses(tables, scale, one, mass);
     st.ended = 1;
-    sm_conclude(st, kept, thr, whole ? bin.count : sm_ties<MASS>(take, bin.count, MASS ? sm_mass(scale, thr) * unit : 0.0), bin.count);
+    sm_conclude(st, kept, thr, whole ? bin.count : sm_ties<MASS>(take, bin.count, mass[0] * unit), bin.count);
 }
 
 // ---- scores of 16 bits: both filters from one histogram of all keys ----------------------------------------------------------------------
@@ -1239,7 +1242,7 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
         __syncthreads();
     }
     SmKept least = { 0u, SM_ALL };
-    if (best != 0 && rule.min_p > 0.0) sm_min_p(scale, best_key, rule.min_p, least);
+    if (best != 0 && rule.min_p > 0.0) sm_min_p(rule, best_key, least);
     if (threadIdx.x != 0) return;
     st.before = kept;
     st.best = best_key;
@@ -1372,7 +1375,7 @@ __device__ __forceinline__ SmKept sm_final(const SmWork& wk, long long r, const 
     if (rule.min_p <= 0.0) return kept;
     if (!wk.best) return st.least > kept.thr ? SmKept{ st.least, SM_ALL } : kept;
     const uint32_t best = sm_best(wk, r);
-    if (best) sm_min_p(sm_scale(rule, best), best, rule.min_p, kept);
+    if (best) sm_min_p(rule, best, kept);
     return kept;
 }
 
@@ -1405,7 +1408,7 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
             best = key[k] > best ? key[k] : best;
         }
         best = sm_block_max(best, sc.b);
-        const SmScale scale = sm_scale(rule, best);
+        const SmScale scale = sm_scale(tables, rule, best);
         double mass[SM_GROUP], sum = 0.0, total, most;
         sm_masses(tables, scale, key, mass);
 #pragma unroll
@@ -1483,7 +1486,7 @@ template <typename Past> __device__ __forceinline__ int sm_rank4(const double* a
 
 template <typename T>
 __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
-                                                      long long R, long long V, long long n, SmRule rule, SmWork wk, long long* __restrict__ out)
+                                                      long long V, long long n, SmRule rule, SmWork wk, long long* __restrict__ out)
 {
     __shared__ double ends[SM_DRAW_ENDS];
     __shared__ SmTables tables;
@@ -1605,7 +1608,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
 }
 
 // second level, and the zone
-__global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, long long n, SmRule rule, SmWork wk, int step)
+__global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, SmRule rule, SmWork wk, int step)
 {
     __shared__ uint32_t h[SM_RBINS];
     __shared__ SmScratch sc;
@@ -1825,7 +1828,6 @@ static bool sm_rule(int logits, double temperature, long long top_k, double top_
     return true;
 }
 
-
 // How a call runs.  Short rows: one workgroup each.  Long ones: the filters by levels of a histogram, or, for 16-bit scores, from one histogram
 // of all keys where its 256 KB a row are little next to the work (R rows at most); what a small top-k leaves goes on as a short row.
 struct SmPlan { bool is_short, top_k, top_p, counts, few; };
@@ -1880,8 +1882,9 @@ template <typename T>
 static void sample_short(const T* scores, long long ss, const float* u, long long us, long long R, long long V, long long n, const SmRule& rule,
                          const uint32_t* names, long long* out, bool distinct, hipStream_t s)
 {
-    // many draws of few rows: several workgroups filter the row again and share its draws (binary searches, 4096 of them cost a filtering)
-    const long long share = (n + 4095) / 4096, most = R < 256 ? 256 / R : 1;
+    // Many draws of few rows: workgroups that would idle filter the row once more and share its draws.  By one workgroup 5000 draws of 1000
+    // scores take 22 us and 100000 of 10000 171 us; with 4096 draws a workgroup 13 and 17 us, with 1024 7 and 12 us (7 and 11 us are 1000 draws).
+    const long long share = (n + 1023) / 1024, most = R < 256 ? 256 / R : 1;
     const dim3 grid((unsigned)R, distinct ? 1u : (unsigned)(share < most ? share : most));
 #define SM_LAUNCH_SHORT(TPB_, EPT_)                                                                                                                            \
     do {                                                                                                                                                       \
@@ -1949,11 +1952,11 @@ static int sample_launch(const T* scores, long long ss, const float* u, long lon
         SmWork sw = wk;
         sw.B = wk.stiles < 5 * wk.B ? wk.stiles : 5 * wk.B;            // (five workgroups of four waves fit a CU)
         hipLaunchKernelGGL((sm_sums_kernel<T>), dim3((unsigned)(R * sw.B)), dim3(256), 0, s, scores, ss, V, rule, sw, wk, step++);
-        hipLaunchKernelGGL((sm_draw_kernel<T>), dim3((unsigned)draws), dim3(256), 0, s, scores, ss, u, us, R, V, n, rule, wk, out);
+        hipLaunchKernelGGL((sm_draw_kernel<T>), dim3((unsigned)draws), dim3(256), 0, s, scores, ss, u, us, V, n, rule, wk, out);
         LG_RETURN_LAST();
     }
     hipLaunchKernelGGL((sm_race_kernel<T>), grid, block, 0, s, scores, ss, u, us, V, n, rule, wk, step++);
-    hipLaunchKernelGGL(sm_race_level_kernel, grid, block, 0, s, V, n, rule, wk, step++);
+    hipLaunchKernelGGL(sm_race_level_kernel, grid, block, 0, s, V, rule, wk, step++);
     SmWork zw = wk;
     zw.B = wk.tiles < wk.B ? wk.tiles : wk.B;
     hipLaunchKernelGGL((sm_zone_kernel<T>), dim3((unsigned)(R * zw.B)), block, 0, s, scores, ss, u, us, V, n, rule, zw, step++);

@@ -137,6 +137,8 @@ def test_dropout_refusals():
         a.update(kw)
         with pytest.raises(ValueError):
             stochastic.dropout(x, **a)
+    with pytest.raises(ValueError, match="columns"):
+        stochastic.dropout(x[:1, 0, :1].expand(1, 2 ** 32 + 8), 0.5, 1, chunk_ids=ids[:1])
     with pytest.raises(RuntimeError):
         stochastic.dropout(x.double(), 0.5, 1)
     with pytest.raises(RuntimeError):
@@ -291,6 +293,17 @@ def test_sampling_of_special_scores(kind, logits, V):
         for kw in RULES if V < 1000 else RULES[:1] + RULES[5:7]:
             check_sample(x, draws_of((2, 50)), logits=logits, **kw)
             check_distinct(x, draws_of((2, V)), V // 4, logits=logits, **kw)
+
+
+@pytest.mark.parametrize("T", [1e-30, 1e-20, 1e-14, 1e-8, 1e-3, 1e20, 1e30])
+@pytest.mark.parametrize("V", [300, 9000, 70001])
+@pytest.mark.parametrize("logits", [True, False])
+def test_far_temperatures(T, V, logits):
+    """equal scores have equal masses however far T magnifies what a logarithm rounds; scores that differ have 2^-24 between them at least"""
+    for kind, dtype in itertools.product(("ties", "normal"), TYPES):
+        x = scores_of(kind, 2, V, dtype, logits, seed=8)
+        for kw in (dict(), dict(top_p=0.8), dict(min_p=0.5), dict(top_k=20, top_p=0.9)):
+            check_sample(x, draws_of((2, 20)), logits=logits, temperature=T, **kw)
 
 
 @pytest.mark.parametrize("V", [5, 5000, 90000])

@@ -77,7 +77,11 @@ class CounterSampler(Sampler):
     score are never picked; where fewer have one than the budget asks for, all of them are."""
 
     def __init__(self, seed: int = 0, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
+        from . import stochastic
         super().__init__(seed)
+        if not 0 <= seed < 1 << 63:
+            raise ValueError(f"CounterSampler: seed must lie in [0, 2^63), got {seed!r}")      # (the keys above are the trainer's: dropout)
+        stochastic.check_rule("CounterSampler", temperature, top_k, top_p, min_p)             # now, not at the first densification
         self.rule = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         self._draw = 0
 

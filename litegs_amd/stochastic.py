@@ -104,6 +104,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Offset = 0, shared: in
             raise ValueError("dropout: chunk_ids must be int64 [A] on the device of x [..., A, S]")
         if shared not in (0, x.dim() - 2):
             raise ValueError("dropout: chunk_ids share the mask over all leading dimensions")
+        if x.shape[-1] >= 1 << 31:
+            raise ValueError("dropout: a chunk has at most 2^31 - 1 columns")
         shared, S, chunk_ids = x.dim() - 2, x.shape[-1], chunk_ids.contiguous()
     M = math.prod(x.shape[shared:])
     lead = math.prod(x.shape[:shared])
@@ -148,16 +150,22 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _sample(what: str, scores, u, n: int, distinct: bool, temperature, top_k, top_p, min_p, logits) -> torch.Tensor:
-    V = scores.shape[-1]
-    if V >= 1 << 31:
-        raise ValueError(f"{what}: at most 2^31 - 1 categories")
+def check_rule(what: str, temperature, top_k, top_p, min_p) -> Tuple[float, int, float, float]:
+    """the samplers' options as numbers, or ValueError"""
     temperature = _real(temperature, what, "temperature", 1e-30, 1e30)
     top_k = _integer(top_k, what, "top_k", 0, 1 << 62)
     top_p = _real(top_p, what, "top_p", 0.0, 1.0)
     min_p = _real(min_p, what, "min_p", 0.0, 1.0)
     if top_p == 0.0:
         raise ValueError(f"{what}: top_p must be more than 0")
+    return temperature, top_k, top_p, min_p
+
+
+def _sample(what: str, scores, u, n: int, distinct: bool, temperature, top_k, top_p, min_p, logits) -> torch.Tensor:
+    V = scores.shape[-1]
+    if V >= 1 << 31:
+        raise ValueError(f"{what}: at most 2^31 - 1 categories")
+    temperature, top_k, top_p, min_p = check_rule(what, temperature, top_k, top_p, min_p)
     x, uu = _rows(scores), _rows(u)
     R = x.shape[0]
     out = torch.empty((*scores.shape[:-1], n), dtype=torch.int64, device=x.device)

@@ -70,9 +70,10 @@ class FrameTrainer:
         self.sched_ticks = 1
         # opacity dropout (stochastic.dropout) of training steps: each step drops this part of the Gaussians and scales the others by
         # 1 / (1 - p).  Operator path only (fused=False): the native executor activates opacities inside its own kernels.  A step's mask is a
-        # function of (opacity_dropout_seed, training_steps, Gaussian), whichever chunks the frame sees.
+        # function of (opacity_dropout_seed, training_steps, Gaussian), whichever chunks the frame sees.  Seeds from 2^63 on are dropout's:
+        # the density controller's draws count epochs under the seeds below, and no two draws of a run may share their words.
         self.opacity_dropout = 0.0
-        self.opacity_dropout_seed = 0
+        self.opacity_dropout_seed = 1 << 63
         self.training_steps = 0
         self.last = {}
         # speculative culling (csrc/fused.hip): culled steps enqueue no gated repeat; a failed step poisons the Adam launches from there on

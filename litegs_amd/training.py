@@ -188,7 +188,7 @@ def start(lp, op, pp, dp, test_epochs: Sequence[int] = (), save_ply: Sequence[in
         cam_state = _learnable_cameras(cameras_info, training_frames, test_frames, frames, test_frames_dev, H, W, device)
     fused = bool(fused) and drop == 0.0               # opacity dropout is a step of the operator path
     trainer = FrameTrainer(params, frames, H, W, opt, sched, pp, sh_degree=0, device=device, fused=fused, extra_slots=len(test_frames_dev))
-    trainer.opacity_dropout, trainer.opacity_dropout_seed = drop, seed
+    trainer.opacity_dropout, trainer.opacity_dropout_seed = drop, 1 << 63 | (seed & (1 << 63) - 1)
     trainer.training_steps = start_epoch * len(frames)
 
     total_epoch = int(op.iterations / len(trainingset))

@@ -124,7 +124,7 @@ def test_training_steps_draw_new_masks_and_evaluation_none():
     tr.close()
 
 
-def test_start_trains_with_dropout_and_counter_sampler(tmp_path):
+def test_start_trains_with_dropout_and_counter_sampler(tmp_path, monkeypatch):
     import make_colmap_scene as M
     from litegs_amd import arguments as A
     from litegs_amd import training
@@ -133,7 +133,16 @@ def test_start_trains_with_dropout_and_counter_sampler(tmp_path):
     lp.source_path, lp.model_path, lp.eval, lp.resolution = str(tmp_path / "scene"), str(tmp_path / "m"), True, 1
     op.iterations, op.opacity_dropout = 7 * 6, 0.1
     dp.target_primitives, dp.densify_from, dp.densification_interval, dp.opacity_reset_interval, dp.sampler, dp.densify_until = 6000, 2, 3, 6, "counter", 6
+    keys = []                                                        # (seed, offset) of every draw of the run
+
+    def spy(name, at):
+        real = getattr(stochastic, name)
+        monkeypatch.setattr(stochastic, name, lambda *a, **kw: (keys.append(tuple(a[at:at + 2])), real(*a, **kw))[1])
+
+    for name, at in (("dropout", 2), ("uniform", 1), ("normal", 1)):
+        spy(name, at)
     trainer, hist = training.start(lp, op, pp, dp, test_epochs=[0, 5], log=lambda *a: None)
+    assert len(keys) > 42 and len(set(keys)) == len(keys) and len({k[0] for k in keys}) == 2
     assert not trainer.fused and trainer.training_steps == 42 and type(trainer.controller.sampler) is D.CounterSampler
     assert all(p.isfinite().all() for p in trainer.params) and hist[-1]["points_after"] > hist[0]["points"]
     op.opacity_dropout = 1.0

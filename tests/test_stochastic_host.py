@@ -109,6 +109,14 @@ def test_sampler_of_the_density_controller_is_chosen_by_its_parameters():
             D.make_sampler(D.DensifyParams(**bad))
 
 
+@pytest.mark.parametrize("bad", [dict(seed=-1), dict(seed=1 << 63), dict(temperature=0.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_k=1.5), dict(top_p=0.0),
+                                 dict(top_p=1.5), dict(min_p=-0.1)])
+def test_counter_sampler_refuses_bad_options_before_training(bad):
+    from litegs_amd import densify as D
+    with pytest.raises(ValueError):
+        D.CounterSampler(**bad)
+
+
 def test_every_draw_of_a_run_has_a_counter_of_its_own():
     from litegs_amd import densify as D
     s, seen = D.CounterSampler(1), []

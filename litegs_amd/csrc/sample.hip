@@ -24,31 +24,28 @@ enum { SM_LOGITS = 0, SM_LINEAR = 1, SM_POWER = 2 };
 
 struct SmRule { int mode; double temperature, top_p, min_p; long long top_k; };
 
-// ---- scores as ordered keys ----------------------------------------------------------------------------------------------------------
+// ---- scores ------------------------------------------------------------------------------------------------------------------------------
+// A row's passes are bound by their instructions (a vector instruction takes a wave four cycles: 69 of them per element were 27 us for 10 M),
+// so that scores are compared as the floats that they are, and taken apart as ordered integers only where a bin is wanted.
 template <typename T> struct SmMax;
 template <> struct SmMax<float> { static constexpr float v = 3.402823466e38f; };
 template <> struct SmMax<LgHalf> { static constexpr float v = 65504.0f; };
 template <> struct SmMax<LgBf16> { static constexpr float v = 3.3895313892515355e38f; };
 
-// larger score <=> larger key; 0 = excluded
-template <typename T> __device__ __forceinline__ uint32_t sm_key(T raw, bool logits)
-{
-    float x = lg_to_float(raw);
-    if (!(x == x) || (logits ? x == -INFINITY : x <= 0.0f)) return 0u;
-    x = fminf(x, SmMax<T>::v) + 0.0f;                                  // (-0 + 0 = +0: equal scores have equal keys)
-    const uint32_t b = __float_as_uint(x);
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-// the score itself; -inf = excluded
-template <typename T> __device__ __forceinline__ float sm_score(T raw, bool logits)
+__device__ __forceinline__ float sm_floor(const SmRule& r) { return r.mode == SM_LOGITS ? -INFINITY : 0.0f; }
+// the score itself (-0 + 0 = +0: equal scores have equal bits); -inf = excluded
+template <typename T> __device__ __forceinline__ float sm_score(T raw, float floor)
 {
     const float x = lg_to_float(raw);
-    return (logits ? x == x : x > 0.0f) ? fminf(x, SmMax<T>::v) + 0.0f : -INFINITY;
+    return x > floor ? fminf(x, SmMax<T>::v) + 0.0f : -INFINITY;
 }
-__device__ __forceinline__ double sm_value(uint32_t key)
+// larger float <=> larger integer, and back
+__device__ __forceinline__ uint32_t sm_order(float k)
 {
-    return (double)__uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+    const uint32_t b = __float_as_uint(k);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float sm_unorder(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
 
 // exp(x) for x <= 0 and log(x) for x > 0 in 64 bits, without the general functions' special cases (which cost as much again, and registers):
 // x = n ln 2 + r with |r| <= ln 2 / 2 and the Taylor polynomial of degree 13 (first term left out < 5e-18);  x = 2^e m with m in
@@ -96,29 +93,28 @@ struct SmScale { int mode; double inv_t, top /*l of the best score, or its weigh
 
 // The best one's l has to come from the function that gives the others' (`ln`): at a temperature of 1e-20 the last bit of a logarithm is
 // as much as e^1000.
-template <typename Ln> __device__ __forceinline__ SmScale sm_scale(const SmRule& r, uint32_t best, const Ln& ln)
+template <typename Ln> __device__ __forceinline__ SmScale sm_scale(const SmRule& r, float best, const Ln& ln)
 {
     SmScale s = { r.mode, 1.0 / r.temperature, 0.0, 1.0 };
-    if (best == 0u) return s;
-    const double x = sm_value(best);
+    if (best == -INFINITY) return s;
+    const double x = (double)best;
     if (r.mode == SM_LOGITS) s.top = x * s.inv_t;
     else if (r.mode == SM_POWER) s.top = ln(x) * s.inv_t;
     else { s.top = x; s.shift = ldexp(1.0, -ilogb(x) - 1); }
     return s;
 }
-__device__ __forceinline__ SmScale sm_scale(const SmRule& r, uint32_t best)                   // for sm_mass
+__device__ __forceinline__ SmScale sm_scale(const SmRule& r, float best)                      // for sm_mass
 {
     return sm_scale(r, best, [](double x) { return sm_ln(x); });
 }
-__device__ __forceinline__ double sm_log(const SmScale& s, uint32_t key)
+__device__ __forceinline__ double sm_log(const SmScale& s, float score)
 {
-    const double x = sm_value(key);
+    const double x = (double)score;
     return s.mode == SM_LOGITS ? x * s.inv_t : s.mode == SM_POWER ? sm_ln(x) * s.inv_t : sm_ln(x);
 }
-__device__ __forceinline__ double sm_mass(const SmScale& s, uint32_t key)
+__device__ __forceinline__ double sm_mass(const SmScale& s, float score)                      // (NaN of a NaN)
 {
-    if (key == 0u) return 0.0;
-    return s.mode == SM_LINEAR ? sm_value(key) : sm_exp(sm_log(s, key) - s.top);
+    return s.mode == SM_LINEAR ? (double)score : sm_exp(sm_log(s, score) - s.top);
 }
 // The same masses in about a third of the instructions, for passes over whole rows, with two tables in LDS that each workgroup works out for
 // itself: 1 / c and log c for the middles c of 128 parts of [1, 2) -- a score has 24 bits, m / c - 1 is one product, below 1 / 256, and six
@@ -159,7 +155,7 @@ __device__ __forceinline__ double sm_ln(const SmTables& t, float x)
     p = fma(r, p, -0.5);
     return fma(n, 6.93147180369123816e-01, fma(n, 1.90821492927058770e-10, t.log[i] + fma(r * r, p, r)));
 }
-__device__ __forceinline__ SmScale sm_scale(const SmTables& t, const SmRule& r, uint32_t best)        // for sm_masses
+__device__ __forceinline__ SmScale sm_scale(const SmTables& t, const SmRule& r, float best)        // for sm_masses
 {
     return sm_scale(r, best, [&](double x) { return sm_ln(t, (float)x); });
 }
@@ -192,21 +188,13 @@ template <int N> __device__ __forceinline__ void sm_masses(const SmTables& t, co
 #pragma unroll
     for (int k = 0; k < N; k++) m[k] = x[k] > -INFINITY ? m[k] : 0.0;
 }
-__device__ __forceinline__ float sm_float(uint32_t key) { return key ? __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key) : -INFINITY; }
-template <int N> __device__ __forceinline__ void sm_masses(const SmTables& t, const SmScale& s, const uint32_t (&key)[N], double (&m)[N])
-{
-    float x[N];
-#pragma unroll
-    for (int k = 0; k < N; k++) x[k] = sm_float(key[k]);
-    sm_masses(t, s, x, m);
-}
 
 // key of the exponential race, ordered as an unsigned integer; 0 = excluded
-__device__ __forceinline__ unsigned long long sm_race(const SmScale& s, uint32_t key, float u)
+__device__ __forceinline__ unsigned long long sm_race(const SmScale& s, float score, float u)
 {
-    if (key == 0u) return 0ull;
+    if (score == -INFINITY) return 0ull;
     u = u == u ? fminf(fmaxf(u, 0x1p-33f), 1.0f - 0x1p-24f) : 1.0f - 0x1p-24f;
-    const double k = sm_log(s, key) - log(-log1p(-(double)u)) + 0.0;
+    const double k = sm_log(s, score) - log(-log1p(-(double)u)) + 0.0;
     const unsigned long long b = (unsigned long long)__double_as_longlong(k);
     return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
 }
@@ -403,28 +391,29 @@ template <bool MASS> __device__ __forceinline__ bool sm_whole_bin(const SmTake& 
     return count == 1 || (!MASS && take.target - (double)take.before_n >= (double)count);
 }
 
-// What passes the filters: key > thr, or key == thr and index <= last (key 0 never does).
-struct SmKept { uint32_t thr, last; };
+// What passes the filters: scores above thr, and those equal to it up to index `end` (thr = -inf, end = 0: all but the excluded)
+struct SmKept { float thr; uint32_t end; };
 #define SM_ALL 0xffffffffu
-__device__ __forceinline__ bool sm_in(const SmKept& k, uint32_t key, uint32_t i) { return key != 0u && (key > k.thr || (key == k.thr && i <= k.last)); }
+__device__ __forceinline__ bool sm_in(const SmKept& k, float x, uint32_t i) { return x > k.thr || (x == k.thr && i < k.end); }
 
-// min-p as a cut of the keys: the smallest key whose mass is at least min_p of the best one's (the mass grows with the key)
-__device__ __forceinline__ void sm_min_p(const SmRule& rule, uint32_t best, SmKept& kept)
+// min-p as a cut of the scores: the smallest one whose mass is at least min_p of the best one's (the mass grows with the score)
+__device__ __forceinline__ void sm_min_p(const SmRule& rule, float best, SmKept& kept)
 {
     const SmScale s = sm_scale(rule, best);
     const double least = rule.min_p * sm_mass(s, best);
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t lo = 1, hi = best;                                        // 64 probes a round; the mass at hi is enough
+    uint32_t lo = s.mode == SM_LOGITS ? 1u : 0x80000001u /*the least weight*/, hi = sm_order(best);      // 64 probes a round; the mass at hi is enough
     while (lo < hi) {
         const uint32_t gap = (hi - lo) / 64 + 1;
         const unsigned long long p = (unsigned long long)lo + (unsigned long long)lane * gap;
-        const unsigned long long ok = __ballot(p >= hi || sm_mass(s, (uint32_t)p) >= least);
+        const unsigned long long ok = __ballot(p >= hi || sm_mass(s, sm_unorder((uint32_t)p)) >= least);
         const uint32_t f = ok ? (uint32_t)__ffsll((long long)ok) - 1 : 64;
         const unsigned long long nhi = (unsigned long long)lo + (unsigned long long)f * gap;
         if (f) lo += (f - 1) * gap + 1;
         hi = nhi < hi ? (uint32_t)nhi : hi;
     }
-    if (lo > kept.thr) kept = SmKept{ lo, SM_ALL };
+    const float thr = sm_unorder(lo);
+    if (thr > kept.thr) kept = SmKept{ thr, SM_ALL };
 }
 
 // ---- approximate race keys ---------------------------------------------------------------------------------------------------------------
@@ -443,13 +432,6 @@ __device__ __forceinline__ float sm_log2(float x)                      // x > 0,
 }
 __device__ __forceinline__ float sm_margin(float k, float slope) { return 0x1p-13f + fabsf(k) * 0x1p-18f + slope * 0x1p-21f; }
 __device__ __forceinline__ float sm_slope(const SmRule& r) { return (float)((r.mode == SM_LOGITS ? 1.4426950408889634 : 1.0) / r.temperature); }
-
-__device__ __forceinline__ uint32_t sm_order(float k)
-{
-    const uint32_t b = __float_as_uint(k);
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float sm_unorder(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
 
 // approximate key of a candidate.  `slope`: log2(e) / T or 1 / T in 32 bits
 __device__ __forceinline__ float sm_race32(bool logits, float slope, float x, float u)
@@ -471,7 +453,7 @@ __device__ __forceinline__ SmZone sm_zone(uint32_t lo, uint32_t hi, float slope)
 }
 
 // (out of line: sixteen of them inlined, with their constants, spill two thousand registers)
-__device__ __attribute__((noinline)) unsigned long long sm_race_call(SmScale s, uint32_t key, float u) { return sm_race(s, key, u); }
+__device__ __attribute__((noinline)) unsigned long long sm_race_call(SmScale s, float x, float u) { return sm_race(s, x, u); }
 
 // ---- short rows: one workgroup per row, EPT consecutive elements of a thread in registers ----------------------------------------------
 // One CU works on a row, so that every instruction an element costs is 0.1 us for 15 k of them: scores are kept as floats (-inf: excluded)
@@ -608,12 +590,9 @@ __device__ __forceinline__ SmBin sm_find_short(const float (&x)[EPT], const doub
     }
 }
 
-// what is left of a row: numbers above thr, and those equal to it up to index last
-struct SmLeft { float thr; uint32_t last; };
-
 // what a top-k (MASS false) or top-p with that target leaves of the candidates
 template <bool MASS, int TPB, int EPT>
-__device__ __forceinline__ SmLeft sm_filter_short(const float (&x)[EPT], const double* mass, bool linear, SmTake take, SmShortLds& h, SmScratch& sc)
+__device__ __forceinline__ SmKept sm_filter_short(const float (&x)[EPT], const double* mass, bool linear, SmTake take, SmShortLds& h, SmScratch& sc)
 {
     SmBins bins;
     const SmBin bin = sm_find_short<MASS, TPB, EPT>(x, mass, linear, take, 64, h.hist, sc, bins);
@@ -627,7 +606,7 @@ __device__ __forceinline__ SmLeft sm_filter_short(const float (&x)[EPT], const d
         }
         __syncthreads();
         const uint32_t ties = sm_ties<MASS>(take, bin.count, MASS ? __longlong_as_double((long long)sc.word[5]) : 0.0);
-        return SmLeft{ bins.lo, ties < bin.count ? sm_nth_short<EPT>(tie, ties, sc) : SM_ALL };
+        return SmKept{ bins.lo, ties < bin.count ? sm_nth_short<EPT>(tie, ties, sc) + 1 : SM_ALL };
     }
     __syncthreads();
     if (threadIdx.x == 0) sc.word[5] = 0;
@@ -659,7 +638,7 @@ __device__ __forceinline__ SmLeft sm_filter_short(const float (&x)[EPT], const d
         if ((int)l == e) { sc.word[0] = __float_as_uint(h.few.x[a]); sc.word[1] = h.few.index[a]; }
     }
     __syncthreads();
-    return SmLeft{ __uint_as_float((uint32_t)sc.word[0]), (uint32_t)sc.word[1] };
+    return SmKept{ __uint_as_float((uint32_t)sc.word[0]), (uint32_t)sc.word[1] + 1 };
 }
 
 template <typename T, int TPB, int EPT, bool DISTINCT>
@@ -676,6 +655,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     const long long r = blockIdx.x;
     const T* row = scores + r * sstride;
     const bool logits = rule.mode == SM_LOGITS;
+    const float floor = sm_floor(rule);
     u += r * ustride;
     out += r * n;
     if (names) names += r * V;
@@ -688,15 +668,14 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         for (int k = 0; k < EPT / 4; k++) v[k] = sm_load4(row, i0 + 4 * k, V, sm_aligned(row));
         sm_tables(tables, rule.mode);                                  // (the first scan is the barrier)
 #pragma unroll
-        for (int k = 0; k < EPT; k++) { x[k] = sm_score(v[k / 4].v[k % 4], logits); most = fmaxf(most, x[k]); }
+        for (int k = 0; k < EPT; k++) { x[k] = sm_score(v[k / 4].v[k % 4], floor); most = fmaxf(most, x[k]); }
     }
     most = sm_unorder(sm_block_max(sm_order(most), sc.a));
     if (most == -INFINITY) {                                           // nothing to draw from
         for (long long j = (long long)blockIdx.y * TPB + threadIdx.x; j < n; j += (long long)gridDim.y * TPB) out[j] = -1;
         return;
     }
-    const uint32_t best = sm_order(most);
-    const SmScale scale = sm_scale(tables, rule, best);
+    const SmScale scale = sm_scale(tables, rule, most);
     // masses, once: linear ones by a power of two below one
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
     auto masses = [&]() {
@@ -712,7 +691,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     // filters: an element that one of them drops becomes -inf
     for (int pass = 0; pass < 2; pass++) {
         SmTake take = { 0.0, 0, { 0, 0 } };
-        SmLeft left;
+        SmKept left;
         if (pass == 0) {
             if (rule.top_k <= 0 || rule.top_k >= V) continue;
             take.target = (double)rule.top_k;
@@ -729,14 +708,13 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             left = sm_filter_short<true, TPB, EPT>(x, mass, logits, take, h, sc);
         }
 #pragma unroll
-        for (int k = 0; k < EPT; k++) if (!(x[k] > left.thr || (x[k] == left.thr && (uint32_t)(i0 + k) <= left.last))) x[k] = -INFINITY;
+        for (int k = 0; k < EPT; k++) if (!sm_in(left, x[k], (uint32_t)(i0 + k))) x[k] = -INFINITY;
     }
     if (rule.min_p > 0.0) {
-        SmKept kept = { 0u, SM_ALL };
-        sm_min_p(rule, best, kept);
-        const float least = sm_float(kept.thr);
+        SmKept kept = { -INFINITY, 0u };
+        sm_min_p(rule, most, kept);
 #pragma unroll
-        for (int k = 0; k < EPT; k++) if (!(x[k] >= least)) x[k] = -INFINITY;
+        for (int k = 0; k < EPT; k++) if (!(x[k] >= kept.thr)) x[k] = -INFINITY;
     }
     if (DISTINCT) {
         float race[EPT];                                               // approximate keys; -inf: not a candidate
@@ -774,7 +752,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         if (found <= SM_BINS) {
             for (uint32_t a = threadIdx.x; a < found; a += TPB) {
                 const uint32_t i = h.zone.index[a];
-                h.zone.rank[a] = sm_race_call(scale, sm_key(row[i], logits), u[i]);
+                h.zone.rank[a] = sm_race_call(scale, sm_score(row[i], floor), u[i]);
             }
             __syncthreads();
             for (uint32_t a = threadIdx.x; a < found; a += TPB) {
@@ -790,7 +768,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             // many elements next to the border (equal numbers, or a slope that spreads nothing): radix selection of their exact keys
             unsigned long long *mine = (unsigned long long*)mass + threadIdx.x, elo;        // (the masses are done)
 #pragma unroll
-            for (int k = 0; k < EPT; k++) mine[k * TPB] = race[k] > -INFINITY && race[k] >= zlo && race[k] <= zhi ? sm_race_call(scale, sm_order(x[k]), u[i0 + k]) : 0ull;
+            for (int k = 0; k < EPT; k++) mine[k * TPB] = race[k] > -INFINITY && race[k] >= zlo && race[k] <= zhi ? sm_race_call(scale, x[k], u[i0 + k]) : 0ull;
             SmTake left = { (double)room, 0, { 0, 0 } };
             const SmBin e = sm_select_short<TPB, EPT>([&](int k, unsigned long long& w) { w = mine[k * TPB]; return w != 0ull; }, left, h.hist, sc, elo);
             const uint32_t ties = e.bin < 0 ? 0 : e.count == 1 ? 1 : sm_ties<false>(left, e.count, 0.0);
@@ -854,12 +832,13 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
 #define SM_GROUP 16                    // elements per stored prefix
 #define SM_STEPS 12
 
-struct SmRowState {
+struct SmRowState {                    // (sm_begin_kernel knows where kept and before are)
     SmKept kept, before;               // what passes the filters; ... before the selection under way
     SmTake take;
     double total, top;                 // with replacement: total mass of the kept; the largest l
     unsigned long long sure;           // race: winners
-    uint32_t prefix, ties, best, least, ended, cut, zone_lo, zone_hi, candidates;
+    float best, least;                 // largest score; least score that passes min-p
+    uint32_t prefix, ties, ended, cut, zone_lo, zone_hi, candidates;
     uint32_t ticket[SM_STEPS], sub[16];
 };
 
@@ -914,12 +893,13 @@ __global__ void __launch_bounds__(SM_LTPB) sm_begin_kernel(const T* __restrict__
     __shared__ SmScratch sc;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
     uint4* clear = (uint4*)(wk.clear + r * wk.clear_bytes);
-    for (long long i = b * SM_LTPB + threadIdx.x; i < wk.clear_bytes / 16; i += wk.B * SM_LTPB) clear[i] = uint4{ 0, 0, 0, 0 };
+    for (long long i = b * SM_LTPB + threadIdx.x; i < wk.clear_bytes / 16; i += wk.B * SM_LTPB) clear[i] = i == 0 ? uint4{ 0xff800000u, 0, 0xff800000u, 0 } : uint4{ 0, 0, 0, 0 };        // (kept, before)
     if (!want_best) return;
     const T* x = scores + r * sstride;
-    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const bool vec = sm_aligned(x);
+    const float floor = sm_floor(rule);
     const long long stride = wk.B * SM_LTPB * 4;
-    uint32_t best = 0;
+    float best = -INFINITY;
     for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += 4 * stride) {
         LgVec4<T> v[4];
 #pragma unroll
@@ -927,28 +907,45 @@ __global__ void __launch_bounds__(SM_LTPB) sm_begin_kernel(const T* __restrict__
 #pragma unroll
         for (int g = 0; g < 4; g++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) { const uint32_t k = sm_key(v[g].v[j], logits); best = k > best ? k : best; }
+            for (int j = 0; j < 4; j++) best = fmaxf(best, sm_score(v[g].v[j], floor));
     }
-    best = sm_block_max(best, sc.a);
-    if (threadIdx.x == 0) wk.best[r * wk.B + b] = best;
+    const uint32_t order = sm_block_max(sm_order(best), sc.a);
+    if (threadIdx.x == 0) wk.best[r * wk.B + b] = order;
 }
 // the row's best (every wave on its own)
-__device__ __forceinline__ uint32_t sm_best(const SmWork& wk, long long r)
+__device__ __forceinline__ float sm_best(const SmWork& wk, long long r)
 {
     uint32_t best = 0;
     for (long long i = threadIdx.x & 63; i < wk.B; i += 64) { const uint32_t k = wk.best[r * wk.B + i]; best = k > best ? k : best; }
-    return sm_lane(sm_wave_scan<false>(best, SmMaxOf()), 63);
+    return sm_unorder(sm_lane(sm_wave_scan<false>(best, SmMaxOf()), 63));
 }
 
-// what a selection leaves in the row's state (one thread): `ties` of `count` elements of key thr are taken, and all above it
-__device__ __forceinline__ void sm_conclude(SmRowState& st, const SmKept& kept, uint32_t thr, uint32_t ties, uint32_t count)
+// what a selection leaves in the row's state (one thread): `ties` of `count` elements of score thr are taken, and all above it
+__device__ __forceinline__ void sm_conclude(SmRowState& st, const SmKept& kept, float thr, uint32_t ties, uint32_t count)
 {
     if (thr < kept.thr) return;                                        // a whole bin around the earlier filter's cut: that one stands
-    st.kept = SmKept{ thr, thr == kept.thr ? kept.last : SM_ALL };
+    st.kept = SmKept{ thr, thr == kept.thr ? kept.end : SM_ALL };
     if (ties < count) { st.cut = 1; st.ties = ties; }
 }
 
-// one level of top-k (MASS false) or top-p: bits [shift - width, shift) of the keys that pass the filters and match the prefix found so far
+// Masses as integers that one addition to LDS adds up: so many of 2^bits parts that a workgroup's share of the row cannot overflow 63 bits
+// (50 bits of the largest mass for short rows, 47 for 10 M scores; two limbs took 6 us more for those 10 M).  The addition of 2^(52 - bits)
+// rounds, and leaves the integer in the low bits.
+struct SmParts { int bits; double one; };
+__device__ __forceinline__ SmParts sm_parts(const SmWork& wk, long long V)
+{
+    const long long share = (V + wk.B * SM_LTPB * 4 - 1) / (wk.B * SM_LTPB * 4) * (SM_LTPB * 4);
+    const int bits = __clzll(share - 1) - 1;                           // 63 - ceil(log2(share))
+    return SmParts{ bits < 51 ? bits : 51, ldexp(1.0, 52 - (bits < 51 ? bits : 51)) };
+}
+__device__ __forceinline__ unsigned long long sm_count_parts(const SmParts& p, double mass, double unit)
+{
+    return (unsigned long long)__double_as_longlong(fma(mass, unit, p.one)) - (unsigned long long)__double_as_longlong(p.one);
+}
+__device__ __forceinline__ SmSum sm_sum_of_parts(const SmParts& p, unsigned long long v) { return SmSum{ v >> (p.bits - 31), (v << (63 - p.bits)) & 0xffffffffull }; }
+
+// one level of top-k (MASS false) or top-p: bits [shift - width, shift) of the ordered scores that pass the filters and match the prefix found
+// so far
 template <typename T, bool MASS>
 __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step,
                                                            int shift, int width)
@@ -962,7 +959,8 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     SmRowState& st = wk.state(r);
     const bool first = shift == 32;
     const T* x = scores + r * sstride;
-    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const bool vec = sm_aligned(x);
+    const float floor = sm_floor(rule);
     const int at = shift - width, nbins = 1 << width, p = width - 6;
     const long long stride = wk.B * SM_LTPB * 4;
     long long i = (b * SM_LTPB + threadIdx.x) * 4;
@@ -971,35 +969,47 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     for (int g = 0; g < G; g++) v[g] = sm_load4(x, i + g * stride, V, vec);
     if (!first && st.ended) return;
     const SmKept kept = first ? st.kept : st.before;
+    const bool filtered = kept.thr > -INFINITY;
     const uint32_t prefix = st.prefix;
-    const uint32_t best = MASS ? (first ? sm_best(wk, r) : st.best) : 0u;
+    // the prefix as a range of scores (its last one is not -0, which equals the first one of the next range)
+    float least = -SmMax<float>::v, most = SmMax<float>::v;
+    if (!first) {
+        const uint32_t last = (prefix << shift) | ((1u << shift) - 1);
+        least = sm_unorder(prefix << shift);
+        most = sm_unorder(last == 0x7fffffffu ? last - 1 : last);
+    }
+    const float best = MASS ? (first ? sm_best(wk, r) : st.best) : 0.0f;
+    const SmParts parts = sm_parts(wk, V);
     const bool counted = !MASS || at == 0;                             // masses need no counts before the last level
     if (MASS) sm_tables(tables, rule.mode);
-    for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { h.n[k] = 0; if (MASS) { h.hi[k] = 0; h.lo[k] = 0; } }
+    for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { h.n[k] = 0; if (MASS) h.lo[k] = 0; }
     __syncthreads();
     const SmScale scale = sm_scale(tables, rule, best);
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
     while (i < V) {
-        uint32_t key[4 * G];
+        float z[4 * G];
+        int found = 0;
 #pragma unroll
         for (int g = 0; g < G; g++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint32_t k = sm_key(v[g].v[j], logits);
-                key[4 * g + j] = sm_in(kept, k, (uint32_t)(i + g * stride + j)) && (first || (k >> shift) == prefix) ? k : 0u;
+                float y = sm_score(v[g].v[j], floor);
+                y = y >= least && y <= most ? y : -INFINITY;
+                if (filtered) y = sm_in(kept, y, (uint32_t)(i + g * stride + j)) ? y : -INFINITY;
+                z[4 * g + j] = y;
+                if (MASS) found += __popcll(__ballot(y > -INFINITY));
             }
         double mass[4 * G];
-        if (MASS && first) sm_masses(tables, scale, key, mass);        // (later levels: few are left, one at a time)
+        const bool many = MASS && found >= 64;                         // (the same for the wave: all masses at once, or one at a time)
+        if (many) sm_masses(tables, scale, z, mass);
 #pragma unroll
         for (int j = 0; j < 4 * G; j++) {
-            if (key[j] == 0u) continue;
-            const int bin = sm_slot((int)(key[j] >> at) & (nbins - 1), p);
+            if (!(z[j] > -INFINITY)) continue;
+            const int bin = sm_slot((int)(sm_order(z[j]) >> at) & (nbins - 1), p);
             if (counted) atomicAdd(&h.n[bin], 1u);
             if (MASS) {
-                if (!first) { const uint32_t one[1] = { key[j] }; double m[1]; sm_masses(tables, scale, one, m); mass[j] = m[0]; }
-                const SmLimbs m = sm_limbs(mass[j] * unit);
-                if (m.hi) atomicAdd(&h.hi[bin], (unsigned long long)m.hi);
-                if (m.lo) atomicAdd(&h.lo[bin], (unsigned long long)m.lo);
+                if (!many) { const float one[1] = { z[j] }; double m[1]; sm_masses(tables, scale, one, m); mass[j] = m[0]; }
+                atomicAdd(&h.lo[bin], sm_count_parts(parts, mass[j], unit));
             }
         }
         i += G * stride;
@@ -1007,6 +1017,9 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
 #pragma unroll
         for (int g = 0; g < G; g++) v[g] = sm_load4(x, i + g * stride, V, vec);
     }
+    __syncthreads();
+    if (MASS)
+        for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { const SmSum m = sm_sum_of_parts(parts, h.lo[k]); h.hi[k] = m.hi; h.lo[k] = m.lo; }
     __syncthreads();
     if (wk.B > 1) {
         SmHist& g = wk.hist(r);
@@ -1057,11 +1070,11 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     const bool whole = counted && sm_whole_bin<MASS>(take, bin.count);
     if (!whole && at > 0) return;
     // the key is found, or the lowest key of a bin that is taken whole; a cut among the equal ones is left to sm_cut_kernel
-    const uint32_t thr = found << at, one[1] = { thr };
+    const float thr = sm_unorder(found << at), one[1] = { thr };
     double mass[1] = { 0.0 };
     if (MASS) sm_masses(tables, scale, one, mass);
     st.ended = 1;
-    sm_conclude(st, kept, thr, whole ? bin.count : sm_ties<MASS>(take, bin.count, mass[0] * unit), bin.count);
+    sm_conclude(st, kept, thr, whole ? bin.count : sm_ties<MASS>(take, bin.count, fma(mass[0], unit, parts.one) - parts.one), bin.count);
 }
 
 // ---- scores of 16 bits: both filters from one histogram of all keys ----------------------------------------------------------------------
@@ -1076,19 +1089,15 @@ template <typename T> __device__ __forceinline__ T sm_from_bits(uint32_t b);
 template <> __device__ __forceinline__ LgHalf sm_from_bits<LgHalf>(uint32_t b) { return __builtin_bit_cast(LgHalf, (uint16_t)b); }
 template <> __device__ __forceinline__ LgBf16 sm_from_bits<LgBf16>(uint32_t b) { return LgBf16{ (uint16_t)b }; }
 
-// ordered key of 16 bits; 0 = excluded.  sm_key(sm_unkey16(k)) orders like k
-template <typename T> __device__ __forceinline__ uint32_t sm_key16(T raw, bool logits)
+// a score as an ordered key of 16 bits, 0 = excluded, and back
+template <typename T> __device__ __forceinline__ uint32_t sm_key16(T raw, float floor)
 {
-    const uint32_t key = sm_key(raw, logits);
-    if (key == 0u) return 0u;
-    const float x = __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);        // canonical: no -0, no infinity
+    const float x = sm_score(raw, floor);
+    if (x == -INFINITY) return 0u;
     const uint32_t b = sm_bits(lg_from_float<T>(x));
     return (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
 }
-template <typename T> __device__ __forceinline__ uint32_t sm_key_of16(uint32_t k, bool logits)
-{
-    return k == 0u ? 0u : sm_key(sm_from_bits<T>((k & 0x8000u) ? (k & 0x7fffu) : (~k & 0xffffu)), logits);
-}
+template <typename T> __device__ __forceinline__ float sm_unkey16(uint32_t k) { return lg_to_float(sm_from_bits<T>((k & 0x8000u) ? (k & 0x7fffu) : (~k & 0xffffu))); }
 
 // per chunk of 64 keys: count, and mass in limbs, of what a filter left
 struct SmChunks { uint32_t n[1024]; unsigned long long hi[1024], lo[1024]; };
@@ -1102,7 +1111,8 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
     SmRowState& st = wk.state(r);
     const T* x = scores + r * sstride;
-    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const bool vec = sm_aligned(x);
+    const float floor = sm_floor(rule);
     const long long stride = wk.B * 4096;
     long long i = (b * 1024 + threadIdx.x) * 4;
     LgVec4<T> v[4];
@@ -1115,7 +1125,7 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
         for (int g = 0; g < 4; g++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint32_t k = sm_key16(v[g].v[j], logits);
+                const uint32_t k = sm_key16(v[g].v[j], floor);
                 if (k) atomicAdd(&h.pair[k >> 1], 1u << (16 * (k & 1)));
             }
         i += 4 * stride;
@@ -1155,10 +1165,10 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
         }
     }
     best = sm_block_max(best, sc.a);
-    const uint32_t best_key = sm_key_of16<T>(best, logits);
-    const SmScale scale = sm_scale(rule, best_key);
+    const float most = best ? sm_unkey16<T>(best) : -INFINITY;
+    const SmScale scale = sm_scale(rule, most);
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
-    SmKept kept = { 0u, SM_ALL };
+    SmKept kept = { -INFINITY, 0u };
     uint32_t cut_key = 0, cut_n = 0;                                   // top-k: keys above cut_key whole, cut_n of it
     uint32_t thr = 0, ties = 0, equal = 0;
     for (int pass = 0; pass < 2 && best != 0; pass++) {
@@ -1172,7 +1182,7 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
         };
         auto limbs = [&](uint32_t k, uint32_t n) {
             SmSum m = { 0, 0 };
-            if (n) { const SmLimbs one = sm_limbs(sm_mass(scale, sm_key_of16<T>(k, logits)) * unit); m = SmSum{ (unsigned long long)one.hi * n, (unsigned long long)one.lo * n }; }
+            if (n) { const SmLimbs one = sm_limbs(sm_mass(scale, sm_unkey16<T>(k)) * unit); m = SmSum{ (unsigned long long)one.hi * n, (unsigned long long)one.lo * n }; }
             return m;
         };
         if (mass) {
@@ -1233,7 +1243,7 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
         thr = sm_lane(k, l);
         take.before_n += sm_lane(in - n2, l);
         if (mass) { take.before_m.hi += sm_lane(in2.hi - m2.hi, l); take.before_m.lo += sm_lane(in2.lo - m2.lo, l); }
-        const double unit_mass = mass ? sm_mass(scale, sm_key_of16<T>(thr, logits)) * unit : 0.0;
+        const double unit_mass = mass ? sm_mass(scale, sm_unkey16<T>(thr)) * unit : 0.0;
         ties = mass ? sm_ties<true>(take, equal, unit_mass) : sm_ties<false>(take, equal, 0.0);
         // equal ones that top-k had left out count as cut too
         equal = sm_peek(&counts[thr]);
@@ -1241,15 +1251,15 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
         cut_n = ties;
         __syncthreads();
     }
-    SmKept least = { 0u, SM_ALL };
-    if (best != 0 && rule.min_p > 0.0) sm_min_p(rule, best_key, least);
+    SmKept least = kept;
+    if (best != 0 && rule.min_p > 0.0) sm_min_p(rule, most, least);
     if (threadIdx.x != 0) return;
     st.before = kept;
-    st.best = best_key;
+    st.best = most;
     st.least = least.thr;
     st.ended = 1;
     st.cut = 0;
-    if (best != 0) sm_conclude(st, kept, sm_key_of16<T>(thr, logits), ties, equal);
+    if (best != 0) sm_conclude(st, kept, sm_unkey16<T>(thr), ties, equal);
 }
 
 // ---- cuts among equal keys, and what top-k left ------------------------------------------------------------------------------------------
@@ -1265,7 +1275,8 @@ __global__ void __launch_bounds__(SM_LTPB) sm_cut_kernel(const T* __restrict__ s
     const bool cut = st.cut;
     if (!GATHER && !cut) return;
     const T* x = scores + r * sstride;
-    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const bool vec = sm_aligned(x);
+    const float floor = sm_floor(rule);
     const SmKept kept = st.kept;
     uint32_t *tile_n = wk.tile_n + r * wk.tiles, *tile_eq = wk.tile_eq + r * wk.tiles;
     for (long long t = b; t < wk.tiles; t += wk.B) {
@@ -1278,9 +1289,10 @@ __global__ void __launch_bounds__(SM_LTPB) sm_cut_kernel(const T* __restrict__ s
         for (int g = 0; g < SM_TILE / SM_LTPB / 4; g++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint32_t k = sm_key(v[g].v[j], logits), i = (uint32_t)(t * SM_TILE + (g * SM_LTPB + threadIdx.x) * 4 + j);
-                eq += k != 0u && k == kept.thr && i <= kept.last;
-                more += k > kept.thr;
+                const float y = sm_score(v[g].v[j], floor);
+                const uint32_t i = (uint32_t)(t * SM_TILE + (g * SM_LTPB + threadIdx.x) * 4 + j);
+                eq += y == kept.thr && i < kept.end;
+                more += y > kept.thr;
             }
         sm_block_scan<uint32_t>(eq, sc.a, total);
         if (threadIdx.x == 0) sm_poke(&tile_eq[t], total);
@@ -1324,12 +1336,11 @@ __global__ void __launch_bounds__(SM_LTPB) sm_cut_kernel(const T* __restrict__ s
     uint32_t is = 0, total;
 #pragma unroll
     for (int k = 0; k < E; k++) {
-        const uint32_t key = sm_key(v[k / 4].v[k % 4], logits);
-        if (key != 0u && key == kept.thr && (uint32_t)(i0 + k) <= kept.last) is |= 1u << k;
+        if (sm_score(v[k / 4].v[k % 4], floor) == kept.thr && (uint32_t)(i0 + k) < kept.end) is |= 1u << k;
     }
     uint32_t before = sm_block_scan<uint32_t>(__popc(is), sc.a, total);
 #pragma unroll
-    for (int k = 0; k < E; k++) if (((is >> k) & 1) && ++before == rest) { st.kept.last = (uint32_t)(i0 + k); st.cut = 0; }
+    for (int k = 0; k < E; k++) if (((is >> k) & 1) && ++before == rest) { st.kept.end = (uint32_t)(i0 + k) + 1; st.cut = 0; }
 }
 
 // what top-k left, in index order: scores, their names and (without replacement) their numbers; rule.top_k places a row, the last ones empty
@@ -1341,7 +1352,8 @@ __global__ void __launch_bounds__(SM_LTPB) sm_gather_kernel(const T* __restrict_
     const long long r = blockIdx.x / wk.tiles, t = blockIdx.x % wk.tiles, K = rule.top_k;
     const SmRowState& st = wk.state(r);
     const T* x = scores + r * sstride;
-    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const bool vec = sm_aligned(x);
+    const float floor = sm_floor(rule);
     const SmKept kept = st.kept;
     constexpr int E = SM_TILE / SM_LTPB;                               // consecutive elements a thread
     const long long i0 = t * SM_TILE + (long long)threadIdx.x * E;
@@ -1350,7 +1362,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_gather_kernel(const T* __restrict_
     for (int g = 0; g < E / 4; g++) v[g] = sm_load4(x, i0 + 4 * g, V, vec);
     uint32_t in = 0, total;
 #pragma unroll
-    for (int k = 0; k < E; k++) if (sm_in(kept, sm_key(v[k / 4].v[k % 4], logits), (uint32_t)(i0 + k))) in |= 1u << k;
+    for (int k = 0; k < E; k++) if (sm_in(kept, sm_score(v[k / 4].v[k % 4], floor), (uint32_t)(i0 + k))) in |= 1u << k;
     long long at = (long long)wk.tile_n[r * wk.tiles + t] + sm_block_scan<uint32_t>(__popc(in), sc.a, total);
     T* few = (T*)wk.few + r * K;
     uint32_t* names = wk.names + r * K;
@@ -1374,8 +1386,8 @@ __device__ __forceinline__ SmKept sm_final(const SmWork& wk, long long r, const 
     SmKept kept = st.kept;
     if (rule.min_p <= 0.0) return kept;
     if (!wk.best) return st.least > kept.thr ? SmKept{ st.least, SM_ALL } : kept;
-    const uint32_t best = sm_best(wk, r);
-    if (best) sm_min_p(rule, best, kept);
+    const float best = sm_best(wk, r);
+    if (best > -INFINITY) sm_min_p(rule, best, kept);
     return kept;
 }
 
@@ -1391,7 +1403,8 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
     SmRowState& st = wk.state(r);
     const T* x = scores + r * sstride;
-    const bool vec = sm_aligned(x), logits = rule.mode == SM_LOGITS;
+    const bool vec = sm_aligned(x);
+    const float floor = sm_floor(rule);
     sm_tables(tables, rule.mode);                                      // (the scans below are the barrier)
     const SmKept kept = sm_final(whole, r, st, rule);
     double *sums = wk.tile_sum + r * wk.stiles, *tops = wk.tile_top + r * wk.stiles, *groups = wk.group + r * wk.stiles * (SM_STILE / SM_GROUP);
@@ -1400,24 +1413,24 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
         LgVec4<T> v[SM_GROUP / 4];
 #pragma unroll
         for (int k = 0; k < SM_GROUP / 4; k++) v[k] = sm_load4(x, i0 + 4 * k, V, vec);
-        uint32_t key[SM_GROUP], best = 0;
+        float z[SM_GROUP], best = -INFINITY;
 #pragma unroll
         for (int k = 0; k < SM_GROUP; k++) {
-            key[k] = sm_key(v[k / 4].v[k % 4], logits);
-            if (!sm_in(kept, key[k], (uint32_t)(i0 + k))) key[k] = 0;
-            best = key[k] > best ? key[k] : best;
+            const float y = sm_score(v[k / 4].v[k % 4], floor);
+            z[k] = sm_in(kept, y, (uint32_t)(i0 + k)) ? y : -INFINITY;
+            best = fmaxf(best, z[k]);
         }
-        best = sm_block_max(best, sc.b);
+        best = sm_unorder(sm_block_max(sm_order(best), sc.b));
         const SmScale scale = sm_scale(tables, rule, best);
         double mass[SM_GROUP], sum = 0.0, total, most;
-        sm_masses(tables, scale, key, mass);
+        sm_masses(tables, scale, z, mass);
 #pragma unroll
         for (int k = 0; k < SM_GROUP; k++) sum += mass[k];
         const double before = sm_block_scan<double>(sum, sc.a, total);
         groups[t * (SM_STILE / SM_GROUP) + threadIdx.x] = sm_block_rise(sum > 0.0 ? before + sum : 0.0, sc.b, most);
         if (threadIdx.x == 0) {
             sm_poke(&sums[t], total);
-            sm_poke(&tops[t], best ? scale.top : -INFINITY);
+            sm_poke(&tops[t], best > -INFINITY ? scale.top : -INFINITY);
         }
     }
     if (!sm_last_block_of_many(&st.ticket[step], st.sub, (uint32_t)b, (uint32_t)wk.B, &ticket)) return;
@@ -1526,14 +1539,14 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
     const bool vec = sm_aligned(x);
 #pragma unroll
     for (int e = 0; e < SM_GROUP / 4; e++) v[e] = sm_load4(x, i0 + 4 * e, V, vec);
-    uint32_t key[SM_GROUP];
+    float z[SM_GROUP];
     double mass[SM_GROUP];
 #pragma unroll
     for (int e = 0; e < SM_GROUP; e++) {
-        key[e] = sm_key(v[e / 4].v[e % 4], rule.mode == SM_LOGITS);
-        if (!sm_in(kept, key[e], (uint32_t)(i0 + e))) key[e] = 0u;
+        const float y = sm_score(v[e / 4].v[e % 4], sm_floor(rule));
+        z[e] = sm_in(kept, y, (uint32_t)(i0 + e)) ? y : -INFINITY;
     }
-    sm_masses(tables, scale, key, mass);
+    sm_masses(tables, scale, z, mass);
 #pragma unroll
     for (int e = 0; e < SM_GROUP; e++) {
         acc += mass[e];
@@ -1557,6 +1570,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
     u += r * ustride;
     uint32_t* keys = wk.keys + r * wk.vpad;
     const bool logits = rule.mode == SM_LOGITS, vec = sm_aligned(x), uvec = sm_aligned(u);
+    const float floor = sm_floor(rule);
     const float slope = sm_slope(rule);
     const SmKept kept = sm_final(wk, r, st, rule);
     const long long stride = wk.B * SM_LTPB * 4;
@@ -1575,8 +1589,8 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
             LgVec4<uint32_t> o;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint32_t key = sm_key(v[g].v[j], logits);
-                o.v[j] = sm_in(kept, key, (uint32_t)(at + j)) ? sm_order(sm_race32(logits, slope, sm_float(key), uk[g].v[j])) : 0u;
+                const float y = sm_score(v[g].v[j], floor);
+                o.v[j] = sm_in(kept, y, (uint32_t)(at + j)) ? sm_order(sm_race32(logits, slope, y, uk[g].v[j])) : 0u;
                 if (o.v[j]) atomicAdd(&h[sm_slot((int)(o.v[j] >> (32 - SM_RBITS1)), SM_RBITS1 - 6)], 1u);
             }
             if (at < V) *(LgVec4<uint32_t>*)(keys + at) = o;           // (padded to a multiple of four: what lies behind V is key 0)
@@ -1699,12 +1713,12 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
     sm_block_scan<unsigned long long>(mine, sc.a, sure);
     const T* x = scores + r * sstride;
     u += r * ustride;
-    const bool logits = rule.mode == SM_LOGITS;
+    const float floor = sm_floor(rule);
     const SmKept kept = st.kept;
-    const SmScale scale = sm_scale(rule, 0u);                          // (race keys need no common scale)
+    const SmScale scale = sm_scale(rule, -INFINITY);                          // (race keys need no common scale)
     auto race = [&](long long i) {
-        const uint32_t k = sm_key(x[i], logits);
-        return sm_race(scale, sm_in(kept, k, (uint32_t)i) ? k : 0u, u[i]);
+        const float y = sm_score(x[i], floor);
+        return sm_race(scale, sm_in(kept, y, (uint32_t)i) ? y : -INFINITY, u[i]);
     };
     auto win = [&](uint32_t i) {
         atomicOr(&words[i >> 6], 1ull << (i & 63));

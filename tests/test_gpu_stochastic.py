@@ -295,14 +295,14 @@ def test_sampling_of_special_scores(kind, logits, V):
             check_distinct(x, draws_of((2, V)), V // 4, logits=logits, **kw)
 
 
-@pytest.mark.parametrize("T", [1e-30, 1e-20, 1e-14, 1e-8, 1e-3, 1e20, 1e30])
+@pytest.mark.parametrize("T", [1e-30, 1e-20, 1e-14, 1e-8, 1e-3, 0.7, 1.7, 1e20, 1e30])
 @pytest.mark.parametrize("V", [300, 9000, 70001])
 @pytest.mark.parametrize("logits", [True, False])
 def test_far_temperatures(T, V, logits):
     """equal scores have equal masses however far T magnifies what a logarithm rounds; scores that differ have 2^-24 between them at least"""
     for kind, dtype in itertools.product(("ties", "normal"), TYPES):
         x = scores_of(kind, 2, V, dtype, logits, seed=8)
-        for kw in (dict(), dict(top_p=0.8), dict(min_p=0.5), dict(top_k=20, top_p=0.9)):
+        for kw in (dict(), dict(top_p=0.8), dict(min_p=0.5), dict(min_p=1e-3), dict(top_k=20, top_p=0.9)):
             check_sample(x, draws_of((2, 20)), logits=logits, temperature=T, **kw)
 
 

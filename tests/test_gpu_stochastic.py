@@ -116,6 +116,29 @@ def test_dropout_second_derivatives():
     assert torch.equal(dxx, 2 * g * m2) and torch.equal(dxg, 2 * x * m2)
 
 
+def test_dropout_in_autograd():
+    x = torch.randn((3, 40), device=DEV, requires_grad=True)
+    with torch.no_grad():
+        assert not stochastic.dropout(x, 0.4, 3).requires_grad
+    with torch.inference_mode():
+        assert stochastic.dropout(x, 0.4, 3).is_inference()
+    assert not stochastic.dropout(x.detach(), 0.4, 3).requires_grad
+    step = torch.tensor([7], device=DEV)
+    y = stochastic.dropout(x * 2, 0.4, 3, step)
+    (a,) = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+    (b,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.equal(a, b) and torch.equal(a != 0, y != 0) and torch.equal(y.detach(), x.detach() * a)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, x, torch.ones_like(y))
+    z = stochastic.dropout(x, 0.4, 3)                                # an output that the loss does not use, a gradient with strides of zero
+    (c,) = torch.autograd.grad(z.sum(), x)
+    assert torch.equal(c != 0, z != 0)
+    (d,) = torch.autograd.grad((stochastic.dropout(x, 0.4, 3) * 0 + x).sum(), x)
+    assert torch.equal(d, torch.ones_like(d))
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+        stochastic.dropout(torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x)), 0.4, 3)
+
+
 def test_offset_tensor_and_its_guard():
     x = torch.randn((1, 7, 128), device=DEV, requires_grad=True)
     step = torch.tensor([41], device=DEV)

@@ -27,7 +27,7 @@
 
 enum { SM_LOGITS = 0, SM_LINEAR = 1, SM_POWER = 2 };
 
-struct SmRule { int mode; double temperature, top_p, min_p; long long top_k; };
+struct SmRule { int mode; double inv_t /*1 / temperature*/, top_p, min_p; long long top_k; };
 
 // ---- scores ------------------------------------------------------------------------------------------------------------------------------
 // A row's passes are bound by their instructions (a vector instruction takes a wave four cycles: 69 of them per element were 27 us for 10 M),
@@ -100,7 +100,7 @@ struct SmScale { int mode; double inv_t, top /*l of the best score, or its weigh
 // as much as e^1000.
 template <typename Ln> __device__ __forceinline__ SmScale sm_scale(const SmRule& r, float best, const Ln& ln)
 {
-    SmScale s = { r.mode, 1.0 / r.temperature, 0.0, 1.0 };
+    SmScale s = { r.mode, r.inv_t, 0.0, 1.0 };
     if (best == -INFINITY) return s;
     const double x = (double)best;
     if (r.mode == SM_LOGITS) s.top = x * s.inv_t;
@@ -401,23 +401,27 @@ struct SmKept { float thr; uint32_t end; };
 #define SM_ALL 0xffffffffu
 __device__ __forceinline__ bool sm_in(const SmKept& k, float x, uint32_t i) { return x > k.thr || (x == k.thr && i < k.end); }
 
-// min-p as a cut of the scores: the smallest one whose mass is at least min_p of the best one's (the mass grows with the score)
-__device__ __forceinline__ void sm_min_p(const SmRule& rule, float best, SmKept& kept)
+// min-p as a cut of the scores: the smallest one whose mass is at least min_p of the best one's (the mass grows with the score), looked for
+// among the ordered integers from `lo` to `hi`, the best one's, that `of` makes scores.  Every wave for itself, 64 probes a round.
+template <typename Of> __device__ __forceinline__ float sm_min_p(const SmRule& rule, uint32_t lo, uint32_t hi, const Of& of)
 {
-    const SmScale s = sm_scale(rule, best);
-    const double least = rule.min_p * sm_mass(s, best);
+    const SmScale s = sm_scale(rule, of(hi));
+    const double least = rule.min_p * sm_mass(s, of(hi));
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t lo = s.mode == SM_LOGITS ? 1u : 0x80000001u /*the least weight*/, hi = sm_order(best);      // 64 probes a round; the mass at hi is enough
     while (lo < hi) {
         const uint32_t gap = (hi - lo) / 64 + 1;
         const unsigned long long p = (unsigned long long)lo + (unsigned long long)lane * gap;
-        const unsigned long long ok = __ballot(p >= hi || sm_mass(s, sm_unorder((uint32_t)p)) >= least);
+        const unsigned long long ok = __ballot(p >= hi || sm_mass(s, of((uint32_t)p)) >= least);
         const uint32_t f = ok ? (uint32_t)__ffsll((long long)ok) - 1 : 64;
         const unsigned long long nhi = (unsigned long long)lo + (unsigned long long)f * gap;
         if (f) lo += (f - 1) * gap + 1;
         hi = nhi < hi ? (uint32_t)nhi : hi;
     }
-    const float thr = sm_unorder(lo);
+    return of(lo);
+}
+__device__ __forceinline__ void sm_min_p(const SmRule& rule, float best, SmKept& kept)
+{
+    const float thr = sm_min_p(rule, rule.mode == SM_LOGITS ? 1u : 0x80000001u /*the least weight*/, sm_order(best), [](uint32_t k) { return sm_unorder(k); });
     if (thr > kept.thr) kept = SmKept{ thr, SM_ALL };
 }
 
@@ -436,7 +440,7 @@ __device__ __forceinline__ float sm_log2(float x)                      // x > 0,
     return __builtin_amdgcn_logf(small ? x * 0x1p64f : x) - (small ? 64.0f : 0.0f);
 }
 __device__ __forceinline__ float sm_margin(float k, float slope) { return 0x1p-13f + fabsf(k) * 0x1p-18f + slope * 0x1p-21f; }
-__device__ __forceinline__ float sm_slope(const SmRule& r) { return (float)((r.mode == SM_LOGITS ? 1.4426950408889634 : 1.0) / r.temperature); }
+__device__ __forceinline__ float sm_slope(const SmRule& r) { return (float)((r.mode == SM_LOGITS ? 1.4426950408889634 : 1.0) * r.inv_t); }
 
 // approximate key of a candidate.  `slope`: log2(e) / T or 1 / T in 32 bits
 __device__ __forceinline__ float sm_race32(bool logits, float slope, float x, float u)
@@ -955,7 +959,7 @@ __device__ __forceinline__ unsigned long long sm_count_parts(const SmParts& p, d
 __device__ __forceinline__ SmSum sm_sum_of_parts(const SmParts& p, unsigned long long v) { return SmSum{ v >> (p.bits - 31), (v << (63 - p.bits)) & 0xffffffffull }; }
 
 // One level of top-k (MASS false) or top-p: bits [shift - width, shift) of the ordered scores that pass the filters and match the prefix found
-// so far.  Three levels of 11, 11 and 10 bits name the last key that is taken, whatever the scores are like; a level of 2^13 bins instead
+// so far.  Three levels of 11, 10 and 11 bits name the last key that is taken, whatever the scores are like; a level of 2^13 bins instead
 // would merge four times as many words.  10 M weights under a temperature: 39 us for the first level (a logarithm and an exponential in 64
 // bits each: the vector pipe), 19 and 18 for the others (2.2 TB/s); 3 M counted: 12 us each, of which the data are 3.
 template <typename T, bool MASS>
@@ -1149,36 +1153,28 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
     }
     __syncthreads();
     uint32_t* counts = wk.counts(r);
-    for (int k = threadIdx.x; k < 32768; k += 1024) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // chunk c: keys 64 c ... 64 c + 63.  A wave merges, and walks at the end, the chunks (b / 2) * 32 + wave * 2 + b % 2, b = 0 ... 63: the scores
+    // that occur lie close together
+    auto chunk_of = [](int b, int w) { return (b >> 1) * 32 + w * 2 + (b & 1); };
+    unsigned long long live = 0;
+    for (int it = 0; it < 32; it++) {
+        const int k = it * 1024 + threadIdx.x;
         const uint32_t w = h.pair[k];
         if (w & 0xffffu) atomicAdd(&counts[2 * k], w & 0xffffu);
         if (w >> 16) atomicAdd(&counts[2 * k + 1], w >> 16);
+        const unsigned long long any = __ballot(w != 0);
+        live |= ((unsigned long long)((uint32_t)any != 0) | (unsigned long long)((any >> 32) != 0) << 1) << (2 * it);
     }
+    unsigned long long* all_live = (unsigned long long*)(counts + 65536);        // a word of each wave, 128 bytes apart (adds to one line wait for each other)
+    if (lane == 0 && live) atomicOr(&all_live[wave * 16], live);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // chunk c: keys 64 c ... 64 c + 63, one a lane; wave w takes the chunks w, w + 16, ... (the scores that occur lie close together)
-    uint32_t best = 0;
-    unsigned long long live = 0;                                       // chunks of this wave with a score in them
-#pragma unroll
-    for (int c0 = 0; c0 < 64; c0 += 32) {
-        uint32_t n[32];
-#pragma unroll
-        for (int c = 0; c < 32; c++) n[c] = sm_peek(&counts[((c0 + c) * 16 + wave) * 64 + lane]);
-#pragma unroll
-        for (int c = 0; c < 32; c++) {
-            const int chunk = (c0 + c) * 16 + wave;
-            const unsigned long long any = __ballot(n[c] != 0);
-            uint32_t sum = 0;
-            if (any) {
-                best = (uint32_t)(chunk * 64 + 63 - __clzll((long long)any));
-                live |= 1ull << (c0 + c);
-                sum = sm_lane(sm_wave_scan<false>(n[c], SmAdd()), 63);
-            }
-            if (lane == 0) h.chunk.n[chunk] = sum;
-        }
-    }
-    best = sm_block_max(best, sc.a);
+    const unsigned long long lives = sm_peek(&all_live[(lane & 15) * 16]);
+    live = sm_lane(lives, wave);
+    const int top = (int)sm_lane(sm_wave_scan<true>(lives ? (uint32_t)chunk_of(63 - __clzll((long long)lives), lane & 15) + 1 : 0u, SmMaxOf()), 15) - 1;
+    uint32_t best = 0;                                                 // every wave on its own
+    if (top >= 0) best = (uint32_t)top * 64 + 63 - __clzll((long long)__ballot(sm_peek(&counts[top * 64 + lane]) != 0));
     const float most = best ? sm_unkey16<T>(best) : -INFINITY;
     const SmScale scale = sm_scale(rule, most);
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
@@ -1199,37 +1195,41 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
             if (n) { const SmLimbs one = sm_limbs(sm_mass(scale, sm_unkey16<T>(k)) * unit); m = SmSum{ (unsigned long long)one.hi * n, (unsigned long long)one.lo * n }; }
             return m;
         };
-        if (mass) {
-            h.chunk.hi[threadIdx.x] = 0;
-            h.chunk.lo[threadIdx.x] = 0;
-            __syncthreads();
-            // four chunks a round: their counts are four round trips to memory otherwise
-            for (unsigned long long todo = live; todo; ) {
-                uint32_t key[4], n[4];
-                int chunk[4];
+        if (mass) { h.chunk.hi[threadIdx.x] = 0; h.chunk.lo[threadIdx.x] = 0; } else h.chunk.n[threadIdx.x] = 0;
+        __syncthreads();
+        // eight chunks a round: their counts are eight round trips to memory otherwise
+        for (unsigned long long todo = live; todo; ) {
+            uint32_t n[8];
+            int chunk[8];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    chunk[q] = todo ? (__ffsll((long long)todo) - 1) * 16 + wave : -1;
-                    todo &= todo - 1;
-                    key[q] = (uint32_t)(chunk[q] < 0 ? 0 : chunk[q]) * 64 + lane;
-                    n[q] = chunk[q] < 0 ? 0u : left(key[q]);
-                }
+            for (int q = 0; q < 8; q++) {
+                chunk[q] = todo ? chunk_of(__ffsll((long long)todo) - 1, wave) : -1;
+                todo &= todo - 1;
+                n[q] = chunk[q] < 0 ? 0u : left((uint32_t)chunk[q] * 64 + lane);
+            }
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    SmSum m = limbs(key[q], n[q]);
+            for (int q = 0; q < 8; q++) {
+                if (chunk[q] < 0) continue;
+                if (mass) {
+                    SmSum m = limbs((uint32_t)chunk[q] * 64 + lane, n[q]);
                     m.hi = sm_lane(sm_wave_scan<false>(m.hi, SmAdd()), 63);
                     m.lo = sm_lane(sm_wave_scan<false>(m.lo, SmAdd()), 63);
-                    if (lane == 0 && chunk[q] >= 0) { h.chunk.hi[chunk[q]] = m.hi; h.chunk.lo[chunk[q]] = m.lo; }
+                    if (lane == 0) { h.chunk.hi[chunk[q]] = m.hi; h.chunk.lo[chunk[q]] = m.lo; }
+                } else {
+                    const uint32_t sum = sm_lane(sm_wave_scan<false>(n[q], SmAdd()), 63);
+                    if (lane == 0) h.chunk.n[chunk[q]] = sum;
                 }
             }
-            __syncthreads();
         }
+        __syncthreads();
         // the chunk in which the selection ends: thread t stands for chunk 1023 - t
         const int chunk = 1023 - (int)threadIdx.x;
-        const uint32_t n = h.chunk.n[chunk];
+        uint32_t n = 0, before = 0, all;
         SmSum m = { 0, 0 }, total = { 0, 0 }, upto = { 0, 0 };
-        uint32_t all, before = sm_block_scan<uint32_t>(n, sc.a, all);
-        if (mass) {
+        if (!mass) {
+            n = h.chunk.n[chunk];
+            before = sm_block_scan<uint32_t>(n, sc.a, all);
+        } else {
             m = SmSum{ h.chunk.hi[chunk], h.chunk.lo[chunk] };
             upto.hi = sm_block_scan<unsigned long long>(m.hi, sc.a, total.hi);
             upto.lo = sm_block_scan<unsigned long long>(m.lo, sc.b, total.lo);
@@ -1265,12 +1265,12 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
         cut_n = ties;
         __syncthreads();
     }
-    SmKept least = kept;
-    if (best != 0 && rule.min_p > 0.0) sm_min_p(rule, most, least);
+    float least = -INFINITY;
+    if (best != 0 && rule.min_p > 0.0) least = sm_min_p(rule, rule.mode == SM_LOGITS ? 1u : 0x8001u, best, [](uint32_t k) { return sm_unkey16<T>(k); });
     if (threadIdx.x != 0) return;
     st.before = kept;
     st.best = most;
-    st.least = least.thr;
+    st.least = least;
     st.ended = 1;
     st.cut = 0;
     if (best != 0) sm_conclude(st, kept, sm_unkey16<T>(thr), ties, equal);
@@ -1549,7 +1549,7 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
     if (k >= ng) k = sm_rank4(g, ng, [&](double s) { return s >= here; });
     // inside the group: the masses once more, in the same order
     const T* x = scores + r * sstride;
-    const SmScale scale = { rule.mode, 1.0 / rule.temperature, tops[t], 1.0 };
+    const SmScale scale = { rule.mode, rule.inv_t, tops[t], 1.0 };
     const SmKept kept = st.kept;
     const long long i0 = (long long)t * SM_STILE + k * SM_GROUP;
     double acc = k ? g[k - 1] : 0.0;
@@ -1859,7 +1859,7 @@ __global__ void __launch_bounds__(SM_TILE / 64) sm_emit_kernel(long long n, SmWo
 static bool sm_rule(int logits, double temperature, long long top_k, double top_p, double min_p, SmRule& r)
 {
     if (!(temperature >= 1e-30 && temperature <= 1e30) || top_k < 0 || !(top_p > 0.0 && top_p <= 1.0) || !(min_p >= 0.0 && min_p <= 1.0)) return false;
-    r = SmRule{ logits ? SM_LOGITS : temperature == 1.0 ? SM_LINEAR : SM_POWER, temperature, top_p, min_p, top_k };
+    r = SmRule{ logits ? SM_LOGITS : temperature == 1.0 ? SM_LINEAR : SM_POWER, 1.0 / temperature, top_p, min_p, top_k };
     return true;
 }
 
@@ -1889,7 +1889,7 @@ static long long sm_layout(const SmPlan& plan, long long R, long long V, int byt
     const bool race = distinct && !plan.few;
     w.rbins_at = align(sizeof(SmRowState));
     w.hist_at = w.rbins_at + (race ? align(SM_RBINS * 4) : 0);
-    w.clear_bytes = w.hist_at + (plan.counts ? 65536 * 4 : plan.top_k || plan.top_p ? align(sizeof(SmHist)) : 0);
+    w.clear_bytes = w.hist_at + (plan.counts ? 65536 * 4 + 16 * 128 : plan.top_k || plan.top_p ? align(sizeof(SmHist)) : 0);
     w.tiles = (V + SM_TILE - 1) / SM_TILE;
     w.stiles = (V + SM_STILE - 1) / SM_STILE;
     w.vpad = (V + 3) & ~3ll;
@@ -1966,7 +1966,7 @@ static int sample_launch(const T* scores, long long ss, const float* u, long lon
         if (plan.counts ? pass == 0 : !(pass == 0 ? plan.top_k : plan.top_p && !plan.few)) continue;
         if (!plan.counts)
             for (int shift = 32; shift > 0; ) {
-                const int width = shift >= 11 ? 11 : shift;
+                const int width = shift == 21 ? 10 : 11;               // 11, 10, 11: the second level is the one that may fill all its bins, and all workgroups merge theirs
                 if (pass == 0) hipLaunchKernelGGL((sm_level_kernel<T, false>), grid, block, 0, s, scores, ss, V, rule, wk, step++, shift, width);
                 else hipLaunchKernelGGL((sm_level_kernel<T, true>), grid, block, 0, s, scores, ss, V, rule, wk, step++, shift, width);
                 shift -= width;

@@ -298,12 +298,19 @@ template <typename V> __device__ __forceinline__ V sm_block_max(V v, void* lds)
 }
 
 // ---- radix selection: histograms of one level, and the bin in which the selection ends -------------------------------------------------
-// Bin b of 64 * 2^p lies at sm_slot(b, p): the 2^p bins of one lane of the wave that walks them lie 64 apart.
+// Bin b of 64 * 2^p lies at sm_slot(b, p) in LDS: the 2^p bins of one lane of the wave that walks them lie 65 apart, so that neither that walk
+// nor one in the bins' order meets a bank twice.  In memory, where workgroups merge them, bins lie in the order of the slots; counts of a level
+// in their own, so that the bins that hold anything lie close together and a wave's additions to one line are one access (top-k of 3 M 54 ->
+// 51 us; top-p's sums of 8 bytes and the race's counts are merged as fast or faster spread out).
 // A row of one workgroup keeps the counts above bit 48 of the low limb's sums (at most SM_SHORT terms: 46 bits), one atomic less an element.
-struct SmHist { uint32_t n[SM_BINS]; unsigned long long hi[SM_BINS], lo[SM_BINS]; };
-union SmShortHist { uint32_t n[SM_BINS]; struct { unsigned long long hi[SM_BINS], lo[SM_BINS]; }; };
+#define SM_SLOTS 2080                  // sm_slots(5)
+struct SmHist { uint32_t n[SM_SLOTS]; unsigned long long hi[SM_SLOTS], lo[SM_SLOTS]; };
+struct SmMerged { uint32_t n[SM_BINS]; unsigned long long hi[SM_BINS], lo[SM_BINS]; };
+union SmShortHist { uint32_t n[SM_SLOTS]; struct { unsigned long long hi[SM_SLOTS], lo[SM_SLOTS]; }; };
 #define SM_PACK 48
-__device__ __forceinline__ int sm_slot(int b, int p) { return ((b & ((1 << p) - 1)) << 6) | (b >> p); }
+__host__ __device__ constexpr int sm_slots(int p) { return 65 << p; }
+__device__ __forceinline__ int sm_slot(int b, int p) { return (b & ((1 << p) - 1)) * 65 + (b >> p); }
+__device__ __forceinline__ int sm_nth_slot(int k) { return (k >> 6) * 65 + (k & 63); }
 
 // An element is taken while what lies before it (best first) is less than the target, counted in elements or in mass.
 struct SmTake { double target; uint32_t before_n; SmSum before_m; };
@@ -327,7 +334,7 @@ __device__ SmBin sm_boundary(const uint32_t* hn, const unsigned long long* hhi, 
         unsigned long long hi = 0, lo = 0;
 #pragma unroll 8
         for (int k = 0; k < per; k++) {
-            const int at = (k << 6) | (63 - lane);
+            const int at = k * 65 + 63 - lane;
             if (!PACKED) n += hn[at];
             if (MASS) { const unsigned long long v = hlo[at]; hi += hhi[at]; lo += v & low; if (PACKED) n += (uint32_t)(v >> SM_PACK); }
         }
@@ -343,7 +350,7 @@ __device__ SmBin sm_boundary(const uint32_t* hn, const unsigned long long* hhi, 
             const int l = 63 - __clzll((long long)enter);
             bn += sm_lane(in - n, l);
             if (MASS) { bm.hi += sm_lane(ihi - hi, l); bm.lo += sm_lane(ilo - lo, l); }
-            const int at = ((per - 1 - lane) << 6) | (63 - l);
+            const int at = (per - 1 - lane) * 65 + 63 - l;
             uint32_t n2 = 0;
             unsigned long long hi2 = 0, lo2 = 0, ihi2 = 0, ilo2 = 0;
             if (lane < per) {
@@ -480,7 +487,7 @@ __device__ __forceinline__ SmBin sm_select_short(const At& at_, SmTake& take, Sm
     while (shift > 0) {
         const int width = shift >= 11 ? 11 : shift < 6 ? 6 : shift, at = shift > width ? shift - width : 0, p = width - 6;
         __syncthreads();
-        for (int i = threadIdx.x; i < 1 << width; i += TPB) h.n[i] = 0;
+        for (int i = threadIdx.x; i < sm_slots(p); i += TPB) h.n[i] = 0;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
@@ -576,7 +583,7 @@ __device__ __forceinline__ SmBin sm_find_short(const float (&x)[EPT], const doub
         sm_range_short<EPT>(x, [&](int k) { return x[k] > -INFINITY && (level == 0 || bins.in(x[k])); }, sc, lo, hi);
         if (!(lo <= hi)) return SmBin{ -1, 0, 0 };
         bins = sm_bins(linear, lo, hi);
-        for (int i = threadIdx.x; i < SM_BINS; i += TPB) { if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } else h.n[i] = 0; }
+        for (int i = threadIdx.x; i < SM_SLOTS; i += TPB) { if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } else h.n[i] = 0; }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
@@ -864,7 +871,7 @@ struct SmWork {                        // workspace of a call
     long long B, tiles, stiles, capacity, vpad;
     __device__ __forceinline__ SmRowState& state(long long r) const { return *(SmRowState*)(clear + r * clear_bytes); }
     __device__ __forceinline__ uint32_t* rbins(long long r) const { return (uint32_t*)(clear + r * clear_bytes + rbins_at); }
-    __device__ __forceinline__ SmHist& hist(long long r) const { return *(SmHist*)(clear + r * clear_bytes + hist_at); }
+    __device__ __forceinline__ SmMerged& hist(long long r) const { return *(SmMerged*)(clear + r * clear_bytes + hist_at); }
     __device__ __forceinline__ uint32_t* counts(long long r) const { return (uint32_t*)(clear + r * clear_bytes + hist_at); }
 };
 
@@ -998,7 +1005,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     const SmParts parts = sm_parts(wk, V);
     const bool counted = !MASS || at == 0;                             // masses need no counts before the last level
     if (MASS) sm_tables(tables, rule.mode);
-    for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { h.n[k] = 0; if (MASS) h.lo[k] = 0; }
+    for (int k = threadIdx.x; k < sm_slots(p); k += SM_LTPB) { h.n[k] = 0; if (MASS) h.lo[k] = 0; }
     __syncthreads();
     const SmScale scale = sm_scale(tables, rule, best);
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
@@ -1035,13 +1042,14 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     }
     __syncthreads();
     if (MASS)
-        for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { const SmSum m = sm_sum_of_parts(parts, h.lo[k]); h.hi[k] = m.hi; h.lo[k] = m.lo; }
+        for (int k = threadIdx.x; k < sm_slots(p); k += SM_LTPB) { const SmSum m = sm_sum_of_parts(parts, h.lo[k]); h.hi[k] = m.hi; h.lo[k] = m.lo; }
     __syncthreads();
     if (wk.B > 1) {
-        SmHist& g = wk.hist(r);
+        SmMerged& g = wk.hist(r);
         for (int k = threadIdx.x; k < nbins; k += SM_LTPB) {
-            if (counted && h.n[k]) atomicAdd(&g.n[k], h.n[k]);
-            if (MASS) { if (h.hi[k]) atomicAdd(&g.hi[k], h.hi[k]); if (h.lo[k]) atomicAdd(&g.lo[k], h.lo[k]); }
+            const int slot = MASS ? sm_nth_slot(k) : sm_slot(k, p);
+            if (counted && h.n[slot]) atomicAdd(&g.n[k], h.n[slot]);
+            if (MASS) { if (h.hi[slot]) atomicAdd(&g.hi[k], h.hi[slot]); if (h.lo[slot]) atomicAdd(&g.lo[k], h.lo[slot]); }
         }
         if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
         // taken over (all loads before the first store: each is a round trip to memory), and left clear for the next level
@@ -1050,15 +1058,16 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
         unsigned long long hi[K], lo[K];
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const int at = k * SM_LTPB + threadIdx.x;
-            n[k] = counted ? sm_peek(&g.n[at]) : 0u;
-            if (MASS) { hi[k] = sm_peek(&g.hi[at]); lo[k] = sm_peek(&g.lo[at]); }
+            const int bin = k * SM_LTPB + threadIdx.x;
+            n[k] = counted ? sm_peek(&g.n[bin]) : 0u;
+            if (MASS) { hi[k] = sm_peek(&g.hi[bin]); lo[k] = sm_peek(&g.lo[bin]); }
         }
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const int at = k * SM_LTPB + threadIdx.x;
-            h.n[at] = n[k]; g.n[at] = 0;
-            if (MASS) { h.hi[at] = hi[k]; h.lo[at] = lo[k]; g.hi[at] = 0; g.lo[at] = 0; }
+            const int bin = k * SM_LTPB + threadIdx.x, slot = MASS ? sm_nth_slot(bin) : sm_slot(bin, p);
+            if (bin >= nbins) continue;
+            h.n[slot] = n[k]; g.n[bin] = 0;
+            if (MASS) { h.hi[slot] = hi[k]; h.lo[slot] = lo[k]; g.hi[bin] = 0; g.lo[bin] = 0; }
         }
         __syncthreads();
     }
@@ -1067,7 +1076,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
         take = SmTake{ (double)rule.top_k, 0, { 0, 0 } };
         if (MASS) {
             SmSum mine = { 0, 0 }, total;
-            for (int k = threadIdx.x; k < nbins; k += SM_LTPB) { mine.hi += h.hi[k]; mine.lo += h.lo[k]; }
+            for (int k = threadIdx.x; k < sm_slots(p); k += SM_LTPB) { mine.hi += h.hi[k]; mine.lo += h.lo[k]; }
             sm_block_scan<unsigned long long>(mine.hi, sc.a, total.hi);
             sm_block_scan<unsigned long long>(mine.lo, sc.b, total.lo);
             take.target = rule.top_p * sm_sum_value(total);
@@ -1581,7 +1590,8 @@ template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                           long long V, long long n, SmRule rule, SmWork wk, int step)
 {
-    __shared__ uint32_t h[SM_RBINS];
+    constexpr int P = SM_RBITS1 - 6;
+    __shared__ uint32_t h[sm_slots(P)];
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
@@ -1600,7 +1610,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
     LgVec4<float> uk[G];
 #pragma unroll
     for (int g = 0; g < G; g++) { v[g] = sm_load4(x, i + g * stride, V, vec); uk[g] = sm_load4(u, i + g * stride, V, uvec); }
-    for (int k = threadIdx.x; k < SM_RBINS; k += SM_LTPB) h[k] = 0;
+    for (int k = threadIdx.x; k < sm_slots(P); k += SM_LTPB) h[k] = 0;
     __syncthreads();
     while (i < V) {
 #pragma unroll
@@ -1611,7 +1621,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
             for (int j = 0; j < 4; j++) {
                 const float y = sm_score(v[g].v[j], floor);
                 o.v[j] = sm_in(kept, y, (uint32_t)(at + j)) ? sm_order(sm_race32(logits, slope, y, uk[g].v[j])) : 0u;
-                if (o.v[j]) atomicAdd(&h[sm_slot((int)(o.v[j] >> (32 - SM_RBITS1)), SM_RBITS1 - 6)], 1u);
+                if (o.v[j]) atomicAdd(&h[sm_slot((int)(o.v[j] >> (32 - SM_RBITS1)), P)], 1u);
             }
             if (at < V) *(LgVec4<uint32_t>*)(keys + at) = o;           // (padded to a multiple of four: what lies behind V is key 0)
         }
@@ -1622,16 +1632,16 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
     }
     __syncthreads();
     uint32_t* g = wk.rbins(r);
-    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) if (h[i]) atomicAdd(&g[i], h[i]);
+    for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) if (const uint32_t c = h[sm_nth_slot(i)]) atomicAdd(&g[i], c);
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
     uint32_t n4[SM_RBINS / SM_LTPB];
 #pragma unroll
     for (int k = 0; k < SM_RBINS / SM_LTPB; k++) n4[k] = sm_peek(&g[k * SM_LTPB + threadIdx.x]);
 #pragma unroll
-    for (int k = 0; k < SM_RBINS / SM_LTPB; k++) { h[k * SM_LTPB + threadIdx.x] = n4[k]; g[k * SM_LTPB + threadIdx.x] = 0; }
+    for (int k = 0; k < SM_RBINS / SM_LTPB; k++) { h[sm_nth_slot(k * SM_LTPB + threadIdx.x)] = n4[k]; g[k * SM_LTPB + threadIdx.x] = 0; }
     __syncthreads();
     SmTake take = { (double)n, 0, { 0, 0 } };
-    const SmBin bin = sm_boundary<false>(h, nullptr, nullptr, SM_RBITS1 - 6, take, sc);
+    const SmBin bin = sm_boundary<false>(h, nullptr, nullptr, P, take, sc);
     if (threadIdx.x != 0) return;
     st.kept = kept;
     st.candidates = 0;
@@ -1644,7 +1654,8 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
 // Second level, and the zone (3 M: 8 us, one read of the keys)
 __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, SmRule rule, SmWork wk, int step)
 {
-    __shared__ uint32_t h[SM_RBINS];
+    constexpr int P = SM_RBITS2 - 6;
+    __shared__ uint32_t h[sm_slots(P)];
     __shared__ SmScratch sc;
     __shared__ uint32_t ticket;
     const long long r = blockIdx.x / wk.B, b = blockIdx.x % wk.B;
@@ -1653,7 +1664,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, SmR
     const uint32_t* keys = wk.keys + r * wk.vpad;
     const uint32_t prefix = st.prefix;
     const int nbins = 1 << SM_RBITS2, at = 32 - SM_RBITS1 - SM_RBITS2;
-    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) h[i] = 0;
+    for (int i = threadIdx.x; i < sm_slots(P); i += SM_LTPB) h[i] = 0;
     __syncthreads();
     const long long stride = wk.B * SM_LTPB * 4;
     for (long long i = (b * SM_LTPB + threadIdx.x) * 4; i < V; i += 4 * stride) {
@@ -1664,16 +1675,16 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, SmR
         for (int g = 0; g < 4; g++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (o[g].v[j] && (o[g].v[j] >> (32 - SM_RBITS1)) == prefix) atomicAdd(&h[sm_slot((int)(o[g].v[j] >> at) & (nbins - 1), SM_RBITS2 - 6)], 1u);
+                if (o[g].v[j] && (o[g].v[j] >> (32 - SM_RBITS1)) == prefix) atomicAdd(&h[sm_slot((int)(o[g].v[j] >> at) & (nbins - 1), P)], 1u);
     }
     __syncthreads();
     uint32_t* g = wk.rbins(r);
-    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) if (h[i]) atomicAdd(&g[i], h[i]);
+    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) if (const uint32_t c = h[sm_nth_slot(i)]) atomicAdd(&g[i], c);
     if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
-    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) h[i] = sm_peek(&g[i]);
+    for (int i = threadIdx.x; i < nbins; i += SM_LTPB) h[sm_nth_slot(i)] = sm_peek(&g[i]);
     __syncthreads();
     SmTake take = st.take;
-    const SmBin bin = sm_boundary<false>(h, nullptr, nullptr, SM_RBITS2 - 6, take, sc);
+    const SmBin bin = sm_boundary<false>(h, nullptr, nullptr, P, take, sc);
     if (threadIdx.x != 0) return;
     const uint32_t lo = (prefix << (32 - SM_RBITS1)) | ((uint32_t)(bin.bin < 0 ? 0 : bin.bin) << at);
     const SmZone zone = sm_zone(lo, lo | ((1u << at) - 1), sm_slope(rule));
@@ -1782,7 +1793,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
             while (shift > 0) {
                 const int width = shift >= 11 ? 11 : shift < 6 ? 6 : shift, low = shift > width ? shift - width : 0;
                 __syncthreads();
-                for (int k = threadIdx.x; k < 1 << width; k += SM_LTPB) h.hist.n[k] = 0;
+                for (int k = threadIdx.x; k < sm_slots(width - 6); k += SM_LTPB) h.hist.n[k] = 0;
                 __syncthreads();
                 for (long long a = threadIdx.x; a < m; a += SM_LTPB) {
                     const unsigned long long k = of(a);
@@ -1889,7 +1900,7 @@ static long long sm_layout(const SmPlan& plan, long long R, long long V, int byt
     const bool race = distinct && !plan.few;
     w.rbins_at = align(sizeof(SmRowState));
     w.hist_at = w.rbins_at + (race ? align(SM_RBINS * 4) : 0);
-    w.clear_bytes = w.hist_at + (plan.counts ? 65536 * 4 + 16 * 128 : plan.top_k || plan.top_p ? align(sizeof(SmHist)) : 0);
+    w.clear_bytes = w.hist_at + (plan.counts ? 65536 * 4 + 16 * 128 : plan.top_k || plan.top_p ? align(sizeof(SmMerged)) : 0);
     w.tiles = (V + SM_TILE - 1) / SM_TILE;
     w.stiles = (V + SM_STILE - 1) / SM_STILE;
     w.vpad = (V + 3) & ~3ll;

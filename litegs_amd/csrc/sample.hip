@@ -891,8 +891,8 @@ __device__ __forceinline__ bool sm_last_block(uint32_t* ticket, uint32_t blocks,
     __syncthreads();
     return *lds != 0;
 }
-// ... of many workgroups: adds to one word take 10 ns each, so sixteen groups draw among themselves first (3 M scores, 733 workgroups: 28.6 us
-// a call, 31.7 with one word).  `sub`: sixteen cleared words
+// ... of many workgroups: adds to one word take 10 ns each, so sixteen groups draw among themselves first (3 M scores, 733 workgroups: 26.5 us
+// a call, 29.0 with one word).  `sub`: sixteen cleared words
 __device__ __forceinline__ bool sm_last_block_of_many(uint32_t* ticket, uint32_t* sub, uint32_t block, uint32_t blocks, uint32_t* lds)
 {
     if (blocks <= 128) return sm_last_block(ticket, blocks, lds);
@@ -967,8 +967,8 @@ __device__ __forceinline__ SmSum sm_sum_of_parts(const SmParts& p, unsigned long
 
 // One level of top-k (MASS false) or top-p: bits [shift - width, shift) of the ordered scores that pass the filters and match the prefix found
 // so far.  Three levels of 11, 10 and 11 bits name the last key that is taken, whatever the scores are like; a level of 2^13 bins instead
-// would merge four times as many words.  10 M weights under a temperature: 39 us for the first level (a logarithm and an exponential in 64
-// bits each: the vector pipe), 19 and 18 for the others (2.2 TB/s); 3 M counted: 12 us each, of which the data are 3.
+// would merge four times as many words.  10 M weights under a temperature: 40 us for the first level (a logarithm and an exponential in 64
+// bits each: the vector pipe), 18 and 18 for the others (2.2 TB/s); 3 M counted: 13, 13 and 10 us, of which the data are 3 each.
 template <typename T, bool MASS>
 __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step,
                                                            int shift, int width)
@@ -1105,9 +1105,9 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
 // ---- scores of 16 bits: both filters from one histogram of all keys ----------------------------------------------------------------------
 // The 65536 ordered keys of a 16-bit type are counted in LDS (two counters a word: a workgroup takes at most SM_SHARE16 elements), added up in
 // memory, and the last workgroup works top-k and top-p out of the counts: one pass over the row and one exponential per distinct score, in
-// the place of one pass for the best and three for each filter.  16 rows of 100 k: 30 us.  Rows of 50 k behind top-p: 1 row 55 us a call (by
-// levels 71), 64 rows 72 (92), 256 rows 164 (195); behind top-k alone 256 rows 131 (124), 512 rows 240 (229).  So up to 256 rows, where the
-// counts are 64 MB.
+// the place of one pass for the best and three for each filter.  16 rows of 100 k: 25 us, about half of it the last workgroup's conclusion.
+// Rows of 50 k behind top-p: 1 row 46 us a call (by levels 63), 64 rows 57 (82), 256 rows 129 (152), 512 rows 228 (275); behind top-k alone 64
+// rows 47 (54), 256 rows 106 (94).  So up to 256 rows, where the counts are 64 MB, and without top-p up to 128.
 #define SM_SHARE16 32768
 __device__ __forceinline__ uint32_t sm_bits(LgHalf v) { return (uint32_t)__builtin_bit_cast(uint16_t, v); }
 __device__ __forceinline__ uint32_t sm_bits(LgBf16 v) { return v.bits; }
@@ -1366,8 +1366,8 @@ __global__ void __launch_bounds__(SM_LTPB) sm_cut_kernel(const T* __restrict__ s
     for (int k = 0; k < E; k++) if (((is >> k) & 1) && ++before == rest) { st.kept.end = (uint32_t)(i0 + k) + 1; st.cut = 0; }
 }
 
-// A top-k of at most SM_SHORT elements leaves a short row, which one more launch finishes: 3 M scores behind top-k 50 and top-p 59 us, by the
-// long way 101; k = 5000 without top-p 67 and 69 (50 k scores: 56 and 51, the one case that loses).
+// A top-k of at most SM_SHORT elements leaves a short row, which one more launch finishes: 3 M scores behind top-k 50 and top-p 58 us, by the
+// long way 99; k = 5000 without top-p 58 and 64 (50 k scores: 54 and 51, the one case that loses).
 // What top-k left, in index order: scores, their names and (without replacement) their numbers; rule.top_k places a row, the last ones empty
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_gather_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u /*nullable*/, long long ustride,
@@ -1585,7 +1585,7 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
 
 // ---- long rows, without replacement ----------------------------------------------------------------------------------------------------
 // Approximate keys and their first level: one pass over scores and numbers, keys written for the passes to come (4 bytes an element in the
-// place of 8, and two logarithms less).  3 M: 18 us (36 MB moved), 10 M 23 us behind top-p.
+// place of 8, and two logarithms less).  3 M: 17 us (36 MB moved), 10 M 23 us behind top-p.
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                           long long V, long long n, SmRule rule, SmWork wk, int step)
@@ -1651,7 +1651,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
     if (bin.total <= (unsigned long long)n) { st.ended = 1; st.zone_lo = 1u; st.zone_hi = 0u; }        // whatever is left wins: nothing to rank
 }
 
-// Second level, and the zone (3 M: 8 us, one read of the keys)
+// Second level, and the zone (3 M: 9 us, one read of the keys)
 __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, SmRule rule, SmWork wk, int step)
 {
     constexpr int P = SM_RBITS2 - 6;
@@ -1874,8 +1874,8 @@ static bool sm_rule(int logits, double temperature, long long top_k, double top_
     return true;
 }
 
-// How a call runs.  Short rows: one workgroup each, as far as its LDS and registers reach (12288 scores, short and long: plain 10 and 19 us, behind
-// top-p 23 and 61, 614 distinct 23 and 26; 64 rows 11 / 21, 24 / 65, 23 / 31).  Long ones: the filters by levels of a histogram, or, for 16-bit
+// How a call runs.  Short rows: one workgroup each, as far as its LDS and registers reach (12288 scores, short and long: plain 10 and 16 us, behind
+// top-p 21 and 53, 614 distinct 21 and 27; 64 rows 10 / 18, 23 / 58, 22 / 29).  Long ones: the filters by levels of a histogram, or, for 16-bit
 // scores, from one histogram of all keys; what a small top-k leaves goes on as a short row.  Both sides of these two stand at their kernels.
 struct SmPlan { bool is_short, top_k, top_p, counts, few; };
 #define SM_COUNTS_ROWS 256
@@ -1886,7 +1886,7 @@ static SmPlan sm_plan(long long R, long long V, int bytes, long long top_k, doub
     p.is_short = V <= SM_SHORT;
     p.top_k = top_k > 0 && top_k < V;
     p.top_p = top_p < 1.0;
-    p.counts = bytes == 2 && (p.top_k || p.top_p) && R <= SM_COUNTS_ROWS;
+    p.counts = bytes == 2 && (p.top_k || p.top_p) && R <= (p.top_p ? SM_COUNTS_ROWS : SM_COUNTS_ROWS / 2);
     p.few = p.top_k && top_k <= SM_SHORT;
     return p;
 }
@@ -1905,8 +1905,8 @@ static long long sm_layout(const SmPlan& plan, long long R, long long V, int byt
     w.stiles = (V + SM_STILE - 1) / SM_STILE;
     w.vpad = (V + 3) & ~3ll;
     w.capacity = V / 256 > 4096 ? V / 256 : 4096;
-    // 256 workgroups fill the chip, and every further one adds its histogram to the same words of memory (3 M scores behind top-p: 89 us with 256,
-    // 105 with 512, 100 with 128)
+    // 256 workgroups fill the chip, and every further one adds its histogram to the same words of memory (3 M scores behind top-p: 79 us with 256,
+    // 95 with 512, 83 with 128)
     const long long want = (V + SM_LTPB * 8 - 1) / (SM_LTPB * 8), most = R >= 256 ? 1 : 256 / R;
     w.B = want < most ? want : most;
     w.clear = take(true, R * w.clear_bytes);
@@ -1939,8 +1939,8 @@ static void sample_short(const T* scores, long long ss, const float* u, long lon
         if (distinct) hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, true>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, names, out);  \
         else hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, false>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, names, out);          \
     } while (0)
-    // 300 scores in 256 x 4, 1024 x 4 and 768 x 16 threads x elements: a plain draw 5.0, 5.2 and 8.1 us, 512 rows of them 5.2, 9.9 and 16; 3000
-    // scores in the last two 5.5 and 8.2, 512 rows 11 and 17
+    // 300 scores in 256 x 4, 1024 x 4 and 768 x 16 threads x elements: a plain draw 4.8, 4.9 and 7.2 us, 512 rows of them 5.2, 9.6 and 15; 3000
+    // scores in the last two 5.4 and 7.4, 512 rows 11 and 16
     if (V <= 1024) SM_LAUNCH_SHORT(256, 4);
     else if (V <= 4096) SM_LAUNCH_SHORT(1024, 4);
     else SM_LAUNCH_SHORT(768, 16);

@@ -97,8 +97,8 @@ __global__ void __launch_bounds__(256) l1_ssim_forward_kernel(const float* __res
     if (hwork) {
         // Four blurred maps instead of five: SSIM needs E[x^2]+E[y^2] and E[xy] only, and both follow from P = blur((x+y)^2) and
         // Q = blur((x-y)^2):  E[x^2]+E[y^2] = (P+Q)/2,  E[xy] = (P-Q)/4  (the blur is linear).  -20 % of the FMAs and LDS traffic.
-        // The kernel is bound by VALU issue (25 M wave instructions, 4 cycles each): the four maps are accumulated as two packed
-        // 2-vectors (v_pk_fma_f32), which halves the multiply-add instructions.
+        // The kernel is bound by VALU issue (25 M wave instructions, 4 cycles each): the four maps are accumulated as two
+        // 2-vectors.  (Packed instructions, which would halve the multiply-adds, are off in this build: litegs_amd/build.py.)
         v2f a01[HSEG], a23[HSEG];
 #pragma unroll
         for (int j = 0; j < HSEG; j++) { a01[j] = v2f{ 0.0f, 0.0f }; a23[j] = v2f{ 0.0f, 0.0f }; }

@@ -335,8 +335,8 @@ __device__ __forceinline__ void fwd_generic_loop(FwdState<PPL>& st, const int* _
     }
 }
 
-// The default 8x16 tile without statistics, forward: the lane's two pixels as packed 2-vectors (exponent, weight, colour accumulation,
-// transmittance: v_pk_* do two pixels per issue slot), splat ids through the scalar path, last_contributor as an add-with-carry of the
+// The default 8x16 tile without statistics, forward: the lane's two pixels as 2-vectors (exponent, weight, colour accumulation,
+// transmittance; the build keeps packed instructions off, so that each is two), splat ids through the scalar path, last_contributor as an add-with-carry of the
 // activity mask, and a splat that no pixel takes (alpha < 1/256 everywhere) leaves after the alpha evaluation -- with alpha = 0 the
 // colour sums and the transmittance keep their values.  36 -> 24 VALU instructions per (tile, splat).
 struct FwdFast {
@@ -1021,9 +1021,9 @@ __device__ __forceinline__ void bwd_splat(BwdState<PPL>& st, const f32x16& rec, 
     const float t0 = __builtin_fmaf(rec[R_A2] * dx, dx, rec[R_LO]);
     float v_r = 0.f, v_g = 0.f, v_b = 0.f, s0 = 0.f, s1 = 0.f, s2 = 0.f, esq = 0.f;
     if constexpr (PPL == 2 && !STAT) {
-        // the lane's two pixels as one 2-vector: packed fp32 ops do two pixels per issue slot
+        // the lane's two pixels as one 2-vector
         const v2f dyv = { rec[R_PY] - st.Y[0], rec[R_PY] - st.Y[1] };
-        const v2f qv = dyv * (rec[R_C2] * dyv + t1) + t0;              // contracted to two v_pk_fma_f32
+        const v2f qv = dyv * (rec[R_C2] * dyv + t1) + t0;              // contracted to multiply-adds
         const float E0 = __builtin_amdgcn_exp2f(qv.x);
         const float E1 = __builtin_amdgcn_exp2f(qv.y);
         const bool val0 = (E0 >= 1.0f / 256) && (j < st.lcrel[0]);

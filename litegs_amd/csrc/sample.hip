@@ -9,9 +9,8 @@
 //   without:             the n largest l_i - log(-log(1 - u_i)), in index order
 //
 // All masses, sums and keys are in 64 bits: an index has to be the same as the definition's however many categories there are.  Masses that
-// are added by atomics (top-p's histograms) are added as integers, so that neither their order nor the launch changes a result: 63 fraction
-// bits of the largest mass where a workgroup holds the row or scores have 16 bits, 50 to 47 bits in the passes over long rows (to 16 M; one
-// bit less per doubling from there).  Floating sums have one fixed order.
+// are added by atomics (top-p's histograms) are added as integers, so that neither their order nor the launch changes a result: of 63 fraction
+// bits of the largest mass.  Floating sums have one fixed order.
 //
 // What bounds it: not the bytes (3 M scores are 3 us of memory, 10 M with their numbers 18).  A short row is the work of one compute unit
 // (100 ns for each instruction that 15 k elements cost); a long one a chain of passes, each of which pays 4 to 5 us to be launched behind the
@@ -949,21 +948,29 @@ __device__ __forceinline__ void sm_conclude(SmRowState& st, const SmKept& kept, 
     if (ties < count) { st.cut = 1; st.ties = ties; }
 }
 
-// Masses as integers that one addition to LDS adds up: so many of 2^bits parts that a workgroup's share of the row cannot overflow 63 bits
-// (50 bits of the largest mass for short rows, 47 for 10 M scores; two limbs took 6 us more for those 10 M).  The addition of 2^(52 - bits)
-// rounds, and leaves the integer in the low bits.
-struct SmParts { int bits; double one; };
+// A mass as two integers that LDS adds up: so many of 2^bits parts that a workgroup's share of the row cannot overflow 63 bits (50 for short
+// rows, 47 for 10 M scores), and what that leaves, of either sign, in 2^-bits of a part.  The addition of 2^(52 - bits) rounds, and leaves the
+// integer in the low bits of the sum.  (One integer alone is 4 us faster for 10 M scores, but then ten million equal scores behind a larger one
+// are cut some elements off.)
+struct SmParts { int bits; double one, rest; };
 __device__ __forceinline__ SmParts sm_parts(const SmWork& wk, long long V)
 {
     const long long share = (V + wk.B * SM_LTPB * 4 - 1) / (wk.B * SM_LTPB * 4) * (SM_LTPB * 4);
-    const int bits = __clzll(share - 1) - 1;                           // 63 - ceil(log2(share))
-    return SmParts{ bits < 51 ? bits : 51, ldexp(1.0, 52 - (bits < 51 ? bits : 51)) };
+    const int b = __clzll(share - 1) - 1, bits = b < 51 ? b : 51;      // 63 - ceil(log2(share))
+    return SmParts{ bits, ldexp(1.0, 52 - bits), ldexp(1.5, 52 - 2 * bits) };
 }
-__device__ __forceinline__ unsigned long long sm_count_parts(const SmParts& p, double mass, double unit)
+__device__ __forceinline__ unsigned long long sm_bits_above(double sum, double one) { return (unsigned long long)__double_as_longlong(sum) - (unsigned long long)__double_as_longlong(one); }
+__device__ __forceinline__ void sm_add_parts(const SmParts& p, double mass, unsigned long long& whole, unsigned long long& rest)
 {
-    return (unsigned long long)__double_as_longlong(fma(mass, unit, p.one)) - (unsigned long long)__double_as_longlong(p.one);
+    const double sum = mass + p.one;
+    atomicAdd(&whole, sm_bits_above(sum, p.one));
+    atomicAdd(&rest, sm_bits_above(mass - (sum - p.one) + p.rest, p.rest));
 }
-__device__ __forceinline__ SmSum sm_sum_of_parts(const SmParts& p, unsigned long long v) { return SmSum{ v >> (p.bits - 31), (v << (63 - p.bits)) & 0xffffffffull }; }
+__device__ __forceinline__ SmSum sm_sum_of_parts(const SmParts& p, unsigned long long whole, unsigned long long rest)
+{
+    const long long lo = (long long)((whole << (63 - p.bits)) & 0xffffffffull) + ((long long)rest >> (2 * p.bits - 63));
+    return SmSum{ (whole >> (p.bits - 31)) + (unsigned long long)(lo >> 32), (unsigned long long)lo & 0xffffffffull };
+}
 
 // One level of top-k (MASS false) or top-p: bits [shift - width, shift) of the ordered scores that pass the filters and match the prefix found
 // so far.  Three levels of 11, 10 and 11 bits name the last key that is taken, whatever the scores are like; a level of 2^13 bins instead
@@ -1005,7 +1012,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     const SmParts parts = sm_parts(wk, V);
     const bool counted = !MASS || at == 0;                             // masses need no counts before the last level
     if (MASS) sm_tables(tables, rule.mode);
-    for (int k = threadIdx.x; k < sm_slots(p); k += SM_LTPB) { h.n[k] = 0; if (MASS) h.lo[k] = 0; }
+    for (int k = threadIdx.x; k < sm_slots(p); k += SM_LTPB) { h.n[k] = 0; if (MASS) { h.hi[k] = 0; h.lo[k] = 0; } }
     __syncthreads();
     const SmScale scale = sm_scale(tables, rule, best);
     const double unit = rule.mode == SM_LINEAR ? scale.shift : 1.0;
@@ -1032,7 +1039,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
             if (counted) atomicAdd(&h.n[bin], 1u);
             if (MASS) {
                 if (!many) { const float one[1] = { z[j] }; double m[1]; sm_masses(tables, scale, one, m); mass[j] = m[0]; }
-                atomicAdd(&h.lo[bin], sm_count_parts(parts, mass[j], unit));
+                sm_add_parts(parts, mass[j] * unit, h.hi[bin], h.lo[bin]);
             }
         }
         i += G * stride;
@@ -1042,7 +1049,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     }
     __syncthreads();
     if (MASS)
-        for (int k = threadIdx.x; k < sm_slots(p); k += SM_LTPB) { const SmSum m = sm_sum_of_parts(parts, h.lo[k]); h.hi[k] = m.hi; h.lo[k] = m.lo; }
+        for (int k = threadIdx.x; k < sm_slots(p); k += SM_LTPB) { const SmSum m = sm_sum_of_parts(parts, h.hi[k], h.lo[k]); h.hi[k] = m.hi; h.lo[k] = m.lo; }
     __syncthreads();
     if (wk.B > 1) {
         SmMerged& g = wk.hist(r);
@@ -1099,7 +1106,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
     double mass[1] = { 0.0 };
     if (MASS) sm_masses(tables, scale, one, mass);
     st.ended = 1;
-    sm_conclude(st, kept, thr, whole ? bin.count : sm_ties<MASS>(take, bin.count, fma(mass[0], unit, parts.one) - parts.one), bin.count);
+    sm_conclude(st, kept, thr, whole ? bin.count : sm_ties<MASS>(take, bin.count, mass[0] * unit), bin.count);
 }
 
 // ---- scores of 16 bits: both filters from one histogram of all keys ----------------------------------------------------------------------

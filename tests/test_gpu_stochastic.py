@@ -395,6 +395,57 @@ def test_distinct_with_many_candidates_next_to_the_border(equal):
         check_distinct(x, u, n, logits=True)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("logits,small", [(True, -21.0), (True, -14.0), (False, 2.0 ** -31 * 1.5), (False, 2.0 ** -20)])
+@pytest.mark.parametrize("V", [12000, 2000001])
+def test_top_p_ends_inside_a_long_tail(V, logits, small, dtype):
+    """one large mass and a tail of equal small ones, cut in its middle: (1 + j m) < top_p (1 + (V - 1) m) holds up to j = V / 2, half a
+    mass away from the border, so that top_p's own rounding (2^-53 of about one: at most 2^-53 / m = 2e-7 of an element here) cannot matter"""
+    if not logits and dtype == torch.float16:
+        small = max(small, 2.0 ** -20)
+    m = math.exp(small) if logits else small
+    x = torch.full((1, V), small, device=DEV).to(dtype)
+    x[0, V // 3] = 0.0 if logits else 1.0
+    assert float(x[0, 0]) == small
+    j = V // 2
+    top_p = (1.0 + (j - 0.5) * m) / (1.0 + (V - 1) * m)
+    last = stochastic.sample(x, torch.ones((1, 1), device=DEV), top_p=top_p, logits=logits)
+    assert int(last) == j                                            # the large one at V / 3, and the first j of the others: 0 ... j
+
+
+def test_rows_of_two_gigabytes_and_more():
+    V = 2 ** 31 - 1
+    x = torch.full((1, V), -math.inf, dtype=torch.bfloat16, device=DEV)
+    x[0, 5], x[0, 2 ** 30], x[0, V - 1] = 1.0, 0.5, 1.0
+    u = torch.tensor([[0.0, 0.3, 0.5, 0.99]], device=DEV)             # masses e, sqrt(e), e: borders at 0.38 and 0.62
+    for dtype in (torch.bfloat16, torch.float32):
+        x = x.to(dtype)
+        for kw, want in ((dict(), [5, 5, 2 ** 30, V - 1]), (dict(top_k=2), [5, 5, V - 1, V - 1]), (dict(top_p=0.9), [5, 5, 2 ** 30, V - 1]), (dict(top_p=0.5), [5, 5, V - 1, V - 1]),
+                         (dict(top_k=20000, min_p=0.9), [5, 5, V - 1, V - 1])):
+            got = stochastic.sample(x, u, **kw).tolist()[0]
+            assert got == want, (dtype, kw, got)
+    del x
+    torch.cuda.empty_cache()
+    w = torch.zeros((1, V), dtype=torch.bfloat16, device=DEV)
+    w[0, 3], w[0, 2 ** 30 + 1], w[0, V - 2] = 1.0, 0.5, 2.0
+    uu = torch.full((1, V), 0.5, device=DEV)
+    assert stochastic.sample_distinct(w, uu, 2, logits=False).tolist() == [[3, V - 2]]
+    assert stochastic.sample_distinct(w, uu, 4, logits=False).tolist() == [[3, 2 ** 30 + 1, V - 2, -1]]
+
+
+def test_dropout_behind_32_bits():
+    lead, M = 9, 2 ** 29 + 4
+    x = torch.ones((lead, M), dtype=torch.bfloat16, device=DEV)
+    y = stochastic.dropout(x, 0.5, 11, 3, shared=1)
+    for at in (0, M - 1000):
+        keep = torch.from_numpy(ref.kept(np.arange(at, at + 1000), 0.5, 11, 3)).to(DEV)
+        assert ((y[:, at:at + 1000] != 0) == keep).all()
+    del y
+    y = stochastic.dropout(x, 0.5, 11, 3)                            # an index of its own for each
+    keep = torch.from_numpy(ref.kept(np.arange(lead * M - 1000, lead * M), 0.5, 11, 3)).to(DEV)
+    assert ((y[-1, -1000:] != 0) == keep).all()
+
+
 def test_sample_of_more_tiles_than_a_workgroup_keeps():
     V = 9000001
     x = scores_of("masked", 1, V, torch.float32, False, seed=4)

@@ -235,6 +235,7 @@ __device__ __forceinline__ unsigned long long sm_lane(unsigned long long v, int 
 {
     return (unsigned long long)sm_lane((uint32_t)v, lane) | (unsigned long long)sm_lane((uint32_t)(v >> 32), lane) << 32;
 }
+__device__ __forceinline__ float sm_lane(float v, int lane) { return __uint_as_float(sm_lane(__float_as_uint(v), lane)); }
 __device__ __forceinline__ double sm_lane(double v, int lane) { return __longlong_as_double((long long)sm_lane((unsigned long long)__double_as_longlong(v), lane)); }
 
 struct SmAdd { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; } };
@@ -529,8 +530,8 @@ template <typename T> __device__ __forceinline__ LgVec4<T> sm_load4(const T* x, 
 }
 template <typename T> __device__ __forceinline__ bool sm_aligned(const T* x) { return (uintptr_t)x % (4 * sizeof(T)) == 0; }
 
-// a boundary bin of at most 64 elements, ranked by a wave
-struct SmFew { unsigned long long hi[64], lo[64]; float x[64]; uint32_t index[64], order[64]; };
+// a boundary bin of at most 64 elements, ranked by a wave; or those and up to 63 above them
+struct SmFew { unsigned long long hi[64], lo[64]; double sum[128]; float x[128], u[128]; uint32_t index[128], order[64], ahead[128]; };
 union SmShortLds { SmShortHist hist; SmFew few; struct { unsigned long long rank[SM_BINS]; uint32_t index[SM_BINS]; } zone; };
 
 // Bins of the numbers from lo to hi, and the one that is wanted (-1: all of them).  Grows with x; lo and hi are never in one bin.
@@ -559,28 +560,34 @@ __device__ __forceinline__ SmBins sm_bins(bool linear, float lo, float hi)
     return b;
 }
 
-// the smallest and the largest of the numbers that are in
+// the smallest and the largest of the numbers that are in (inf and -inf: none is)
 template <int EPT, typename In> __device__ __forceinline__ void sm_range_short(const float (&x)[EPT], const In& in, SmScratch& sc, float& lo, float& hi)
 {
     float a = INFINITY, b = -INFINITY;
 #pragma unroll
     for (int k = 0; k < EPT; k++) if (in(k)) { a = fminf(a, x[k]); b = fmaxf(b, x[k]); }
-    hi = sm_unorder(sm_block_max(sm_order(b), sc.a));
-    lo = sm_unorder(~sm_block_max(~sm_order(a), sc.b));
+    const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    uint32_t low = sm_wave_scan<false>(~sm_order(a), SmMaxOf()), high = sm_wave_scan<false>(sm_order(b), SmMaxOf());
+    __syncthreads();
+    if (lane == 63) sc.a[threadIdx.x >> 6] = (unsigned long long)high << 32 | low;
+    __syncthreads();
+    const unsigned long long part = (lane & 15) < waves ? sc.a[lane & 15] : 0ull;
+    low = sm_lane(sm_wave_scan<true>((uint32_t)part, SmMaxOf()), 15);
+    high = sm_lane(sm_wave_scan<true>((uint32_t)(part >> 32), SmMaxOf()), 15);
+    lo = sm_unorder(~low);
+    hi = sm_unorder(high);
 }
 
-// Where a selection of the candidates x (> -inf) ends: the bins that are left hold at most `small` elements, or only equal ones (lo == hi).
+// Where a selection of the candidates x (> -inf; from lo to hi) ends: the bins that are left hold at most `small` elements, or only equal ones (lo == hi).
 // take.before_* is what lies above them, the result their count and the number of candidates (0: there are none).
 template <bool MASS, int TPB, int EPT>
-__device__ __forceinline__ SmBin sm_find_short(const float (&x)[EPT], const double* mass /*LDS, [EPT][TPB], at most one each*/, bool linear, SmTake& take, uint32_t small, SmShortHist& h, SmScratch& sc,
-                               SmBins& bins)
+__device__ __forceinline__ SmBin sm_find_short(const float (&x)[EPT], const double* mass /*LDS, [EPT][TPB], at most one each*/, bool linear, float lo, float hi, SmTake& take, uint32_t small,
+                               SmShortHist& h, SmScratch& sc, SmBins& bins)
 {
     uint32_t candidates = 0;
-    bins.want = -1;
+    if (!(lo <= hi)) return SmBin{ -1, 0, 0 };
     for (int level = 0; ; level++) {
-        float lo, hi;
-        sm_range_short<EPT>(x, [&](int k) { return x[k] > -INFINITY && (level == 0 || bins.in(x[k])); }, sc, lo, hi);
-        if (!(lo <= hi)) return SmBin{ -1, 0, 0 };
+        if (level) sm_range_short<EPT>(x, [&](int k) { return x[k] > -INFINITY && bins.in(x[k]); }, sc, lo, hi);
         bins = sm_bins(linear, lo, hi);
         for (int i = threadIdx.x; i < SM_SLOTS; i += TPB) { if (MASS) { h.hi[i] = 0; h.lo[i] = 0; } else h.n[i] = 0; }
         __syncthreads();
@@ -607,10 +614,10 @@ __device__ __forceinline__ SmBin sm_find_short(const float (&x)[EPT], const doub
 
 // what a top-k (MASS false) or top-p with that target leaves of the candidates
 template <bool MASS, int TPB, int EPT>
-__device__ __forceinline__ SmKept sm_filter_short(const float (&x)[EPT], const double* mass, bool linear, SmTake take, SmShortLds& h, SmScratch& sc)
+__device__ __forceinline__ SmKept sm_filter_short(const float (&x)[EPT], const double* mass, bool linear, float lo, float hi, SmTake take, SmShortLds& h, SmScratch& sc)
 {
     SmBins bins;
-    const SmBin bin = sm_find_short<MASS, TPB, EPT>(x, mass, linear, take, 64, h.hist, sc, bins);
+    const SmBin bin = sm_find_short<MASS, TPB, EPT>(x, mass, linear, lo, hi, take, 64, h.hist, sc, bins);
     if (bin.count > 64) {                                              // equal ones: the first of them
         bool tie[EPT];
         __syncthreads();
@@ -639,7 +646,7 @@ __device__ __forceinline__ SmKept sm_filter_short(const float (&x)[EPT], const d
         const uint32_t n = bin.count, l = threadIdx.x, i = l < n ? h.few.index[l] : 0u;
         const float mine = l < n ? h.few.x[l] : 0.0f;
         uint32_t ahead = 0;
-        for (uint32_t c = 0; c < n; c++) ahead += h.few.x[c] > mine || (h.few.x[c] == mine && h.few.index[c] < i);
+        for (uint32_t c = 0; c < n; c++) { const float other = sm_lane(mine, (int)c); ahead += other > mine || (other == mine && sm_lane(i, (int)c) < i); }
         if (l < n) h.few.order[ahead] = l;
         __threadfence_block();                                         // (one wave: in order, and the compiler is told)
         const uint32_t a = l < n ? h.few.order[l] : 0u;                // the l-th best
@@ -679,7 +686,8 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     if (names) names += r * V;
     auto name = [&](uint32_t i) { return names ? (long long)names[i] : (long long)i; };          // of element i, where the row is what a filter left
     const int i0 = threadIdx.x * EPT;
-    float x[EPT], most = -INFINITY;
+    const bool filtered = (rule.top_k > 0 && rule.top_k < V) || rule.top_p < 1.0;
+    float x[EPT], most = -INFINITY, lowest = -INFINITY;
     {
         LgVec4<T> v[EPT / 4];
 #pragma unroll
@@ -688,7 +696,8 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
 #pragma unroll
         for (int k = 0; k < EPT; k++) { x[k] = sm_score(v[k / 4].v[k % 4], floor); most = fmaxf(most, x[k]); }
     }
-    most = sm_unorder(sm_block_max(sm_order(most), sc.a));
+    if (filtered) sm_range_short<EPT>(x, [&](int k) { return x[k] > -INFINITY; }, sc, lowest, most);
+    else most = sm_unorder(sm_block_max(sm_order(most), sc.a));
     if (most == -INFINITY) {                                           // nothing to draw from
         for (long long j = (long long)blockIdx.y * TPB + threadIdx.x; j < n; j += (long long)gridDim.y * TPB) out[j] = -1;
         return;
@@ -706,6 +715,100 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             for (int j = 0; j < 4; j++) mass[(k + j) * TPB + threadIdx.x] = m[j] * unit;
         }
     };
+    if (rule.top_k > 0 && rule.top_k <= 64 && rule.top_k < V) {
+        // What such a top-k leaves is the work of one wave: the bin in which it ends and what lies above are listed in index order and ranked by
+        // all threads; the first wave applies the other filters, best first, and sums or ranks (10 k scores: 1 behind top-k 50 and
+        // top-p 24 -> 10 us, 10 distinct 31 -> 15, behind top-k alone 20 -> 15; 300 scores 11.5 -> 7.2, 15.5 -> 11, 10.3 -> 10.7)
+        SmTake take = { (double)rule.top_k, 0, { 0, 0 } };
+        SmBins bins;
+        const SmBin bin = sm_find_short<false, TPB, EPT>(x, mass, logits, lowest, most, take, 64, h.hist, sc, bins);
+        if (bin.count <= 64) {                                         // (else equal numbers)
+            uint32_t in = 0, found;
+#pragma unroll
+            for (int k = 0; k < EPT; k++) if (x[k] >= bins.lo && bins.of(x[k]) >= bins.want) in |= 1u << k;
+            uint32_t at = sm_block_scan<uint32_t>(__popc(in), sc.a, found);          // at most 63 + 64
+#pragma unroll
+            for (int k = 0; k < EPT; k++) if ((in >> k) & 1) {
+                    h.few.x[at] = x[k];
+                    if (DISTINCT) h.few.u[at] = u[i0 + k];
+                    h.few.index[at++] = i0 + k;
+                }
+            if (threadIdx.x < 128) { h.few.ahead[threadIdx.x] = 0; h.few.sum[threadIdx.x] = 0.0; }
+            __syncthreads();
+            {
+                constexpr uint32_t PARTS = TPB / 128;                  // threads that share an element's comparisons
+                const uint32_t a = threadIdx.x % 128, each = (found + PARTS - 1) / PARTS, from = threadIdx.x / 128 * each;
+                if (a < found) {
+                    const float mine = h.few.x[a];
+                    uint32_t ahead = 0;
+#pragma unroll 4
+                    for (uint32_t c = from; c < found && c < from + each; c++) ahead += h.few.x[c] > mine || (h.few.x[c] == mine && c < a);
+                    if (ahead) atomicAdd(&h.few.ahead[a], ahead);
+                }
+            }
+            __syncthreads();
+            if (threadIdx.x < 64) {
+                const uint32_t l = threadIdx.x, K = found < (uint32_t)rule.top_k ? found : (uint32_t)rule.top_k;
+                for (uint32_t a = l; a < found; a += 64) if (h.few.ahead[a] < K) h.few.order[h.few.ahead[a]] = a;
+                __threadfence_block();                                 // (one wave: in order, and the compiler is told)
+                const uint32_t a = l < K ? h.few.order[l] : 0u;        // the l-th best
+                const float z[1] = { l < K ? h.few.x[a] : -INFINITY };
+                double m[1];
+                sm_masses(tables, scale, z, m);
+                bool keep = l < K;
+                if (rule.top_p < 1.0) {
+                    const SmLimbs one = sm_limbs(m[0] * unit);
+                    const unsigned long long hi = sm_wave_scan<false>((unsigned long long)one.hi, SmAdd()), lo = sm_wave_scan<false>((unsigned long long)one.lo, SmAdd());
+                    const SmTake part = { rule.top_p * sm_sum_value(SmSum{ sm_lane(hi, 63), sm_lane(lo, 63) }), 0, { 0, 0 } };
+                    keep = keep && sm_room<true>(part, 0, hi - one.hi, lo - one.lo);
+                }
+                if (rule.min_p > 0.0) keep = keep && m[0] >= rule.min_p * sm_lane(m[0], 0);
+                h.few.ahead[l] = 0;
+                h.few.ahead[l + 64] = 0;
+                __threadfence_block();
+                if (DISTINCT) {
+                    uint32_t ahead = 0;
+                    if (__popcll(__ballot(keep)) > n) {                // (else all of them win)
+                        const unsigned long long key = keep ? sm_race_call(scale, z[0], h.few.u[a]) : 0ull;
+                        for (uint32_t c = 0; c < K; c++) { const unsigned long long other = sm_lane(key, (int)c); ahead += other > key || (other == key && sm_lane(a, (int)c) < a); }
+                    }
+                    if (keep && ahead < n) h.few.ahead[a] = 1;
+                    __threadfence_block();
+                    // in index order, two a lane
+                    const uint32_t w0 = h.few.ahead[2 * l], w1 = h.few.ahead[2 * l + 1], upto = sm_wave_scan<false>(w0 + w1, SmAdd());
+                    if (w0) out[upto - w0 - w1] = name(h.few.index[2 * l]);
+                    if (w1) out[upto - w1] = name(h.few.index[2 * l + 1]);
+                    if (l == 63) sc.word[0] = upto;
+                } else {
+                    if (keep) h.few.sum[a] = m[0];
+                    __threadfence_block();
+                    const double m0 = h.few.sum[2 * l], m1 = h.few.sum[2 * l + 1], upto = sm_wave_scan<false>(m0 + m1, SmAdd()), before = sm_dpp<0x138, 0xf>(upto);
+                    const double c0 = m0 > 0.0 ? before + m0 : 0.0, c1 = m1 > 0.0 ? fmax(c0, before + (m0 + m1)) : c0;        // rise with a mass only
+                    const double risen = sm_dpp<0x138, 0xf>(sm_wave_scan<false>(c1, SmMaxOf()));
+                    h.few.sum[2 * l] = fmax(risen, c0);
+                    h.few.sum[2 * l + 1] = fmax(risen, c1);
+                    const unsigned long long b0 = __ballot(m0 > 0.0), b1 = __ballot(m1 > 0.0);
+                    const int l0 = 2 * (63 - (b0 ? __clzll((long long)b0) : 64)), l1 = 2 * (63 - (b1 ? __clzll((long long)b1) : 64)) + 1;
+                    if (l == 63) { sc.word[0] = (unsigned long long)__double_as_longlong(upto); sc.word[1] = (unsigned long long)(l0 > l1 ? l0 : l1); }
+                }
+            }
+            __syncthreads();
+            if (DISTINCT) {
+                for (long long j = (long long)sc.word[0] + threadIdx.x; j < n; j += TPB) out[j] = -1;
+            } else {
+                const double total = __longlong_as_double((long long)sc.word[0]);
+                const uint32_t last = (uint32_t)sc.word[1];
+                for (long long j = (long long)blockIdx.y * TPB + threadIdx.x; j < n; j += (long long)gridDim.y * TPB) {
+                    const float uj = u[j];
+                    const double t = (uj > 0.0f ? (double)uj : 0.0) * total;
+                    uint32_t lo = 0, hi = last;                        // the first sum that passes t, or the last one
+                    while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (h.few.sum[mid] > t) hi = mid; else lo = mid + 1; }
+                    out[j] = name(h.few.index[lo]);
+                }
+            }
+            return;
+        }
+    }
     // filters: an element that one of them drops becomes -inf
     for (int pass = 0; pass < 2; pass++) {
         SmTake take = { 0.0, 0, { 0, 0 } };
@@ -713,7 +816,8 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         if (pass == 0) {
             if (rule.top_k <= 0 || rule.top_k >= V) continue;
             take.target = (double)rule.top_k;
-            left = sm_filter_short<false, TPB, EPT>(x, mass, logits, take, h, sc);
+            left = sm_filter_short<false, TPB, EPT>(x, mass, logits, lowest, most, take, h, sc);
+            lowest = left.thr;
         } else {
             if (rule.top_p >= 1.0) continue;
             SmSum mine = { 0, 0 }, total;
@@ -723,7 +827,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
             sm_block_scan<unsigned long long>(mine.hi, sc.a, total.hi);
             sm_block_scan<unsigned long long>(mine.lo, sc.b, total.lo);
             take.target = rule.top_p * sm_sum_value(total);
-            left = sm_filter_short<true, TPB, EPT>(x, mass, logits, take, h, sc);
+            left = sm_filter_short<true, TPB, EPT>(x, mass, logits, lowest, most, take, h, sc);
         }
 #pragma unroll
         for (int k = 0; k < EPT; k++) if (!sm_in(left, x[k], (uint32_t)(i0 + k))) x[k] = -INFINITY;
@@ -739,12 +843,18 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         uint32_t wins = 0;
         const float slope = sm_slope(rule);
 #pragma unroll
-        for (int k = 0; k < EPT; k++) race[k] = x[k] > -INFINITY ? u[i0 + k] : 0.0f;              // (loads first; -inf behind V)
+        for (int k = 0; k < EPT / 4; k++) {                            // (loads first)
+            const LgVec4<float> four = sm_load4(u, i0 + 4 * k, V, sm_aligned(u));
+#pragma unroll
+            for (int j = 0; j < 4; j++) race[4 * k + j] = four.v[j];
+        }
 #pragma unroll
         for (int k = 0; k < EPT; k++) race[k] = x[k] > -INFINITY ? sm_race32(logits, slope, x[k], race[k]) : -INFINITY;
+        float rlo, rhi;
+        sm_range_short<EPT>(race, [&](int k) { return race[k] > -INFINITY; }, sc, rlo, rhi);
         SmTake take = { (double)n, 0, { 0, 0 } };
         SmBins bins;
-        const SmBin bin = sm_find_short<false, TPB, EPT>(race, nullptr, true, take, 64, h.hist, sc, bins);
+        const SmBin bin = sm_find_short<false, TPB, EPT>(race, nullptr, true, rlo, rhi, take, 64, h.hist, sc, bins);
         float zlo = -INFINITY, zhi = -INFINITY;                        // nothing to rank where everything wins
         const bool ranked = bin.total > (uint32_t)n;
         if (ranked) {

@@ -318,6 +318,22 @@ def test_sampling_of_special_scores(kind, logits, V):
             check_distinct(x, draws_of((2, V)), V // 4, logits=logits, **kw)
 
 
+@pytest.mark.parametrize("kind", ["normal", "ties", "masked", "nan", "wide", "inf", "near", "empty", "tiny"])
+@pytest.mark.parametrize("V", [64, 65, 130, 1025, 5000, 12288])
+@pytest.mark.parametrize("logits", [True, False])
+def test_top_k_around_a_wave(kind, V, logits):
+    """top-k of up to 64 is finished by one wave, unless equal scores at the border are too many for it"""
+    for k, dtype in zip((1, 2, 50, 63, 64, 65), itertools.cycle(TYPES)):
+        x = scores_of(kind, 3, V, dtype, logits, seed=k)
+        if kind == "masked":
+            x[1, : V - 20] = -math.inf if logits else 0.0             # fewer left than k
+        for kw in (dict(), dict(top_p=0.7), dict(min_p=0.2), dict(temperature=0.6, top_p=0.9, min_p=0.05)):
+            check_sample(x, draws_of((3, 40), k), logits=logits, top_k=k, **kw)
+            for n in (1, 20, 64):
+                check_distinct(x, draws_of((3, V), k), n, logits=logits, top_k=k, **kw)
+    check_sample(x[:1], draws_of((1, 5000)), logits=logits, top_k=40, top_p=0.9)      # draws shared by workgroups
+
+
 @pytest.mark.parametrize("T", [1e-30, 1e-20, 1e-14, 1e-8, 1e-3, 0.7, 1.7, 1e20, 1e30])
 @pytest.mark.parametrize("V", [300, 9000, 70001])
 @pytest.mark.parametrize("logits", [True, False])

@@ -967,7 +967,7 @@ struct SmRowState {                    // (sm_begin_kernel knows where kept and 
     unsigned long long sure;           // race: winners
     float best, least;                 // largest score; least score that passes min-p
     uint32_t prefix, ties, ended, cut, zone_lo, zone_hi, candidates;
-    uint32_t ticket[SM_STEPS], sub[16];
+    uint32_t ticket[SM_STEPS], sub[16][32];       // (sub: one of 32 words, 128 bytes apart)
 };
 
 struct SmWork {                        // workspace of a call
@@ -991,25 +991,26 @@ template <typename V> __device__ __forceinline__ void sm_poke(V* p, V v) { __hip
 // go through the XCD's own L2) and is read by sm_peek: each wave waits for its own to be done before the ticket is drawn, and no L2 has to be
 // written back (a release fence in every wave of every workgroup took longer than the pass over the data).
 __device__ __forceinline__ uint32_t sm_draw_ticket(uint32_t* t) { return __hip_atomic_fetch_add(t, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ bool sm_last_block(uint32_t* ticket, uint32_t blocks, uint32_t* lds)
+// Adds to one line of memory take 5 ns each, so of more than 128 workgroups sixteen groups draw among themselves first, on lines of their own (3 M
+// scores: a plain draw, 733 workgroups, 26.5 -> 23.5 us, top-k of 1.5 M, four steps of 256, 51.8 -> 48.1).  The last of a group leaves its word
+// clear for the next step.
+__device__ __forceinline__ bool sm_last_block(SmRowState& st, int step, uint32_t block, uint32_t blocks, uint32_t* lds)
 {
     if (blocks == 1) { __syncthreads(); return true; }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) *lds = sm_draw_ticket(ticket) == blocks - 1;
-    __syncthreads();
-    return *lds != 0;
-}
-// ... of many workgroups: adds to one word take 10 ns each, so sixteen groups draw among themselves first (3 M scores, 733 workgroups: 26.5 us
-// a call, 29.0 with one word).  `sub`: sixteen cleared words
-__device__ __forceinline__ bool sm_last_block_of_many(uint32_t* ticket, uint32_t* sub, uint32_t block, uint32_t blocks, uint32_t* lds)
-{
-    if (blocks <= 128) return sm_last_block(ticket, blocks, lds);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
     if (threadIdx.x == 0) {
-        const uint32_t g = block & 15;
-        *lds = sm_draw_ticket(&sub[g]) == (blocks - g + 15) / 16 - 1 && sm_draw_ticket(ticket) == 15;
+        bool last;
+        if (blocks <= 128) last = sm_draw_ticket(&st.ticket[step]) == blocks - 1;
+        else {
+            const uint32_t g = block & 15;
+            last = sm_draw_ticket(st.sub[g]) == (blocks - g + 15) / 16 - 1;
+            if (last) {
+                sm_poke(st.sub[g], 0u);
+                last = sm_draw_ticket(&st.ticket[step]) == 15;
+            }
+        }
+        *lds = last;
     }
     __syncthreads();
     return *lds != 0;
@@ -1168,7 +1169,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
             if (counted && h.n[slot]) atomicAdd(&g.n[k], h.n[slot]);
             if (MASS) { if (h.hi[slot]) atomicAdd(&g.hi[k], h.hi[slot]); if (h.lo[slot]) atomicAdd(&g.lo[k], h.lo[slot]); }
         }
-        if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+        if (!sm_last_block(st, step, (uint32_t)b, (uint32_t)wk.B, &ticket)) return;
         // taken over (all loads before the first store: each is a round trip to memory), and left clear for the next level
         constexpr int K = SM_BINS / SM_LTPB;
         uint32_t n[K];
@@ -1295,7 +1296,7 @@ __global__ void __launch_bounds__(1024) sm_count16_kernel(const T* __restrict__ 
     unsigned long long* all_live = (unsigned long long*)(counts + 65536);        // a word of each wave, 128 bytes apart (adds to one line wait for each other)
     if (lane == 0 && live) atomicOr(&all_live[wave * 16], live);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    if (!sm_last_block(st, step, (uint32_t)b, (uint32_t)wk.B, &ticket)) return;
     const unsigned long long lives = sm_peek(&all_live[(lane & 15) * 16]);
     live = sm_lane(lives, wave);
     const int top = (int)sm_lane(sm_wave_scan<true>(lives ? (uint32_t)chunk_of(63 - __clzll((long long)lives), lane & 15) + 1 : 0u, SmMaxOf()), 15) - 1;
@@ -1441,7 +1442,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_cut_kernel(const T* __restrict__ s
             if (threadIdx.x == 0) sm_poke(&tile_n[t], total);
         }
     }
-    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    if (!sm_last_block(st, step, (uint32_t)b, (uint32_t)wk.B, &ticket)) return;
     const uint32_t want = cut ? st.ties : SM_ALL;                      // equal elements that are kept
     unsigned long long equal = 0, run = 0;
     long long tile = -1;
@@ -1576,7 +1577,7 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
             sm_poke(&tops[t], best > -INFINITY ? scale.top : -INFINITY);
         }
     }
-    if (!sm_last_block_of_many(&st.ticket[step], st.sub, (uint32_t)b, (uint32_t)wk.B, &ticket)) return;
+    if (!sm_last_block(st, step, (uint32_t)b, (uint32_t)wk.B, &ticket)) return;
     double top = -INFINITY;
     for (long long t = threadIdx.x; t < wk.stiles; t += 256) top = fmax(top, sm_peek(&tops[t]));
     const unsigned long long ordered = (unsigned long long)__double_as_longlong(top + 0.0);
@@ -1750,7 +1751,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_kernel(const T* __restrict__ 
     __syncthreads();
     uint32_t* g = wk.rbins(r);
     for (int i = threadIdx.x; i < SM_RBINS; i += SM_LTPB) if (const uint32_t c = h[sm_nth_slot(i)]) atomicAdd(&g[i], c);
-    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    if (!sm_last_block(st, step, (uint32_t)b, (uint32_t)wk.B, &ticket)) return;
     uint32_t n4[SM_RBINS / SM_LTPB];
 #pragma unroll
     for (int k = 0; k < SM_RBINS / SM_LTPB; k++) n4[k] = sm_peek(&g[k * SM_LTPB + threadIdx.x]);
@@ -1797,7 +1798,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, SmR
     __syncthreads();
     uint32_t* g = wk.rbins(r);
     for (int i = threadIdx.x; i < nbins; i += SM_LTPB) if (const uint32_t c = h[sm_nth_slot(i)]) atomicAdd(&g[i], c);
-    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    if (!sm_last_block(st, step, (uint32_t)b, (uint32_t)wk.B, &ticket)) return;
     for (int i = threadIdx.x; i < nbins; i += SM_LTPB) h[sm_nth_slot(i)] = sm_peek(&g[i]);
     __syncthreads();
     SmTake take = st.take;
@@ -1849,7 +1850,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ 
         sm_block_scan<uint32_t>(c, sc.a, total);
         if (threadIdx.x == 0) { sm_poke(&tile_n[t], total); }
     }
-    if (!sm_last_block(&st.ticket[step], (uint32_t)wk.B, &ticket)) return;
+    if (!sm_last_block(st, step, (uint32_t)b, (uint32_t)wk.B, &ticket)) return;
     unsigned long long mine = 0, sure;
     const bool in_lds = wk.tiles <= SM_ZTILES;
     const uint32_t found = sm_peek(&st.candidates);

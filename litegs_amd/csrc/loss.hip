@@ -151,10 +151,17 @@ __global__ void __launch_bounds__(256) l1_ssim_forward_kernel(const float* __res
         if (gx < W && gy < H) {
             const float C1 = 0.01f * 0.01f, C2 = 0.03f * 0.03f;
             float mu1 = m[0][j], mu2 = m[1][j];
-            float e2sum = 0.5f * (m[2][j] + m[3][j]), exy = 0.25f * (m[2][j] - m[3][j]);       // E[x^2]+E[y^2], E[xy]
+            float exy = 0.25f * (m[2][j] - m[3][j]);                      // E[xy]; E[x^2]+E[y^2] is half the sum
             float s12 = exy - mu1 * mu2;
             float A1 = 2.0f * mu1 * mu2 + C1, A2 = 2.0f * s12 + C2;
-            float B1 = mu1 * mu1 + mu2 * mu2 + C1, B2 = (e2sum - mu1 * mu1 - mu2 * mu2) + C2;
+            // squares rounded by themselves, whatever the compiler would contract: a training run's last bits depend on it
+            float B1, B2;
+            {
+#pragma clang fp contract(off)
+                const float q1 = mu1 * mu1, q2 = mu2 * mu2;
+                B1 = q1 + q2 + C1;
+                B2 = fmaf(0.5f, m[2][j] + m[3][j], -q1) - q2 + C2;
+            }
             const float rB2 = __builtin_amdgcn_rcpf(B2);               // B1, B2 >= C1, C2 > 0: v_rcp_f32 (1 ulp) instead of two IEEE divisions
             float inv = __builtin_amdgcn_rcpf(B1) * rB2;
             float s_val = A1 * A2 * inv;
@@ -360,7 +367,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(7, 8))
             float xv = clamp01 ? fminf(fmaxf(xr, 0.0f), 1.0f) : xr;
             float d = xv - yv;
             float sgn = (d > 0.0f) ? 1.0f : ((d < 0.0f) ? -1.0f : 0.0f);
-            float gr = g * (-lam * inv_n * (b[0][j] + 2.0f * xv * b[1][j] + yv * b[2][j]) + (1.0f - lam) * inv_n * sgn);
+            float gr;
+            {
+#pragma clang fp contract(off)                                             // (as in the forward kernel)
+                gr = g * (-lam * inv_n * fmaf(yv, b[2][j], b[0][j] + 2.0f * xv * b[1][j]) + (1.0f - lam) * inv_n * sgn);
+            }
             if (clamp01 && !(xr >= 0.0f && xr <= 1.0f)) gr = 0.0f;
             d_img[oi] = gr;
         } else if (gx < Wp && gy < Hp) {

@@ -87,7 +87,7 @@ static int dropout_launch(const T* x, T* y, long long lead, long long M, unsigne
                           const long long* ids, int S, hipStream_t s)
 {
     const long long items = (M + 3) / 4 * ((lead + DR_ROWS - 1) / DR_ROWS), blocks = (items + DR_TPB - 1) / DR_TPB;
-    if (blocks > 0x7fffffffll) return (int)hipErrorInvalidValue;
+    if (blocks > 0xffffffll) return (int)hipErrorInvalidValue;         // (threads of a launch: 32 bits; four elements each)
     const bool vec = M % 4 == 0 && ((uintptr_t)x | (uintptr_t)y) % (4 * sizeof(T)) == 0;
     const dim3 grid((unsigned)blocks);
     if (vec) hipLaunchKernelGGL((dropout_kernel<T, true>), grid, dim3(DR_TPB), 0, s, x, y, lead, M, threshold, scale, key, ids, S);
@@ -181,7 +181,7 @@ template <typename T>
 static int draw_launch(const T* std_, T* out, long long n, const DrKey& key, float top, hipStream_t s)
 {
     const long long blocks = ((n + 3) / 4 + DR_TPB - 1) / DR_TPB;
-    if (blocks > 0x7fffffffll) return (int)hipErrorInvalidValue;
+    if (blocks > 0xffffffll) return (int)hipErrorInvalidValue;         // (threads of a launch: 32 bits; four elements each)
     const bool vec = ((uintptr_t)std_ | (uintptr_t)out) % (4 * sizeof(T)) == 0;
     const dim3 grid((unsigned)blocks);
     if (std_ && vec) hipLaunchKernelGGL((draw_kernel<T, true, true>), grid, dim3(DR_TPB), 0, s, std_, out, n, key, top);

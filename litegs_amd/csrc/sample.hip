@@ -664,7 +664,7 @@ __device__ __forceinline__ SmKept sm_filter_short(const float (&x)[EPT], const d
 }
 
 // A row from beginning to end in one launch: scores in registers, masses in LDS (worked out once), and one histogram level a filter as a rule.
-// 10 k scores: a plain draw 9.5 us, behind top-k and top-p 24, 500 distinct 19; a launch alone is 5.  64 rows take what one takes (a compute
+// 10 k scores: a plain draw 9.5 us, behind top-k 50 and top-p 10, behind top-p 20, 500 distinct 18; a launch alone is 5.  64 rows take what one takes (a compute
 // unit each).
 template <typename T, int TPB, int EPT, bool DISTINCT>
 __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
@@ -1085,8 +1085,8 @@ __device__ __forceinline__ SmSum sm_sum_of_parts(const SmParts& p, unsigned long
 
 // One level of top-k (MASS false) or top-p: bits [shift - width, shift) of the ordered scores that pass the filters and match the prefix found
 // so far.  Three levels of 11, 10 and 11 bits name the last key that is taken, whatever the scores are like; a level of 2^13 bins instead
-// would merge four times as many words.  10 M weights under a temperature: 40 us for the first level (a logarithm and an exponential in 64
-// bits each: the vector pipe), 18 and 18 for the others (2.2 TB/s); 3 M counted: 13, 13 and 10 us, of which the data are 3 each.
+// would merge four times as many words.  10 M weights under a temperature: 42 us for the first level (a logarithm and an exponential in 64
+// bits each: the vector pipe), 18 and 17 for the others (2.2 TB/s); 3 M counted: 13, 13 and 8 us, of which the data are 3 each.
 template <typename T, bool MASS>
 __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, int step,
                                                            int shift, int width)
@@ -1223,7 +1223,7 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
 // ---- scores of 16 bits: both filters from one histogram of all keys ----------------------------------------------------------------------
 // The 65536 ordered keys of a 16-bit type are counted in LDS (two counters a word: a workgroup takes at most SM_SHARE16 elements), added up in
 // memory, and the last workgroup works top-k and top-p out of the counts: one pass over the row and one exponential per distinct score, in
-// the place of one pass for the best and three for each filter.  16 rows of 100 k: 25 us, about half of it the last workgroup's conclusion.
+// the place of one pass for the best and three for each filter.  16 rows of 100 k: 24 us, about half of it the last workgroup's conclusion.
 // Rows of 50 k behind top-p: 1 row 46 us a call (by levels 63), 64 rows 57 (82), 256 rows 129 (152), 512 rows 228 (275); behind top-k alone 64
 // rows 47 (54), 256 rows 106 (94).  So up to 256 rows, where the counts are 64 MB, and without top-p up to 128.
 #define SM_SHARE16 32768
@@ -1537,7 +1537,7 @@ __device__ __forceinline__ SmKept sm_final(const SmWork& wk, long long r, const 
 // ---- long rows, with replacement -------------------------------------------------------------------------------------------------------
 // Prefix sums of the kept masses inside tiles, one stored per SM_GROUP elements, relative to the tile's best element (so that no pass for the
 // row's best is needed); the last workgroup puts the tiles on a common scale.  Fixed order everywhere.  Workgroups of 256, five a compute unit,
-// hide each other's scans: 3 M weights 14 us, 10 M scores 31 (1.3 TB/s: the exponentials; 26 for weights, which have none).
+// hide each other's scans: 3 M weights 12 us, 10 M scores 31 (1.3 TB/s: the exponentials; 26 for weights, which have none).
 template <typename T>
 __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, SmWork whole, int step)
 {
@@ -1993,7 +1993,7 @@ static bool sm_rule(int logits, double temperature, long long top_k, double top_
 }
 
 // How a call runs.  Short rows: one workgroup each, as far as its LDS and registers reach (12288 scores, short and long: plain 10 and 16 us, behind
-// top-p 21 and 53, 614 distinct 21 and 27; 64 rows 10 / 18, 23 / 58, 22 / 29).  Long ones: the filters by levels of a histogram, or, for 16-bit
+// top-p 20 and 53, 614 distinct 17 and 27; 64 rows 10 / 18, 22 / 58, 18 / 29).  Long ones: the filters by levels of a histogram, or, for 16-bit
 // scores, from one histogram of all keys; what a small top-k leaves goes on as a short row.  Both sides of these two stand at their kernels.
 struct SmPlan { bool is_short, top_k, top_p, counts, few; };
 #define SM_COUNTS_ROWS 256
@@ -2051,18 +2051,25 @@ static void sample_short(const T* scores, long long ss, const float* u, long lon
     // Many draws of few rows: workgroups that would idle filter the row once more and share its draws.  By one workgroup 5000 draws of 1000
     // scores take 22 us and 100000 of 10000 171 us; with 4096 draws a workgroup 13 and 17 us, with 1024 7 and 12 us (7 and 11 us are 1000 draws).
     const long long share = (n + 1023) / 1024, most = R < 256 ? 256 / R : 1;
-    const dim3 grid((unsigned)R, distinct ? 1u : (unsigned)(share < most ? share : most));
-#define SM_LAUNCH_SHORT(TPB_, EPT_)                                                                                                                            \
-    do {                                                                                                                                                       \
-        if (distinct) hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, true>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, names, out);  \
-        else hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, false>), grid, dim3(TPB_), 0, s, scores, ss, u, us, (int)V, n, rule, names, out);          \
+    const long long rows = 1ll << 21;                                  // of a launch: its threads are counted in 32 bits
+    for (long long r = 0; r < R; r += rows) {
+        const dim3 grid((unsigned)(R - r < rows ? R - r : rows), distinct ? 1u : (unsigned)(share < most ? share : most));
+        const T* x = scores + r * ss;
+        const float* v = u + r * us;
+        const uint32_t* nm = names ? names + r * V : nullptr;
+        long long* o = out + r * n;
+#define SM_LAUNCH_SHORT(TPB_, EPT_)                                                                                                                 \
+    do {                                                                                                                                            \
+        if (distinct) hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, true>), grid, dim3(TPB_), 0, s, x, ss, v, us, (int)V, n, rule, nm, o); \
+        else hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, false>), grid, dim3(TPB_), 0, s, x, ss, v, us, (int)V, n, rule, nm, o);         \
     } while (0)
-    // 300 scores in 256 x 4, 1024 x 4 and 768 x 16 threads x elements: a plain draw 4.8, 4.9 and 7.2 us, 512 rows of them 5.2, 9.6 and 15; 3000
-    // scores in the last two 5.4 and 7.4, 512 rows 11 and 16
-    if (V <= 1024) SM_LAUNCH_SHORT(256, 4);
-    else if (V <= 4096) SM_LAUNCH_SHORT(1024, 4);
-    else SM_LAUNCH_SHORT(768, 16);
+        // 300 scores in 256 x 4, 1024 x 4 and 768 x 16 threads x elements: a plain draw 4.8, 4.9 and 7.2 us, 512 rows of them 5.2, 9.6 and 15; 3000
+        // scores in the last two 5.4 and 7.4, 512 rows 11 and 16
+        if (V <= 1024) SM_LAUNCH_SHORT(256, 4);
+        else if (V <= 4096) SM_LAUNCH_SHORT(1024, 4);
+        else SM_LAUNCH_SHORT(768, 16);
 #undef SM_LAUNCH_SHORT
+    }
 }
 
 template <typename T>
@@ -2077,7 +2084,7 @@ static int sample_launch(const T* scores, long long ss, const float* u, long lon
     SmWork wk;
     const long long need = sm_layout(plan, R, V, (int)sizeof(T), distinct, rule.top_k, (char*)temp, wk);
     const long long draws = R * ((n + 255) / 256);
-    if (temp == nullptr || temp_bytes < need || (uintptr_t)temp % 16 != 0 || R * wk.tiles > 0x7fffffffll || draws > 0x7fffffffll) return (int)hipErrorInvalidValue;
+    if (temp == nullptr || temp_bytes < need || (uintptr_t)temp % 16 != 0 || R * wk.tiles > 0x3fffffll || draws > 0xffffffll) return (int)hipErrorInvalidValue;        // (threads of a launch: 32 bits)
     const dim3 grid((unsigned)(R * wk.B)), block(SM_LTPB);
     int step = 0;
     const int want_best = !plan.counts && (plan.top_p || rule.min_p > 0.0);
@@ -2087,7 +2094,6 @@ static int sample_launch(const T* scores, long long ss, const float* u, long lon
             SmWork cw = wk;                                            // counters of 16 bits: a bounded share of the row each
             const long long shares = (V + SM_SHARE16 - 1) / SM_SHARE16;
             cw.B = shares > wk.B ? shares : wk.B;
-            if (R * cw.B > 0x7fffffffll) return (int)hipErrorInvalidValue;
             hipLaunchKernelGGL((sm_count16_kernel<T>), dim3((unsigned)(R * cw.B)), dim3(1024), 0, s, scores, ss, V, rule, cw, step++, (int)plan.top_k, (int)plan.top_p);
         }
     }

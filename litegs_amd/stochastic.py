@@ -166,8 +166,10 @@ def _sample(what: str, scores, u, n: int, distinct: bool, temperature, top_k, to
     if V >= 1 << 31:
         raise ValueError(f"{what}: at most 2^31 - 1 categories")
     temperature, top_k, top_p, min_p = check_rule(what, temperature, top_k, top_p, min_p)
+    R = math.prod(scores.shape[:-1])
+    if V > 12288 and (R * ((V + 8191) // 8192) >= 1 << 22 or R * ((n + 255) // 256) >= 1 << 24):
+        raise ValueError(f"{what}: {R} rows of {V} categories and {n} draws are too many for one call")
     x, uu = _rows(scores), _rows(u)
-    R = x.shape[0]
     out = torch.empty((*scores.shape[:-1], n), dtype=torch.int64, device=x.device)
     if _C is not None:
         _C.sample(x, uu, out, n, distinct, bool(logits), temperature, top_k, top_p, min_p)

@@ -449,6 +449,14 @@ def test_rows_of_two_gigabytes_and_more():
     assert stochastic.sample_distinct(w, uu, 4, logits=False).tolist() == [[3, 2 ** 30 + 1, V - 2, -1]]
 
 
+def test_more_rows_than_a_launch_has_threads_for():
+    few, R = 1000, 2 ** 24 + 5                                       # (256 threads a row: more than 2^32)
+    x, u = scores_of("normal", few, 3, torch.float32, True), draws_of((few, 3))
+    rows = torch.arange(R, device=DEV) % few
+    for got, want in ((stochastic.sample(x[rows], u[rows][:, :1]), stochastic.sample(x, u[:, :1])), (stochastic.sample_distinct(x[rows], u[rows], 2), stochastic.sample_distinct(x, u, 2))):
+        assert torch.equal(got, want[rows])
+
+
 def test_dropout_behind_32_bits():
     lead, M = 9, 2 ** 29 + 4
     x = torch.ones((lead, M), dtype=torch.bfloat16, device=DEV)
@@ -525,6 +533,14 @@ def test_empty_calls():
     assert stochastic.sample_distinct(torch.zeros((2, 5), device=DEV), draws_of((2, 5)), 0).shape == (2, 0)
     assert stochastic.sample_distinct(z, z, 0).shape == (2, 0)
     assert stochastic.sample(torch.zeros((0, 5), device=DEV), draws_of((0, 3))).shape == (0, 3)
+
+
+def test_too_many_rows_or_draws_are_refused():
+    x, u = torch.zeros((1, 1), device=DEV), torch.zeros((1, 1), device=DEV)
+    with pytest.raises(ValueError, match="too many"):
+        stochastic.sample(x.expand(2 ** 21, 13000), u.expand(2 ** 21, 1))
+    with pytest.raises(ValueError, match="too many"):
+        stochastic.sample(x.expand(2 ** 12, 13000), u.expand(2 ** 12, 2 ** 20))
 
 
 def test_sampling_refusals():

@@ -29,9 +29,9 @@ __device__ __forceinline__ float dr_product(float a, float b)
     asm volatile("" : "+v"(c));
     return c;
 }
-// Measured: 3 M float32 10 us a direction behind an idle gap (24 MB), 45 rows of 500 k 34 us (180 MB: 5.3 TB/s, part of it
-// from the last-level cache); what a forward and a backward pass take of a user's program for less than 20 M elements is the autograd
-// engine's host time (45 us).
+// Measured, launch behind launch: 3 M float32 4.6 us a direction (24 MB: 5.2 TB/s), by chunk id 5.6, 45 rows of 500 k 27 us (180 MB: 6.6 TB/s, part
+// of it from the last-level cache), 8 M bfloat16 9.1 (their words' issue alone 7).  What a forward and a backward pass take of a user's program
+// for less than 10 M elements is the autograd engine's host time (40 us).
 // Work items are (block of DR_ROWS rows, group), groups innermost, so that short rows fill a workgroup too.
 #define DR_ROWS 8
 template <typename T, bool VEC>
@@ -53,8 +53,12 @@ __global__ void __launch_bounds__(DR_TPB) dropout_kernel(const T* __restrict__ x
         const LgWords w = lg_philox((unsigned long long)g, offset, key.seed);
 #pragma unroll
         for (int k = 0; k < 4; k++) keep[k] = w.w[k] >= threshold;
-    } else {
-        // four consecutive columns lie in one block of words when S is a multiple of four; otherwise the block may change at each of them
+    } else if (S % 4 == 0) {                                           // four consecutive columns are one block of words
+        const long long a = (i0 | S) >> 32 ? i0 / S : (long long)((uint32_t)i0 / (uint32_t)S);
+        const LgWords w = lg_philox(((unsigned long long)chunk_ids[a] * (unsigned)S + (unsigned long long)(i0 - a * S)) >> 2, offset, key.seed);
+#pragma unroll
+        for (int k = 0; k < 4; k++) keep[k] = w.w[k] >= threshold;
+    } else {                                                           // the block may change at each of them
         unsigned long long block = ~0ull;
         LgWords w = {};
 #pragma unroll

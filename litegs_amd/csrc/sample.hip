@@ -277,6 +277,14 @@ template <typename V> __device__ __forceinline__ V sm_block_scan(V v, void* lds,
     V before;
     return sm_block_op(v, SmAdd(), lds, before, total) - v;
 }
+// The same for floating sums: handed up one lane (and one wave), not the inclusive sum less the thread's own, which would lose what lies before
+// a thread whose own is 2^53 times as large.
+__device__ __forceinline__ double sm_block_sum_before(double v, void* lds, double& total)
+{
+    double before;
+    const double prev = sm_dpp<0x138, 0xf>(sm_block_op(v, SmAdd(), lds, before, total));        // one lane up; lane 0: 0
+    return (threadIdx.x & 63) ? prev : before;
+}
 // inclusive maximum over the threads up to this one: sums that rounding made fall, or rise without a mass, are flat again
 __device__ __forceinline__ double sm_block_rise(double v, void* lds, double& total)
 {
@@ -675,7 +683,6 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
     __shared__ SmShortLds h;
     __shared__ SmTables tables;
     __shared__ uint32_t won[DISTINCT ? TPB * EPT / 32 : 1];
-    __shared__ uint16_t pos[DISTINCT ? 1 : TPB];
     __shared__ SmScratch sc;
     const long long r = blockIdx.x;
     const T* row = scores + r * sstride;
@@ -921,28 +928,33 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         for (int k = 0; k < EPT; k++) if ((wins >> k) & 1) out[at++] = name(i0 + k);
         for (long long j = (long long)total + threadIdx.x; j < n; j += TPB) out[j] = -1;
     } else {
-        double m[EPT], sum = 0.0, total;
-        uint32_t positive = 0, last = 0;
+        double m[EPT], sum = 0.0, total, most_sum;
+        uint32_t last = 0;
         if (rule.top_p >= 1.0) masses();
 #pragma unroll
         for (int k = 0; k < EPT; k++) m[k] = x[k] > -INFINITY ? mass[k * TPB + threadIdx.x] : 0.0;
 #pragma unroll
         for (int k = 0; k < EPT; k++) {
             sum += m[k];
-            if (m[k] > 0.0) { positive |= 1u << k; last = (uint32_t)(i0 + k) + 1; }
+            if (m[k] > 0.0) last = (uint32_t)(i0 + k) + 1;
         }
-        double at = sm_block_scan<double>(sum, sc.a, total);
+        // cumulative masses that rise at elements with a mass only, and never fall (a sum along the lanes and one along a thread's elements
+        // round differently): the search then ends at an element that can be drawn
+        const double before = sm_block_sum_before(sum, sc.a, total);
         last = sm_block_max(last, sc.b);
+        double at = before, high = 0.0;
 #pragma unroll
-        for (int k = 0; k < EPT; k++) { at += m[k]; mass[k * TPB + threadIdx.x] = at; }
-        pos[threadIdx.x] = (uint16_t)positive;
+        for (int k = 0; k < EPT; k++) { at += m[k]; if (m[k] > 0.0) high = fmax(high, at); }
+        high = sm_block_rise_before(high, sc.a, most_sum);
+        at = before;
+#pragma unroll
+        for (int k = 0; k < EPT; k++) { at += m[k]; if (m[k] > 0.0) high = fmax(high, at); mass[k * TPB + threadIdx.x] = high; }
         __syncthreads();
         for (long long j = (long long)blockIdx.y * TPB + threadIdx.x; j < n; j += (long long)gridDim.y * TPB) {         // (blockIdx.y: its share of the draws)
             const float uj = u[j];
             const double t = (uj > 0.0f ? (double)uj : 0.0) * total;
             uint32_t lo = 0, hi = last - 1;                            // first element whose sum passes t; at the end the last one with a mass
             while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (mass[mid % EPT * TPB + mid / EPT] > t) hi = mid; else lo = mid + 1; }
-            while (lo < last - 1 && !((pos[lo / EPT] >> (lo % EPT)) & 1)) lo++;      // rounding at a border never lands on a masked element
             out[j] = name(lo);
         }
     }

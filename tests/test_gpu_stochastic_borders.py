@@ -1,0 +1,39 @@
+"""The samplers where the masses before and behind a category differ by many powers of two, and at the ends of the range of ``u``: against
+the 64-bit forms, index for index."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from litegs_amd import stochastic
+from tests.test_gpu_stochastic import DEV, TYPES, check_sample, scores_of
+
+pytestmark = pytest.mark.gpu
+
+SMALL = [0.0, -1.0, math.nan, 1e-45, 1e-38, 1e-30, 1e-20, 1e-12, 1e-6]
+
+
+def numbers(values, R):
+    return torch.tensor(values, dtype=torch.float32, device=DEV).expand(R, len(values))
+
+
+def test_a_far_larger_mass_behind_does_not_hide_a_small_one():
+    """the threads of a workgroup hold four scores each: 1 lies in the first one's, 7 and 11 at the ends of the others'.  The masses are
+    e^-40 = 4.2e-18, 1 and 1, so that 1e-18 of their total, 2e-18, still lies in the first"""
+    x = torch.full((1, 12), -math.inf, device=DEV)
+    x[0, 1], x[0, 7], x[0, 11] = -40.0, 0.0, 0.0
+    assert stochastic.sample(x, numbers([0.0, -1.0, math.nan, 1e-45, 1e-18, 0.25, 0.75], 1)).tolist() == [[1, 1, 1, 1, 1, 7, 11]]
+
+
+@pytest.mark.parametrize("V", [5, 12, 64, 300, 1000, 1024, 1025, 4096, 4097, 9000, 12288])
+@pytest.mark.parametrize("T", [0.05, 0.1, 1.0])
+def test_small_numbers_in_short_rows(V, T):
+    for dtype in TYPES:
+        for seed in range(4):
+            x = scores_of("masked", 16, V, dtype, True, seed=seed)
+            for kw in (dict(), dict(top_k=V // 2 + 65), dict(top_p=0.9999), dict(min_p=1e-30)):
+                check_sample(x, numbers(SMALL, 16), logits=True, temperature=T, **kw)
+        x = scores_of("steps", 16, V, dtype, False, seed=V)             # weights over the whole range of the type
+        for kw in (dict(), dict(temperature=0.5), dict(top_k=V // 2 + 65)):
+            check_sample(x, numbers(SMALL, 16), logits=False, **kw)

@@ -1610,7 +1610,7 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
             if (rule.mode != SM_LINEAR) mass[k] = tt[k] == -INFINITY ? 0.0 : mass[k] * sm_exp(tables, tt[k] - top);
             sum += mass[k];
         }
-        double at = run + sm_block_scan<double>(sum, sc.a, total);
+        double at = run + sm_block_sum_before(sum, sc.a, total);
         double rise[K], high = 0.0;
 #pragma unroll
         for (int k = 0; k < K; k++) {

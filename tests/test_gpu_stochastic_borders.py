@@ -37,3 +37,27 @@ def test_small_numbers_in_short_rows(V, T):
         x = scores_of("steps", 16, V, dtype, False, seed=V)             # weights over the whole range of the type
         for kw in (dict(), dict(temperature=0.5), dict(top_k=V // 2 + 65)):
             check_sample(x, numbers(SMALL, 16), logits=False, **kw)
+
+
+# A long row's masses are added up tile by tile (4096 scores), four tiles a thread
+TILE = 4096
+
+
+def test_a_far_larger_tile_behind_does_not_hide_a_small_one():
+    x = torch.full((1, 9 * TILE), -math.inf, device=DEV)
+    x[0, 5], x[0, 4 * TILE + 9], x[0, 7 * TILE + 3] = -80.0, -80.0 + math.log(1.5), 0.0
+    p = math.exp(-80.0)
+    assert stochastic.sample(x, numbers([0.5 * p, 1.2 * p, 2.0 * p, 3.0 * p], 1)).tolist() == [[5, 4 * TILE + 9, 4 * TILE + 9, 7 * TILE + 3]]
+
+
+@pytest.mark.parametrize("V", [12289, 40000, 300001])
+@pytest.mark.parametrize("T", [0.05, 0.1, 1.0])
+def test_small_numbers_in_long_rows(V, T):
+    """masses that fall by tiles and rise again, so that a thread's tiles hold sums far apart"""
+    for dtype in TYPES:
+        x = scores_of("masked", 3, V, dtype, True, seed=V)
+        far = torch.rand(3, (V + TILE - 1) // TILE, generator=torch.Generator(device=DEV).manual_seed(V), device=DEV).mul(-60.0)
+        y = (x.float() + far.repeat_interleave(TILE, dim=1)[:, :V] * T).to(dtype)
+        for z in (x, y):
+            for kw in (dict(), dict(top_k=V // 2), dict(top_p=0.9999), dict(min_p=1e-20)):
+                check_sample(z, numbers(SMALL, 3), logits=True, temperature=T, **kw)

@@ -8,7 +8,8 @@
 //   with replacement:    smallest i with (w_0 + ... + w_i) > u * total
 //   without:             the n largest l_i - log(-log(1 - u_i)), in index order
 //
-// All masses, sums and keys are in 64 bits: an index has to be the same as the definition's however many categories there are.  Masses that
+// All masses, sums and keys are in 64 bits: an index has to be the same as the definition's however many categories there are.  A mass below
+// 2^-1074 of the row's best is 0 and never drawn.  Masses that
 // are added by atomics (top-p's histograms) are added as integers, so that neither their order nor the launch changes a result: of 63 fraction
 // bits of the largest mass.  Floating sums have one fixed order.
 //
@@ -1686,31 +1687,37 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
     const double local = fmax((target - (t ? sums[t - 1] : 0.0)) / scale_up, 0.0), here = g[ng - 1];
     int k = sm_rank4(g, ng, [&](double s) { return s > local; });
     if (k >= ng) k = sm_rank4(g, ng, [&](double s) { return s >= here; });
-    // inside the group: the masses once more, in the same order
+    // Inside the group: the masses once more, in the same order.  A mass that is nothing next to the row's best (below 2^-1074 of it) may be
+    // something next to the tile's: it is not drawn, and where a group holds no other, the next that does is taken.  There is one: the tile's sum is
+    // something, and so is its best.
     const T* x = scores + r * sstride;
     const SmScale scale = { rule.mode, rule.inv_t, tops[t], 1.0 };
     const SmKept kept = st.kept;
-    const long long i0 = (long long)t * SM_STILE + k * SM_GROUP;
-    double acc = k ? g[k - 1] : 0.0;
-    int found = -1, any = -1;
-    LgVec4<T> v[SM_GROUP / 4];
     const bool vec = sm_aligned(x);
+    long long drawn = -1;
+    for (int q = 0; q < ng && drawn < 0; q++, k = k + 1 < ng ? k + 1 : 0) {
+        const long long i0 = (long long)t * SM_STILE + k * SM_GROUP;
+        double acc = k ? g[k - 1] : 0.0;
+        LgVec4<T> v[SM_GROUP / 4];
 #pragma unroll
-    for (int e = 0; e < SM_GROUP / 4; e++) v[e] = sm_load4(x, i0 + 4 * e, V, vec);
-    float z[SM_GROUP];
-    double mass[SM_GROUP];
+        for (int e = 0; e < SM_GROUP / 4; e++) v[e] = sm_load4(x, i0 + 4 * e, V, vec);
+        float z[SM_GROUP];
+        double mass[SM_GROUP];
 #pragma unroll
-    for (int e = 0; e < SM_GROUP; e++) {
-        const float y = sm_score(v[e / 4].v[e % 4], sm_floor(rule));
-        z[e] = sm_in(kept, y, (uint32_t)(i0 + e)) ? y : -INFINITY;
+        for (int e = 0; e < SM_GROUP; e++) {
+            const float y = sm_score(v[e / 4].v[e % 4], sm_floor(rule));
+            z[e] = sm_in(kept, y, (uint32_t)(i0 + e)) ? y : -INFINITY;
+        }
+        sm_masses(tables, scale, z, mass);
+        int found = -1, any = -1;
+#pragma unroll
+        for (int e = 0; e < SM_GROUP; e++) {
+            acc += mass[e];
+            if (mass[e] * scale_up > 0.0) { any = e; if (found < 0 && acc > local) found = e; }
+        }
+        if (any >= 0) drawn = i0 + (found >= 0 ? found : any);
     }
-    sm_masses(tables, scale, z, mass);
-#pragma unroll
-    for (int e = 0; e < SM_GROUP; e++) {
-        acc += mass[e];
-        if (mass[e] > 0.0) { any = e; if (found < 0 && acc > local) found = e; }
-    }
-    out[at] = i0 + (found >= 0 ? found : any);
+    out[at] = drawn;
 }
 
 // ---- long rows, without replacement ----------------------------------------------------------------------------------------------------

@@ -61,3 +61,23 @@ def test_small_numbers_in_long_rows(V, T):
         for z in (x, y):
             for kw in (dict(), dict(top_k=V // 2), dict(top_p=0.9999), dict(min_p=1e-20)):
                 check_sample(z, numbers(SMALL, 3), logits=True, temperature=T, **kw)
+
+
+@pytest.mark.parametrize("V", [12, 12288, 12289, 5 * TILE])
+@pytest.mark.parametrize("logits", [True, False])
+def test_a_mass_below_the_least_number_is_none(V, logits):
+    """masses are exp(l - max l) in 64 bits, whatever lies next to a score: exp(-750) is 0, exp(-100) is not"""
+    T = 0.01
+    x = torch.full((1, V), -math.inf if logits else 0.0, device=DEV)
+    x[0, 1], x[0, 3], x[0, V - 1] = (-7.5, -1.0, 0.0) if logits else (math.exp(-7.5), math.exp(-1.0), 1.0)
+    assert stochastic.sample(x, numbers([0.0, -1.0, math.nan, 1e-45, 0.5], 1), logits=logits, temperature=T).tolist() == [[3, 3, 3, 3, V - 1]]
+
+
+@pytest.mark.parametrize("V", [300, 9000, 12289, 40000])
+@pytest.mark.parametrize("T", [1e-30, 1e-3, 0.004, 0.01, 0.03])
+def test_nothing_without_a_mass_is_drawn_by_a_small_number(V, T):
+    for dtype in TYPES:
+        for kind in ("normal", "masked", "ties"):
+            x = scores_of(kind, 3, V, dtype, True, seed=V)
+            for kw in (dict(), dict(top_k=V // 2), dict(top_p=0.99)):
+                check_sample(x, numbers(SMALL, 3), logits=True, temperature=T, **kw)

@@ -809,7 +809,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
                 for (long long j = (long long)blockIdx.y * TPB + threadIdx.x; j < n; j += (long long)gridDim.y * TPB) {
                     const float uj = u[j];
                     const double t = (uj > 0.0f ? (double)uj : 0.0) * total;
-                    uint32_t lo = 0, hi = last;                        // the first sum that passes t, or the last one
+                    uint32_t lo = uj >= 1.0f ? last : 0, hi = last;    // the first sum that passes t, or the last one
                     while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (h.few.sum[mid] > t) hi = mid; else lo = mid + 1; }
                     out[j] = name(h.few.index[lo]);
                 }
@@ -954,7 +954,7 @@ __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__
         for (long long j = (long long)blockIdx.y * TPB + threadIdx.x; j < n; j += (long long)gridDim.y * TPB) {         // (blockIdx.y: its share of the draws)
             const float uj = u[j];
             const double t = (uj > 0.0f ? (double)uj : 0.0) * total;
-            uint32_t lo = 0, hi = last - 1;                            // first element whose sum passes t; at the end the last one with a mass
+            uint32_t lo = uj >= 1.0f ? last - 1 : 0, hi = last - 1;    // first element whose sum passes t; from one on the last one with a mass
             while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (mass[mid % EPT * TPB + mid / EPT] > t) hi = mid; else lo = mid + 1; }
             out[j] = name(lo);
         }
@@ -979,7 +979,7 @@ struct SmRowState {                    // (sm_begin_kernel knows where kept and 
     double total, top;                 // with replacement: total mass of the kept; the largest l
     unsigned long long sure;           // race: winners
     float best, least;                 // largest score; least score that passes min-p
-    uint32_t prefix, ties, ended, cut, zone_lo, zone_hi, candidates;
+    uint32_t prefix, ties, ended, cut, zone_lo, zone_hi, candidates, end_tile /*with replacement: the last tile with a mass*/;
     uint32_t ticket[SM_STEPS], sub[16][32];       // (sub: one of 32 words, 128 bytes apart)
 };
 
@@ -1597,6 +1597,7 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
     const unsigned long long m = sm_block_max<unsigned long long>((ordered >> 63) ? ~ordered : (ordered | 0x8000000000000000ull), sc.b);
     top = __longlong_as_double((long long)((m >> 63) ? (m & 0x7fffffffffffffffull) : ~m));
     double run = 0.0, risen = 0.0;
+    uint32_t end = 0;
     constexpr int K = 4;                                               // tiles a thread
     for (long long base = 0; base < wk.stiles; base += 256 * K) {
         const long long t0 = base + threadIdx.x * K;
@@ -1616,7 +1617,7 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
 #pragma unroll
         for (int k = 0; k < K; k++) {
             at += mass[k];
-            if (mass[k] > 0.0 && at > high) high = at;
+            if (mass[k] > 0.0) { end = (uint32_t)(t0 + k); if (at > high) high = at; }
             rise[k] = high;
         }
         const double below = fmax(sm_block_rise_before(high, sc.b, most), risen);
@@ -1625,6 +1626,8 @@ __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scor
         risen = fmax(risen, most);
         run += total;
     }
+    end = sm_wave_scan<false>(end, SmMaxOf());
+    if ((threadIdx.x & 63) == 63) atomicMax(&st.end_tile, end);
     if (threadIdx.x == 0) { st.total = run; st.top = top; st.kept = kept; }
 }
 
@@ -1679,23 +1682,24 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
         const int k = sm_rank(ends, ngroups, past), t = k * group;
         return k < ngroups && group > 1 ? t + sm_rank(sums + t, t + group < tiles ? group : tiles - t, past) : t;
     };
-    int t = tile_of([&](double s) { return s > target; });
-    if (t >= tiles) t = tile_of([&](double s) { return s >= total; });                                  // rounding, or u >= 1: where the masses end
+    int t = uj >= 1.0f ? tiles : tile_of([&](double s) { return s > target; });
+    const bool last = t >= tiles;                                      // (or rounding: the last one with a mass)
+    if (last) t = (int)st.end_tile;
     const double* g = wk.group + (r * wk.stiles + t) * (long long)(SM_STILE / SM_GROUP);
     const int ng = SM_STILE / SM_GROUP;
     const double scale_up = rule.mode == SM_LINEAR ? 1.0 : sm_exp(tables, tops[t] - st.top);
     const double local = fmax((target - (t ? sums[t - 1] : 0.0)) / scale_up, 0.0), here = g[ng - 1];
-    int k = sm_rank4(g, ng, [&](double s) { return s > local; });
+    int k = last ? ng - 1 : sm_rank4(g, ng, [&](double s) { return s > local; });
     if (k >= ng) k = sm_rank4(g, ng, [&](double s) { return s >= here; });
     // Inside the group: the masses once more, in the same order.  A mass that is nothing next to the row's best (below 2^-1074 of it) may be
-    // something next to the tile's: it is not drawn, and where a group holds no other, the next that does is taken.  There is one: the tile's sum is
-    // something, and so is its best.
+    // something next to the tile's: it is not drawn, and where a group holds no other, the next that does is taken (the one before, on the way to
+    // the last).  There is one: the tile's sum is something, and so is its best.
     const T* x = scores + r * sstride;
     const SmScale scale = { rule.mode, rule.inv_t, tops[t], 1.0 };
     const SmKept kept = st.kept;
     const bool vec = sm_aligned(x);
     long long drawn = -1;
-    for (int q = 0; q < ng && drawn < 0; q++, k = k + 1 < ng ? k + 1 : 0) {
+    for (int q = 0; q < ng && drawn < 0; q++, k = last ? k - 1 : k + 1 < ng ? k + 1 : 0) {
         const long long i0 = (long long)t * SM_STILE + k * SM_GROUP;
         double acc = k ? g[k - 1] : 0.0;
         LgVec4<T> v[SM_GROUP / 4];
@@ -1713,7 +1717,7 @@ __global__ void __launch_bounds__(256) sm_draw_kernel(const T* __restrict__ scor
 #pragma unroll
         for (int e = 0; e < SM_GROUP; e++) {
             acc += mass[e];
-            if (mass[e] * scale_up > 0.0) { any = e; if (found < 0 && acc > local) found = e; }
+            if (mass[e] * scale_up > 0.0) { any = e; if (found < 0 && !last && acc > local) found = e; }
         }
         if (any >= 0) drawn = i0 + (found >= 0 ? found : any);
     }

@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from litegs_amd import stochastic
-from tests.test_gpu_stochastic import DEV, TYPES, check_sample, scores_of
+from tests import stochastic_reference as ref
+from tests.test_gpu_stochastic import DEV, TYPES, check_sample, rule, scores_of
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +82,25 @@ def test_nothing_without_a_mass_is_drawn_by_a_small_number(V, T):
             x = scores_of(kind, 3, V, dtype, True, seed=V)
             for kw in (dict(), dict(top_k=V // 2), dict(top_p=0.99)):
                 check_sample(x, numbers(SMALL, 3), logits=True, temperature=T, **kw)
+
+
+@pytest.mark.parametrize("V", [12, 300, 4097, 12288, 12289, 40000, 300001])
+@pytest.mark.parametrize("T", [1e-30, 0.004, 0.03, 0.1, 1.0])
+def test_numbers_from_one_on_draw_the_last(V, T):
+    """... with a mass, however small: what follows the large ones does not move their sum.  (The 64-bit form rounds the total, and what is
+    above the rounded one is found before the last: from one on the answer is the definition's own, the last category with a mass.)"""
+    def check(x, logits, **kw):
+        a = rule(kw, logits)
+        got = stochastic.sample(x, numbers([1.0, 1.5, math.inf], x.shape[0]), **a).cpu()
+        for r, row in zip(x.double().cpu().numpy(), got.tolist()):
+            who, _, mass = ref.filtered(r, big=torch.finfo(x.dtype).max, **a)
+            assert row == [int(who[mass > 0][-1])] * 3, (x.shape, x.dtype, kw)
+        check_sample(x, numbers([1.0 - 2.0 ** -24], x.shape[0]), logits=logits, **kw)
+
+    for dtype in TYPES:
+        for kind in ("normal", "masked"):
+            x = scores_of(kind, 3, V, dtype, True, seed=V)
+            x[0, V // 3], x[1, 0] = 30.0, 30.0
+            for kw in (dict(), dict(top_k=V // 2), dict(top_k=min(V // 2, 50)), dict(top_p=0.99), dict(min_p=1e-30)):
+                check(x, True, temperature=T, **kw)
+        check(scores_of("steps", 3, V, dtype, False, seed=V), False)

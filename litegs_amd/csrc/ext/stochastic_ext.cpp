@@ -4,7 +4,10 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <mutex>
 #include <optional>
@@ -29,6 +32,16 @@ inline int dtype_code(const Tensor& t, const char* what)
     return -1;
 }
 inline const int64_t* words(const OptTensor& t) { return t.has_value() && t->defined() ? t->data_ptr<int64_t>() : nullptr; }
+
+// Whether torch's calls are being recorded (a trace, a proxy or functional mode) or only their shapes worked out (a fake mode).  The kernels here
+// write into empty tensors behind the dispatcher's back, so that a recording would hold the empty tensor alone.
+bool traced()
+{
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Key = c10::impl::TorchDispatchModeKey;
+    if (torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch)) return true;
+    return Modes::stack_len() > 0 && (Modes::get_mode(Key::PROXY).has_value() || Modes::get_mode(Key::FAKE).has_value() || Modes::get_mode(Key::FUNCTIONAL).has_value());
+}
 
 struct Mask {                          // which elements a call keeps: the arguments of lg_dropout behind the type
     int64_t lead, M;
@@ -63,6 +76,7 @@ struct DropoutBackward : public torch::autograd::Node {
 Tensor dropout(const Tensor& x, const Mask& m, const OptTensor& offset_dev, const OptTensor& chunk_ids)
 {
     TORCH_CHECK(!torch::autograd::isFwGradDefined(x), "dropout: no forward-mode derivative");
+    TORCH_CHECK(!traced(), "dropout: cannot be traced (the kernel would not be part of the trace)");        // (a backward pass comes here without the Python function)
     const bool graph = at::GradMode::is_enabled() && x.requires_grad();
     Tensor y;
     {
@@ -112,6 +126,7 @@ void sample(const Tensor& scores, const Tensor& u, Tensor out, int64_t n, bool d
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
+    m.def("traced", &traced);
     m.def("dropout", &dropout_call);
     m.def("random_draw", &random_draw);
     m.def("sample", &sample);

@@ -7,7 +7,8 @@ backward pass instead of being stored, and a run can be repeated from any step. 
 an int64 tensor of one element on the device it is read by the kernel, and a captured graph draws anew on every replay that changes it.
 
 The reference draws with ``torch.multinomial`` (at most 2^24 categories) and ``torch.normal`` (litegs/training/densify.py:296-310); it has
-no dropout.  GPU tensors only; everything runs on the current stream.
+no dropout.  GPU tensors only; everything runs on the current stream.  The calls are no operators of torch's dispatcher: a trace
+(``torch.jit.trace``, ``make_fx``, ``torch.export``) or a fake-tensor mode would not see the kernels, and is refused.
 """
 from __future__ import annotations
 
@@ -33,6 +34,20 @@ def _s() -> int:
 def _on(device: torch.device):
     """launches go to the tensor's device, whichever is current"""
     return nullcontext() if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _traced() -> bool:
+    """the compiled binding's ``traced`` (csrc/ext/stochastic_ext.cpp)"""
+    c = torch._C
+    if c._get_tracing_state() is not None or c._dispatch_tls_is_dispatch_key_included(c.DispatchKey.PreDispatch):
+        return True
+    keys = c._TorchDispatchModeKey
+    return c._len_torch_dispatch_stack() > 0 and any(c._get_dispatch_mode(k) is not None for k in (keys.PROXY, keys.FAKE, keys.FUNCTIONAL))
+
+
+def _not_traced(what: str) -> None:
+    if _traced() if _C is None else _C.traced():
+        raise RuntimeError(f"{what}: cannot be traced (the kernel would not be part of the trace)")
 
 
 def _float_tensor(t, what: str) -> None:
@@ -70,6 +85,7 @@ class _Dropout(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, lead, M, p, seed, offset, offset_dev, chunk_ids, S):
+        _not_traced("dropout")
         ctx.meta = (lead, M, p, seed, offset, S)
         ctx.save_for_backward(offset_dev, chunk_ids)        # a step counter advanced in between is reported by autograd, not used
         x = x.contiguous()
@@ -94,6 +110,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Offset = 0, shared: in
     [R,3,chunks,S] drops whole Gaussians).  ``chunk_ids`` int64 [A] for ``x`` [..., A, S]: column ``s`` of slot ``a`` belongs to Gaussian
     ``chunk_ids[a] * S + s``, and that is its index, shared by all leading dimensions -- a Gaussian's decision is the same in every view,
     whatever slot its chunk was compacted to.  ``p = 1`` drops everything."""
+    _not_traced("dropout")
     _float_tensor(x, "dropout")
     p = _real(p, "dropout", "p", 0.0, 1.0)
     key = _key(seed, offset, x.device, "dropout")
@@ -123,6 +140,7 @@ def _draw(std, out, seed, offset, offset_dev, what: str) -> None:
 
 def uniform(shape, seed: int, offset: Offset = 0, dtype: torch.dtype = torch.float32, device: Optional[torch.device] = None) -> torch.Tensor:
     """``(word(i) + 1/2) / 2^32`` rounded to ``dtype`` and kept below one: in (0, 1) in float32 (in half width the smallest round to 0)"""
+    _not_traced("uniform")
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if device.type != "cuda" or dtype not in _DTYPES:
         raise RuntimeError("uniform: float32, float16 or bfloat16 on a GPU (no CPU path)")
@@ -134,6 +152,7 @@ def uniform(shape, seed: int, offset: Offset = 0, dtype: torch.dtype = torch.flo
 
 def normal(std: torch.Tensor, seed: int, offset: Offset = 0) -> torch.Tensor:
     """``std * N(0,1)``, element for element (Box-Muller: the words 2j and 2j + 1 give the elements 2j and 2j + 1); not differentiable"""
+    _not_traced("normal")
     _float_tensor(std, "normal")
     seed, offset, offset_dev = _key(seed, offset, std.device, "normal")
     std = std.detach().contiguous()
@@ -184,6 +203,7 @@ def _sample(what: str, scores, u, n: int, distinct: bool, temperature, top_k, to
 
 
 def _check_scores(scores, u, what: str) -> None:
+    _not_traced(what)
     _float_tensor(scores, what)
     if not isinstance(u, torch.Tensor) or u.dtype != torch.float32 or u.device != scores.device:
         raise RuntimeError(f"{what}: u must be float32 on the device of the scores")

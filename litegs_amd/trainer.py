@@ -70,7 +70,9 @@ class FrameTrainer:
         self.sched_ticks = 1
         # opacity dropout (stochastic.dropout) of training steps: each step drops this part of the Gaussians and scales the others by
         # 1 / (1 - p).  Operator path only (fused=False): the native executor activates opacities inside its own kernels.  A step's mask is a
-        # function of (opacity_dropout_seed, training_steps, Gaussian), whichever chunks the frame sees.  Seeds from 2^63 on are dropout's:
+        # function of (opacity_dropout_seed, training_steps, Gaussian), whichever chunks the frame sees.  While statistics are collected nothing
+        # is dropped: a dropped Gaussian leaves no trace in a frame, and density control would take one that every frame of the epoch dropped
+        # for invisible, and prune it.  Seeds from 2^63 on are dropout's:
         # the density controller's draws count epochs under the seeds below, and no two draws of a run may share their words.
         self.opacity_dropout = 0.0
         self.opacity_dropout_seed = 1 << 63
@@ -107,7 +109,7 @@ class FrameTrainer:
         vis_id, vis_num, cx, cs, cr, cc, co = R.render_preprocess(
             self.cluster_origin, self.cluster_extend, frame.planes, frame.view, xyz, scale, rot, sh_0, sh_rest, opacity,
             self.feedback_visible_chunks_num, frame.idx_tensor, self.pp, self.degree,
-            (self.opacity_dropout, self.opacity_dropout_seed, self.training_steps) if training and self.opacity_dropout > 0.0 else None)
+            (0.0 if STATS.active else self.opacity_dropout, self.opacity_dropout_seed, self.training_steps) if training and self.opacity_dropout > 0.0 else None)
         valid_length = vis_num * self.pp.cluster_size
         img, trans, depth, normal, prim_vis = R.render(frame.view, frame.proj, cx, cs, cr, cc, co, valid_length,
                                                        self.feedback_binning_allocate_size, frame.idx_tensor, self.degree,

@@ -19,7 +19,7 @@ Differences from the reference, all deliberate:
   so the exchange's per-set size predictions stay valid.  Only rank 0 writes files and prints;
 * frames are drawn by a seeded permutation per epoch instead of a ``DataLoader(shuffle=True)`` (same distribution, reproducible);
 * ``op.opacity_dropout`` (not in the reference): every training step drops that part of the Gaussians (litegs_amd/stochastic.py), on the
-  operator path; evaluation renders all of them;
+  operator path; evaluation renders all of them, and so do the epochs whose statistics density control decides by;
 * ``op.learnable_viewproj`` (trainer.py:84-91, 117-123, 158-162, 183-191, 221-222): the cameras are built from their parameters -- the
   frames' COLMAP poses as a sparse ``nn.Embedding`` [frames, 7] (quaternion + translation) and the first camera's 1 / tan(fov_x / 2) --
   by the ``create_viewproj`` operator, ``SparseAdam(lr 1e-4)`` steps the embedding after every iteration, evaluation frames take the

@@ -68,13 +68,18 @@ class Sampler:
     def multinomial(self, score: torch.Tensor, budget: int) -> torch.Tensor:
         return torch.multinomial(score, budget, replacement=False, generator=self._gen["g"])
 
+    def mixed(self, picked: torch.Tensor) -> torch.Tensor:
+        """the picks in an order that says nothing of their place (torch.multinomial's is that of the draws): the last ones may be left out"""
+        return picked
+
     def normal(self, std: torch.Tensor) -> torch.Tensor:
         return torch.normal(mean=torch.zeros_like(std), std=std, generator=self._gen["g"])
 
 
 class CounterSampler(Sampler):
     """The same draws from ``litegs_amd.stochastic``: functions of (seed, epoch, number of the draw, Gaussian) alone.  Gaussians without a
-    score are never picked; where fewer have one than the budget asks for, all of them are."""
+    score are never picked; where fewer have one than the budget asks for, all of them are.  Picks come in ascending order, ``mixed`` brings
+    them into a random one."""
 
     def __init__(self, seed: int = 0, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
         from . import stochastic
@@ -97,6 +102,10 @@ class CounterSampler(Sampler):
         u = stochastic.uniform(score.shape, self.seed, self._next(), device=score.device)
         picked = stochastic.sample_distinct(score, u, budget, logits=False, **self.rule)
         return picked[picked >= 0]
+
+    def mixed(self, picked: torch.Tensor) -> torch.Tensor:
+        from . import stochastic
+        return picked[stochastic.uniform(picked.shape, self.seed, self._next(), device=picked.device).argsort(stable=True)]
 
     def normal(self, std: torch.Tensor) -> torch.Tensor:
         from . import stochastic
@@ -232,7 +241,7 @@ class DensityController:
         n = xyz.shape[-1]
         prune_num = int(self.prune_mask(opacity.sigmoid()).sum())
         budget = self.budget(epoch, n, prune_num)
-        picked = self.sampler.multinomial(self.score(opacity), budget)
+        picked = self.sampler.mixed(self.sampler.multinomial(self.score(opacity), budget))       # (which of them the truncation below drops is chance)
         largest = scale[:, picked].exp().max(dim=0).values
         limit = self.p.percent_dense * self.screen_extent
         clone_idx, split_idx = picked[largest <= limit], picked[largest > limit]

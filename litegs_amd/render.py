@@ -56,7 +56,8 @@ def render_preprocess(cluster_origin: Optional[torch.Tensor], cluster_extend: Op
     """-> (visible_chunkid, visible_chunks_num, culled_xyz, culled_scale, culled_rot, color, culled_opacity).
 
     ``opacity_dropout`` (not in the reference): (p, seed, offset) of ``stochastic.dropout`` on the activated opacities; a Gaussian's decision
-    depends on its place in the whole cloud, not on the chunks that this view keeps.  A dropped Gaussian (opacity 0) emits no tile instances."""
+    depends on its place in the whole cloud, not on the chunks that this view keeps.  A dropped Gaussian (opacity 0) emits no tile instances.
+    The others' opacities are divided by 1 - p and may exceed one: ``render`` them with ``limit_opacity``."""
     visible_chunkid = None
     visible_chunks_num = None
     if pp.cluster_size:
@@ -88,8 +89,14 @@ def render_preprocess(cluster_origin: Optional[torch.Tensor], cluster_extend: Op
 def render(view_matrix: torch.Tensor, proj_matrix: torch.Tensor, xyz: torch.Tensor, scale: torch.Tensor, rot: torch.Tensor,
            color: torch.Tensor, opacity: torch.Tensor, valid_length: Optional[torch.Tensor],
            feedback_binning_allocate_size: Optional[torch.Tensor], idx_tensor: Optional[torch.Tensor],
-           actived_sh_degree: int, output_shape: Tuple[int, int], pp):
-    """-> (img[V,3,H,W] clamped to [0,1], transmitance|None, depth|None, normal=None, primitive_visible)."""
+           actived_sh_degree: int, output_shape: Tuple[int, int], pp, limit_opacity: bool = False):
+    """-> (img[V,3,H,W] clamped to [0,1], transmitance|None, depth|None, normal=None, primitive_visible).
+
+    ``limit_opacity`` (not in the reference): opacities above one (``opacity_dropout``) count as one, and get no gradient.  Without it they
+    saturate the blend's alpha over a whole core, through which its backward pass hands the gradient as if alpha still grew (a limit at
+    255/256 that opacities of at most one reach by 1/256: the reference's choice)."""
+    if limit_opacity:
+        opacity = opacity.clamp(max=1.0)
     view_pos, ndc_pos = wrapper.MVPTransform.apply(xyz, view_matrix, proj_matrix, valid_length)
     transform_matrix = wrapper.CreateTransformMatrix.call_fused(scale, rot, valid_length)
     J = wrapper.CreateRaySpaceTransformMatrix.call_fused(view_pos, proj_matrix, output_shape, valid_length)

@@ -106,14 +106,15 @@ class FrameTrainer:
             fn = self.renderer.render_raw if raw else self.renderer.render
             img, vis_id, vis_num = fn(frame.cam, self.cluster_origin, self.cluster_extend, xyz, scale, rot, sh_0, sh_rest, opacity, self.degree)
             return img, vis_id, vis_num, None
+        drop = training and self.opacity_dropout > 0.0
         vis_id, vis_num, cx, cs, cr, cc, co = R.render_preprocess(
             self.cluster_origin, self.cluster_extend, frame.planes, frame.view, xyz, scale, rot, sh_0, sh_rest, opacity,
             self.feedback_visible_chunks_num, frame.idx_tensor, self.pp, self.degree,
-            (0.0 if STATS.active else self.opacity_dropout, self.opacity_dropout_seed, self.training_steps) if training and self.opacity_dropout > 0.0 else None)
+            (0.0 if STATS.active else self.opacity_dropout, self.opacity_dropout_seed, self.training_steps) if drop else None)
         valid_length = vis_num * self.pp.cluster_size
         img, trans, depth, normal, prim_vis = R.render(frame.view, frame.proj, cx, cs, cr, cc, co, valid_length,
                                                        self.feedback_binning_allocate_size, frame.idx_tensor, self.degree,
-                                                       (self.H, self.W), self.pp)
+                                                       (self.H, self.W), self.pp, limit_opacity=drop)
         return img, vis_id, vis_num, prim_vis
 
     def step(self, frame_index: int, grad_hook=None, hook_slot: int = 0, peer_frames=None):

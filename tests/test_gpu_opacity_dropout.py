@@ -101,3 +101,25 @@ def test_training_steps_limit_opacities(monkeypatch):
         assert seen == [1.0]
     finally:
         tr.close()
+
+
+# ---- the executor --------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fused,drop,warned", [(True, 0.1, True), (False, 0.1, False), (True, 0.0, False)])
+def test_start_says_that_it_leaves_the_executor(fused, drop, warned, tmp_path):
+    import os
+    import sys
+    import warnings
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tools"))
+    import make_colmap_scene as M
+    from litegs_amd import arguments as A
+    from litegs_amd import training
+    M.make(str(tmp_path / "scene"), points=1024, frames=2, width=96, height=64, focal=80.0, sfm_fraction=0.6, seed=3)
+    lp, op, pp, dp = A.get_default_arg()
+    lp.source_path, lp.model_path, lp.eval, lp.resolution = str(tmp_path / "scene"), str(tmp_path / "m"), False, 1
+    op.iterations, op.opacity_dropout = 2, drop
+    with warnings.catch_warnings(record=True) as seen:
+        warnings.simplefilter("always")
+        trainer, _ = training.start(lp, op, pp, dp, fused=fused, log=lambda *a: None)
+    assert any("without the native executor" in str(w.message) for w in seen) == warned
+    assert trainer.fused == (fused and not drop)
+    trainer.close()

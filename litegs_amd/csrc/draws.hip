@@ -29,8 +29,8 @@ __device__ __forceinline__ float dr_product(float a, float b)
     asm volatile("" : "+v"(c));
     return c;
 }
-// Measured, launch behind launch: 3 M float32 4.6 us a direction (24 MB: 5.2 TB/s), by chunk id 5.6, 45 rows of 500 k 27 us (180 MB: 6.6 TB/s, part
-// of it from the last-level cache), 8 M bfloat16 9.1 (their words' issue alone 7).  What a forward and a backward pass take of a user's program
+// Measured, launch behind launch: 3 M float32 4.9 us a direction (24 MB: 4.9 TB/s), by chunk id 5.6, 45 rows of 500 k 27.5 us (180 MB: 6.5 TB/s, part
+// of it from the last-level cache), 8 M bfloat16 8.7 (their words' issue alone 7).  What a forward and a backward pass take of a user's program
 // for less than 10 M elements is the autograd engine's host time (40 us).
 // Work items are (block of DR_ROWS rows, group), groups innermost, so that short rows fill a workgroup too.
 #define DR_ROWS 8
@@ -141,7 +141,9 @@ __device__ __forceinline__ void dr_cos_sin(uint32_t k, float& c, float& s)
     s = (q >= 2 && q < 4) ? -b : b;
 }
 
-// One thread, one block of four words.  10 M uniform float32 9.2 us (40 MB: 4.4 TB/s), 150 k normal ones 3 us (a launch).
+// One thread, one block of four words.  10 M uniform float32 9.1 us (40 MB: 4.4 TB/s); normal ones 15.5 us (80 MB: 5.2 TB/s), 3 M 6.8, 150 k 2.6
+// (a launch).  Radius, angle and product are worked out in 32 bits: float32 results are then off by some 6e-8 of the largest where 64 bits would
+// leave 3e-8, which is no use to a random number and costs several times the instructions.
 template <typename T, bool NORMAL, bool VEC>
 __global__ void __launch_bounds__(DR_TPB) draw_kernel(const T* __restrict__ std_, T* __restrict__ out, long long n, DrKey key, float top)
 {

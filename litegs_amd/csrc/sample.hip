@@ -446,10 +446,12 @@ __device__ __forceinline__ void sm_min_p(const SmRule& rule, float best, SmKept&
 // float bound it to a bin; what lies above the bin by more than twice the approximation's error wins, what lies below by as much loses, and
 // the few in the zone between are ranked by their exact 64-bit keys.
 //
-// Error of k: the logarithm instruction is good to a step of its result or 2^-22 (arguments next to one), log2(e) / T and the products round
-// three times, -ln(1 - u) is good to 2^-19 relative (below 2^-6 a series, above it 1 - u is off by 2^-25 of at least 2^-6): together less
-// than 2^-17 + |log2(mass)| 2^-21 + |log2(-ln(1-u))| 2^-21, the last at most 33, and for weights 2^-22 of the slope 1 / T (the logarithm of a
-// weight next to one).  sm_margin allows twice that and more.
+// Error of k, with the logarithm instruction good to a step of its result or, for arguments next to one, to 2^-22:
+//   -ln(1 - u): below u = 2^-6 a series, good to 2^-21 relative.  From there on log2(1 - u) is at least 2^-5.5 and off by the instruction's
+//   2^-22 and by the rounding of 1 - u (2^-25, i.e. 2^-23.5 in the logarithm): 2^-16 relative, so that its own logarithm is off by 2^-15.4;
+//   that logarithm (at most 33), log2(mass) (at most |k| + 33), slope and products round by 2^-21 of them at most: 2^-15.9 + |k| 2^-21;
+//   the logarithm of a weight next to one: 2^-22 of the slope.
+// Together less than 2^-14.6 + |k| 2^-21 + slope 2^-22.  sm_margin allows twice each of the three and more.
 __device__ __forceinline__ float sm_log2(float x)                      // x > 0, subnormals too
 {
     const bool small = x < 0x1p-100f;
@@ -673,7 +675,7 @@ __device__ __forceinline__ SmKept sm_filter_short(const float (&x)[EPT], const d
 }
 
 // A row from beginning to end in one launch: scores in registers, masses in LDS (worked out once), and one histogram level a filter as a rule.
-// 10 k scores: a plain draw 9.5 us, behind top-k 50 and top-p 10, behind top-p 20, 500 distinct 18; a launch alone is 5.  64 rows take what one takes (a compute
+// 10 k scores: a plain draw 10.4 us, behind top-k 50 and top-p 10, behind top-p 21, 500 distinct 18; a launch alone is 5.  64 rows take what one takes (a compute
 // unit each).
 template <typename T, int TPB, int EPT, bool DISTINCT>
 __global__ void __launch_bounds__(TPB) sample_short_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
@@ -1237,8 +1239,8 @@ __global__ void __launch_bounds__(SM_LTPB) sm_level_kernel(const T* __restrict__
 // The 65536 ordered keys of a 16-bit type are counted in LDS (two counters a word: a workgroup takes at most SM_SHARE16 elements), added up in
 // memory, and the last workgroup works top-k and top-p out of the counts: one pass over the row and one exponential per distinct score, in
 // the place of one pass for the best and three for each filter.  16 rows of 100 k: 24 us, about half of it the last workgroup's conclusion.
-// Rows of 50 k behind top-p: 1 row 46 us a call (by levels 63), 64 rows 57 (82), 256 rows 129 (152), 512 rows 228 (275); behind top-k alone 64
-// rows 47 (54), 256 rows 106 (94).  So up to 256 rows, where the counts are 64 MB, and without top-p up to 128.
+// Rows of 50 k behind top-p: 1 row 45 us a call (by levels 63), 64 rows 58 (83), 256 rows 131 (160), 512 rows 231 (287); behind top-k alone 64
+// rows 51 (57), 128 rows 72 (82), 256 rows 118 (110).  So up to 256 rows, where the counts are 64 MB, and without top-p up to 128.
 #define SM_SHARE16 32768
 __device__ __forceinline__ uint32_t sm_bits(LgHalf v) { return (uint32_t)__builtin_bit_cast(uint16_t, v); }
 __device__ __forceinline__ uint32_t sm_bits(LgBf16 v) { return v.bits; }
@@ -1497,8 +1499,9 @@ __global__ void __launch_bounds__(SM_LTPB) sm_cut_kernel(const T* __restrict__ s
     for (int k = 0; k < E; k++) if (((is >> k) & 1) && ++before == rest) { st.kept.end = (uint32_t)(i0 + k) + 1; st.cut = 0; }
 }
 
-// A top-k of at most SM_SHORT elements leaves a short row, which one more launch finishes: 3 M scores behind top-k 50 and top-p 58 us, by the
-// long way 99; k = 5000 without top-p 58 and 64 (50 k scores: 54 and 51, the one case that loses).
+// A top-k of at most SM_SHORT elements leaves a short row, which one more launch finishes: 3 M scores behind top-k 50 and top-p 46 us, by the
+// long way 83; behind k = 5000 alone, where the long way is shortest, a draw 55 and 54, 500 distinct 65 and 70 (of 50 k scores 43 and 36, 53 and
+// 44: the case that loses).
 // What top-k left, in index order: scores, their names and (without replacement) their numbers; rule.top_k places a row, the last ones empty
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_gather_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u /*nullable*/, long long ustride,
@@ -1550,7 +1553,7 @@ __device__ __forceinline__ SmKept sm_final(const SmWork& wk, long long r, const 
 // ---- long rows, with replacement -------------------------------------------------------------------------------------------------------
 // Prefix sums of the kept masses inside tiles, one stored per SM_GROUP elements, relative to the tile's best element (so that no pass for the
 // row's best is needed); the last workgroup puts the tiles on a common scale.  Fixed order everywhere.  Workgroups of 256, five a compute unit,
-// hide each other's scans: 3 M weights 12 us, 10 M scores 31 (1.3 TB/s: the exponentials; 26 for weights, which have none).
+// hide each other's scans: 3 M weights 12.6 us, scores 14 (the exponentials; a plain draw of 10 M scores 40.7 us, of weights 34).
 template <typename T>
 __global__ void __launch_bounds__(256) sm_sums_kernel(const T* __restrict__ scores, long long sstride, long long V, SmRule rule, SmWork wk, SmWork whole, int step)
 {
@@ -1835,7 +1838,10 @@ __global__ void __launch_bounds__(SM_LTPB) sm_race_level_kernel(long long V, SmR
 
 #define SM_ZTILES 4096                 // tiles whose winners are counted in LDS
 // Winners as a bit per element, the zone's elements as a list, winners counted per tile; the last workgroup ranks the list (3 M: 13 us, 10 M
-// 18)
+// 18).  That holds while the zone is small.  Where a good part of the row has one key next to the border -- equal scores at a temperature of a
+// thousandth of them or less, which outweigh the numbers, or equal scores with equal numbers -- every one of them is added to the list by an
+// atomic on one word, and one workgroup works out their exact keys again and again: a call for 5 % of 100 k, 1 M and 10 M such scores takes 1.6, 18
+// and 190 ms (2.4, 25 and 250 with one number for all).
 template <typename T>
 __global__ void __launch_bounds__(SM_LTPB) sm_zone_kernel(const T* __restrict__ scores, long long sstride, const float* __restrict__ u, long long ustride,
                                                           long long V, long long n, SmRule rule, SmWork wk, int step)
@@ -2015,8 +2021,8 @@ static bool sm_rule(int logits, double temperature, long long top_k, double top_
     return true;
 }
 
-// How a call runs.  Short rows: one workgroup each, as far as its LDS and registers reach (12288 scores, short and long: plain 10 and 16 us, behind
-// top-p 20 and 53, 614 distinct 17 and 27; 64 rows 10 / 18, 22 / 58, 18 / 29).  Long ones: the filters by levels of a histogram, or, for 16-bit
+// How a call runs.  Short rows: one workgroup each, as far as its LDS and registers reach (12288 scores, short and long: plain 10 and 17 us, behind
+// top-p 22 and 53, 614 distinct 18 and 25; 64 rows 11 / 18, 22 / 59, 19 / 28).  Long ones: the filters by levels of a histogram, or, for 16-bit
 // scores, from one histogram of all keys; what a small top-k leaves goes on as a short row.  Both sides of these two stand at their kernels.
 struct SmPlan { bool is_short, top_k, top_p, counts, few; };
 #define SM_COUNTS_ROWS 256
@@ -2072,7 +2078,7 @@ static void sample_short(const T* scores, long long ss, const float* u, long lon
                          const uint32_t* names, long long* out, bool distinct, hipStream_t s)
 {
     // Many draws of few rows: workgroups that would idle filter the row once more and share its draws.  By one workgroup 5000 draws of 1000
-    // scores take 22 us and 100000 of 10000 171 us; with 4096 draws a workgroup 13 and 17 us, with 1024 7 and 12 us (7 and 11 us are 1000 draws).
+    // scores take 22 us and 100000 of 10000 171 us; with 4096 draws a workgroup 13 and 17 us, with 1024 7 and 12 us (7 and 12 us are 1000 draws).
     const long long share = (n + 1023) / 1024, most = R < 256 ? 256 / R : 1;
     const long long rows = 1ll << 21;                                  // of a launch: its threads are counted in 32 bits
     for (long long r = 0; r < R; r += rows) {
@@ -2086,8 +2092,8 @@ static void sample_short(const T* scores, long long ss, const float* u, long lon
         if (distinct) hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, true>), grid, dim3(TPB_), 0, s, x, ss, v, us, (int)V, n, rule, nm, o); \
         else hipLaunchKernelGGL((sample_short_kernel<T, TPB_, EPT_, false>), grid, dim3(TPB_), 0, s, x, ss, v, us, (int)V, n, rule, nm, o);         \
     } while (0)
-        // 300 scores in 256 x 4, 1024 x 4 and 768 x 16 threads x elements: a plain draw 4.8, 4.9 and 7.2 us, 512 rows of them 5.2, 9.6 and 15; 3000
-        // scores in the last two 5.4 and 7.4, 512 rows 11 and 16
+        // 300 scores in 256 x 4, 1024 x 4 and 768 x 16 threads x elements: a plain draw 4.4, 5.8 and 8.4 us, 512 rows of them 5.4, 11.3 and 16.6; 3000
+        // scores in the last two 5.9 and 8.6, 512 rows 12.3 and 17.2
         if (V <= 1024) SM_LAUNCH_SHORT(256, 4);
         else if (V <= 4096) SM_LAUNCH_SHORT(1024, 4);
         else SM_LAUNCH_SHORT(768, 16);

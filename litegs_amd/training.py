@@ -188,7 +188,7 @@ def start(lp, op, pp, dp, test_epochs: Sequence[int] = (), save_ply: Sequence[in
     if getattr(op, "learnable_viewproj", False):
         cam_state = _learnable_cameras(cameras_info, training_frames, test_frames, frames, test_frames_dev, H, W, device)
     if fused and drop > 0.0:
-        warnings.warn("op.opacity_dropout is a step of the operator path: training without the native executor, whose steps take about half the time", stacklevel=2)
+        warnings.warn("op.opacity_dropout is a step of the operator path: training without the native executor, whose steps are 1.3 to 2.3 times as fast", stacklevel=2)
     fused = bool(fused) and drop == 0.0
     trainer = FrameTrainer(params, frames, H, W, opt, sched, pp, sh_degree=0, device=device, fused=fused, extra_slots=len(test_frames_dev))
     trainer.opacity_dropout, trainer.opacity_dropout_seed = drop, 1 << 63 | (seed & (1 << 63) - 1)
